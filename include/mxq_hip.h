@@ -35,8 +35,9 @@ typedef void* mxq_stream_t;
  *   3  mxq_mx_pack_bytes; the MXQ_EBUSY status of mxq_systolic_noalloc.
  *   4  mxq_attend_windows writes one flag word per call and 64 query rows, each whole (was one per call, zeroed
  *      by the caller).
- *   5  mxq_systolic_plan_of. */
-#define MXQ_ABI_VERSION 5
+ *   5  mxq_systolic_plan_of.
+ *   6  mxq_route, mxq_dispatch, mxq_combine, mxq_packed_linear, mxq_expert_linear and their specs. */
+#define MXQ_ABI_VERSION 6
 
 enum { MXQ_OK = 0, MXQ_EINVAL = 1, MXQ_EHIP = 2, MXQ_EBUSY = 3 };
 
@@ -470,6 +471,74 @@ int mxq_block_lut_workspace(int64_t K, int64_t n, int32_t group, int32_t fmt_e, 
  * first minimum.  Codes already checked in range by the caller.  Replaces mxq/lut/formats.py:140-159. */
 int mxq_lut_finder(const int64_t* codes, int64_t K, int64_t n, int32_t group, const int64_t* fx_all,
                    int32_t ncodes, const int64_t* lut_fx, int64_t mask, int64_t* out, mxq_stream_t stream);
+
+/* ---- a mixture-of-experts layer on packed weights (no counterpart in the reference) ------------------------ */
+
+enum { MXQ_SCORE_SOFTMAX = 0, MXQ_SCORE_SIGMOID = 1 };
+enum { MXQ_ACT_NONE = 0, MXQ_ACT_SILU = 1, MXQ_ACT_GELU = 2, MXQ_ACT_GELU_TANH = 3, MXQ_ACT_RELU = 4 };
+/* Element formats of packed weights: one code a byte as mxq_pack writes them, MXQ_FMT_E2M1_PAIRS two codes a byte, the
+ * even column in the low nibble. */
+enum { MXQ_FMT_E4M3 = 0, MXQ_FMT_E5M2 = 1, MXQ_FMT_E3M2 = 2, MXQ_FMT_E2M3 = 3, MXQ_FMT_E2M1 = 4, MXQ_FMT_E2M1_PAIRS = 5 };
+
+typedef struct mxq_route_spec {
+  int32_t score;        /* MXQ_SCORE_* */
+  int32_t top_k;        /* 1 to min(64, E) */
+  int32_t groups;       /* divides E, at most 64; 1: no groups */
+  int32_t top_groups;   /* 1 to groups */
+  int32_t renormalize;  /* divide the chosen scores by their sum */
+  float scale;          /* multiplies the weights */
+} mxq_route_spec;
+
+/* Routing of T tokens to E <= 1024 experts.  Scores are softmax or sigmoid of the logits (T x E of dtype MXQ_DT_*),
+ * in 64 bits; experts are ranked by score + bias (float32, NULL: none), ties to the lowest index, among those whose
+ * logit is not -inf and whose group (E / groups neighbours) is one of the top_groups by the sum of its two best; the
+ * weights (T x top_k float32) are the chosen scores without the bias.  Where fewer than top_k are open the rest is
+ * expert -1 with weight 0.  A row with a NaN (under softmax also +inf) gets NaN weights and experts -1.
+ * mxq_route_grad: the logits' gradient (their dtype) from the weights' (float32), given mxq_route's experts. */
+int mxq_route(const void* logits, int32_t dtype, const float* bias, int64_t T, int64_t E, const mxq_route_spec* spec,
+              float* weights, int32_t* experts, mxq_stream_t stream);
+int mxq_route_grad(const void* logits, int32_t dtype, const int32_t* experts, const float* grad, int64_t T, int64_t E,
+                   const mxq_route_spec* spec, void* out, mxq_stream_t stream);
+
+/* The n slots (slot t * k + j: token t's j-th choice) sorted by expert, stably: order (n) the slots, offsets (E + 1)
+ * each expert's first row, positions (n) each slot's row.  A slot whose expert is not in [0, E) comes after the last
+ * expert's rows, its position given as -1 - row. */
+int mxq_dispatch(const int32_t* experts, int64_t n, int64_t E, int32_t* order, int32_t* offsets, int32_t* positions,
+                 mxq_stream_t stream);
+
+/* out (T x D) = residual (NULL: none) + sum over j of weights[t, j] y[positions[t, j]], summed in float32 in the order
+ * of j and rounded once; y (T k x D), residual and out of one dtype.  A slot of no expert adds nothing, unless its
+ * weight is NaN.  mxq_combine_grad: dy (T k x D, zeros for slots of no expert) and dw (T x k float32), either NULL. */
+int mxq_combine(const void* y, int32_t dtype, const float* weights, const int32_t* positions, const void* residual,
+                void* out, int64_t T, int64_t k, int64_t D, mxq_stream_t stream);
+int mxq_combine_grad(const void* grad, int32_t dtype, const void* y, const float* weights, const int32_t* positions,
+                     void* dy, float* dw, int64_t T, int64_t k, int64_t D, mxq_stream_t stream);
+
+typedef struct mxq_linear_spec {
+  int32_t x_dtype, bias_dtype, residual_dtype, y_dtype;   /* MXQ_DT_* */
+  int32_t format;       /* MXQ_FMT_* */
+  int32_t activation;   /* MXQ_ACT_* */
+  int32_t gated;        /* the weight has 2 N rows: y = act(x G^T + b) * (x U^T + c), G its first N rows, U the others */
+  int32_t top_k;        /* mxq_expert_linear: x's row is slot / top_k; 0: x's rows are in the experts' order */
+  int64_t ld_x, ld_residual, ld_y;                        /* row strides, in elements */
+  int64_t ld_codes, ld_scales;                            /* row strides, in bytes */
+  int64_t batch_codes, batch_scales, batch_bias;          /* mxq_expert_linear: strides between experts' matrices */
+} mxq_linear_spec;
+
+/* y (M x N) = act(x W^T + bias) [* (x U^T + bias of U)] + residual, W's rows packed codes (K of them a row) with one
+ * E8M0 byte for 32 columns; bias and residual NULL for none.  Products are exact, sums float32, y is rounded once.  A
+ * weight below 2^-126 is rounded to bfloat16's subnormals; scale byte 255 makes its block NaN.  `workspace`: device
+ * memory of mxq_packed_linear_workspace bytes, 256-byte aligned (NULL where that is 0).
+ * mxq_expert_linear: n rows sorted by expert (mxq_dispatch's order and offsets; order is read where top_k > 0), row r
+ * of expert e multiplied by matrix e; rows past the last expert's become zeros. */
+int64_t mxq_packed_linear_workspace(int64_t M, int64_t N, int64_t K, const mxq_linear_spec* spec);
+int mxq_packed_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias,
+                      const void* residual, void* y, int64_t M, int64_t N, int64_t K, const mxq_linear_spec* spec,
+                      void* workspace, mxq_stream_t stream);
+int64_t mxq_expert_linear_workspace(int64_t n, int64_t N, int64_t K, int64_t E, const mxq_linear_spec* spec);
+int mxq_expert_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias, void* y, int64_t n,
+                      int64_t N, int64_t K, int64_t E, const int32_t* order, const int32_t* offsets,
+                      const mxq_linear_spec* spec, void* workspace, mxq_stream_t stream);
 
 /* ---- elementwise primitives over flat arrays of n elements (the caller broadcasts) ---------------------- */
 

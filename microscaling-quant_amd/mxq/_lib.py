@@ -26,7 +26,7 @@ _lib: Optional[ctypes.CDLL] = None
 _FN = {}            # entry point name -> its ctypes function, filled by load()
 
 #: the MXQ_ABI_VERSION of include/mxq_hip.h these signatures follow; a library reporting another is refused
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 c_i32, c_i64, c_f32, c_f64, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
 
@@ -77,6 +77,20 @@ class SystolicPlan(ctypes.Structure):
 class AnchorSpec(ctypes.Structure):
     """mxq_anchor_spec (include/mxq_hip.h)."""
     _fields_ = [(n, c_i32) for n in ("width", "drop", "headroom", "has_emin", "emin", "nbits")]
+
+
+class RouteSpec(ctypes.Structure):
+    """mxq_route_spec (include/mxq_hip.h)."""
+    _fields_ = [("score", c_i32), ("top_k", c_i32), ("groups", c_i32), ("top_groups", c_i32), ("renormalize", c_i32),
+                ("scale", c_f32)]
+
+
+class LinearSpec(ctypes.Structure):
+    """mxq_linear_spec (include/mxq_hip.h)."""
+    _fields_ = [(n, c_i32) for n in ("x_dtype", "bias_dtype", "residual_dtype", "y_dtype", "format", "activation",
+                                     "gated", "top_k")] + \
+               [(n, c_i64) for n in ("ld_x", "ld_residual", "ld_y", "ld_codes", "ld_scales", "batch_codes",
+                                     "batch_scales", "batch_bias")]
 
 
 # exported symbol -> (restype, argtypes); every symbol include/mxq_hip.h declares
@@ -148,8 +162,21 @@ SIGNATURES = {
     "mxq_truncate_significand": (c_i32, [c_ptr, c_ptr, c_i64, c_i32, c_ptr]),
     "mxq_flush_product": (c_i32, [c_ptr, c_ptr, c_i64, c_f32, c_ptr]),
     "mxq_saturate": (c_i32, [c_ptr, c_ptr, c_i64, c_f32, c_f32, c_ptr]),
+    "mxq_route": (c_i32, [c_ptr, c_i32, c_ptr, c_i64, c_i64, ctypes.POINTER(RouteSpec), c_ptr, c_ptr, c_ptr]),
+    "mxq_route_grad": (c_i32, [c_ptr, c_i32, c_ptr, c_ptr, c_i64, c_i64, ctypes.POINTER(RouteSpec), c_ptr, c_ptr]),
+    "mxq_dispatch": (c_i32, [c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "mxq_combine": (c_i32, [c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr]),
+    "mxq_combine_grad": (c_i32, [c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr]),
+    "mxq_packed_linear_workspace": (c_i64, [c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
+    "mxq_packed_linear": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64,
+                                  ctypes.POINTER(LinearSpec), c_ptr, c_ptr]),
+    "mxq_expert_linear_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
+    "mxq_expert_linear": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr,
+                                  ctypes.POINTER(LinearSpec), c_ptr, c_ptr]),
 }
 
+# MXQ_DT_* codes
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # mxq_block_spec codes
 SCALE_NONE, SCALE_MXQUANT, SCALE_OCP, SCALE_OCP_NO_CLIP = 0, 1, 2, 3
 ELEM_NONE, ELEM_QTORCH, ELEM_IEEE, ELEM_OCP, ELEM_MICROSOFT = 0, 1, 2, 3, 4
@@ -263,13 +290,18 @@ def numel(shape: Sequence[int]) -> int:
     return n
 
 
-def run(name: str, *args) -> None:
-    """Call entry point `name` with args; raise RuntimeError on a nonzero status."""
+def call(name: str, *args):
+    """Call entry point `name` with args; its result."""
     fn = _FN.get(name)
     if fn is None:
         load()
         fn = _FN[name] if name in _FN else getattr(load(), name)
-    rc = fn(*args)
+    return fn(*args)
+
+
+def run(name: str, *args) -> None:
+    """Call entry point `name` with args; raise RuntimeError on a nonzero status."""
+    rc = call(name, *args)
     if rc != 0:
         check(rc, name)
 
