@@ -1,0 +1,266 @@
+// Products of many rows with packed weights on the matrix cores.
+//
+// A workgroup owns BM rows of x by BN rows of the weight and goes through the contraction 64 columns at a time.  x (64
+// bfloat16, 128 bytes a row) and the codes (64 or 32 bytes a row) come straight from global memory into LDS, three stages
+// deep: while one is multiplied the next has landed and the third is on its way.  The codes stay codes in LDS, half the
+// bytes, and become bfloat16 when a wave takes its operands: one conversion for two values with their scale, beside the
+// matrix instructions.  Lane (r, h) takes block h of row r's 64 columns, so a lane's 32 codes share one scale.
+// Chunks of 16 bytes are permuted within a row by its number, so that eight rows' chunks lie in different banks.
+// float16 and float32 activations have been split into bfloat16 planes one after another along a longer row: the walk
+// goes through the weight once a plane.
+#pragma once
+
+#include "packed_linear_common.h"
+
+namespace mxq {
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// Global memory straight into LDS, 16 bytes (or one byte, as a word) a lane, lane i's at base + 16 i (4 i).  Written as
+// assembly because the compiler would wait for all such loads before every LDS read; the waits are wait_stage's.
+__device__ __forceinline__ void dma16(uint32_t base, const void* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
+}
+__device__ __forceinline__ void dma1(uint32_t base, const void* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(base), "v"(p) : "memory");
+}
+
+// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; DIRECT: codes by DMA (K a multiple of 64, rows 16-byte
+// aligned), through registers otherwise.
+template <int FAM, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k_linear_tile(TileArgs ta) {
+  constexpr int WAVES_N = BN / (32 * WN), WAVES = BM / (32 * WM) * WAVES_N, THREADS = 64 * WAVES;
+  constexpr int WB = 2 * kBlockBytes<FAM>, CH = WB / 16;                 // a weight row's bytes and chunks of one stage
+  constexpr int XL = BM * 8 / THREADS, WL = BN * CH / THREADS, SL = BN * 2 / THREADS;   // loads a thread and stage
+  static_assert(WN == 2, "a wave's two tiles are neighbours, or G's and U's of the same outputs");
+  static_assert(XL >= 1 && WL >= 1 && SL >= 1 && BM * 8 % THREADS == 0, "whole loads");
+  struct Stage {
+    uint8_t x[BM * 128];
+    uint8_t w[BN * WB];
+    uint32_t s[BN * 2];
+  };
+  constexpr int PITCH = 32 * WN + 4;
+  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = 3 * sizeof(Stage);
+  __shared__ __attribute__((aligned(16))) uint8_t memory[kStages > kEpilogue ? kStages : kEpilogue];
+  Stage* stage = (Stage*)memory;
+
+  const LinearArgs& a = ta.l;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, h = lane >> 5, wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const bool gated = a.sp.gated;
+  const int outputs = gated ? BN / 2 : BN;
+
+  // Consecutive workgroups go to the eight XCDs in turn; each XCD gets a run of tiles, in strips of eight row tiles, so
+  // that what its L2 holds serves its neighbours.
+  const int total = ta.tiles_m * ta.tiles_n;
+  int at = blockIdx.x;
+  {
+    const int xcd = at & 7, local = at >> 3, base = total >> 3, more = total & 7;
+    at = xcd * base + (xcd < more ? xcd : more) + local;
+  }
+  const int strip = at / (8 * ta.tiles_n), in = at - strip * 8 * ta.tiles_n;
+  const int deep = ta.tiles_m - strip * 8 < 8 ? ta.tiles_m - strip * 8 : 8;
+  const int tile_n = in / deep;
+  const RowTile t = row_tile(a, BM, strip * 8 + in % deep);
+  if (t.expert < 0) return;
+  const int64_t n0 = (int64_t)tile_n * outputs;
+
+  // the weight row of LDS row q; gated: of every 64 rows the first 32 from G, the others the same outputs' from U
+  auto weight_row = [&](int q) {
+    int64_t n = gated ? n0 + (q >> 6) * 32 + (q & 31) : n0 + q;
+    if (n >= a.N) n = a.N - 1;
+    return gated && (q & 32) ? n + a.N : n;
+  };
+
+  f32x16 acc[WN][WM];
+#pragma unroll
+  for (int i = 0; i < WN; ++i)
+#pragma unroll
+    for (int m = 0; m < WM; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][m][e] = 0.0f;
+
+  const int all = ta.steps * ta.planes, per = (all + ta.split - 1) / ta.split;
+  const int first = (int)blockIdx.y * per, last = first + per < all ? first + per : all;
+
+  if (!t.zeros && first < last) {
+    const uint8_t *xp[XL], *wp[WL], *sp[SL];
+    const uint8_t* codes = a.codes + t.expert * a.sp.batch_codes;
+    const uint8_t* scales = a.scales + t.expert * a.sp.batch_scales;
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+      const int q = i * THREADS + tid, row = q >> 3, c = (q & 7) ^ (row & 7);
+      xp[i] = (const uint8_t*)(ta.x + x_row(a, t.row0 + (row < t.rows ? row : t.rows - 1)) * ta.ld_x) + c * 16;
+    }
+    int wc = 0;
+#pragma unroll
+    for (int i = 0; i < WL; ++i) {
+      const int q = i * THREADS + tid, row = q / CH;
+      wc = (q % CH) ^ (CH == 4 ? row >> 1 & 3 : row >> 2 & 1);
+      wp[i] = codes + weight_row(row) * a.sp.ld_codes + wc * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int q = i * THREADS + tid;
+      sp[i] = scales + weight_row(q >> 1) * a.sp.ld_scales;
+    }
+    const int blocks = (int)((a.K + 31) >> 5);
+    u32x4 held[DIRECT ? 1 : WL];
+
+    // step st into stage b
+    auto issue = [&](int st, int b) {
+      const int k = ta.planes == 1 ? st : st % ta.steps;
+      const uint32_t xo = lds_offset(stage[b].x) + wave * 1024;
+#pragma unroll
+      for (int i = 0; i < XL; ++i) dma16(xo + i * THREADS * 16, xp[i] + (int64_t)st * 128);
+      const uint32_t so = lds_offset(stage[b].s) + wave * 256;
+#pragma unroll
+      for (int i = 0; i < SL; ++i) {
+        const int block = 2 * k + (tid & 1);
+        dma1(so + i * THREADS * 4, sp[i] + (block < blocks ? block : blocks - 1));
+      }
+      if constexpr (DIRECT) {
+        const uint32_t wo = lds_offset(stage[b].w) + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < WL; ++i) dma16(wo + i * THREADS * 16, wp[i] + (int64_t)k * WB);
+      } else {
+        const int64_t left = a.K - (int64_t)k * 64 - wc * (FAM == kPairs ? 32 : 16);      // codes from this chunk on
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+          const uint8_t* p = wp[i] + (int64_t)k * WB;
+          if (left >= (FAM == kPairs ? 32 : 16)) {
+            held[i] = *(const u32x4_any*)p;
+          } else {
+            const int valid = left < 0 ? 0 : (int)left;
+            held[i] = load_part(p, FAM == kPairs ? (valid + 1) / 2 : valid);
+            if (FAM == kPairs && (valid & 1)) clear_odd(held[i], valid);
+          }
+        }
+      }
+    };
+    auto put = [&](int b) {
+      if constexpr (!DIRECT) {
+#pragma unroll
+        for (int i = 0; i < WL; ++i) *(u32x4*)&stage[b].w[(i * THREADS + tid) * 16] = held[i];
+      }
+    };
+    constexpr int kInFlight = XL + SL + WL;                              // one stage's loads
+    static_assert(kInFlight < 16, "the count below has one digit's four bits");
+
+    issue(first, 0);
+    if constexpr (!DIRECT) put(0);
+    if (first + 1 < last) {
+      issue(first + 1, 1);
+      if constexpr (!DIRECT) put(1);
+    }
+    int b = 0;
+    for (int st = first; st < last; ++st) {
+      if (DIRECT && st + 1 < last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_barrier" ::: "memory");
+      const int two = b >= 1 ? b - 1 : 2;                                // (b + 2) % 3
+      if (st + 2 < last) issue(st + 2, two);
+      const Stage& now = stage[b];
+
+      bf16x8 wv[WN][4];
+#pragma unroll
+      for (int i = 0; i < WN; ++i) {
+        const int row = (wn * WN + i) * 32 + r;
+        uint32_t w[kWords<FAM>];
+#pragma unroll
+        for (int c = 0; c < kWords<FAM> / 4; ++c) {
+          const int chunk = h * (CH / 2) + c;
+          const u32x4 v = *(const u32x4*)&now.w[row * WB + (chunk ^ (CH == 4 ? row >> 1 & 3 : row >> 2 & 1)) * 16];
+          __builtin_memcpy(&w[4 * c], &v, 16);
+        }
+        if (FAM == kE5M2 && st >= ta.steps) {                            // an infinite weight meets no zero of a lower plane
+#pragma unroll
+          for (int c = 0; c < kWords<FAM>; ++c) w[c] = without_infinities(w[c]);
+        }
+        weights_of<FAM>(w, now.s[row * 2 + h], ta.map, wv[i]);
+      }
+#pragma unroll
+      for (int m = 0; m < WM; ++m) {
+        const int row = (wm * WM + m) * 32 + r;
+        bf16x8 xv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[j] = *(const bf16x8*)&now.x[row * 128 + ((h * 4 + j) ^ (row & 7)) * 16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < WN; ++i) acc[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i][j], xv[j], acc[i][m], 0, 0, 0);
+      }
+      if (!DIRECT && st + 2 < last) put(two);
+      b = b == 2 ? 0 : b + 1;
+    }
+  }
+
+  // acc[i][m][e]: row m * 32 + (lane & 31), weight row i * 32 + 8 (e / 4) + 4 h + e % 4
+  if (ta.split > 1) {
+    const int64_t width = gated ? 2 * a.N : a.N;
+#pragma unroll
+    for (int m = 0; m < WM; ++m) {
+      const int row = (wm * WM + m) * 32 + r;
+      if (row >= t.rows) continue;
+      float* out = ta.partial + ((int64_t)blockIdx.y * a.M + t.row0 + row) * width;
+#pragma unroll
+      for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int q = (wn * WN + i) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+          const int64_t n = gated ? n0 + (q >> 6) * 32 + (q & 31) : n0 + q;
+          if (n < a.N) out[gated && (q & 32) ? n + a.N : n] = acc[i][m][e];
+        }
+    }
+    return;
+  }
+
+  __syncthreads();                                                       // the stages become the waves' own transposes
+  float* mine = (float*)memory + wave * 32 * PITCH;
+  const int64_t nw = n0 + wn * (gated ? 32 : 64);                       // this wave's first output
+#pragma unroll
+  for (int m = 0; m < WM; ++m) {
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& v = acc[i][m];
+        *(f32x4*)&mine[r * PITCH + i * 32 + 8 * q + 4 * h] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int shift = gated ? 2 : 3;                                     // log2 of the groups of eight outputs a row
+#pragma unroll 1
+    for (int p = lane; p < 32 << shift; p += 64) {
+      const int row = p >> shift, g = p & ((1 << shift) - 1), rr = (wm * WM + m) * 32 + row;
+      if (rr >= t.rows || nw + g * 8 >= a.N) continue;
+      float z[8], up[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float* at = &mine[row * PITCH + g * 8 + 4 * i];
+        const f32x4 u = *(const f32x4*)at, v = *(const f32x4*)(at + (gated ? 32 : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[4 * i + e] = u[e], up[4 * i + e] = v[e];
+      }
+      finish_eight(a, t, t.row0 + rr, nw + g * 8, z, up);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int FAM> void launch_tile_family(const TileArgs& ta, const TilePlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(ta.tiles_m * ta.tiles_n), (unsigned)p.split);
+  auto go = [&](auto direct) {
+    constexpr bool D = decltype(direct)::value;
+    KernelTimer timer("k_linear_tile", st);
+    if (p.shape == 0) k_linear_tile<FAM, 256, 256, 4, 2, D><<<grid, 512, 0, st>>>(ta);
+    else if (p.shape == 1) k_linear_tile<FAM, 128, 128, 2, 2, D><<<grid, 256, 0, st>>>(ta);
+    else k_linear_tile<FAM, 64, 128, 1, 2, D><<<grid, 256, 0, st>>>(ta);
+  };
+  if (p.direct) go(std::true_type());
+  else go(std::false_type());
+}
+
+}  // namespace mxq

@@ -1,5 +1,5 @@
-// What the kernels of products with packed weights share: arguments, the tiles of rows by expert, codes as values, the
-// epilogue.
+// What the kernels of products with packed weights share: arguments, the tiles of rows by expert, codes as bfloat16
+// values, the epilogue.
 #pragma once
 
 #include "mxq_common.h"
@@ -89,26 +89,142 @@ __device__ __forceinline__ int64_t x_row(const LinearArgs& a, int64_t r) {
   return (slot < 0 || slot >= a.M ? 0 : slot) / a.sp.top_k;
 }
 
-__device__ __forceinline__ float code_value(const uint8_t* row, int64_t k, int format) {
-  if (format == MXQ_FMT_E4M3) return __builtin_amdgcn_cvt_f32_fp8(row[k], 0);
-  if (format == MXQ_FMT_E5M2) return __builtin_amdgcn_cvt_f32_bf8(row[k], 0);
-  const int e = format == MXQ_FMT_E3M2 ? 3 : 2, m = format == MXQ_FMT_E3M2 ? 2 : format == MXQ_FMT_E2M3 ? 3 : 1;
-  const int c = format == MXQ_FMT_E2M1_PAIRS ? row[k >> 1] >> (k & 1) * 4 : row[k];
-  const int exponent = c >> m & ((1 << e) - 1), fraction = c & ((1 << m) - 1), bias = (1 << (e - 1)) - 1;
-  const float v = exponent ? ldexpf((float)(fraction + (1 << m)), exponent - bias - m) : ldexpf((float)fraction, 1 - bias - m);
-  return c >> (e + m) & 1 ? -v : v;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));       // at any address
+
+// How a format's bytes become bfloat16.  kMapped: the formats of 4 and 6 bits a byte, put into E4M3's fields first.
+enum Family { kE4M3 = 0, kE5M2 = 1, kMapped = 2, kPairs = 3 };
+
+// 32 codes of one row with one scale: eight words, four of MXFP4's pairs.
+template <int FAM> constexpr int kWords = FAM == kPairs ? 4 : 8;
+template <int FAM> constexpr int kBlockBytes = FAM == kPairs ? 16 : 32;
+
+// E3M2 and E2M1 move up to E4M3's fields (value times 2^4 and 2^6 too small: the exponents' biases differ), E2M3 keeps
+// its place (2^6).
+struct CodeMap {
+  uint32_t mask;        // magnitude bits, in every byte
+  int shift, sign;      // how far they and the sign move up
+  int power;            // what the scale's exponent gains
+};
+inline CodeMap code_map(int format) {
+  if (format == MXQ_FMT_E3M2) return CodeMap{0x1F1F1F1Fu, 1, 2, 4};
+  if (format == MXQ_FMT_E2M3) return CodeMap{0x1F1F1F1Fu, 0, 2, 6};
+  return CodeMap{0x07070707u, 2, 4, 6};
 }
 
-__device__ __forceinline__ float scale_value(int s) { return s == 255 ? NAN : ldexpf(1.0f, s - 127); }
+// The E8M0 byte as the conversions take it: a float's exponent field, 0 standing for 2^-127 and 255 for NaN.
+__device__ __forceinline__ float scale_float(uint32_t s) { return __uint_as_float(s << 23); }
+
+// The j-th eight of the 32 codes as bfloat16, times the scale: exact (a code has at most 4 significant bits), but for
+// values below 2^-126, rounded to bfloat16's subnormals.  One instruction makes two values.
+template <int FAM> __device__ __forceinline__ bf16x8 eight(const uint32_t (&w)[kWords<FAM>], float scale, int j) {
+  bf16x2 v[4];
+  if constexpr (FAM == kPairs) {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 0);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 1);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 2);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 3);
+  } else if constexpr (FAM == kE5M2) {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j], scale, false);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j], scale, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j + 1], scale, false);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j + 1], scale, true);
+  } else {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j], scale, false);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j], scale, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j + 1], scale, false);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j + 1], scale, true);
+  }
+  bf16x8 r;
+  __builtin_memcpy(&r, v, 16);
+  return r;
+}
+
+// The arguments of k_linear_tile.
+struct TileArgs {
+  LinearArgs l;
+  const uint16_t* x;      // bfloat16, rows of ld_x, every one a whole number of 64s in each plane, 16-byte aligned
+  int64_t ld_x;
+  int32_t steps, planes;  // 64 columns a step, steps a plane
+  int32_t tiles_m, tiles_n, split;
+  float* partial;         // split > 1: split x M x rows of the weight
+  CodeMap map;
+};
+
+struct TilePlan {
+  int shape;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128
+  int split;
+  bool direct;
+};
+
+// The 32 codes and the scale byte as the four operands of the matrix instructions.  kMapped: a scale past 2^127 after the
+// map's power is applied in two steps, in a branch that no trained weight takes.
+template <int FAM> __device__ __forceinline__ void weights_of(const uint32_t (&codes)[kWords<FAM>], uint32_t s, const CodeMap& map,
+                                                              bf16x8 (&out)[4]) {
+  uint32_t w[kWords<FAM>];
+  uint32_t left = 0;
+#pragma unroll
+  for (int i = 0; i < kWords<FAM>; ++i) w[i] = codes[i];
+  if constexpr (FAM == kMapped) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (w[i] & map.mask) << map.shift | (w[i] << map.sign & 0x80808080u);
+    if (s != 255) {
+      s += map.power;
+      if (s > 254) left = s - 254, s = 254;
+    }
+  }
+  const float scale = scale_float(s);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = eight<FAM>(w, scale, j);
+  if constexpr (FAM == kMapped) {
+    if (__builtin_expect(__any(left), 0)) {
+      const float more = __uint_as_float((127 + left) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[j][i] = (__bf16)((float)out[j][i] * more);
+    }
+  }
+}
+
+// E5M2's codes with zeros for its infinities.
+__device__ __forceinline__ uint32_t without_infinities(uint32_t w) {
+  const uint32_t z = ~(((w & 0x7F7F7F7Fu) ^ 0x7C7C7C7Cu) + 0x7F7F7F7Fu) & 0x80808080u;     // 0x80 in the bytes that hold one
+  return w & ~((z << 1) - (z >> 7));
+}
+
+// 16 bytes of which the first `valid` exist; zeros for the others.
+__device__ __forceinline__ u32x4 load_part(const uint8_t* p, int valid) {
+  u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < valid) v[i >> 2] |= (uint32_t)p[i] << (i & 3) * 8;
+  return v;
+}
+
+// sigmoid by the hardware's exp2 and reciprocal, each within one unit in the last place.
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+
+// Of an odd number of MXFP4 codes the last byte's high half is no code.
+__device__ __forceinline__ void clear_odd(u32x4& v, int valid) {
+  const uint32_t keep = ~(0xF0u << (valid >> 1 & 3) * 8);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (c == valid >> 3) v[c] &= keep;
+}
 
 __device__ __forceinline__ float activate(float z, int activation) {
   switch (activation) {
-    case MXQ_ACT_SILU: return z / (1.0f + expf(-z));
+    case MXQ_ACT_SILU: return z * sigmoid(z);
     case MXQ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case MXQ_ACT_GELU_TANH: {
-      const float t = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-      return 0.5f * z * (1.0f + tanhf(t));
-    }
+    case MXQ_ACT_GELU_TANH: return z * sigmoid(1.59576912160573071f * (z + 0.044715f * z * z * z));
     case MXQ_ACT_RELU: return z < 0.0f ? 0.0f : z;
     default: return z;
   }
@@ -126,6 +242,84 @@ __device__ __forceinline__ float epilogue(const LinearArgs& a, const RowTile& t,
   if (a.sp.gated) z *= up;
   if (a.residual) z += load_elem(a.residual, a.sp.residual_dtype, row * a.sp.ld_residual + n);
   return z;
+}
+
+// v[i] += p[at + i], eight neighbours.
+__device__ __forceinline__ void add_eight(float (&v)[8], const void* p, int dtype, int64_t at) {
+  if (dtype == MXQ_DT_F32) {
+    const u32x4 x = *(const u32x4_any*)((const float*)p + at), y = *(const u32x4_any*)((const float*)p + at + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(x[i]), v[i + 4] += __uint_as_float(y[i]);
+    return;
+  }
+  const u32x4 x = *(const u32x4_any*)((const uint16_t*)p + at);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t b = (uint16_t)(x[i >> 1] >> (i & 1) * 16);
+    v[i] += load_elem(&b, dtype, 0);
+  }
+}
+
+__device__ __forceinline__ void activate_eight(float (&v)[8], int activation) {
+  switch (activation) {
+#define MXQ_EACH(ACT)                                        \
+  case ACT:                                                  \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] = activate(v[i], ACT); \
+    break;
+    MXQ_EACH(MXQ_ACT_SILU)
+    MXQ_EACH(MXQ_ACT_GELU)
+    MXQ_EACH(MXQ_ACT_GELU_TANH)
+    MXQ_EACH(MXQ_ACT_RELU)
+#undef MXQ_EACH
+  }
+}
+
+// epilogue and store of eight neighbouring outputs of a row.
+__device__ __forceinline__ void finish_eight(const LinearArgs& a, const RowTile& t, int64_t row, int64_t n, float (&z)[8], float (&up)[8]) {
+  if (n + 8 > a.N) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < a.N) store_elem(a.y, a.sp.y_dtype, row * a.sp.ld_y + n + i, epilogue(a, t, row, n + i, z[i], up[i]));
+    return;
+  }
+  if (t.zeros) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = 0.0f;
+  } else {
+    const int64_t first = t.expert * a.sp.batch_bias + n;
+    if (a.bias) add_eight(z, a.bias, a.sp.bias_dtype, first);
+    activate_eight(z, a.sp.activation);
+    if (a.sp.gated) {
+      if (a.bias) add_eight(up, a.bias, a.sp.bias_dtype, first + a.N);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] *= up[i];
+    }
+    if (a.residual) add_eight(z, a.residual, a.sp.residual_dtype, row * a.sp.ld_residual + n);
+  }
+  const int64_t at = row * a.sp.ld_y + n;
+  if (a.sp.y_dtype == MXQ_DT_F32) {
+    u32x4 p, q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __float_as_uint(z[i]), q[i] = __float_as_uint(z[i + 4]);
+    *(u32x4_any*)((float*)a.y + at) = p;
+    *(u32x4_any*)((float*)a.y + at + 4) = q;
+    return;
+  }
+  u32x4 p;
+  if (a.sp.y_dtype == MXQ_DT_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x2 b = {(__bf16)z[2 * i], (__bf16)z[2 * i + 1]};
+      __builtin_memcpy((char*)&p + 4 * i, &b, 4);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f16x2 b = {(_Float16)z[2 * i], (_Float16)z[2 * i + 1]};
+      __builtin_memcpy((char*)&p + 4 * i, &b, 4);
+    }
+  }
+  *(u32x4_any*)((uint16_t*)a.y + at) = p;
 }
 
 }  // namespace mxq

@@ -79,6 +79,38 @@ def test_outputs(cuda, M, N):
     _run(rng, M, N, 128, "MXFP6_E3M2", torch.float16)
 
 
+@pytest.mark.parametrize("M, N, K", [(2049, 6180, 96), (4096, 4096, 64), (1100, 2050, 128), (130, 70, 4128), (200, 700, 1090)])
+def test_many_outputs_and_long_contractions(cuda, M, N, K):
+    """The large tiles, whole and cut off, and contractions shared among workgroups."""
+    rng = np.random.default_rng(M)
+    _run(rng, M, N, K, "MXFP8_E4M3", bias=True, activation="gelu", residual=True)
+    _run(rng, M, N, K, "MXFP8_E5M2", torch.float16, bias=True, residual=True)
+    _run(rng, M, N // 2, K, "MXFP4", bias=True, activation="silu", gated=True, residual=True, pairs=True)
+    _run(rng, M, N // 2, K + 3, "MXFP6_E2M3", torch.float32, bias=True, gated=True)
+
+
+def test_experts_of_many_rows(cuda):
+    rng = np.random.default_rng(21)
+    _experts(rng, 1500, 2, 4, 1030, 128, "MXFP8_E4M3", bias=True, activation="silu", gated=True)
+    _experts(rng, 1500, 2, 4, 2100, 70, "MXFP4", torch.float16, pairs=True, sorted_rows=True)
+    _experts(rng, 900, 4, 30, 516, 192, "MXFP8_E5M2", sorted_rows=True)
+
+
+def test_largest_scales_of_narrow_codes(cuda):
+    """Scale bytes up to 254 of formats that are put into wider fields first."""
+    for fmt, K in (("MXFP6_E3M2", 64), ("MXFP6_E2M3", 64), ("MXFP4", 64)):
+        codes = torch.full((6, K), {"MXFP6_E3M2": 1, "MXFP6_E2M3": 1, "MXFP4": 1}[fmt], dtype=torch.uint8)
+        scales = torch.tensor([[0, 1], [127, 247], [248, 249], [250, 251], [252, 253], [254, 255]], dtype=torch.uint8)
+        for M in (3, 100):
+            x = torch.zeros(M, K)
+            x[:, 0], x[:, 40] = 2.0 ** -3, 2.0 ** -4
+            y = nn.packed_linear(x.cuda(), codes.cuda(), scales.cuda(), fmt).double().cpu()
+            want = x.double() @ _matrix(codes, scales, fmt, K).cpu().t()
+            assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.isnan(y[:, 5]).all()
+            assert torch.equal(y[:, 1:5], want[:, 1:5]), fmt
+            assert ((y[:, 0] - want[:, 0]).abs() <= 2.0 ** -133).all()          # a weight below 2^-126: bfloat16's subnormals
+
+
 @pytest.mark.parametrize("activation", [None, "silu", "gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("M", [3, 40, 290])
