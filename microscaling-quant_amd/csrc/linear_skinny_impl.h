@@ -161,12 +161,20 @@ __global__ __launch_bounds__(64 * kSkinnyWaves, 2) void k_linear_skinny(LinearAr
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           bf16x8 wv[4], wl[4];
-          weights_of<FAM>(w[u][i], s[u][i], map, wv);
+          uint32_t left;
+          const float scale = scale_of<FAM>(s[u][i], map, left);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wv[j] = eight<FAM>(w[u][i], scale, j, map);
+          if (FAM == kMapped && __builtin_expect(__any(left), 0)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) apply_left(wv[j], left);
+          }
           if constexpr (P > 1 && FAM == kE5M2) {                       // an infinite weight meets no zero of a lower plane
             uint32_t f[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) f[c] = without_infinities(w[u][i][c]);
-            weights_of<FAM>(f, s[u][i], map, wl);
+            for (int c = 0; c < 8; ++c) f[c] = without_infinities(w[u][i][c], ~0u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wl[j] = eight<FAM>(f, scale, j, map);
           }
 #pragma unroll
           for (int m = 0; m < MT; ++m)

@@ -5,7 +5,8 @@
 // deep: while one is multiplied the next has landed and the third is on its way.  The codes stay codes in LDS, half the
 // bytes, and become bfloat16 when a wave takes its operands: one conversion for two values with their scale, beside the
 // matrix instructions.  Lane (r, h) takes block h of row r's 64 columns, so a lane's 32 codes share one scale.
-// Chunks of 16 bytes are permuted within a row by its number, so that eight rows' chunks lie in different banks.
+// Chunks of 16 bytes are permuted within a row by its number, so that the sixteen rows an LDS cycle pair reads lie in
+// different ones of the 64 banks.
 // float16 and float32 activations have been split into bfloat16 planes one after another along a longer row: the walk
 // goes through the weight once a plane.
 #pragma once
@@ -17,7 +18,7 @@ namespace mxq {
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
-// Global memory straight into LDS, 16 bytes (or one byte, as a word) a lane, lane i's at base + 16 i (4 i).  Written as
+// Global memory straight into LDS, 16 or 4 bytes (or one byte, as a word) a lane, lane i's at base + 16 i or 4 i.  Written as
 // assembly because the compiler would wait for all such loads before every LDS read; the waits are wait_stage's.
 __device__ __forceinline__ void dma16(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
@@ -26,24 +27,31 @@ __device__ __forceinline__ void dma1(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(base), "v"(p) : "memory");
 }
 
-// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; DIRECT: codes by DMA (K a multiple of 64, rows 16-byte
-// aligned), through registers otherwise.
+__device__ __forceinline__ void dma4(uint32_t base, const void* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
+}
+
+// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; DIRECT: codes by DMA (K a multiple of 128, rows of codes
+// 16-byte and of scales 4-byte aligned), through registers otherwise.
 template <int FAM, int BM, int BN, int WM, int WN, bool DIRECT>
 __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k_linear_tile(TileArgs ta) {
   constexpr int WAVES_N = BN / (32 * WN), WAVES = BM / (32 * WM) * WAVES_N, THREADS = 64 * WAVES;
   constexpr int WB = 2 * kBlockBytes<FAM>, CH = WB / 16;                 // a weight row's bytes and chunks of one stage
   constexpr int XL = BM * 8 / THREADS, WL = BN * CH / THREADS, SL = BN * 2 / THREADS;   // loads a thread and stage
+  constexpr int SC = BN * 4 / THREADS;                                   // DIRECT: loads of scales a thread and eight steps
   static_assert(WN == 2, "a wave's two tiles are neighbours, or G's and U's of the same outputs");
   static_assert(XL >= 1 && WL >= 1 && SL >= 1 && BM * 8 % THREADS == 0, "whole loads");
   struct Stage {
     uint8_t x[BM * 128];
     uint8_t w[BN * WB];
-    uint32_t s[BN * 2];
   };
+  // DIRECT: rings of two times eight steps' scale bytes; otherwise of three steps', a word each
+  constexpr int kScales = DIRECT ? 2 * BN * 16 : 3 * BN * 8;
   constexpr int PITCH = 32 * WN + 4;
-  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = 3 * sizeof(Stage);
+  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = 3 * sizeof(Stage) + kScales;
   __shared__ __attribute__((aligned(16))) uint8_t memory[kStages > kEpilogue ? kStages : kEpilogue];
   Stage* stage = (Stage*)memory;
+  uint8_t* scale_ring = memory + 3 * sizeof(Stage);
 
   const LinearArgs& a = ta.l;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -81,50 +89,62 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][m][e] = 0.0f;
 
-  const int all = ta.steps * ta.planes, per = (all + ta.split - 1) / ta.split;
+  const int all = ta.steps * ta.planes, per = ((all + ta.split - 1) / ta.split + 1) & ~1;         // even: a word of scales is two steps'
   const int first = (int)blockIdx.y * per, last = first + per < all ? first + per : all;
 
   if (!t.zeros && first < last) {
-    const uint8_t *xp[XL], *wp[WL], *sp[SL];
+    const uint8_t *xp[XL], *wp[WL], *sp[DIRECT ? SC : SL];
     const uint8_t* codes = a.codes + t.expert * a.sp.batch_codes;
     const uint8_t* scales = a.scales + t.expert * a.sp.batch_scales;
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-      const int q = i * THREADS + tid, row = q >> 3, c = (q & 7) ^ (row & 7);
+      const int q = i * THREADS + tid, row = q >> 3, c = (q & 7) ^ (row >> 1 & 7);
       xp[i] = (const uint8_t*)(ta.x + x_row(a, t.row0 + (row < t.rows ? row : t.rows - 1)) * ta.ld_x) + c * 16;
     }
     int wc = 0;
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
       const int q = i * THREADS + tid, row = q / CH;
-      wc = (q % CH) ^ (CH == 4 ? row >> 1 & 3 : row >> 2 & 1);
+      wc = (q % CH) ^ (CH == 4 ? row >> 2 & 3 : row >> 3 & 1);
       wp[i] = codes + weight_row(row) * a.sp.ld_codes + wc * 16;
     }
 #pragma unroll
-    for (int i = 0; i < SL; ++i) {
+    for (int i = 0; i < (DIRECT ? SC : SL); ++i) {
       const int q = i * THREADS + tid;
-      sp[i] = scales + weight_row(q >> 1) * a.sp.ld_scales;
+      sp[i] = scales + weight_row(DIRECT ? q >> 2 : q >> 1) * a.sp.ld_scales;
     }
     const int blocks = (int)((a.K + 31) >> 5);
     u32x4 held[DIRECT ? 1 : WL];
 
-    // step st into stage b
-    auto issue = [&](int st, int b) {
-      const int k = ta.planes == 1 ? st : st % ta.steps;
-      const uint32_t xo = lds_offset(stage[b].x) + wave * 1024;
+    // A third of the next step's loads into stage b, in the order codes and scales, x, x: loads of a step issued at once
+    // would keep the wave from its multiplications while the memory pipeline takes them.  The last step again after it, so
+    // that every step waits for as many loads.
+    int st = first, k = first % ta.steps;
+    auto issue = [&](int b, int part) {
+      if (part == 1 || part == 2) {
+        const uint32_t xo = lds_offset(stage[b].x) + wave * 1024;
 #pragma unroll
-      for (int i = 0; i < XL; ++i) dma16(xo + i * THREADS * 16, xp[i] + (int64_t)st * 128);
-      const uint32_t so = lds_offset(stage[b].s) + wave * 256;
-#pragma unroll
-      for (int i = 0; i < SL; ++i) {
-        const int block = 2 * k + (tid & 1);
-        dma1(so + i * THREADS * 4, sp[i] + (block < blocks ? block : blocks - 1));
+        for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) dma16(xo + i * THREADS * 16, xp[i] + (int64_t)st * 128);
+        return;
       }
       if constexpr (DIRECT) {
+        const int chunk = st - first;
+        if ((chunk & 7) == 0) {
+          const uint32_t so = lds_offset(scale_ring) + (chunk >> 3 & 1) * BN * 16 + wave * 256;
+          const int two = (k + 2 * (tid & 3)) % ta.steps;
+#pragma unroll
+          for (int i = 0; i < SC; ++i) dma4(so + i * THREADS * 4, sp[i] + two * 2);
+        }
         const uint32_t wo = lds_offset(stage[b].w) + wave * 1024;
 #pragma unroll
         for (int i = 0; i < WL; ++i) dma16(wo + i * THREADS * 16, wp[i] + (int64_t)k * WB);
       } else {
+        const uint32_t so = lds_offset(scale_ring) + b * BN * 8 + wave * 256;
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+          const int block = 2 * k + (tid & 1);
+          dma1(so + i * THREADS * 4, sp[i] + (block < blocks ? block : blocks - 1));
+        }
         const int64_t left = a.K - (int64_t)k * 64 - wc * (FAM == kPairs ? 32 : 16);      // codes from this chunk on
 #pragma unroll
         for (int i = 0; i < WL; ++i) {
@@ -139,61 +159,108 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
         }
       }
     };
+    auto advance = [&]() {
+      if (st + 1 < last) ++st, k = k + 1 == ta.steps ? 0 : k + 1;
+    };
     auto put = [&](int b) {
       if constexpr (!DIRECT) {
 #pragma unroll
         for (int i = 0; i < WL; ++i) *(u32x4*)&stage[b].w[(i * THREADS + tid) * 16] = held[i];
       }
     };
-    constexpr int kInFlight = XL + SL + WL;                              // one stage's loads
-    static_assert(kInFlight < 16, "the count below has one digit's four bits");
-
-    issue(first, 0);
-    if constexpr (!DIRECT) put(0);
-    if (first + 1 < last) {
-      issue(first + 1, 1);
-      if constexpr (!DIRECT) put(1);
-    }
-    int b = 0;
-    for (int st = first; st < last; ++st) {
-      if (DIRECT && st + 1 < last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      asm volatile("s_barrier" ::: "memory");
-      const int two = b >= 1 ? b - 1 : 2;                                // (b + 2) % 3
-      if (st + 2 < last) issue(st + 2, two);
-      const Stage& now = stage[b];
-
-      bf16x8 wv[WN][4];
+    // one stage's loads, without the scales that come before them every eighth time: the waits below then ask for a little
+    // more than they need
+    constexpr int kInFlight = XL + WL;
+    // A step is four phases of eight columns a lane.  A phase reads and converts the next one's operands while its own are
+    // multiplied; the last phase of a step first waits for the next stage, whose loads began two steps ago, and hands its
+    // own buffer to the stage after the one in flight.
+    uint32_t code[WN][kWords<FAM>];
+    float scale[WN];
+    uint32_t left[WN];
+    bf16x8 wv[2][WN], xv[2][WM];
+    auto read_w = [&](int b, int st) {
+      const Stage& s = stage[b];
 #pragma unroll
       for (int i = 0; i < WN; ++i) {
         const int row = (wn * WN + i) * 32 + r;
-        uint32_t w[kWords<FAM>];
 #pragma unroll
         for (int c = 0; c < kWords<FAM> / 4; ++c) {
           const int chunk = h * (CH / 2) + c;
-          const u32x4 v = *(const u32x4*)&now.w[row * WB + (chunk ^ (CH == 4 ? row >> 1 & 3 : row >> 2 & 1)) * 16];
-          __builtin_memcpy(&w[4 * c], &v, 16);
+          const u32x4 v = *(const u32x4*)&s.w[row * WB + (chunk ^ (CH == 4 ? row >> 2 & 3 : row >> 3 & 1)) * 16];
+          __builtin_memcpy(&code[i][4 * c], &v, 16);
         }
-        if (FAM == kE5M2 && st >= ta.steps) {                            // an infinite weight meets no zero of a lower plane
+        if constexpr (FAM == kE5M2Wide) {
+          const uint32_t drop = st >= ta.steps ? ~0u : 0u;
 #pragma unroll
-          for (int c = 0; c < kWords<FAM>; ++c) w[c] = without_infinities(w[c]);
+          for (int c = 0; c < kWords<FAM>; ++c) code[i][c] = without_infinities(code[i][c], drop);
         }
-        weights_of<FAM>(w, now.s[row * 2 + h], ta.map, wv[i]);
+        const int since = st - first;
+        const uint8_t* at = DIRECT ? scale_ring + (since >> 3 & 1) * BN * 16 + row * 16 + (since & 7) * 2 + h
+                                   : scale_ring + b * BN * 8 + (row * 2 + h) * 4;
+        scale[i] = scale_of<FAM>(*at, ta.map, left[i]);
       }
+    };
+    auto read_x = [&](const Stage& s, int j) {
 #pragma unroll
       for (int m = 0; m < WM; ++m) {
         const int row = (wm * WM + m) * 32 + r;
-        bf16x8 xv[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) xv[j] = *(const bf16x8*)&now.x[row * 128 + ((h * 4 + j) ^ (row & 7)) * 16];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < WN; ++i) acc[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i][j], xv[j], acc[i][m], 0, 0, 0);
+        xv[j & 1][m] = *(const bf16x8*)&s.x[row * 128 + ((h * 4 + j) ^ (row >> 1 & 7)) * 16];
       }
-      if (!DIRECT && st + 2 < last) put(two);
-      b = b == 2 ? 0 : b + 1;
+    };
+    auto convert = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i) wv[j & 1][i] = eight<FAM>(code[i], scale[i], j, ta.map);
+      if (FAM == kMapped && __builtin_expect(__any(left[0] | left[1]), 0)) {
+#pragma unroll
+        for (int i = 0; i < WN; ++i) apply_left(wv[j & 1][i], left[i]);
+      }
+    };
+    auto multiply = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i)
+#pragma unroll
+        for (int m = 0; m < WM; ++m) acc[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[j & 1][i], xv[j & 1][m], acc[i][m], 0, 0, 0);
+    };
+
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        if (s < 2 || p == 0) issue(s, p);
+      if (s < 2) put(s), advance();
     }
+    if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + WL) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    read_w(0, first);
+    read_x(stage[0], 0);
+    convert(0);
+    int b = 0;
+    for (int now = first; now < last; ++now) {
+      const int nb = b == 2 ? 0 : b + 1;
+      const int pb = nb == 2 ? 0 : nb + 1;                               // the stage whose loads are being issued
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        read_x(stage[b], j + 1);
+        __builtin_amdgcn_sched_barrier(0);                               // the compiler would sink the reads to their uses
+        if (j < 2) issue(pb, j + 1);
+        multiply(j);
+        convert(j + 1);
+      }
+      put(pb);
+      if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_barrier" ::: "memory");
+      advance();
+      read_w(nb, now + 1);                                        // after the last step: a stage that no sum takes
+      read_x(stage[nb], 0);
+      __builtin_amdgcn_sched_barrier(0);
+      issue(b, 0);
+      multiply(3);
+      convert(0);
+      b = nb;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
 
   // acc[i][m][e]: row m * 32 + (lane & 31), weight row i * 32 + 8 (e / 4) + 4 h + e % 4

@@ -153,7 +153,8 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
     t.ld_x = kp * p.planes;
   }
   TilePlan tp = p.tile;
-  tp.direct = a.K % 64 == 0 && (uintptr_t)a.codes % 16 == 0 && a.sp.ld_codes % 16 == 0 && a.sp.batch_codes % 16 == 0;
+  tp.direct = a.K % 128 == 0 && (uintptr_t)a.codes % 16 == 0 && a.sp.ld_codes % 16 == 0 && a.sp.batch_codes % 16 == 0 &&
+              (uintptr_t)a.scales % 4 == 0 && a.sp.ld_scales % 4 == 0 && a.sp.batch_scales % 4 == 0;
   (fam == kE4M3 ? launch_tile_e4m3 : fam == kE5M2 ? launch_tile_e5m2 : fam == kPairs ? launch_tile_pairs : launch_tile_mapped)(t, tp, st);
   if (tp.split > 1) {
     KernelTimer timer("k_linear_finish", st);

@@ -98,18 +98,19 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));       // at any address
 
 // How a format's bytes become bfloat16.  kMapped: the formats of 4 and 6 bits a byte, put into E4M3's fields first.
-enum Family { kE4M3 = 0, kE5M2 = 1, kMapped = 2, kPairs = 3 };
+// kE5M2Wide: E5M2 under activations of several planes, whose lower ones see zeros in the place of infinities.
+enum Family { kE4M3 = 0, kE5M2 = 1, kMapped = 2, kPairs = 3, kE5M2Wide = 4 };
 
 // 32 codes of one row with one scale: eight words, four of MXFP4's pairs.
 template <int FAM> constexpr int kWords = FAM == kPairs ? 4 : 8;
 template <int FAM> constexpr int kBlockBytes = FAM == kPairs ? 16 : 32;
 
-// E3M2 and E2M1 move up to E4M3's fields (value times 2^4 and 2^6 too small: the exponents' biases differ), E2M3 keeps
-// its place (2^6).
+// E3M2 and E2M1 move up to E4M3's fields, E2M3 keeps its place.  The exponents' biases differ, so that the fields alone
+// are 2^4 or 2^6 too small; the scale makes up for it.
 struct CodeMap {
   uint32_t mask;        // magnitude bits, in every byte
   int shift, sign;      // how far they and the sign move up
-  int power;            // what the scale's exponent gains
+  uint32_t power;       // what the scale's exponent gains
 };
 inline CodeMap code_map(int format) {
   if (format == MXQ_FMT_E3M2) return CodeMap{0x1F1F1F1Fu, 1, 2, 4};
@@ -117,28 +118,45 @@ inline CodeMap code_map(int format) {
   return CodeMap{0x07070707u, 2, 4, 6};
 }
 
-// The E8M0 byte as the conversions take it: a float's exponent field, 0 standing for 2^-127 and 255 for NaN.
-__device__ __forceinline__ float scale_float(uint32_t s) { return __uint_as_float(s << 23); }
+// The E8M0 byte as the conversions take it: a float's exponent field, 0 standing for 2^-127 and 255 for NaN.  kMapped: a
+// scale past 2^127 with the map's power leaves the excess in `left` for apply_left.
+template <int FAM> __device__ __forceinline__ float scale_of(uint32_t s, const CodeMap& map, uint32_t& left) {
+  left = 0;
+  if constexpr (FAM == kMapped) {
+    const uint32_t t = s + map.power;
+    left = s != 255 && t > 254 ? t - 254 : 0;
+    s = s == 255 ? 255 : t < 254 ? t : 254;
+  }
+  return __uint_as_float(s << 23);
+}
+__device__ __forceinline__ void apply_left(bf16x8& w, uint32_t left) {
+  const float more = __uint_as_float((127 + left) << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = (__bf16)((float)w[i] * more);
+}
 
 // The j-th eight of the 32 codes as bfloat16, times the scale: exact (a code has at most 4 significant bits), but for
 // values below 2^-126, rounded to bfloat16's subnormals.  One instruction makes two values.
-template <int FAM> __device__ __forceinline__ bf16x8 eight(const uint32_t (&w)[kWords<FAM>], float scale, int j) {
+template <int FAM> __device__ __forceinline__ bf16x8 eight(const uint32_t (&w)[kWords<FAM>], float scale, int j, const CodeMap& map) {
   bf16x2 v[4];
   if constexpr (FAM == kPairs) {
     v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 0);
     v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 1);
     v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 2);
     v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 3);
-  } else if constexpr (FAM == kE5M2) {
-    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j], scale, false);
-    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j], scale, true);
-    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j + 1], scale, false);
-    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[2 * j + 1], scale, true);
   } else {
-    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j], scale, false);
-    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j], scale, true);
-    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j + 1], scale, false);
-    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[2 * j + 1], scale, true);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t c = w[2 * j + i];
+      if constexpr (FAM == kE5M2 || FAM == kE5M2Wide) {
+        v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(c, scale, false);
+        v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(c, scale, true);
+      } else {
+        if constexpr (FAM == kMapped) c = (c & map.mask) << map.shift | (c << map.sign & 0x80808080u);
+        v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false);
+        v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true);
+      }
+    }
   }
   bf16x8 r;
   __builtin_memcpy(&r, v, 16);
@@ -162,40 +180,10 @@ struct TilePlan {
   bool direct;
 };
 
-// The 32 codes and the scale byte as the four operands of the matrix instructions.  kMapped: a scale past 2^127 after the
-// map's power is applied in two steps, in a branch that no trained weight takes.
-template <int FAM> __device__ __forceinline__ void weights_of(const uint32_t (&codes)[kWords<FAM>], uint32_t s, const CodeMap& map,
-                                                              bf16x8 (&out)[4]) {
-  uint32_t w[kWords<FAM>];
-  uint32_t left = 0;
-#pragma unroll
-  for (int i = 0; i < kWords<FAM>; ++i) w[i] = codes[i];
-  if constexpr (FAM == kMapped) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = (w[i] & map.mask) << map.shift | (w[i] << map.sign & 0x80808080u);
-    if (s != 255) {
-      s += map.power;
-      if (s > 254) left = s - 254, s = 254;
-    }
-  }
-  const float scale = scale_float(s);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) out[j] = eight<FAM>(w, scale, j);
-  if constexpr (FAM == kMapped) {
-    if (__builtin_expect(__any(left), 0)) {
-      const float more = __uint_as_float((127 + left) << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[j][i] = (__bf16)((float)out[j][i] * more);
-    }
-  }
-}
-
-// E5M2's codes with zeros for its infinities.
-__device__ __forceinline__ uint32_t without_infinities(uint32_t w) {
+// E5M2's codes, the infinities' bits under `drop` cleared.
+__device__ __forceinline__ uint32_t without_infinities(uint32_t w, uint32_t drop) {
   const uint32_t z = ~(((w & 0x7F7F7F7Fu) ^ 0x7C7C7C7Cu) + 0x7F7F7F7Fu) & 0x80808080u;     // 0x80 in the bytes that hold one
-  return w & ~((z << 1) - (z >> 7));
+  return w & ~(((z << 1) - (z >> 7)) & drop);
 }
 
 // 16 bytes of which the first `valid` exist; zeros for the others.
@@ -220,10 +208,23 @@ __device__ __forceinline__ void clear_odd(u32x4& v, int valid) {
     if (c == valid >> 3) v[c] &= keep;
 }
 
+// The normal distribution's share below z: with t = 1 / (1 + 0.39 |z| / sqrt 2), half of erfc(|z| / sqrt 2) is
+// t p(t) exp(-z^2 / 2), p fitted here to 8e-9 of erfc; z times it is off by at most 2.2e-7 |z|.
+__device__ __forceinline__ float normal_below(float z) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.27577164f, __builtin_fabsf(z), 1.0f));
+  float p = __builtin_fmaf(-0.113768743f, t, 0.443332924f);
+  p = __builtin_fmaf(p, t, -0.317701341f);
+  p = __builtin_fmaf(p, t, 0.32478067f);
+  p = __builtin_fmaf(p, t, 0.0456938178f);
+  p = __builtin_fmaf(p, t, 0.117662672f);
+  const float q = t * p * __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  return z < 0.0f ? q : 1.0f - q;
+}
+
 __device__ __forceinline__ float activate(float z, int activation) {
   switch (activation) {
     case MXQ_ACT_SILU: return z * sigmoid(z);
-    case MXQ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case MXQ_ACT_GELU: return z * normal_below(z);
     case MXQ_ACT_GELU_TANH: return z * sigmoid(1.59576912160573071f * (z + 0.044715f * z * z * z));
     case MXQ_ACT_RELU: return z < 0.0f ? 0.0f : z;
     default: return z;
