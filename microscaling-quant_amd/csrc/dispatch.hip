@@ -6,65 +6,84 @@ namespace mxq {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopK = 64;
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kAhead = 4;
 
-// A stable counting sort by one workgroup: counts, their prefix, then 1024 slots at a time each to its expert's next
-// places.  A slot's rank among its wave's equal ones is a population count of the lanes with the same key; the waves
-// before it add theirs from LDS.  Integer sums throughout: the same order whatever the timing.
-__global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* experts, int n, int E, int bits,
+// A stable counting sort by one workgroup.  Each wave owns a run of whole 64s of the slots and counts its experts into its
+// own row of LDS; the rows' and the experts' prefix sums turn the counts into the places where the wave's slots go; then it
+// goes through its run again, 64 slots at a time, on its own: a slot's rank among the wave's equal ones is a population
+// count of the lanes with the same key, which ballots over the key's bits find.  Three barriers whatever n is, and integer
+// sums throughout: the same order whatever the timing.
+__global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* experts, int n, int E, int bits, int run,
                                                            int32_t* order, int32_t* offsets, int32_t* positions) {
-  __shared__ int base[kMaxExperts + 1];
+  __shared__ int place[kSortWaves][kMaxExperts + 1];
   __shared__ int scan[kSortWaves];
-  __shared__ uint16_t cnt[kSortWaves][kMaxExperts + 1];      // a wave's counts, at most 64 each
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto key_of = [&](int i) {
-    const int e = experts[i];
-    return (unsigned)e < (unsigned)E ? e : E;                     // E: the slots of no expert, sorted last
-  };
-  for (int e = tid; e <= E; e += kSortThreads) base[e] = 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, used = n ? (n - 1) / run + 1 : 0;
+  const int first = wave * run, last = first + run < n ? first + run : n;
+  volatile int* mine = place[wave];
+  auto key_of = [&](int e) { return (unsigned)e < (unsigned)E ? e : E; };        // E: the slots of no expert, sorted last
+  if (wave < used) {
+    for (int e = lane; e <= E; e += 64) mine[e] = 0;
+    for (int i = first + lane; i < last; i += 64 * kAhead) {
+      int e[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) e[u] = i + u * 64 < last ? experts[i + u * 64] : 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u * 64 < last) atomicAdd(&place[wave][key_of(e[u])], 1);
+    }
+  }
   __syncthreads();
-  for (int i = tid; i < n; i += kSortThreads) atomicAdd(&base[key_of(i)], 1);
-  __syncthreads();
-  // exclusive prefix over the E + 1 <= 1025 counts: one a thread, the last by itself
-  int c = tid < E ? base[tid] : 0, p = c;
+  // one expert a thread: its count, the prefix over the experts, then the rows' places; slots of none follow all others
+  int c = 0;
+  if (tid < E)
+    for (int w = 0; w < used; ++w) c += place[w][tid];
+  int p = c;
   for (int o = 1; o < 64; o <<= 1) {
     const int q = __shfl_up(p, o);
     if (lane >= o) p += q;
   }
   if (lane == 63) scan[wave] = p;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < wave; ++w) before += scan[w];
-  p += before;
-  __syncthreads();
-  if (tid < E) base[tid] = p - c, offsets[tid] = p - c;
-  if (tid == kSortThreads - 1) base[E] = p, offsets[E] = p;
-  __syncthreads();
-  for (int first = 0; first < n; first += kSortThreads) {
-    for (int w = 0; w < kSortWaves; ++w)
-      for (int e = tid; e <= E; e += kSortThreads) cnt[w][e] = 0;
-    __syncthreads();
-    const int i = first + tid;
-    const int key = i < n ? key_of(i) : -1;
-    uint64_t same = __ballot(i < n);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot(key >> b & 1);
-      same &= key >> b & 1 ? set : ~set;
+  int before = 0, all = 0;
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (w == wave) before = all;
+    all += scan[w];
+  }
+  p += before - c;
+  if (tid < E) offsets[tid] = p;
+  if (tid == 0) offsets[E] = all;
+  for (int w = 0, at = p; w < used && tid < E; ++w) {
+    const int q = place[w][tid];
+    place[w][tid] = at;
+    at += q;
+  }
+  if (tid == kSortThreads - 1)                                    // after its expert, should it have one
+    for (int w = 0, at = all; w < used; ++w) {
+      const int q = place[w][E];
+      place[w][E] = at;
+      at += q;
     }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    if (i < n && rank == 0) cnt[wave][key] = (uint16_t)__popcll(same);
-    __syncthreads();
-    int place = 0;
-    if (i < n) {
-      place = base[key] + rank;
-      for (int w = 0; w < wave; ++w) place += cnt[w][key];
-      order[place] = i;
-      positions[i] = key < E ? place : -1 - place;
+  __syncthreads();
+  if (wave >= used) return;
+  for (int i0 = first; i0 < last; i0 += 64 * kAhead) {
+    int e[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) e[u] = i0 + u * 64 + lane < last ? experts[i0 + u * 64 + lane] : 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * 64 + lane, key = key_of(e[u]);
+      uint64_t same = __ballot(i < last);
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot(key >> b & 1);
+        same &= key >> b & 1 ? set : ~set;
+      }
+      if (i < last) {
+        const int rank = __popcll(same & ((1ull << lane) - 1)), at = mine[key] + rank;
+        order[at] = i;
+        positions[i] = key < E ? at : -1 - at;
+        if (rank == 0) mine[key] = at + __popcll(same);
+      }
     }
-    __syncthreads();
-    for (int e = tid; e <= E; e += kSortThreads)
-      for (int w = 0; w < kSortWaves; ++w) base[e] += cnt[w][e];
-    __syncthreads();
   }
 }
 
@@ -73,50 +92,145 @@ template <> struct Elem<MXQ_DT_F32> { typedef float type; };
 template <> struct Elem<MXQ_DT_BF16> { typedef __bf16 type; };
 template <> struct Elem<MXQ_DT_F16> { typedef _Float16 type; };
 
-// out[t] = residual[t] + sum_j w[t, j] y[position[t, j]] in float32, j in order, rounded once.
+// 16 bytes of a row at any address, element i of them as float32; the row's last ones one by one.
+template <int DT> struct Pack {
+  typedef typename Elem<DT>::type E;
+  static constexpr int N = 16 / sizeof(E);
+  typedef E Any __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+  E v[N];
+  __device__ __forceinline__ void load(const E* p, int64_t left) {
+    if (left >= N) {
+      const Any a = *(const Any*)p;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = a[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = i < left ? p[i] : (E)0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(E* p, int64_t left) const {
+    if (left >= N) {
+      Any a;
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = v[i];
+      *(Any*)p = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) p[i] = v[i];
+    }
+  }
+};
+
+constexpr int kRows = 4;                                          // experts' rows in flight
+
+// out[t] = residual[t] + sum_j w[t, j] y[position[t, j]] in float32, j in order, rounded once.  Reading y bounds it: 16
+// bytes a thread, four rows' loads in flight before the first is added.
 template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y_, const float* weights, const int32_t* positions,
                                                                    const void* residual_, void* out_, int64_t T, int k, int64_t D) {
-  typedef typename Elem<DT>::type E;
+  typedef Pack<DT> P;
+  typedef typename P::E E;
   const E *y = (const E*)y_, *residual = (const E*)residual_;
   E* out = (E*)out_;
-  for (int64_t t = blockIdx.x; t < T; t += gridDim.x)
-    for (int64_t d = (int64_t)blockIdx.y * 256 + threadIdx.x; d < D; d += (int64_t)gridDim.y * 256) {
-      float sum = residual ? (float)residual[t * D + d] : 0.0f;
-      for (int j = 0; j < k; ++j) {
-        const float w = weights[t * k + j];
-        const int p = positions[t * k + j];
-        if (p >= 0) sum = __builtin_fmaf(w, (float)y[p * D + d], sum);
-        else if (w != w) sum = w;                               // a NaN weight of no expert stays visible
+  const int64_t groups = (D + P::N - 1) / P::N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < T * groups; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / groups, d = (i - t * groups) * P::N, left = D - d;
+    float sum[P::N];
+    P res, row[kRows];
+    if (residual) res.load(residual + t * D + d, left);
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) sum[e] = 0.0f;
+    for (int j0 = 0; j0 < k; j0 += kRows) {
+      float w[kRows];
+      int p[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const bool in = j0 + j < k;
+        w[j] = in ? weights[t * k + j0 + j] : 0.0f;
+        p[j] = in ? positions[t * k + j0 + j] : -1;
       }
-      out[t * D + d] = (E)sum;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (p[j] >= 0) row[j].load(y + p[j] * D + d, left);
+      if (residual && j0 == 0) {
+#pragma unroll
+        for (int e = 0; e < P::N; ++e) sum[e] = (float)res.v[e];
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        if (p[j] >= 0) {
+#pragma unroll
+          for (int e = 0; e < P::N; ++e) sum[e] = __builtin_fmaf(w[j], (float)row[j].v[e], sum[e]);
+        } else if (w[j] != w[j]) {                                // a NaN weight of no expert stays visible
+#pragma unroll
+          for (int e = 0; e < P::N; ++e) sum[e] = w[j];
+        }
+      }
     }
+    P o;
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) o.v[e] = (E)sum[e];
+    o.store(out + t * D + d, left);
+  }
 }
 
-// dy[position] = w g[t] (zeros for a slot of no expert), dw = <g[t], y[position]>: a workgroup a token.
+// dy[position] = w g[t] (zeros for a slot of no expert), dw = <g[t], y[position]>: a workgroup a token, the gradient's row
+// read once for four slots, their rows' loads in flight together.
 template <int DT> __global__ __launch_bounds__(256) void k_combine_grad(const void* grad_, const void* y_, const float* weights,
                                                                         const int32_t* positions, void* dy_, float* dw, int64_t T,
                                                                         int k, int64_t D) {
-  typedef typename Elem<DT>::type E;
-  __shared__ float part[4];
+  typedef Pack<DT> P;
+  typedef typename P::E E;
+  __shared__ float part[2][kRows][4];
   const E *y = (const E*)y_, *grad = (const E*)grad_;
   E* dy = (E*)dy_;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int turn = 0;
   for (int64_t t = blockIdx.x; t < T; t += gridDim.x)
-    for (int j = 0; j < k; ++j) {
-      const int p = positions[t * k + j];
-      const int64_t row = p >= 0 ? p : -1 - (int64_t)p;
-      const float w = p >= 0 ? weights[t * k + j] : 0.0f;
-      float dot = 0.0f;
-      for (int64_t d = threadIdx.x; d < D; d += 256) {
-        const float g = (float)grad[t * D + d];
-        if (dw && p >= 0) dot = __builtin_fmaf(g, (float)y[row * D + d], dot);
-        if (dy) dy[row * D + d] = (E)(p >= 0 ? w * g : 0.0f);
+    for (int j0 = 0; j0 < k; j0 += kRows, turn ^= 1) {
+      float w[kRows], dot[kRows];
+      int64_t at[kRows];
+      bool live[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int p = j0 + j < k ? positions[t * k + j0 + j] : 0;
+        live[j] = j0 + j < k && p >= 0;
+        at[j] = (p >= 0 ? p : -1 - (int64_t)p) * D;
+        w[j] = live[j] ? weights[t * k + j0 + j] : 0.0f;
+        dot[j] = 0.0f;
+      }
+      for (int64_t d = (int64_t)threadIdx.x * P::N; d < D; d += 256 * P::N) {
+        const int64_t left = D - d;
+        P g, row[kRows];
+        g.load(grad + t * D + d, left);
+#pragma unroll
+        for (int j = 0; j < kRows; ++j)
+          if (dw && live[j]) row[j].load(y + at[j] + d, left);
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+          if (dw && live[j]) {
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) dot[j] = __builtin_fmaf((float)g.v[e], (float)row[j].v[e], dot[j]);
+          }
+          if (dy && j0 + j < k) {
+            P o;
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) o.v[e] = (E)(live[j] ? w[j] * (float)g.v[e] : 0.0f);
+            o.store(dy + at[j] + d, left);
+          }
+        }
       }
       if (!dw) continue;
-      for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
-      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) dw[t * k + j] = part[0] + part[1] + part[2] + part[3];
-      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        for (int o = 32; o; o >>= 1) dot[j] += __shfl_xor(dot[j], o);
+        if (lane == 0) part[turn][j][wave] = dot[j];
+      }
+      __syncthreads();                                            // the other half of `part` is the next turn's
+      if (threadIdx.x < kRows && j0 + (int)threadIdx.x < k) {
+        const float* p = part[turn][threadIdx.x];
+        dw[t * k + j0 + threadIdx.x] = p[0] + p[1] + p[2] + p[3];
+      }
     }
 }
 
@@ -147,8 +261,9 @@ extern "C" int mxq_dispatch(const int32_t* experts, int64_t n, int64_t E, int32_
   if (!offsets || (n && (!experts || !order || !positions))) return invalid("mxq_dispatch: NULL argument");
   int bits = 0;
   while ((E >> bits) != 0) ++bits;                                // keys 0 .. E
+  const int64_t run = n ? ceil_div(ceil_div(n, kSortWaves), 64) * 64 : 64;
   KernelTimer timer("k_dispatch", as_stream(stream));
-  k_dispatch<<<1, kSortThreads, 0, as_stream(stream)>>>(experts, (int)n, (int)E, bits, order, offsets, positions);
+  k_dispatch<<<1, kSortThreads, 0, as_stream(stream)>>>(experts, (int)n, (int)E, bits, (int)run, order, offsets, positions);
   return check_launch("mxq_dispatch");
 }
 
@@ -157,7 +272,8 @@ extern "C" int mxq_combine(const void* y, int32_t dtype, const float* weights, c
   if (int rc = check_combine("mxq_combine", dtype, T, k, D)) return rc;
   if (T == 0 || D == 0) return MXQ_OK;
   if (!y || !weights || !positions || !out) return invalid("mxq_combine: NULL argument");
-  const dim3 grid((unsigned)T, (unsigned)(ceil_div(D, 256) < 65535 ? ceil_div(D, 256) : 65535));
+  const int64_t blocks = ceil_div(T * ceil_div(D, dtype == MXQ_DT_F32 ? 4 : 8), 256);
+  const dim3 grid((unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff));
   with_dtype(dtype, [&](auto dt) {
     KernelTimer timer("k_combine", as_stream(stream));
     k_combine<decltype(dt)::value><<<grid, 256, 0, as_stream(stream)>>>(y, weights, positions, residual, out, T, (int)k, D);

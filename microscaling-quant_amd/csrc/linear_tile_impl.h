@@ -286,8 +286,22 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
   __syncthreads();                                                       // the stages become the waves' own transposes
   float* mine = (float*)memory + wave * 32 * PITCH;
   const int64_t nw = n0 + wn * (gated ? 32 : 64);                       // this wave's first output
+  const int shift = gated ? 2 : 3, groups = 1 << shift;                  // of eight outputs a row
+  const int64_t n = nw + (lane & (groups - 1)) * 8;
+  // the residual of the next 32 rows is asked for before these are finished: a wait for memory a tile, not one for each row
+  Eight residual[2][4];
+  auto ask = [&](int m) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int row = (wm * WM + m) * 32 + ((p * 64 + lane) >> shift);
+      if (a.residual && p * 64 < 32 * groups && row < t.rows && n + 8 <= a.N)
+        residual[m & 1][p] = load_eight(a.residual, a.sp.residual_dtype, (t.row0 + row) * a.sp.ld_residual + n);
+    }
+  };
+  ask(0);
 #pragma unroll
   for (int m = 0; m < WM; ++m) {
+    if (m + 1 < WM) ask(m + 1);
 #pragma unroll
     for (int i = 0; i < WN; ++i)
 #pragma unroll
@@ -297,20 +311,30 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int shift = gated ? 2 : 3;                                     // log2 of the groups of eight outputs a row
-#pragma unroll 1
-    for (int p = lane; p < 32 << shift; p += 64) {
-      const int row = p >> shift, g = p & ((1 << shift) - 1), rr = (wm * WM + m) * 32 + row;
-      if (rr >= t.rows || nw + g * 8 >= a.N) continue;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int row = (p * 64 + lane) >> shift, rr = (wm * WM + m) * 32 + row;
+      if (p * 64 >= 32 * groups || rr >= t.rows || n + 8 > a.N) continue;
       float z[8], up[8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float* at = &mine[row * PITCH + g * 8 + 4 * i];
+        const float* at = &mine[row * PITCH + (lane & (groups - 1)) * 8 + 4 * i];
         const f32x4 u = *(const f32x4*)at, v = *(const f32x4*)(at + (gated ? 32 : 0));
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[4 * i + e] = u[e], up[4 * i + e] = v[e];
       }
-      finish_eight(a, t, t.row0 + rr, nw + g * 8, z, up);
+      finish_eight(a, t, t.row0 + rr, n, z, up, residual[m & 1][p]);
+    }
+    if (n < a.N && n + 8 > a.N) {                                        // the last outputs, one by one
+#pragma unroll 1
+      for (int row = lane >> shift; row < 32; row += 64 >> shift) {
+        const int rr = (wm * WM + m) * 32 + row;
+        const float* at = &mine[row * PITCH + (lane & (groups - 1)) * 8];
+        if (rr < t.rows)
+#pragma unroll 1
+          for (int64_t e = n; e < a.N; ++e, ++at)
+            store_elem(a.y, a.sp.y_dtype, (t.row0 + rr) * a.sp.ld_y + e, epilogue(a, t, t.row0 + rr, e, at[0], at[gated ? 32 : 0]));
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();

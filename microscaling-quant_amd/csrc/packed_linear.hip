@@ -53,24 +53,29 @@ __global__ __launch_bounds__(256) void k_linear_finish(LinearArgs a, const float
   const int64_t groups = (a.N + 7) / 8, width = a.sp.gated ? 2 * a.N : a.N;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.M * groups; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / groups, n = i % groups * 8;
+    const RowTile t{0, 0, 0, false};
+    const float* p = partial + row * width + n;
+    if (n + 8 > a.N) {
+      for (int64_t e = n; e < a.N; ++e, ++p) {
+        float z = 0.0f, up = 0.0f;
+        for (int s = 0; s < split; ++s) {
+          z += p[s * a.M * width];
+          if (a.sp.gated) up += p[s * a.M * width + a.N];
+        }
+        store_elem(a.y, a.sp.y_dtype, row * a.sp.ld_y + e, epilogue(a, t, row, e, z, up));
+      }
+      continue;
+    }
     float z[8], up[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[e] = up[e] = 0.0f;
-    for (int s = 0; s < split; ++s) {
-      const float* p = partial + (s * a.M + row) * width + n;
-      if (n + 8 <= a.N) {
-        add_eight(z, p, MXQ_DT_F32, 0);
-        if (a.sp.gated) add_eight(up, p + a.N, MXQ_DT_F32, 0);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < a.N) {
-            z[e] += p[e];
-            if (a.sp.gated) up[e] += p[a.N + e];
-          }
-      }
+    for (int s = 0; s < split; ++s, p += a.M * width) {
+      add_eight(z, p, MXQ_DT_F32, 0);
+      if (a.sp.gated) add_eight(up, p + a.N, MXQ_DT_F32, 0);
     }
-    finish_eight(a, RowTile{0, 0, 0, false}, row, n, z, up);
+    Eight residual = {};
+    if (a.residual) residual = load_eight(a.residual, a.sp.residual_dtype, row * a.sp.ld_residual + n);
+    finish_eight(a, t, row, n, z, up, residual);
   }
 }
 

@@ -245,21 +245,41 @@ __device__ __forceinline__ float epilogue(const LinearArgs& a, const RowTile& t,
   return z;
 }
 
-// v[i] += p[at + i], eight neighbours.
-__device__ __forceinline__ void add_eight(float (&v)[8], const void* p, int dtype, int64_t at) {
+// Eight neighbours as they lie in memory (float32's second half in `more`), and their sum with v.
+struct Eight {
+  u32x4 first, more;
+};
+__device__ __forceinline__ Eight load_eight(const void* p, int dtype, int64_t at) {
+  Eight e;
   if (dtype == MXQ_DT_F32) {
-    const u32x4 x = *(const u32x4_any*)((const float*)p + at), y = *(const u32x4_any*)((const float*)p + at + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(x[i]), v[i + 4] += __uint_as_float(y[i]);
-    return;
+    e.first = *(const u32x4_any*)((const float*)p + at);
+    e.more = *(const u32x4_any*)((const float*)p + at + 4);
+  } else {
+    e.first = *(const u32x4_any*)((const uint16_t*)p + at);
   }
-  const u32x4 x = *(const u32x4_any*)((const uint16_t*)p + at);
+  return e;
+}
+__device__ __forceinline__ void add_eight(float (&v)[8], const Eight& e, int dtype) {
+  if (dtype == MXQ_DT_F32) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint16_t b = (uint16_t)(x[i >> 1] >> (i & 1) * 16);
-    v[i] += load_elem(&b, dtype, 0);
+    for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(e.first[i]), v[i + 4] += __uint_as_float(e.more[i]);
+  } else if (dtype == MXQ_DT_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] += __uint_as_float(e.first[i] << 16);
+      v[2 * i + 1] += __uint_as_float(e.first[i] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f16x2 b;
+      __builtin_memcpy(&b, (const char*)&e.first + 4 * i, 4);
+      v[2 * i] += (float)b[0];
+      v[2 * i + 1] += (float)b[1];
+    }
   }
 }
+__device__ __forceinline__ void add_eight(float (&v)[8], const void* p, int dtype, int64_t at) { add_eight(v, load_eight(p, dtype, at), dtype); }
 
 __device__ __forceinline__ void activate_eight(float (&v)[8], int activation) {
   switch (activation) {
@@ -275,14 +295,9 @@ __device__ __forceinline__ void activate_eight(float (&v)[8], int activation) {
   }
 }
 
-// epilogue and store of eight neighbouring outputs of a row.
-__device__ __forceinline__ void finish_eight(const LinearArgs& a, const RowTile& t, int64_t row, int64_t n, float (&z)[8], float (&up)[8]) {
-  if (n + 8 > a.N) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n + i < a.N) store_elem(a.y, a.sp.y_dtype, row * a.sp.ld_y + n + i, epilogue(a, t, row, n + i, z[i], up[i]));
-    return;
-  }
+// epilogue and store of eight neighbouring outputs of a row, all below N; residual: theirs, if there is one.
+__device__ __forceinline__ void finish_eight(const LinearArgs& a, const RowTile& t, int64_t row, int64_t n, float (&z)[8], float (&up)[8],
+                                             const Eight& residual) {
   if (t.zeros) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] = 0.0f;
@@ -295,7 +310,7 @@ __device__ __forceinline__ void finish_eight(const LinearArgs& a, const RowTile&
 #pragma unroll
       for (int i = 0; i < 8; ++i) z[i] *= up[i];
     }
-    if (a.residual) add_eight(z, a.residual, a.sp.residual_dtype, row * a.sp.ld_residual + n);
+    if (a.residual) add_eight(z, residual, a.sp.residual_dtype);
   }
   const int64_t at = row * a.sp.ld_y + n;
   if (a.sp.y_dtype == MXQ_DT_F32) {

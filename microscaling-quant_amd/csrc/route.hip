@@ -4,9 +4,12 @@
 //   groups > 1: a group's score is the sum of its two best r; experts outside the top_groups best groups: r = -inf
 //   the k experts of largest r, ties to the lowest index;  w_j = scale s_{e_j} [/ sum of the k s]
 //
-// One wave a token, expert e in register e / 64 of lane e % 64.  Scores are 64-bit: an expert is taken or left by values
-// that lie close together (16384 tokens of 256 experts hold a pair of neighbours at rank k within 1e-8 of each other),
-// and float32's exp would decide those by its rounding.
+// Scores are 64-bit: an expert is taken or left by values that lie close together (16384 tokens of 256 experts hold a pair
+// of neighbours at rank k within 1e-8 of each other), and float32's exp would decide those by its rounding.
+//
+// Up to 512 experts a token has 16 lanes, so that a maximum over its lanes is four rotations within a row of lanes and a
+// wave chooses for four tokens at once; beyond, a whole wave.  Expert e is register e / L of lane e % L.  What bounds it is
+// instructions: about 25 for a score and seven a register and choice.
 #include "mxq_common.h"
 
 namespace mxq {
@@ -27,175 +30,260 @@ template <int DT> __device__ __forceinline__ void store_from_float(void* p, int6
   if constexpr (DT == MXQ_DT_F16) ((_Float16*)p)[i] = (_Float16)v;
 }
 
-__device__ __forceinline__ double wave_max(double v) {
-  for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-  return v;
+// Rotation by N within each row of 16 lanes.
+template <int N> __device__ __forceinline__ int rotate(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x120 + N, 0xF, 0xF, false); }
+template <int N> __device__ __forceinline__ double rotate(double v) {
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t lo = rotate<N>((int)(uint32_t)b), hi = rotate<N>((int)(uint32_t)(b >> 32));
+  return __longlong_as_double((uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// The wave's best (value, index), the larger value first, the lower index among equals.
-__device__ __forceinline__ void wave_best(double& v, int& i) {
-  for (int o = 32; o; o >>= 1) {
-    const double ov = __shfl_xor(v, o);
-    const int oi = __shfl_xor(i, o);
-    if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
+// f over the L lanes of a token, the same value in each.
+template <int L, typename T, typename F> __device__ __forceinline__ T over_lanes(T v, F f) {
+  v = f(v, rotate<8>(v));
+  v = f(v, rotate<4>(v));
+  v = f(v, rotate<2>(v));
+  v = f(v, rotate<1>(v));
+  if constexpr (L == 64) {
+    v = f(v, __shfl_xor(v, 16));
+    v = f(v, __shfl_xor(v, 32));
   }
+  return v;
+}
+template <int L> __device__ __forceinline__ double lanes_max(double v) {
+  return over_lanes<L>(v, [](double a, double b) { return fmax(a, b); });
+}
+template <int L> __device__ __forceinline__ double lanes_sum(double v) {
+  return over_lanes<L>(v, [](double a, double b) { return a + b; });
+}
+template <int L> __device__ __forceinline__ int lanes_min(int v) {
+  return over_lanes<L>(v, [](int a, int b) { return a < b ? a : b; });
+}
+template <int L> __device__ __forceinline__ bool lanes_any(bool b) {
+  const uint64_t all = __ballot(b);
+  if constexpr (L == 64) return all != 0;
+  return (all >> (threadIdx.x & 48) & 0xFFFF) != 0;
 }
 
-// s[]: the scores of the lane's experts; true if the row holds a NaN, or +inf under softmax, which has no score.
-template <int DT, int V> __device__ __forceinline__ bool scores_of(const void* logits, int64_t row, int E, int softmax,
-                                                                   float (&l)[V], double (&s)[V]) {
-  const int lane = threadIdx.x & 63;
-  double top = -INFINITY;
+// e^x for x <= 709.78, zero below -746: x = n ln 2 + r with |r| <= ln(2) / 2, Taylor's series of e^r to r^13 (the next term
+// is below 4e-18), times 2^n.
+__device__ __forceinline__ double exp64(double x) {
+  x = fmax(x, -746.0);
+  const double n = rint(x * 1.4426950408889634);
+  const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994531, x));
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+
+// 1 / d for 1 <= d < 2^1000: the hardware's estimate and two steps of Newton's iteration.
+__device__ __forceinline__ double inverse(double d) {
+  double y = __builtin_amdgcn_rcp(d);
+  y = fma(fma(-d, y, 1.0), y, y);
+  return fma(fma(-d, y, 1.0), y, y);
+}
+
+// The row's largest logit and the inverse of its sum of powers, under softmax.
+struct Norm {
+  double top, inverse;
+};
+
+__device__ __forceinline__ double score_of(float l, int softmax, const Norm& n) {
+  if (softmax) return exp64((double)l - n.top) * n.inverse;
+  return -l > 709.0f ? 0.0 : inverse(1.0 + exp64(-(double)l));
+}
+
+// l[]: the lane's logits, s[]: their scores; true if the row holds a NaN, or +inf under softmax, which has no score.
+template <int DT, int L, int V> __device__ __forceinline__ bool scores_of(const void* logits, int64_t row, int E, int softmax, float (&l)[V],
+                                                                          double (&s)[V], Norm& n) {
+  const int lane = threadIdx.x & (L - 1);
   bool bad = false;
+  double top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < V; ++v) l[v] = v * L + lane < E ? load_as_float<DT>(logits, row * E + v * L + lane) : -INFINITY;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    l[v] = e < E ? load_as_float<DT>(logits, row * E + e) : -INFINITY;
     bad |= l[v] != l[v] || (softmax && l[v] == INFINITY);
     top = fmax(top, (double)l[v]);
   }
-  bad = __any(bad);
+  bad = lanes_any<L>(bad);
+  n = Norm{0.0, 1.0};
   if (softmax) {
-    top = wave_max(top);
-    if (top == -INFINITY) top = 0.0;
+    top = lanes_max<L>(top);
+    n.top = top == -INFINITY ? 0.0 : top;
     double sum = 0.0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum += s[v] = exp((double)l[v] - top);
-    sum = wave_sum(sum);
-    if (sum == 0.0) sum = 1.0;
+    for (int v = 0; v < V; ++v) sum += s[v] = l[v] == -INFINITY ? 0.0 : exp64((double)l[v] - n.top);
+    sum = lanes_sum<L>(sum);
+    n.inverse = sum < 1.0 ? 1.0 : inverse(sum);                   // an open row's sum is at least 1
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] /= sum;
+    for (int v = 0; v < V; ++v) s[v] *= n.inverse;
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = 1.0 / (1.0 + exp(-(double)l[v]));
+    for (int v = 0; v < V; ++v) s[v] = score_of(l[v], 0, n);
   }
   return bad;
 }
 
-template <int DT, int V>
+template <int DT, int L, int V>
 __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const float* bias, int64_t T, int E,
-                                                       mxq_route_spec sp, float* weights, int32_t* experts) {
-  __shared__ double ranked[kWaves][V * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + wave;
-  if (row >= T) return;
+                                                       mxq_route_spec sp, DivU31 per, float* weights, int32_t* experts) {
+  extern __shared__ double shared[];                              // groups > 1: E ranks and 64 scores a token
+  constexpr int kSlots = kMaxTopK / L;
+  const int lane = threadIdx.x & (L - 1), token = threadIdx.x / L;
+  const int64_t at = (int64_t)blockIdx.x * (blockDim.x / L) + token, row = at < T ? at : T - 1;
+  const bool softmax = sp.score == MXQ_SCORE_SOFTMAX, out = at < T;     // lanes past the end go along: the row's lanes work together
   const int k = sp.top_k;
   float l[V];
-  double s[V], r[V];
-  bool bad = scores_of<DT, V>(logits, row, E, sp.score == MXQ_SCORE_SOFTMAX, l, s);
+  double r[V];
+  Norm norm;
+  bool bad = scores_of<DT, L, V>(logits, row, E, softmax, l, r, norm);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    r[v] = bias && e < E ? s[v] + (double)bias[e] : s[v];
+    const int e = v * L + lane;
+    if (bias && e < E) r[v] += (double)bias[e];
     if (l[v] == -INFINITY) r[v] = -INFINITY;
     bad |= r[v] != r[v];
   }
-  if (__any(bad)) {
-    if (lane < k) weights[row * k + lane] = NAN, experts[row * k + lane] = -1;
-    return;
-  }
+  bad = lanes_any<L>(bad);
   if (sp.groups > 1) {
-    double* mine = ranked[wave];
+    volatile double* ranks = shared + (size_t)token * (E + kMaxGroups);
+    volatile double* scores = ranks + E;
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine[v * 64 + lane] = r[v];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int per = E / sp.groups;
-    double a = -INFINITY, b = -INFINITY;
-    if (lane < sp.groups)
-      for (int j = 0; j < per; ++j) {
-        const double x = mine[lane * per + j];
-        if (x > a) b = a, a = x;
-        else if (x > b) b = x;
+    for (int v = 0; v < V; ++v)
+      if (v * L + lane < E) ranks[v * L + lane] = r[v];
+    for (int g = lane; g < sp.groups; g += L) {
+      double a = -INFINITY, b = -INFINITY;
+      for (int j = 0; j < (int)per.d; ++j) {
+        const double x = ranks[g * per.d + j];
+        b = fmax(b, fmin(a, x));
+        a = fmax(a, x);
       }
-    double score = a == -INFINITY ? a : b == -INFINITY ? a : a + b;
+      scores[g] = b == -INFINITY ? a : a + b;
+    }
+    // a group is kept if fewer than top_groups come before it
     uint64_t kept = 0;
-    for (int j = 0; j < sp.top_groups; ++j) {
-      double x = score;
-      int i = lane < sp.groups && !(kept >> lane & 1) ? lane : 64;
-      if (i == 64) x = -INFINITY;
-      wave_best(x, i);
-      if (i < 64) kept |= 1ull << i;
+    for (int g0 = 0; g0 < sp.groups; g0 += L) {
+      const int g = g0 + lane;
+      const double mine = g < sp.groups ? scores[g] : 0.0;
+      int before = 0;
+      for (int h = 0; h < sp.groups; ++h) {
+        const double x = scores[h];
+        before += x > mine || (x == mine && h < g);
+      }
+      const uint64_t all = __ballot(g < sp.groups && before < sp.top_groups);
+      kept |= (L == 64 ? all : all >> (threadIdx.x & 48) & 0xFFFF) << g0;
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int g = (v * 64 + lane) / per;
-      if (g >= sp.groups || !(kept >> g & 1)) r[v] = -INFINITY;
+      const uint32_t g = divu31(v * L + lane, per);
+      if (!(kept >> (g & 63) & 1)) r[v] = -INFINITY;
     }
   }
-  double own = 0.0;
-  int pick = -1;
-  for (int j = 0; j < k; ++j) {
-    double x = r[0], sx = s[0];
-    int i = lane;
+  int pick[kSlots];
 #pragma unroll
-    for (int v = 1; v < V; ++v)
-      if (r[v] > x) x = r[v], sx = s[v], i = v * 64 + lane;
-    wave_best(x, i);
-    if (x == -INFINITY) break;
-    sx = __shfl(sx, i & 63);
-    if (lane == j) own = sx, pick = i;
+  for (int q = 0; q < kSlots; ++q) {
+    pick[q] = -1;
+    for (int j = q * L; j < k && j < (q + 1) * L; ++j) {
+      double best = r[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (i == v * 64 + lane) r[v] = -INFINITY;
+      for (int v = 1; v < V; ++v) best = fmax(best, r[v]);
+      best = lanes_max<L>(best);
+      int i = 0x7fffffff;
+#pragma unroll
+      for (int v = V - 1; v >= 0; --v)
+        if (r[v] == best) i = v * L + lane;
+      i = lanes_min<L>(i);
+      if (lane == j - q * L && best > -INFINITY) pick[q] = i;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (i == v * L + lane) r[v] = -INFINITY;
+    }
   }
-  double total = 1.0;
-  if (sp.renormalize) {
-    total = wave_sum(own);
-    if (total == 0.0) total = 1.0;
+  double own[kSlots], total = 0.0;
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q) {
+    own[q] = 0.0;
+    if (pick[q] >= 0 && !bad) own[q] = score_of(load_as_float<DT>(logits, row * E + pick[q]), softmax, norm);
+    total += own[q];
   }
-  if (lane < k) {
-    weights[row * k + lane] = (float)(own / total * (double)sp.scale);
-    experts[row * k + lane] = pick;
+  total = lanes_sum<L>(total);
+  if (!sp.renormalize || total == 0.0) total = 1.0;
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q) {
+    const int j = q * L + lane;
+    if (j >= k || !out) continue;
+    weights[row * k + j] = bad ? NAN : (float)(own[q] / total * (double)sp.scale);
+    experts[row * k + j] = bad ? -1 : pick[q];
   }
 }
 
 // The gradient of the logits: with u_j the chosen scores and U their sum, du_j = scale (g_j - sum_i g_i u_i / U) / U
 // where renormalized, scale g_j otherwise; softmax: dl_e = s_e (du_e - sum_j du_j u_j); sigmoid: dl_e = du_e s_e (1 - s_e).
-template <int DT, int V>
+template <int DT, int L, int V>
 __global__ __launch_bounds__(64 * kWaves) void k_route_grad(const void* logits, const int32_t* experts, const float* grad,
                                                             int64_t T, int E, mxq_route_spec sp, void* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + wave;
-  if (row >= T) return;
+  constexpr int kSlots = kMaxTopK / L;
+  const int lane = threadIdx.x & (L - 1), first = threadIdx.x & 63 & ~(L - 1);
+  const int64_t at = (int64_t)blockIdx.x * (64 * kWaves / L) + threadIdx.x / L, row = at < T ? at : T - 1;
+  const bool softmax = sp.score == MXQ_SCORE_SOFTMAX;
   const int k = sp.top_k;
   float l[V];
   double s[V], d[V];
-  const bool bad = scores_of<DT, V>(logits, row, E, sp.score == MXQ_SCORE_SOFTMAX, l, s);
-  const int pick = lane < k ? experts[row * k + lane] : -1;
-  const double g = lane < k && pick >= 0 ? (double)grad[row * k + lane] : 0.0;
-  double u = 0.0;
+  Norm norm;
+  const bool bad = scores_of<DT, L, V>(logits, row, E, softmax, l, s, norm);
+  int pick[kSlots];
+  double u[kSlots], du[kSlots], U = 0.0, gu = 0.0;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const double x = __shfl(s[v], pick & 63);
-    if (pick >= 0 && pick >> 6 == v) u = x;
-    d[v] = 0.0;
+  for (int q = 0; q < kSlots; ++q) {
+    const int j = q * L + lane;
+    const int e = j < k ? experts[row * k + j] : -1;
+    pick[q] = e < E ? e : -1;
+    u[q] = pick[q] >= 0 ? score_of(load_as_float<DT>(logits, row * E + pick[q]), softmax, norm) : 0.0;
+    du[q] = pick[q] >= 0 ? (double)grad[row * k + j] * (double)sp.scale : 0.0;
+    U += u[q];
+    gu += du[q] * u[q];
   }
-  double du = g * (double)sp.scale;
   if (sp.renormalize) {
-    double U = wave_sum(u);
+    U = lanes_sum<L>(U);
+    gu = lanes_sum<L>(gu);
     if (U == 0.0) U = 1.0;
-    du = (du - wave_sum(du * u) / U) / U;
-    if (pick < 0) du = 0.0;
-  }
-  const double dot = sp.score == MXQ_SCORE_SOFTMAX ? wave_sum(du * u) : 0.0;
-  for (int j = 0; j < k; ++j) {
-    const int e = __shfl(pick, j);
-    const double x = __shfl(du, j);
+    const double mean = gu / U;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e == v * 64 + lane) d[v] = x;
+    for (int q = 0; q < kSlots; ++q) du[q] = pick[q] >= 0 ? (du[q] - mean) / U : 0.0;
   }
+  double dot = 0.0;
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q) dot += du[q] * u[q];
+  dot = softmax ? lanes_sum<L>(dot) : 0.0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) d[v] = 0.0;
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q)
+    for (int j = q * L; j < k && j < (q + 1) * L; ++j) {
+      const int e = __shfl(pick[q], first + j - q * L);
+      const double x = __shfl(du[q], first + j - q * L);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (e == v * L + lane) d[v] = x;
+    }
+  if (at >= T) return;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    double x = sp.score == MXQ_SCORE_SOFTMAX ? s[v] * (d[v] - dot) : d[v] * s[v] * (1.0 - s[v]);
-    if (bad) x = NAN;
-    if (e < E) store_from_float<DT>(out, row * E + e, (float)x);
+    const int e = v * L + lane;
+    const double x = softmax ? s[v] * (d[v] - dot) : d[v] * s[v] * (1.0 - s[v]);
+    if (e < E) store_from_float<DT>(out, row * E + e, bad ? NAN : (float)x);
   }
 }
 
@@ -212,18 +300,21 @@ int check_spec(const char* who, int32_t dtype, int64_t T, int64_t E, const mxq_r
   return MXQ_OK;
 }
 
-// f(DT, V) with the dtype and the registers a lane needs for E experts as compile-time constants.
+// f(DT, L, V): the dtype, the lanes of a token and the registers of a lane, as compile-time constants.
 template <typename F> void with_shape(int32_t dtype, int64_t E, F f) {
-  auto by_v = [&](auto dt) {
-    if (E <= 64) f(dt, std::integral_constant<int, 1>());
-    else if (E <= 128) f(dt, std::integral_constant<int, 2>());
-    else if (E <= 256) f(dt, std::integral_constant<int, 4>());
-    else if (E <= 512) f(dt, std::integral_constant<int, 8>());
-    else f(dt, std::integral_constant<int, 16>());
+  auto by_experts = [&](auto dt) {
+    std::integral_constant<int, 16> row;
+    if (E <= 16) f(dt, row, std::integral_constant<int, 1>());
+    else if (E <= 32) f(dt, row, std::integral_constant<int, 2>());
+    else if (E <= 64) f(dt, row, std::integral_constant<int, 4>());
+    else if (E <= 128) f(dt, row, std::integral_constant<int, 8>());
+    else if (E <= 256) f(dt, row, std::integral_constant<int, 16>());
+    else if (E <= 512) f(dt, row, std::integral_constant<int, 32>());
+    else f(dt, std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
   };
-  if (dtype == MXQ_DT_F32) by_v(std::integral_constant<int, MXQ_DT_F32>());
-  else if (dtype == MXQ_DT_BF16) by_v(std::integral_constant<int, MXQ_DT_BF16>());
-  else by_v(std::integral_constant<int, MXQ_DT_F16>());
+  if (dtype == MXQ_DT_F32) by_experts(std::integral_constant<int, MXQ_DT_F32>());
+  else if (dtype == MXQ_DT_BF16) by_experts(std::integral_constant<int, MXQ_DT_BF16>());
+  else by_experts(std::integral_constant<int, MXQ_DT_F16>());
 }
 
 }  // namespace
@@ -236,10 +327,13 @@ extern "C" int mxq_route(const void* logits, int32_t dtype, const float* bias, i
   if (int rc = check_spec("mxq_route", dtype, T, E, spec)) return rc;
   if (T == 0) return MXQ_OK;
   if (!logits || !weights || !experts) return invalid("mxq_route: NULL argument");
-  with_shape(dtype, E, [&](auto dt, auto v) {
+  with_shape(dtype, E, [&](auto dt, auto lanes, auto v) {
+    constexpr int L = decltype(lanes)::value;
+    const int threads = spec->groups > 1 && E > 256 ? 32 * kWaves : 64 * kWaves, tokens = threads / L;   // below 64 KB of LDS
+    const size_t lds = spec->groups > 1 ? tokens * (size_t)(E + kMaxGroups) * sizeof(double) : 0;
     KernelTimer timer("k_route", as_stream(stream));
-    k_route<decltype(dt)::value, decltype(v)::value><<<dim3((unsigned)ceil_div(T, kWaves)), 64 * kWaves, 0, as_stream(stream)>>>(
-        logits, bias, T, (int)E, *spec, weights, experts);
+    k_route<decltype(dt)::value, L, decltype(v)::value><<<dim3((unsigned)ceil_div(T, tokens)), threads, lds, as_stream(stream)>>>(
+        logits, bias, T, (int)E, *spec, make_divu31((uint32_t)(E / spec->groups)), weights, experts);
   });
   return check_launch("mxq_route");
 }
@@ -249,9 +343,10 @@ extern "C" int mxq_route_grad(const void* logits, int32_t dtype, const int32_t* 
   if (int rc = check_spec("mxq_route_grad", dtype, T, E, spec)) return rc;
   if (T == 0) return MXQ_OK;
   if (!logits || !experts || !grad || !out) return invalid("mxq_route_grad: NULL argument");
-  with_shape(dtype, E, [&](auto dt, auto v) {
+  with_shape(dtype, E, [&](auto dt, auto lanes, auto v) {
+    constexpr int L = decltype(lanes)::value, kTokens = 64 * kWaves / L;
     KernelTimer timer("k_route_grad", as_stream(stream));
-    k_route_grad<decltype(dt)::value, decltype(v)::value><<<dim3((unsigned)ceil_div(T, kWaves)), 64 * kWaves, 0, as_stream(stream)>>>(
+    k_route_grad<decltype(dt)::value, L, decltype(v)::value><<<dim3((unsigned)ceil_div(T, kTokens)), 64 * kWaves, 0, as_stream(stream)>>>(
         logits, experts, grad, T, (int)E, *spec, out);
   });
   return check_launch("mxq_route_grad");
