@@ -8,35 +8,39 @@ namespace {
 constexpr int kMaxExperts = 1024, kMaxTopK = 64;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kAhead = 4;
 
-// A stable counting sort by one workgroup.  Each wave owns a run of whole 64s of the slots and counts its experts into its
-// own row of LDS; the rows' and the experts' prefix sums turn the counts into the places where the wave's slots go; then it
-// goes through its run again, 64 slots at a time, on its own: a slot's rank among the wave's equal ones is a population
-// count of the lanes with the same key, which ballots over the key's bits find.  Three barriers whatever n is, and integer
-// sums throughout: the same order whatever the timing.
+// A stable counting sort.  A workgroup owns 16 runs of whole 64s of the slots, one a wave.  It counts the whole array's
+// experts itself, those before its runs apart from the others (reading 4 bytes a slot again costs less than a second
+// launch and a workspace), and each wave its own run's; prefix sums over the experts and the waves turn the counts into the
+// places where each wave's slots go.  A slot's rank among its wave's equal ones is a population count of the lanes with
+// the same key, which ballots over the key's bits find.  Integer sums throughout: the same order whatever the timing.
 __global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* experts, int n, int E, int bits, int run,
                                                            int32_t* order, int32_t* offsets, int32_t* positions) {
   __shared__ int place[kSortWaves][kMaxExperts + 1];
+  __shared__ int before_me[kMaxExperts + 1], others[kMaxExperts + 1];
   __shared__ int scan[kSortWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, used = n ? (n - 1) / run + 1 : 0;
-  const int first = wave * run, last = first + run < n ? first + run : n;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, begin = blockIdx.x * (kSortWaves * run);
+  const int left = n - begin, used = left <= 0 ? 0 : left > (kSortWaves - 1) * run ? kSortWaves : (left - 1) / run + 1;
+  const int first = begin + wave * run, last = wave >= used ? first : n - first < run ? n : first + run;
   volatile int* mine = place[wave];
   auto key_of = [&](int e) { return (unsigned)e < (unsigned)E ? e : E; };        // E: the slots of no expert, sorted last
-  if (wave < used) {
+  for (int e = tid; e <= E; e += kSortThreads) before_me[e] = others[e] = 0;
+  if (wave < used)
     for (int e = lane; e <= E; e += 64) mine[e] = 0;
-    for (int i = first + lane; i < last; i += 64 * kAhead) {
-      int e[kAhead];
+  __syncthreads();
+  for (int i = tid; i < n; i += kSortThreads * kAhead) {
+    int e[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) e[u] = i + u * 64 < last ? experts[i + u * 64] : 0;
+    for (int u = 0; u < kAhead; ++u) e[u] = i + u * kSortThreads < n ? experts[i + u * kSortThreads] : 0;
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i + u * 64 < last) atomicAdd(&place[wave][key_of(e[u])], 1);
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = i + u * kSortThreads;
+      if (at < n) atomicAdd(at < begin ? &before_me[key_of(e[u])] : &others[key_of(e[u])], 1);
     }
   }
+  for (int i = first + lane; i < last; i += 64) atomicAdd(&place[wave][key_of(experts[i])], 1);
   __syncthreads();
-  // one expert a thread: its count, the prefix over the experts, then the rows' places; slots of none follow all others
-  int c = 0;
-  if (tid < E)
-    for (int w = 0; w < used; ++w) c += place[w][tid];
+  // one expert a thread: its count, the prefix over the experts, then the runs' places; slots of none follow all others
+  const int c = tid < E ? before_me[tid] + others[tid] : 0;
   int p = c;
   for (int o = 1; o < 64; o <<= 1) {
     const int q = __shfl_up(p, o);
@@ -44,25 +48,23 @@ __global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* expert
   }
   if (lane == 63) scan[wave] = p;
   __syncthreads();
-  int before = 0, all = 0;
+  int ahead = 0, all = 0;
   for (int w = 0; w < kSortWaves; ++w) {
-    if (w == wave) before = all;
+    if (w == wave) ahead = all;
     all += scan[w];
   }
-  p += before - c;
-  if (tid < E) offsets[tid] = p;
-  if (tid == 0) offsets[E] = all;
-  for (int w = 0, at = p; w < used && tid < E; ++w) {
-    const int q = place[w][tid];
-    place[w][tid] = at;
-    at += q;
-  }
-  if (tid == kSortThreads - 1)                                    // after its expert, should it have one
-    for (int w = 0, at = all; w < used; ++w) {
-      const int q = place[w][E];
-      place[w][E] = at;
+  p += ahead - c;
+  if (blockIdx.x == 0 && tid < E) offsets[tid] = p;
+  if (blockIdx.x == 0 && tid == 0) offsets[E] = all;
+  auto runs = [&](int e, int at) {
+    for (int w = 0; w < used; ++w) {
+      const int q = place[w][e];
+      place[w][e] = at;
       at += q;
     }
+  };
+  if (tid < E) runs(tid, p + before_me[tid]);
+  if (tid == kSortThreads - 1) runs(E, all + before_me[E]);
   __syncthreads();
   if (wave >= used) return;
   for (int i0 = first; i0 < last; i0 += 64 * kAhead) {
@@ -256,14 +258,15 @@ using namespace mxq;
 
 extern "C" int mxq_dispatch(const int32_t* experts, int64_t n, int64_t E, int32_t* order, int32_t* offsets,
                             int32_t* positions, mxq_stream_t stream) {
-  if (n < 0 || n > 0x7fffffff - kSortThreads) return invalid("mxq_dispatch: n out of range");
+  if (n < 0 || n > 0x7fffffff - 2 * kSortThreads * kAhead) return invalid("mxq_dispatch: n out of range");
   if (E < 1 || E > kMaxExperts) return invalid("mxq_dispatch: 1 to 1024 experts");
   if (!offsets || (n && (!experts || !order || !positions))) return invalid("mxq_dispatch: NULL argument");
   int bits = 0;
   while ((E >> bits) != 0) ++bits;                                // keys 0 .. E
-  const int64_t run = n ? ceil_div(ceil_div(n, kSortWaves), 64) * 64 : 64;
+  // a workgroup has 1024 slots, or more where that would be over 256 workgroups counting
+  const int64_t run = n ? ceil_div(n, 256 * kSortThreads) * 64 : 64, blocks = n ? ceil_div(n, run * kSortWaves) : 1;
   KernelTimer timer("k_dispatch", as_stream(stream));
-  k_dispatch<<<1, kSortThreads, 0, as_stream(stream)>>>(experts, (int)n, (int)E, bits, (int)run, order, offsets, positions);
+  k_dispatch<<<dim3((unsigned)blocks), kSortThreads, 0, as_stream(stream)>>>(experts, (int)n, (int)E, bits, (int)run, order, offsets, positions);
   return check_launch("mxq_dispatch");
 }
 
