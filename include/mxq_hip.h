@@ -531,12 +531,13 @@ typedef struct mxq_linear_spec {
  * memory of mxq_packed_linear_workspace bytes, 256-byte aligned (NULL where that is 0).
  * mxq_expert_linear: n rows sorted by expert (mxq_dispatch's order and offsets; order is read where top_k > 0), row r
  * of expert e multiplied by matrix e; rows past the last expert's become zeros. */
-int64_t mxq_packed_linear_workspace(const void* x, int64_t M, int64_t N, int64_t K, const mxq_linear_spec* spec);
+int64_t mxq_packed_linear_workspace(const void* x, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t N,
+                                    int64_t K, const mxq_linear_spec* spec);
 int mxq_packed_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias,
                       const void* residual, void* y, int64_t M, int64_t N, int64_t K, const mxq_linear_spec* spec,
                       void* workspace, mxq_stream_t stream);
-int64_t mxq_expert_linear_workspace(const void* x, int64_t n, int64_t N, int64_t K, int64_t E,
-                                    const mxq_linear_spec* spec);
+int64_t mxq_expert_linear_workspace(const void* x, const uint8_t* codes, const uint8_t* scales, int64_t n, int64_t N,
+                                    int64_t K, int64_t E, const mxq_linear_spec* spec);
 int mxq_expert_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias, void* y, int64_t n,
                       int64_t N, int64_t K, int64_t E, const int32_t* order, const int32_t* offsets,
                       const mxq_linear_spec* spec, void* workspace, mxq_stream_t stream);

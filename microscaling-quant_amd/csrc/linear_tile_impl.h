@@ -18,40 +18,38 @@ namespace mxq {
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
-// Global memory straight into LDS, 16 or 4 bytes (or one byte, as a word) a lane, lane i's at base + 16 i or 4 i.  Written as
+// Global memory straight into LDS, 16 or 4 bytes a lane, lane i's at base + 16 i or 4 i.  Written as
 // assembly because the compiler would wait for all such loads before every LDS read; the waits are wait_stage's.
 __device__ __forceinline__ void dma16(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
-}
-__device__ __forceinline__ void dma1(uint32_t base, const void* p) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(base), "v"(p) : "memory");
 }
 
 __device__ __forceinline__ void dma4(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
 }
 
-// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; DIRECT: codes by DMA (K a multiple of 128, rows of codes
-// 16-byte and of scales 4-byte aligned), through registers otherwise.
-template <int FAM, int BM, int BN, int WM, int WN, bool DIRECT>
+// What a chunk past the last column is loaded from.
+static __device__ const u32x4 kNothing = {0, 0, 0, 0};
+
+// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; STAGES of 64 columns in LDS.
+template <int FAM, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k_linear_tile(TileArgs ta) {
   constexpr int WAVES_N = BN / (32 * WN), WAVES = BM / (32 * WM) * WAVES_N, THREADS = 64 * WAVES;
   constexpr int WB = 2 * kBlockBytes<FAM>, CH = WB / 16;                 // a weight row's bytes and chunks of one stage
-  constexpr int XL = BM * 8 / THREADS, WL = BN * CH / THREADS, SL = BN * 2 / THREADS;   // loads a thread and stage
-  constexpr int SC = BN * 4 / THREADS;                                   // DIRECT: loads of scales a thread and eight steps
+  constexpr int XL = BM * 8 / THREADS, WL = BN * CH / THREADS;   // loads a thread and stage
+  constexpr int SC = BN * 4 / THREADS;                                   // loads of scales a thread and eight steps
   static_assert(WN == 2, "a wave's two tiles are neighbours, or G's and U's of the same outputs");
-  static_assert(XL >= 1 && WL >= 1 && SL >= 1 && BM * 8 % THREADS == 0, "whole loads");
+  static_assert(XL >= 2 && WL >= 1 && SC >= 1 && BM * 8 % THREADS == 0, "whole loads");
   struct Stage {
     uint8_t x[BM * 128];
     uint8_t w[BN * WB];
   };
-  // DIRECT: rings of two times eight steps' scale bytes; otherwise of three steps', a word each
-  constexpr int kScales = DIRECT ? 2 * BN * 16 : 3 * BN * 8;
+  constexpr int kScales = 2 * BN * 16;                                   // a ring of two times eight steps' scale bytes
   constexpr int PITCH = 32 * WN + 4;
-  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = 3 * sizeof(Stage) + kScales;
+  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = STAGES * sizeof(Stage) + kScales;
   __shared__ __attribute__((aligned(16))) uint8_t memory[kStages > kEpilogue ? kStages : kEpilogue];
   Stage* stage = (Stage*)memory;
-  uint8_t* scale_ring = memory + 3 * sizeof(Stage);
+  uint8_t* scale_ring = memory + STAGES * sizeof(Stage);
 
   const LinearArgs& a = ta.l;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -93,84 +91,52 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
   const int first = (int)blockIdx.y * per, last = first + per < all ? first + per : all;
 
   if (!t.zeros && first < last) {
-    const uint8_t *xp[XL], *wp[WL], *sp[DIRECT ? SC : SL];
+    const uint8_t *xp[XL], *wp[WL], *sp[SC];
     const uint8_t* codes = a.codes + t.expert * a.sp.batch_codes;
     const uint8_t* scales = a.scales + t.expert * a.sp.batch_scales;
+    const int xc = (tid & 7) ^ (tid >> 4 & 7);                           // this thread's chunk of a row, the same in all its rows
+    const int wc = (tid % CH) ^ (CH == 4 ? tid >> 4 & 3 : tid >> 4 & 1);
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-      const int q = i * THREADS + tid, row = q >> 3, c = (q & 7) ^ (row >> 1 & 7);
-      xp[i] = (const uint8_t*)(ta.x + x_row(a, t.row0 + (row < t.rows ? row : t.rows - 1)) * ta.ld_x) + c * 16;
-    }
-    int wc = 0;
-#pragma unroll
-    for (int i = 0; i < WL; ++i) {
-      const int q = i * THREADS + tid, row = q / CH;
-      wc = (q % CH) ^ (CH == 4 ? row >> 2 & 3 : row >> 3 & 1);
-      wp[i] = codes + weight_row(row) * a.sp.ld_codes + wc * 16;
+      const int row = (i * THREADS + tid) >> 3;
+      xp[i] = (const uint8_t*)(ta.x + x_row(a, t.row0 + (row < t.rows ? row : t.rows - 1)) * ta.ld_x) + xc * 16;
     }
 #pragma unroll
-    for (int i = 0; i < (DIRECT ? SC : SL); ++i) {
-      const int q = i * THREADS + tid;
-      sp[i] = scales + weight_row(DIRECT ? q >> 2 : q >> 1) * a.sp.ld_scales;
-    }
-    const int blocks = (int)((a.K + 31) >> 5);
-    u32x4 held[DIRECT ? 1 : WL];
+    for (int i = 0; i < WL; ++i) wp[i] = codes + weight_row((i * THREADS + tid) / CH) * a.sp.ld_codes + wc * 16;
+#pragma unroll
+    for (int i = 0; i < SC; ++i) sp[i] = scales + weight_row((i * THREADS + tid) >> 2) * a.sp.ld_scales;
 
     // A third of the next step's loads into stage b, in the order codes and scales, x, x: loads of a step issued at once
     // would keep the wave from its multiplications while the memory pipeline takes them.  The last step again after it, so
     // that every step waits for as many loads.
     int st = first, k = first % ta.steps;
     auto issue = [&](int b, int part) {
+      const uint8_t* nothing = (const uint8_t*)&kNothing;
       if (part == 1 || part == 2) {
         const uint32_t xo = lds_offset(stage[b].x) + wave * 1024;
+        const bool past = k * 64 + xc * 8 >= ta.x_columns;
 #pragma unroll
-        for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) dma16(xo + i * THREADS * 16, xp[i] + (int64_t)st * 128);
+        for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) dma16(xo + i * THREADS * 16, past ? nothing : xp[i] + (int64_t)st * 128);
         return;
       }
-      if constexpr (DIRECT) {
-        const int chunk = st - first;
-        if ((chunk & 7) == 0) {
-          const uint32_t so = lds_offset(scale_ring) + (chunk >> 3 & 1) * BN * 16 + wave * 256;
-          const int two = (k + 2 * (tid & 3)) % ta.steps;
+      const int chunk = st - first;
+      if ((chunk & 7) == 0) {
+        const uint32_t so = lds_offset(scale_ring) + (chunk >> 3 & 1) * BN * 16 + wave * 256;
+        const int two = (k + 2 * (tid & 3)) % ta.steps;
 #pragma unroll
-          for (int i = 0; i < SC; ++i) dma4(so + i * THREADS * 4, sp[i] + two * 2);
-        }
-        const uint32_t wo = lds_offset(stage[b].w) + wave * 1024;
-#pragma unroll
-        for (int i = 0; i < WL; ++i) dma16(wo + i * THREADS * 16, wp[i] + (int64_t)k * WB);
-      } else {
-        const uint32_t so = lds_offset(scale_ring) + b * BN * 8 + wave * 256;
-#pragma unroll
-        for (int i = 0; i < SL; ++i) {
-          const int block = 2 * k + (tid & 1);
-          dma1(so + i * THREADS * 4, sp[i] + (block < blocks ? block : blocks - 1));
-        }
-        const int64_t left = a.K - (int64_t)k * 64 - wc * (FAM == kPairs ? 32 : 16);      // codes from this chunk on
-#pragma unroll
-        for (int i = 0; i < WL; ++i) {
-          const uint8_t* p = wp[i] + (int64_t)k * WB;
-          if (left >= (FAM == kPairs ? 32 : 16)) {
-            held[i] = *(const u32x4_any*)p;
-          } else {
-            const int valid = left < 0 ? 0 : (int)left;
-            held[i] = load_part(p, FAM == kPairs ? (valid + 1) / 2 : valid);
-            if (FAM == kPairs && (valid & 1)) clear_odd(held[i], valid);
-          }
-        }
+        for (int i = 0; i < SC; ++i) dma4(so + i * THREADS * 4, sp[i] + two * 2);
       }
+      const uint32_t wo = lds_offset(stage[b].w) + wave * 1024;
+      const bool past = k * 64 + wc * (FAM == kPairs ? 32 : 16) >= ta.w_columns;
+#pragma unroll
+      for (int i = 0; i < WL; ++i) dma16(wo + i * THREADS * 16, past ? nothing : wp[i] + (int64_t)k * WB);
     };
     auto advance = [&]() {
       if (st + 1 < last) ++st, k = k + 1 == ta.steps ? 0 : k + 1;
     };
-    auto put = [&](int b) {
-      if constexpr (!DIRECT) {
-#pragma unroll
-        for (int i = 0; i < WL; ++i) *(u32x4*)&stage[b].w[(i * THREADS + tid) * 16] = held[i];
-      }
-    };
-    // one stage's loads, without the scales that come before them every eighth time: the waits below then ask for a little
+    // the later stages' loads, without the scales that come before them every eighth time: the waits below then ask for a little
     // more than they need
-    constexpr int kInFlight = XL + WL;
+    constexpr int kInFlight = (STAGES - 2) * (XL + WL);
     // A step is four phases of eight columns a lane.  A phase reads and converts the next one's operands while its own are
     // multiplied; the last phase of a step first waits for the next stage, whose loads began two steps ago, and hands its
     // own buffer to the stage after the one in flight.
@@ -195,8 +161,7 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
           for (int c = 0; c < kWords<FAM>; ++c) code[i][c] = without_infinities(code[i][c], drop);
         }
         const int since = st - first;
-        const uint8_t* at = DIRECT ? scale_ring + (since >> 3 & 1) * BN * 16 + row * 16 + (since & 7) * 2 + h
-                                   : scale_ring + b * BN * 8 + (row * 2 + h) * 4;
+        const uint8_t* at = scale_ring + (since >> 3 & 1) * BN * 16 + row * 16 + (since & 7) * 2 + h;
         scale[i] = scale_of<FAM>(*at, ta.map, left[i]);
       }
     };
@@ -223,22 +188,21 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
     };
 
 #pragma unroll
-    for (int s = 0; s < 3; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
 #pragma unroll
       for (int p = 0; p < 3; ++p)
-        if (s < 2 || p == 0) issue(s, p);
-      if (s < 2) put(s), advance();
+        if (s < STAGES - 1 || p == 0) issue(s, p);
+      if (s < STAGES - 1) advance();
     }
-    if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + WL) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + WL) : "memory");
     asm volatile("s_barrier" ::: "memory");
     read_w(0, first);
     read_x(stage[0], 0);
     convert(0);
     int b = 0;
     for (int now = first; now < last; ++now) {
-      const int nb = b == 2 ? 0 : b + 1;
-      const int pb = nb == 2 ? 0 : nb + 1;                               // the stage whose loads are being issued
+      const int nb = b == STAGES - 1 ? 0 : b + 1;
+      const int pb = b == 0 ? STAGES - 1 : b - 1;                             // the stage whose loads are being issued
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
         read_x(stage[b], j + 1);
@@ -247,9 +211,7 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
         multiply(j);
         convert(j + 1);
       }
-      put(pb);
-      if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
       asm volatile("s_barrier" ::: "memory");
       advance();
       read_w(nb, now + 1);                                        // after the last step: a stage that no sum takes
@@ -343,15 +305,10 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
 
 template <int FAM> void launch_tile_family(const TileArgs& ta, const TilePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)(ta.tiles_m * ta.tiles_n), (unsigned)p.split);
-  auto go = [&](auto direct) {
-    constexpr bool D = decltype(direct)::value;
-    KernelTimer timer("k_linear_tile", st);
-    if (p.shape == 0) k_linear_tile<FAM, 256, 256, 4, 2, D><<<grid, 512, 0, st>>>(ta);
-    else if (p.shape == 1) k_linear_tile<FAM, 128, 128, 2, 2, D><<<grid, 256, 0, st>>>(ta);
-    else k_linear_tile<FAM, 64, 128, 1, 2, D><<<grid, 256, 0, st>>>(ta);
-  };
-  if (p.direct) go(std::true_type());
-  else go(std::false_type());
+  KernelTimer timer("k_linear_tile", st);
+  if (p.shape == 0) k_linear_tile<FAM, 256, 256, 4, 2, 3><<<grid, 512, 0, st>>>(ta);
+  else if (p.shape == 1) k_linear_tile<FAM, 128, 128, 2, 2, 3><<<grid, 256, 0, st>>>(ta);
+  else k_linear_tile<FAM, 64, 128, 1, 2, 3><<<grid, 256, 0, st>>>(ta);
 }
 
 }  // namespace mxq

@@ -17,33 +17,68 @@ void launch_tile_pairs(const TileArgs&, const TilePlan&, hipStream_t);
 
 namespace {
 
-// x's rows as bfloat16 planes of kp = 64 steps values, one after another along a row, zeros past K: each plane the leading
-// bits of what the ones before leave, so that their sum is the value.
-__global__ __launch_bounds__(256) void k_planes(const void* x, int dtype, int64_t ld, int64_t rows, int64_t K, int64_t kp, int planes,
-                                                uint16_t* out) {
-  const int64_t groups = kp / 8;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * groups; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / groups, k = i % groups * 8;
-    float v[8];
+// What k_linear_tile's direct loads cannot take as it lies is laid out first, by one launch.
+//   x: bfloat16 planes of kp values, one after another along a row, zeros past K: each plane the leading bits of what the
+//      ones before leave, so that their sum is the value.  Eight values a thread.
+//   codes: rows of whole 128 columns, zeros past K.  16 bytes a thread.
+//   scales: rows of whole words.  Four bytes a thread.
+// Experts without rows are left out.
+struct PrepareArgs {
+  LinearArgs l;
+  int64_t kp, x_rows, w_rows;          // columns a plane, rows of x, rows of one weight
+  int32_t planes;
+  int64_t x_items, code_items, items;  // threads of x, of x and codes, of all
+  uint16_t* x;
+  uint8_t *codes, *scales;
+};
+__global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
+  const LinearArgs& a = p.l;
+  const bool pairs = a.sp.format == MXQ_FMT_E2M1_PAIRS;
+  auto used = [&](int64_t e) { return !a.offsets || a.offsets[e + 1] > a.offsets[e]; };
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.items; i += (int64_t)gridDim.x * 256) {
+    if (i < p.x_items) {
+      const int64_t groups = p.kp / 8, row = i / groups, k = (i - row * groups) * 8;
+      float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (k + 8 <= K) {
-      add_eight(v, x, dtype, row * ld + k);
-    } else {
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      if (k + 8 <= a.K) {
+        add_eight(v, a.x, a.sp.x_dtype, row * a.sp.ld_x + k);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k + e < K) v[e] = load_elem(x, dtype, row * ld + k + e);
-    }
-    for (int p = 0; p < planes; ++p) {
-      u32x4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_perm(__float_as_uint(v[2 * e + 1]), __float_as_uint(v[2 * e]), 0x07060302u);
-      *(u32x4*)(out + (row * planes + p) * kp + k) = w;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float hi = __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
-        v[e] = v[e] == hi ? 0.0f : v[e] - hi;                            // infinities leave nothing
+        for (int e = 0; e < 8; ++e)
+          if (k + e < a.K) v[e] = load_elem(a.x, a.sp.x_dtype, row * a.sp.ld_x + k + e);
       }
+      for (int q = 0; q < p.planes; ++q) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_perm(__float_as_uint(v[2 * e + 1]), __float_as_uint(v[2 * e]), 0x07060302u);
+        *(u32x4*)(p.x + (row * p.planes + q) * p.kp + k) = w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float hi = __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+          v[e] = v[e] == hi ? 0.0f : v[e] - hi;                          // infinities leave nothing
+        }
+      }
+    } else if (i < p.code_items) {
+      const int64_t bytes = pairs ? p.kp / 2 : p.kp, chunks = bytes / 16, all = (i - p.x_items) / chunks, e = all / p.w_rows;
+      if (!used(e)) continue;
+      const int64_t at = (i - p.x_items - all * chunks) * 16, have = pairs ? (a.K + 1) / 2 : a.K, left = have - at;
+      const uint8_t* from = a.codes + e * a.sp.batch_codes + (all - e * p.w_rows) * a.sp.ld_codes + at;
+      u32x4 v;
+      if (left >= 16) v = *(const u32x4_any*)from;
+      else v = load_part(from, left < 0 ? 0 : (int)left);
+      if (pairs && (a.K & 1) && left > 0 && left <= 16) clear_odd(v, (int)left * 2 - 1);
+      *(u32x4*)(p.codes + all * bytes + at) = v;
+    } else {
+      const int64_t words = p.kp / 128, all = (i - p.code_items) / words, e = all / p.w_rows;
+      if (!used(e)) continue;
+      const int64_t at = (i - p.code_items - all * words) * 4, left = (a.K + 31) / 32 - at;
+      const uint8_t* from = a.scales + e * a.sp.batch_scales + (all - e * p.w_rows) * a.sp.ld_scales + at;
+      uint32_t v = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (b < left) v |= (uint32_t)from[b] << 8 * b;
+      *(uint32_t*)(p.scales + (all * words) * 4 + at) = v;
     }
   }
 }
@@ -99,24 +134,30 @@ struct Plan {
   TilePlan tile;
   int64_t tiles_m, tiles_n;    // of either
   int steps, planes;
-  bool convert;                // x goes through k_planes
-  int64_t plane_bytes, bytes;  // workspace: the planes, everything
+  bool lay_x, lay_codes, lay_scales;                  // what goes through k_prepare
+  int64_t x_rows, w_rows;
+  int64_t at_codes, at_scales, at_partial, bytes;     // workspace: x, codes, scales, partial sums
 };
 
 constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128};
 
-// E = 0: one matrix.
-Plan plan_of(const void* x, int64_t M, int64_t N, int64_t K, int64_t E, const mxq_linear_spec& sp) {
+// a.E = 0: one matrix.
+Plan plan_of(const LinearArgs& a) {
+  const mxq_linear_spec& sp = a.sp;
+  const int64_t M = a.M, N = a.N, K = a.K, E = a.E;
   Plan p{};
   const int64_t each = E ? ceil_div(M, E) : M, width = sp.gated ? 2 * N : N;
   auto row_tiles = [&](int64_t bm) { return E ? M / bm + (M < E + 1 ? M : E + 1) : ceil_div(M, bm); };
-  if (each <= 64) {
-    const int most = sp.x_dtype == MXQ_DT_F32 ? 2 : 4;
-    p.mt = each <= 16 ? 1 : each <= 32 || most == 2 ? 2 : 4;
+  const bool pairs = sp.format == MXQ_FMT_E2M1_PAIRS;
+  p.lay_codes = K % (pairs ? 32 : 16) || (uintptr_t)a.codes % 16 || sp.ld_codes % 16 || sp.batch_codes % 16;
+  p.lay_scales = K % 128 || (uintptr_t)a.scales % 4 || sp.ld_scales % 4 || sp.batch_scales % 4;
+  // by the sizes alone: strides and addresses do not change a result's bits
+  if (each <= 16) {
+    p.mt = 1;
     p.tiles_m = row_tiles(16 * p.mt);
     return p;
   }
-  p.steps = (int)ceil_div(K, 64);
+  p.steps = (int)(2 * ceil_div(K, 128));
   p.planes = sp.x_dtype == MXQ_DT_BF16 ? 1 : sp.x_dtype == MXQ_DT_F16 ? 2 : 3;
   auto tiles = [&](int s) { return ceil_div(each, kTileM[s]) * (E ? E : 1) * ceil_div(width, kTileN[s]); };
   p.tile.shape = tiles(0) >= 192 && each > 128 ? 0 : tiles(1) >= 128 && each > 64 ? 1 : 2;
@@ -125,17 +166,22 @@ Plan plan_of(const void* x, int64_t M, int64_t N, int64_t K, int64_t E, const mx
   p.tile.split = 1;
   if (!E) {
     const int64_t have = p.tiles_m * p.tiles_n, all = (int64_t)p.steps * p.planes;
-    while (p.tile.split < 8 && have * p.tile.split * 2 <= 512 && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
+    while (p.tile.split < 8 && have * p.tile.split * 2 <= 320 && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
   }
-  p.convert = sp.x_dtype != MXQ_DT_BF16 || K % 64 || sp.ld_x % 8 || (uintptr_t)x % 16;
-  const int64_t rows = E && sp.top_k ? ceil_div(M, sp.top_k) : M;
-  if (p.convert) p.plane_bytes = ceil_div(rows * p.planes * p.steps * 128, 256) * 256;
-  p.bytes = p.plane_bytes + (p.tile.split > 1 ? p.tile.split * M * width * 4 : 0);
+  p.lay_x = sp.x_dtype != MXQ_DT_BF16 || K % 8 || sp.ld_x % 8 || (uintptr_t)a.x % 16;
+  p.x_rows = E && sp.top_k ? ceil_div(M, sp.top_k) : M;
+  p.w_rows = width;
+  auto whole = [](int64_t bytes) { return ceil_div(bytes, 256) * 256; };
+  const int64_t kp = (int64_t)p.steps * 64, matrices = (E ? E : 1) * width;
+  p.at_codes = p.lay_x ? whole(p.x_rows * p.planes * kp * 2) : 0;
+  p.at_scales = p.at_codes + (p.lay_codes ? whole(matrices * (pairs ? kp / 2 : kp)) : 0);
+  p.at_partial = p.at_scales + (p.lay_scales ? whole(matrices * (kp / 32)) : 0);
+  p.bytes = p.at_partial + (p.tile.split > 1 ? p.tile.split * M * width * 4 : 0);
   return p;
 }
 
 int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st) {
-  const Plan p = plan_of(a.x, a.M, a.N, a.K, a.E, a.sp);
+  const Plan p = plan_of(a);
   if (p.bytes && !workspace) return invalid(std::string(who) + ": NULL workspace");
   const int fam = family(a.sp.format);
   if (p.mt) {
@@ -144,27 +190,31 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
     return check_launch(who);
   }
   if (p.tiles_m * p.tiles_n > 0x7fffffff) return invalid(std::string(who) + ": too many outputs");
-  TileArgs t{a, (const uint16_t*)a.x, a.sp.ld_x, p.steps, p.planes, (int32_t)p.tiles_m, (int32_t)p.tiles_n, p.tile.split,
-             (float*)((uint8_t*)workspace + p.plane_bytes), code_map(a.sp.format)};
-  if (p.convert) {
-    const int64_t kp = (int64_t)p.steps * 64, rows = a.E && a.sp.top_k ? ceil_div(a.M, a.sp.top_k) : a.M;
-    if (kp) {
-      KernelTimer timer("k_planes", st);
-      const int64_t blocks = ceil_div(rows * kp / 8, 256);
-      k_planes<<<dim3((unsigned)(blocks < 16384 ? blocks : 16384)), 256, 0, st>>>(a.x, a.sp.x_dtype, a.sp.ld_x, rows, a.K, kp, p.planes,
-                                                                               (uint16_t*)workspace);
+  uint8_t* work = (uint8_t*)workspace;
+  const bool pairs = fam == kPairs;
+  const int64_t kp = (int64_t)p.steps * 64, matrices = (a.E ? a.E : 1) * p.w_rows;
+  TileArgs t{a, (const uint16_t*)a.x, a.sp.ld_x, p.steps, p.planes, (int32_t)a.K, (int32_t)a.K, (int32_t)p.tiles_m, (int32_t)p.tiles_n,
+             p.tile.split, (float*)(work + p.at_partial), code_map(a.sp.format)};
+  if (kp && (p.lay_x || p.lay_codes || p.lay_scales)) {
+    PrepareArgs q{a, kp, p.x_rows, p.w_rows, p.planes, 0, 0, 0, (uint16_t*)work, work + p.at_codes, work + p.at_scales};
+    q.x_items = p.lay_x ? p.x_rows * (kp / 8) : 0;
+    q.code_items = q.x_items + (p.lay_codes ? matrices * (kp / (pairs ? 32 : 16)) : 0);
+    q.items = q.code_items + (p.lay_scales ? matrices * (kp / 128) : 0);
+    const int64_t blocks = ceil_div(q.items, 256);
+    KernelTimer timer("k_prepare", st);
+    k_prepare<<<dim3((unsigned)(blocks < 32768 ? blocks : 32768)), 256, 0, st>>>(q);
+    if (p.lay_x) t.x = q.x, t.ld_x = kp * p.planes, t.x_columns = (int32_t)kp;
+    if (p.lay_codes) {
+      t.l.codes = q.codes, t.l.sp.ld_codes = pairs ? kp / 2 : kp, t.l.sp.batch_codes = t.l.sp.ld_codes * p.w_rows;
+      t.w_columns = (int32_t)kp;
     }
-    t.x = (const uint16_t*)workspace;
-    t.ld_x = kp * p.planes;
+    if (p.lay_scales) t.l.scales = q.scales, t.l.sp.ld_scales = kp / 32, t.l.sp.batch_scales = kp / 32 * p.w_rows;
   }
-  TilePlan tp = p.tile;
-  tp.direct = a.K % 128 == 0 && (uintptr_t)a.codes % 16 == 0 && a.sp.ld_codes % 16 == 0 && a.sp.batch_codes % 16 == 0 &&
-              (uintptr_t)a.scales % 4 == 0 && a.sp.ld_scales % 4 == 0 && a.sp.batch_scales % 4 == 0;
-  (fam == kE4M3 ? launch_tile_e4m3 : fam == kE5M2 ? launch_tile_e5m2 : fam == kPairs ? launch_tile_pairs : launch_tile_mapped)(t, tp, st);
-  if (tp.split > 1) {
+  (fam == kE4M3 ? launch_tile_e4m3 : fam == kE5M2 ? launch_tile_e5m2 : fam == kPairs ? launch_tile_pairs : launch_tile_mapped)(t, p.tile, st);
+  if (p.tile.split > 1) {
     KernelTimer timer("k_linear_finish", st);
     const int64_t blocks = ceil_div(a.M * ceil_div(a.N, 8), 256);
-    k_linear_finish<<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), 256, 0, st>>>(a, t.partial, tp.split);
+    k_linear_finish<<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), 256, 0, st>>>(a, t.partial, p.tile.split);
   }
   return check_launch(who);
 }
@@ -174,11 +224,15 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
 
 using namespace mxq;
 
-extern "C" int64_t mxq_packed_linear_workspace(const void* x, int64_t M, int64_t N, int64_t K, const mxq_linear_spec* spec) {
-  return check_spec("mxq_packed_linear_workspace", M, N, K, spec) || !M || !N ? 0 : plan_of(x, M, N, K, 0, *spec).bytes;
+extern "C" int64_t mxq_packed_linear_workspace(const void* x, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t N,
+                                               int64_t K, const mxq_linear_spec* spec) {
+  if (check_spec("mxq_packed_linear_workspace", M, N, K, spec) || !M || !N) return 0;
+  return plan_of(LinearArgs{x, codes, scales, nullptr, nullptr, nullptr, nullptr, nullptr, M, N, K, 0, *spec}).bytes;
 }
-extern "C" int64_t mxq_expert_linear_workspace(const void* x, int64_t n, int64_t N, int64_t K, int64_t E, const mxq_linear_spec* spec) {
-  return check_spec("mxq_expert_linear_workspace", n, N, K, spec) || !n || !N || E < 1 || E > 1024 ? 0 : plan_of(x, n, N, K, E, *spec).bytes;
+extern "C" int64_t mxq_expert_linear_workspace(const void* x, const uint8_t* codes, const uint8_t* scales, int64_t n, int64_t N,
+                                               int64_t K, int64_t E, const mxq_linear_spec* spec) {
+  if (check_spec("mxq_expert_linear_workspace", n, N, K, spec) || !n || !N || E < 1 || E > 1024) return 0;
+  return plan_of(LinearArgs{x, codes, scales, nullptr, nullptr, nullptr, nullptr, nullptr, n, N, K, (int32_t)E, *spec}).bytes;
 }
 
 extern "C" int mxq_packed_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias,

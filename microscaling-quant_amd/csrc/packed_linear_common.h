@@ -166,9 +166,10 @@ template <int FAM> __device__ __forceinline__ bf16x8 eight(const uint32_t (&w)[k
 // The arguments of k_linear_tile.
 struct TileArgs {
   LinearArgs l;
-  const uint16_t* x;      // bfloat16, rows of ld_x, every one a whole number of 64s in each plane, 16-byte aligned
+  const uint16_t* x;      // bfloat16 planes one after another along a row, rows of ld_x, 16-byte aligned
   int64_t ld_x;
-  int32_t steps, planes;  // 64 columns a step, steps a plane
+  int32_t steps, planes;  // 64 columns a step, an even number of steps a plane
+  int32_t x_columns, w_columns;   // that exist in a plane of x and in a row of codes; the others are zeros
   int32_t tiles_m, tiles_n, split;
   float* partial;         // split > 1: split x M x rows of the weight
   CodeMap map;
@@ -177,7 +178,6 @@ struct TileArgs {
 struct TilePlan {
   int shape;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128
   int split;
-  bool direct;
 };
 
 // E5M2's codes, the infinities' bits under `drop` cleared.

@@ -167,10 +167,10 @@ SIGNATURES = {
     "mxq_dispatch": (c_i32, [c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr]),
     "mxq_combine": (c_i32, [c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr]),
     "mxq_combine_grad": (c_i32, [c_ptr, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr]),
-    "mxq_packed_linear_workspace": (c_i64, [c_ptr, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
+    "mxq_packed_linear_workspace": (c_i64, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
     "mxq_packed_linear": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64,
                                   ctypes.POINTER(LinearSpec), c_ptr, c_ptr]),
-    "mxq_expert_linear_workspace": (c_i64, [c_ptr, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
+    "mxq_expert_linear_workspace": (c_i64, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
     "mxq_expert_linear": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr,
                                   ctypes.POINTER(LinearSpec), c_ptr, c_ptr]),
 }

@@ -123,7 +123,7 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
     spec = _spec(xd, bd, rd, y, cd, sd, code, activation, gated)
     with _lib.on(dev):
-        work = _workspace("mxq_packed_linear_workspace", dev, _lib.ptr(xd), M, N, K, spec)
+        work = _workspace("mxq_packed_linear_workspace", dev, _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), M, N, K, spec)
         _lib.run("mxq_packed_linear", _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), _lib.ptr(bd), _lib.ptr(rd),
                  _lib.ptr(y), M, N, K, spec, _lib.ptr(work), _lib.stream(dev))
     return _lib.back(y.reshape(shape), x)
@@ -157,7 +157,7 @@ def expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
     y = torch.empty((n, N), dtype=out_dtype, device=dev)
     spec = _spec(xd, bd, None, y, cd, sd, code, activation, gated, 0 if sorted_rows else k)
     with _lib.on(dev):
-        work = _workspace("mxq_expert_linear_workspace", dev, _lib.ptr(xd), n, N, K, E, spec)
+        work = _workspace("mxq_expert_linear_workspace", dev, _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), n, N, K, E, spec)
         _lib.run("mxq_expert_linear", _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), _lib.ptr(bd), _lib.ptr(y), n, N, K, E,
                  _lib.ptr(order), _lib.ptr(offsets), spec, _lib.ptr(work), _lib.stream(dev))
     return _lib.back(y, x)
