@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
   };
   constexpr int kScales = 2 * BN * 16;                                   // a ring of two times eight steps' scale bytes
   constexpr int PITCH = 32 * WN + 4;
-  constexpr size_t kEpilogue = (size_t)WAVES * 32 * PITCH * 4, kStages = STAGES * sizeof(Stage) + kScales;
+  constexpr int kHeld = WM < 2 ? WM : 2;                                 // 32-row pieces of a wave's sums in LDS at a time
+  constexpr size_t kEpilogue = (size_t)WAVES * kHeld * 32 * PITCH * 4, kStages = STAGES * sizeof(Stage) + kScales;
   __shared__ __attribute__((aligned(16))) uint8_t memory[kStages > kEpilogue ? kStages : kEpilogue];
   Stage* stage = (Stage*)memory;
   uint8_t* scale_ring = memory + STAGES * sizeof(Stage);
@@ -137,169 +138,229 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
     // the later stages' loads, without the scales that come before them every eighth time: the waits below then ask for a little
     // more than they need
     constexpr int kInFlight = (STAGES - 2) * (XL + WL);
-    // A step is four phases of eight columns a lane.  A phase reads and converts the next one's operands while its own are
-    // multiplied; the last phase of a step first waits for the next stage, whose loads began two steps ago, and hands its
-    // own buffer to the stage after the one in flight.
-    uint32_t code[WN][kWords<FAM>];
-    float scale[WN];
-    uint32_t left[WN];
-    bf16x8 wv[2][WN], xv[2][WM];
-    auto read_w = [&](int b, int st) {
-      const Stage& s = stage[b];
+    auto read_codes = [&](int b, int st, uint32_t (&code)[WN][kWords<FAM>], float (&scale)[WN], uint32_t (&left)[WN]) {
 #pragma unroll
       for (int i = 0; i < WN; ++i) {
-        const int row = (wn * WN + i) * 32 + r;
+        const int row = (wn * WN + i) * 32 + r, since = st - first;
 #pragma unroll
         for (int c = 0; c < kWords<FAM> / 4; ++c) {
           const int chunk = h * (CH / 2) + c;
-          const u32x4 v = *(const u32x4*)&s.w[row * WB + (chunk ^ (CH == 4 ? row >> 2 & 3 : row >> 3 & 1)) * 16];
+          const u32x4 v = *(const u32x4*)&stage[b].w[row * WB + (chunk ^ (CH == 4 ? row >> 2 & 3 : row >> 3 & 1)) * 16];
           __builtin_memcpy(&code[i][4 * c], &v, 16);
         }
-        if constexpr (FAM == kE5M2Wide) {
-          const uint32_t drop = st >= ta.steps ? ~0u : 0u;
-#pragma unroll
-          for (int c = 0; c < kWords<FAM>; ++c) code[i][c] = without_infinities(code[i][c], drop);
-        }
-        const int since = st - first;
         const uint8_t* at = scale_ring + (since >> 3 & 1) * BN * 16 + row * 16 + (since & 7) * 2 + h;
         scale[i] = scale_of<FAM>(*at, ta.map, left[i]);
       }
     };
-    auto read_x = [&](const Stage& s, int j) {
+    auto drop_infinities = [&](int st, uint32_t (&code)[WN][kWords<FAM>]) {
+      if constexpr (FAM == kE5M2Wide) {
+        const uint32_t drop = st >= ta.steps ? ~0u : 0u;
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+#pragma unroll
+          for (int c = 0; c < kWords<FAM>; ++c) code[i][c] = without_infinities(code[i][c], drop);
+      }
+    };
+    auto read_x = [&](int b, int j, bf16x8 (&x)[WM]) {
 #pragma unroll
       for (int m = 0; m < WM; ++m) {
         const int row = (wm * WM + m) * 32 + r;
-        xv[j & 1][m] = *(const bf16x8*)&s.x[row * 128 + ((h * 4 + j) ^ (row >> 1 & 7)) * 16];
+        x[m] = *(const bf16x8*)&stage[b].x[row * 128 + ((h * 4 + j) ^ (row >> 1 & 7)) * 16];
       }
     };
-    auto convert = [&](int j) {
+    auto convert = [&](const uint32_t (&code)[WN][kWords<FAM>], const float (&scale)[WN], const uint32_t (&left)[WN], int j, bf16x8 (&w)[WN]) {
+      uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < WN; ++i) wv[j & 1][i] = eight<FAM>(code[i], scale[i], j, ta.map);
-      if (FAM == kMapped && __builtin_expect(__any(left[0] | left[1]), 0)) {
+      for (int i = 0; i < WN; ++i) w[i] = eight<FAM>(code[i], scale[i], j, ta.map), any |= left[i];
+      if (FAM == kMapped && __builtin_expect(__any(any), 0)) {
 #pragma unroll
-        for (int i = 0; i < WN; ++i) apply_left(wv[j & 1][i], left[i]);
+        for (int i = 0; i < WN; ++i) apply_left(w[i], left[i]);
       }
     };
-    auto multiply = [&](int j) {
+    auto multiply = [&](const bf16x8 (&w)[WN], const bf16x8 (&x)[WM]) {
 #pragma unroll
       for (int i = 0; i < WN; ++i)
 #pragma unroll
-        for (int m = 0; m < WM; ++m) acc[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[j & 1][i], xv[j & 1][m], acc[i][m], 0, 0, 0);
+        for (int m = 0; m < WM; ++m) acc[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[i], x[m], acc[i][m], 0, 0, 0);
     };
+    auto next = [](int b) { return b == STAGES - 1 ? 0 : b + 1; };
 
+    if constexpr (WM <= 2) {
+      // Few rows: a step's operands are all read a step ahead, one wait for LDS a step, since a phase of the larger tile's
+      // walk would hold too few products to hide it.
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s) {
+      for (int s = 0; s < STAGES; ++s) {
+        if (s) advance();
 #pragma unroll
-      for (int p = 0; p < 3; ++p)
-        if (s < STAGES - 1 || p == 0) issue(s, p);
-      if (s < STAGES - 1) advance();
-    }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + WL) : "memory");
-    asm volatile("s_barrier" ::: "memory");
-    read_w(0, first);
-    read_x(stage[0], 0);
-    convert(0);
-    int b = 0;
-    for (int now = first; now < last; ++now) {
-      const int nb = b == STAGES - 1 ? 0 : b + 1;
-      const int pb = b == 0 ? STAGES - 1 : b - 1;                             // the stage whose loads are being issued
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        read_x(stage[b], j + 1);
-        __builtin_amdgcn_sched_barrier(0);                               // the compiler would sink the reads to their uses
-        if (j < 2) issue(pb, j + 1);
-        multiply(j);
-        convert(j + 1);
+        for (int p = 0; p < 3; ++p) issue(s, p);
       }
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + XL + WL) : "memory");
       asm volatile("s_barrier" ::: "memory");
-      advance();
-      read_w(nb, now + 1);                                        // after the last step: a stage that no sum takes
-      read_x(stage[nb], 0);
-      __builtin_amdgcn_sched_barrier(0);
-      issue(b, 0);
-      multiply(3);
-      convert(0);
-      b = nb;
+      uint32_t code[2][WN][kWords<FAM>], left[2][WN];
+      float scale[2][WN];
+      bf16x8 xv[2][4][WM];
+      auto read = [&](int b, int st, int turn) {
+        read_codes(b, st, code[turn], scale[turn], left[turn]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) read_x(b, j, xv[turn][j]);
+      };
+      int b = 0;
+      read(0, first, 0);
+      for (int now = first; now < last; now += 2) {                      // an even number of steps
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+          asm volatile("s_barrier" ::: "memory");
+          advance();
+#pragma unroll
+          for (int p = 0; p < 3; ++p) issue(b, p);
+          b = next(b);
+          read(b, now + turn + 1, 1 - turn);                             // after the last step: what no sum takes
+          __builtin_amdgcn_sched_barrier(0);                             // the compiler would sink the reads to their uses
+          drop_infinities(now + turn, code[turn]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            bf16x8 w[WN];
+            convert(code[turn], scale[turn], left[turn], j, w);
+            multiply(w, xv[turn][j]);
+          }
+        }
+      }
+    } else {
+      // A step is four phases of eight columns a lane.  A phase reads and converts the next one's operands while its own
+      // are multiplied; the last phase of a step first waits for the next stage, whose loads began two steps ago, and
+      // hands its own buffer to the stage after the one in flight.
+      uint32_t code[WN][kWords<FAM>], left[WN];
+      float scale[WN];
+      bf16x8 wv[2][WN], xv[2][WM];
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          if (s < STAGES - 1 || p == 0) issue(s, p);
+        if (s < STAGES - 1) advance();
+      }
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kInFlight + WL) : "memory");
+      asm volatile("s_barrier" ::: "memory");
+      read_codes(0, first, code, scale, left);
+      drop_infinities(first, code);
+      read_x(0, 0, xv[0]);
+      convert(code, scale, left, 0, wv[0]);
+      int b = 0;
+      for (int now = first; now < last; ++now) {
+        const int nb = next(b), pb = b == 0 ? STAGES - 1 : b - 1;        // the stage whose loads are being issued
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          read_x(b, j + 1, xv[(j + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);                             // the compiler would sink the reads to their uses
+          if (j < 2) issue(pb, j + 1);
+          multiply(wv[j & 1], xv[j & 1]);
+          convert(code, scale, left, j + 1, wv[(j + 1) & 1]);
+        }
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kInFlight) : "memory");
+        asm volatile("s_barrier" ::: "memory");
+        advance();
+        read_codes(nb, now + 1, code, scale, left);                      // after the last step: what no sum takes
+        read_x(nb, 0, xv[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(b, 0);
+        multiply(wv[1], xv[1]);
+        drop_infinities(now + 1, code);
+        convert(code, scale, left, 0, wv[0]);
+        b = nb;
+      }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
 
-  // acc[i][m][e]: row m * 32 + (lane & 31), weight row i * 32 + 8 (e / 4) + 4 h + e % 4
-  if (ta.split > 1) {
-    const int64_t width = gated ? 2 * a.N : a.N;
-#pragma unroll
-    for (int m = 0; m < WM; ++m) {
-      const int row = (wm * WM + m) * 32 + r;
-      if (row >= t.rows) continue;
-      float* out = ta.partial + ((int64_t)blockIdx.y * a.M + t.row0 + row) * width;
-#pragma unroll
-      for (int i = 0; i < WN; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int q = (wn * WN + i) * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-          const int64_t n = gated ? n0 + (q >> 6) * 32 + (q & 31) : n0 + q;
-          if (n < a.N) out[gated && (q & 32) ? n + a.N : n] = acc[i][m][e];
-        }
-    }
-    return;
-  }
-
-  __syncthreads();                                                       // the stages become the waves' own transposes
-  float* mine = (float*)memory + wave * 32 * PITCH;
-  const int64_t nw = n0 + wn * (gated ? 32 : 64);                       // this wave's first output
-  const int shift = gated ? 2 : 3, groups = 1 << shift;                  // of eight outputs a row
-  const int64_t n = nw + (lane & (groups - 1)) * 8;
-  // the residual of the next 32 rows is asked for before these are finished: a wait for memory a tile, not one for each row
-  Eight residual[2][4];
-  auto ask = [&](int m) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int row = (wm * WM + m) * 32 + ((p * 64 + lane) >> shift);
-      if (a.residual && p * 64 < 32 * groups && row < t.rows && n + 8 <= a.N)
-        residual[m & 1][p] = load_eight(a.residual, a.sp.residual_dtype, (t.row0 + row) * a.sp.ld_residual + n);
-    }
-  };
-  ask(0);
-#pragma unroll
-  for (int m = 0; m < WM; ++m) {
-    if (m + 1 < WM) ask(m + 1);
+  // acc[i][m][e]: row m * 32 + (lane & 31), weight row i * 32 + 8 (e / 4) + 4 h + e % 4.  The stages become the waves' own
+  // transposes, from which a lane takes eight neighbouring outputs of a row.  The loop stays a loop: unrolled, its code was
+  // read from memory once a workgroup, 5 us that nothing hid.
+  __syncthreads();
+  const int shift = gated ? 2 : 3, groups = 1 << shift, passes = groups / 2, group = lane & (groups - 1);       // of a row, of 32
+  const int64_t n = n0 + wn * (gated ? 32 : 64) + group * 8, width = gated ? 2 * a.N : a.N;
+  float* mine = (float*)memory + wave * (kHeld * 32 * PITCH);
+  auto hold = [&](int m, int at) {
 #pragma unroll
     for (int i = 0; i < WN; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const f32x16& v = acc[i][m];
-        *(f32x4*)&mine[r * PITCH + i * 32 + 8 * q + 4 * h] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        *(f32x4*)&mine[(at * 32 + r) * PITCH + i * 32 + 8 * q + 4 * h] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
       }
+  };
+  auto in_order = [&]() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  const bool split = ta.split > 1, whole = n + 8 <= a.N;
+  Bias bias = {};
+  if (whole && !split && !t.zeros) bias = load_bias(a, t, n);
+  // a residual of 16 bits: these 32 rows', and the next's, asked for before them
+  const bool early = a.residual && a.sp.residual_dtype != MXQ_DT_F32 && !split && whole;
+  u32x4 residual[4], coming[4];
+  auto ask = [&](int m) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      const int row = (p * 64 + lane) >> shift, rr = (wm * WM + m) * 32 + row;
-      if (p * 64 >= 32 * groups || rr >= t.rows || n + 8 > a.N) continue;
-      float z[8], up[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float* at = &mine[row * PITCH + (lane & (groups - 1)) * 8 + 4 * i];
-        const f32x4 u = *(const f32x4*)at, v = *(const f32x4*)(at + (gated ? 32 : 0));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[4 * i + e] = u[e], up[4 * i + e] = v[e];
-      }
-      finish_eight(a, t, t.row0 + rr, n, z, up, residual[m & 1][p]);
+      const int row = (wm * WM + m) * 32 + ((p * 64 + lane) >> shift);
+      if (early && p < passes && row < t.rows)
+        coming[p] = *(const u32x4_any*)((const uint16_t*)a.residual + (t.row0 + row) * a.sp.ld_residual + n);
     }
-    if (n < a.N && n + 8 > a.N) {                                        // the last outputs, one by one
+  };
+  ask(0);
+#pragma unroll
+  for (int some = 0; some < WM; some += kHeld) {
+    if (some) in_order();
+#pragma unroll
+    for (int m = 0; m < kHeld; ++m) hold(some + m, m);
+    in_order();
 #pragma unroll 1
-      for (int row = lane >> shift; row < 32; row += 64 >> shift) {
-        const int rr = (wm * WM + m) * 32 + row;
-        const float* at = &mine[row * PITCH + (lane & (groups - 1)) * 8];
-        if (rr < t.rows)
+    for (int held = 0; held < kHeld; ++held) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) residual[p] = coming[p];
+      if (some + held + 1 < WM) ask(some + held + 1);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int line = (p * 64 + lane) >> shift, row = (wm * WM + some + held) * 32 + line;
+        if (p >= passes || row >= t.rows || n >= a.N) continue;
+        const float* at = &mine[(held * 32 + line) * PITCH + group * 8];
+        float z[8], up[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 u = *(const f32x4*)(at + 4 * i), v = *(const f32x4*)(at + 4 * i + (gated ? 32 : 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[4 * i + e] = u[e], up[4 * i + e] = v[e];
+        }
+        const int64_t y = t.row0 + row;
+        if (split) {
+          float* out = ta.partial + ((int64_t)blockIdx.y * a.M + y) * width + n;
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              u32x4 first4, second4;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) first4[e] = __float_as_uint(z[4 * i + e]), second4[e] = __float_as_uint(up[4 * i + e]);
+              *(u32x4_any*)(out + 4 * i) = first4;
+              if (gated) *(u32x4_any*)(out + a.N + 4 * i) = second4;
+            }
+          } else {
 #pragma unroll 1
-          for (int64_t e = n; e < a.N; ++e, ++at)
-            store_elem(a.y, a.sp.y_dtype, (t.row0 + rr) * a.sp.ld_y + e, epilogue(a, t, t.row0 + rr, e, at[0], at[gated ? 32 : 0]));
+            for (int e = 0; n + e < a.N; ++e) {
+              out[e] = at[e];
+              if (gated) out[a.N + e] = at[32 + e];
+            }
+          }
+        } else if (whole) {
+          Eight r8;
+          r8.first = residual[p];
+          if (a.residual && !early) r8 = load_eight(a.residual, a.sp.residual_dtype, y * a.sp.ld_residual + n);
+          finish_eight(a, t, y, n, z, up, bias, r8);
+        } else {
+#pragma unroll 1
+          for (int e = 0; n + e < a.N; ++e) store_elem(a.y, a.sp.y_dtype, y * a.sp.ld_y + n + e, epilogue(a, t, y, n + e, at[e], at[gated ? 32 + e : 0]));
+        }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 

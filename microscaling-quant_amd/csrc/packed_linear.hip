@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256) void k_linear_finish(LinearArgs a, const float
     }
     Eight residual = {};
     if (a.residual) residual = load_eight(a.residual, a.sp.residual_dtype, row * a.sp.ld_residual + n);
-    finish_eight(a, t, row, n, z, up, residual);
+    finish_eight(a, t, row, n, z, up, load_bias(a, t, n), residual);
   }
 }
 

@@ -295,20 +295,31 @@ __device__ __forceinline__ void activate_eight(float (&v)[8], int activation) {
   }
 }
 
+// The biases of eight neighbouring outputs, all below N: of z and, gated, of up.
+struct Bias {
+  float z[8], up[8];
+};
+__device__ __forceinline__ Bias load_bias(const LinearArgs& a, const RowTile& t, int64_t n) {
+  Bias b = {};
+  const int64_t first = t.expert * a.sp.batch_bias + n;
+  if (a.bias) add_eight(b.z, a.bias, a.sp.bias_dtype, first);
+  if (a.bias && a.sp.gated) add_eight(b.up, a.bias, a.sp.bias_dtype, first + a.N);
+  return b;
+}
+
 // epilogue and store of eight neighbouring outputs of a row, all below N; residual: theirs, if there is one.
 __device__ __forceinline__ void finish_eight(const LinearArgs& a, const RowTile& t, int64_t row, int64_t n, float (&z)[8], float (&up)[8],
-                                             const Eight& residual) {
+                                             const Bias& bias, const Eight& residual) {
   if (t.zeros) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] = 0.0f;
   } else {
-    const int64_t first = t.expert * a.sp.batch_bias + n;
-    if (a.bias) add_eight(z, a.bias, a.sp.bias_dtype, first);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] += bias.z[i];
     activate_eight(z, a.sp.activation);
     if (a.sp.gated) {
-      if (a.bias) add_eight(up, a.bias, a.sp.bias_dtype, first + a.N);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] *= up[i];
+      for (int i = 0; i < 8; ++i) z[i] *= up[i] + bias.up[i];
     }
     if (a.residual) add_eight(z, residual, a.sp.residual_dtype);
   }
