@@ -35,16 +35,34 @@ def _whole(value, who: str, what: str, low: int, high: int) -> int:
     return value
 
 
+@_lib.memo_spec
+def _route_spec(E, top_k, score, groups, top_groups, renormalize, scale):
+    _whole(E, "route", "the number of experts", 1, MAX_EXPERTS)
+    _whole(top_k, "route", "top_k", 1, min(MAX_TOP_K, E))
+    _whole(groups, "route", "groups", 1, min(MAX_GROUPS, E))
+    if E % groups:
+        raise ValueError(f"mxq.nn.route: groups {groups} must divide the {E} experts")
+    _whole(top_groups, "route", "top_groups", 1, groups)
+    if score not in SCORES:
+        raise ValueError(f"mxq.nn.route: score must be one of {SCORES}, got {score!r}")
+    return _lib.RouteSpec(SCORES.index(score), top_k, groups, top_groups, int(bool(renormalize)), float(scale))
+
+
+def _route(logits, bias, spec):
+    T, E = logits.shape
+    dev = logits.device
+    weights = logits.new_empty((T, spec.top_k), dtype=torch.float32)
+    experts = logits.new_empty((T, spec.top_k), dtype=torch.int32)
+    with _lib.on(dev):
+        _lib.run("mxq_route", logits.data_ptr(), _DTYPES[logits.dtype], _lib.ptr(bias), T, E, spec, weights.data_ptr(),
+                 experts.data_ptr(), _lib.stream(dev))
+    return weights, experts
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, spec):
-        T, E = logits.shape
-        dev = logits.device
-        weights = torch.empty((T, spec.top_k), dtype=torch.float32, device=dev)
-        experts = torch.empty((T, spec.top_k), dtype=torch.int32, device=dev)
-        with _lib.on(dev):
-            _lib.run("mxq_route", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(bias), T, E, spec,
-                     _lib.ptr(weights), _lib.ptr(experts), _lib.stream(dev))
+        weights, experts = _route(logits, bias, spec)
         ctx.save_for_backward(logits, experts)
         ctx.spec = spec
         ctx.mark_non_differentiable(experts)
@@ -58,8 +76,8 @@ class _Route(torch.autograd.Function):
         grad = grad.to(torch.float32).contiguous()
         out = torch.empty_like(logits)
         with _lib.on(dev):
-            _lib.run("mxq_route_grad", _lib.ptr(logits), _DTYPES[logits.dtype], _lib.ptr(experts), _lib.ptr(grad),
-                     logits.shape[0], logits.shape[1], ctx.spec, _lib.ptr(out), _lib.stream(dev))
+            _lib.run("mxq_route_grad", logits.data_ptr(), _DTYPES[logits.dtype], experts.data_ptr(), grad.data_ptr(),
+                     logits.shape[0], logits.shape[1], ctx.spec, out.data_ptr(), _lib.stream(dev))
         return out, None, None
 
 
@@ -80,24 +98,20 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
     if logits.ndim < 1:
         raise ValueError("mxq.nn.route: logits must have an experts axis")
     E = logits.shape[-1]
-    _whole(E, "route", "the number of experts", 1, MAX_EXPERTS)
-    _whole(top_k, "route", "top_k", 1, min(MAX_TOP_K, E))
-    _whole(groups, "route", "groups", 1, min(MAX_GROUPS, E))
-    if E % groups:
-        raise ValueError(f"mxq.nn.route: groups {groups} must divide the {E} experts")
-    _whole(top_groups, "route", "top_groups", 1, groups)
-    if score not in SCORES:
-        raise ValueError(f"mxq.nn.route: score must be one of {SCORES}, got {score!r}")
+    spec = _route_spec(E, top_k, score, groups, top_groups, renormalize, scale)
     if bias is not None and tuple(bias.shape) != (E,):
         raise ValueError(f"mxq.nn.route: bias must hold {E} values, got shape {tuple(bias.shape)}")
     dev = _lib.compute_device(logits)
-    spec = _lib.RouteSpec(SCORES.index(score), top_k, groups, top_groups, int(bool(renormalize)), float(scale))
     if bias is not None:
         bias = _lib.to_device(bias.detach(), dev).to(torch.float32).contiguous()
-    lead = logits.shape[:-1]
-    flat = _lib.to_device(logits, dev).reshape(-1, E).contiguous()
-    weights, experts = _Route.apply(flat, bias, spec)
-    return _lib.back(weights.reshape(*lead, top_k), logits), _lib.back(experts.reshape(*lead, top_k), logits)
+    flat = logits if logits.ndim == 2 else logits.reshape(-1, E)
+    flat = _lib.to_device(flat, dev).contiguous()
+    grad = flat.requires_grad and torch.is_grad_enabled()
+    weights, experts = (_Route.apply if grad else _route)(flat, bias, spec)
+    if logits.ndim != 2:
+        lead = logits.shape[:-1]
+        weights, experts = weights.reshape(*lead, top_k), experts.reshape(*lead, top_k)
+    return _lib.back(weights, logits), _lib.back(experts, logits)
 
 
 class Dispatch(NamedTuple):
@@ -132,32 +146,39 @@ def dispatch(experts: torch.Tensor, num_experts: int) -> Dispatch:
         e = e.clamp(-1, num_experts).to(torch.int32)             # a far index must not wrap into the range
     e = e.contiguous()
     n = e.numel()
-    order = torch.empty(n, dtype=torch.int32, device=dev)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    positions = torch.empty(tuple(e.shape), dtype=torch.int32, device=dev)
+    order = e.new_empty(n, dtype=torch.int32)
+    offsets = e.new_empty(num_experts + 1, dtype=torch.int32)
+    positions = torch.empty_like(e)
     with _lib.on(dev):
-        _lib.run("mxq_dispatch", _lib.ptr(e), n, num_experts, _lib.ptr(order), _lib.ptr(offsets), _lib.ptr(positions),
-                 _lib.stream(dev))
+        _lib.run("mxq_dispatch", e.data_ptr(), n, num_experts, order.data_ptr(), offsets.data_ptr(),
+                 positions.data_ptr(), _lib.stream(dev))
     return Dispatch(_lib.back(order, experts), _lib.back(offsets, experts), _lib.back(positions, experts))
 
 
 def _check_plan(plan, who: str) -> None:
     if not isinstance(plan, Dispatch):
         raise TypeError(f"mxq.nn.{who}: plan must be dispatch's, got {type(plan).__name__}")
-    if any(t.dtype != torch.int32 for t in plan) or plan.positions.ndim != 2 or \
-            plan.order.shape != (plan.positions.numel(),) or plan.offsets.ndim != 1 or len(plan.offsets) < 2:
+    order, offsets, positions = plan
+    if order.dtype != torch.int32 or offsets.dtype != torch.int32 or positions.dtype != torch.int32 or \
+            positions.ndim != 2 or order.ndim != 1 or len(order) != positions.numel() or offsets.ndim != 1 or \
+            len(offsets) < 2:
         raise ValueError(f"mxq.nn.{who}: plan does not hold dispatch's tensors")
+
+
+def _combine(y, weights, positions, residual):
+    T, k = positions.shape
+    D, dev = y.shape[1], y.device
+    out = y.new_empty((T, D))
+    with _lib.on(dev):
+        _lib.run("mxq_combine", y.data_ptr(), _DTYPES[y.dtype], weights.data_ptr(), positions.data_ptr(),
+                 _lib.ptr(residual), out.data_ptr(), T, k, D, _lib.stream(dev))
+    return out
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, positions, residual):
-        T, k = positions.shape
-        D, dev = y.shape[1], y.device
-        out = torch.empty((T, D), dtype=y.dtype, device=dev)
-        with _lib.on(dev):
-            _lib.run("mxq_combine", _lib.ptr(y), _DTYPES[y.dtype], _lib.ptr(weights), _lib.ptr(positions),
-                     _lib.ptr(residual), _lib.ptr(out), T, k, D, _lib.stream(dev))
+        out = _combine(y, weights, positions, residual)
         ctx.save_for_backward(y, weights, positions)
         return out
 
@@ -194,7 +215,9 @@ def combine(y: torch.Tensor, weights: torch.Tensor, plan: Dispatch,
         raise ValueError(f"mxq.nn.combine: residual must be {T} x {y.shape[1]} {y.dtype}, got "
                          f"{tuple(residual.shape)} {residual.dtype}")
     dev = _lib.compute_device(y, weights)
-    out = _Combine.apply(_lib.to_device(y, dev).contiguous(), _lib.to_device(weights, dev).to(torch.float32).contiguous(),
-                         _lib.to_device(plan.positions, dev).contiguous(),
-                         None if residual is None else _lib.to_device(residual, dev).contiguous())
-    return _lib.back(out, y)
+    yd = _lib.to_device(y, dev).contiguous()
+    wd = _lib.to_device(weights, dev).to(torch.float32).contiguous()
+    pd = _lib.to_device(plan.positions, dev).contiguous()
+    rd = None if residual is None else _lib.to_device(residual, dev).contiguous()
+    grad = torch.is_grad_enabled() and (yd.requires_grad or wd.requires_grad or (rd is not None and rd.requires_grad))
+    return _lib.back((_Combine.apply if grad else _combine)(yd, wd, pd, rd), y)

@@ -25,36 +25,39 @@ _PAIRS = 5
 BLOCK = 32
 
 
-def _weight(codes, scales, fmt, K: int, ndim: int, who: str):
-    """(format code, row count) of a weight of K columns, its shapes checked."""
+@_lib.memo_spec
+def _weight(fmt, codes_shape, codes_dtype, scales_shape, scales_dtype, K, ndim, who):
+    """The format code of a weight of K columns, its types and shapes checked."""
     f = get(fmt)
     code = None if f is None else _FORMATS.get(f.name)
     if code is None:
         raise ValueError(f"mxq.nn.{who}: fmt must name one of {tuple(_FORMATS)}, got {fmt!r}")
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise TypeError(f"mxq.nn.{who}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-    if codes.ndim != ndim:
-        raise ValueError(f"mxq.nn.{who}: codes must have {ndim} axes, got shape {tuple(codes.shape)}")
-    if codes.shape[-1] != K:
-        if code != _FORMATS["MXFP4"] or codes.shape[-1] != (K + 1) // 2:
-            raise ValueError(f"mxq.nn.{who}: codes of shape {tuple(codes.shape)} do not hold {K} columns")
+    if codes_dtype != torch.uint8 or scales_dtype != torch.uint8:
+        raise TypeError(f"mxq.nn.{who}: codes and scales must be uint8, got {codes_dtype} and {scales_dtype}")
+    if len(codes_shape) != ndim:
+        raise ValueError(f"mxq.nn.{who}: codes must have {ndim} axes, got shape {tuple(codes_shape)}")
+    if codes_shape[-1] != K:
+        if code != _FORMATS["MXFP4"] or codes_shape[-1] != (K + 1) // 2:
+            raise ValueError(f"mxq.nn.{who}: codes of shape {tuple(codes_shape)} do not hold {K} columns")
         code = _PAIRS
-    if tuple(scales.shape) != (*codes.shape[:-1], -(-K // BLOCK)):
-        raise ValueError(f"mxq.nn.{who}: scales must be {(*codes.shape[:-1], -(-K // BLOCK))}, got "
-                         f"{tuple(scales.shape)}")
+    if tuple(scales_shape) != (*codes_shape[:-1], -(-K // BLOCK)):
+        raise ValueError(f"mxq.nn.{who}: scales must be {(*codes_shape[:-1], -(-K // BLOCK))}, got "
+                         f"{tuple(scales_shape)}")
     return code
 
 
 def _no_grad(who: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"mxq.nn.{who}: packed weights are for inference; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"mxq.nn.{who}: packed weights are for inference; call it under torch.no_grad()")
 
 
 def _rows(t: Optional[torch.Tensor], dev) -> Optional[torch.Tensor]:
     """t on dev, its last axis's elements next to each other."""
     if t is None:
         return None
-    t = _lib.to_device(t.detach(), dev)
+    t = _lib.to_device(t, dev)
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
@@ -88,7 +91,10 @@ def _spec(x, bias, residual, y, codes, scales, code, activation, gated, top_k=0)
         scales.stride(0) if batched else 0, bias.stride(0) if batched and bias is not None else 0)
 
 
-def _workspace(name: str, dev, *args) -> Optional[torch.Tensor]:
+def _workspace(name: str, rows: int, each: int, dev, *args) -> Optional[torch.Tensor]:
+    """What the kernels of this call need; nothing where a matrix has at most 16 rows of x."""
+    if rows <= 16 * each:
+        return None
     size = _lib.call(name, *args)
     return torch.empty(size, dtype=torch.uint8, device=dev) if size else None
 
@@ -107,7 +113,7 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
     if x.ndim < 1:
         raise ValueError("mxq.nn.packed_linear: x must have a last axis to contract")
     K = x.shape[-1]
-    code = _weight(codes, scales, fmt, K, 2, who)
+    code = _weight(fmt, codes.shape, codes.dtype, scales.shape, scales.dtype, K, 2, who)
     N = _outputs(codes.shape[0], gated, who)
     out_dtype = _checked(x, bias, (codes.shape[0],), activation, out_dtype, who)
     shape = (*x.shape[:-1], N)
@@ -117,16 +123,18 @@ def packed_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
             raise ValueError(f"mxq.nn.packed_linear: residual must have shape {shape}, got {tuple(residual.shape)}")
     dev = _lib.compute_device(x, codes)
     M = _lib.numel(shape[:-1])
-    xd = _rows(_lib.to_device(x, dev).reshape(M, K), dev)
+    xd = _rows(x if x.ndim == 2 else x.reshape(M, K), dev)
     cd, sd, bd = _rows(codes, dev), _rows(scales, dev), _rows(bias, dev)
-    rd = None if residual is None else _rows(_lib.to_device(residual, dev).reshape(M, N), dev)
+    rd = residual if residual is None or residual.ndim == 2 else residual.reshape(M, N)
+    rd = _rows(rd, dev)
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
     spec = _spec(xd, bd, rd, y, cd, sd, code, activation, gated)
+    xp, cp, sp = xd.data_ptr(), cd.data_ptr(), sd.data_ptr()
     with _lib.on(dev):
-        work = _workspace("mxq_packed_linear_workspace", dev, _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), M, N, K, spec)
-        _lib.run("mxq_packed_linear", _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), _lib.ptr(bd), _lib.ptr(rd),
-                 _lib.ptr(y), M, N, K, spec, _lib.ptr(work), _lib.stream(dev))
-    return _lib.back(y.reshape(shape), x)
+        work = _workspace("mxq_packed_linear_workspace", M, 1, dev, xp, cp, sp, M, N, K, spec)
+        _lib.run("mxq_packed_linear", xp, cp, sp, _lib.ptr(bd), _lib.ptr(rd), y.data_ptr(), M, N, K, spec,
+                 _lib.ptr(work), _lib.stream(dev))
+    return _lib.back(y if x.ndim == 2 else y.reshape(shape), x)
 
 
 def expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fmt: Union[str, Format], plan: Dispatch,
@@ -146,7 +154,7 @@ def expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
         raise ValueError(f"mxq.nn.expert_linear: x must have {n if sorted_rows else T} rows, got shape "
                          f"{tuple(x.shape)}")
     K = x.shape[1]
-    code = _weight(codes, scales, fmt, K, 3, who)
+    code = _weight(fmt, codes.shape, codes.dtype, scales.shape, scales.dtype, K, 3, who)
     if codes.shape[0] != E or E > MAX_EXPERTS:
         raise ValueError(f"mxq.nn.expert_linear: codes of {codes.shape[0]} experts, plan has {E}")
     N = _outputs(codes.shape[1], gated, who)
@@ -156,8 +164,9 @@ def expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, fm
     order, offsets = (_lib.to_device(t, dev).contiguous() for t in (plan.order, plan.offsets))
     y = torch.empty((n, N), dtype=out_dtype, device=dev)
     spec = _spec(xd, bd, None, y, cd, sd, code, activation, gated, 0 if sorted_rows else k)
+    xp, cp, sp = xd.data_ptr(), cd.data_ptr(), sd.data_ptr()
     with _lib.on(dev):
-        work = _workspace("mxq_expert_linear_workspace", dev, _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), n, N, K, E, spec)
-        _lib.run("mxq_expert_linear", _lib.ptr(xd), _lib.ptr(cd), _lib.ptr(sd), _lib.ptr(bd), _lib.ptr(y), n, N, K, E,
-                 _lib.ptr(order), _lib.ptr(offsets), spec, _lib.ptr(work), _lib.stream(dev))
+        work = _workspace("mxq_expert_linear_workspace", n, E, dev, xp, cp, sp, n, N, K, E, spec)
+        _lib.run("mxq_expert_linear", xp, cp, sp, _lib.ptr(bd), y.data_ptr(), n, N, K, E, order.data_ptr(),
+                 offsets.data_ptr(), spec, _lib.ptr(work), _lib.stream(dev))
     return _lib.back(y, x)
