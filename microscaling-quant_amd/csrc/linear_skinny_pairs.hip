@@ -1,5 +1,5 @@
 #include "linear_skinny_impl.h"
 
 namespace mxq {
-void launch_skinny_pairs(const LinearArgs& a, int mt, int64_t tiles, hipStream_t st) { launch_skinny_family<kPairs>(a, mt, tiles, st); }
+void launch_skinny_pairs(const LinearArgs& a, int64_t tiles, hipStream_t st) { launch_skinny_family<kPairs>(a, tiles, st); }
 }  // namespace mxq

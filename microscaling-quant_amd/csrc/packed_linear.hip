@@ -6,10 +6,10 @@
 
 namespace mxq {
 
-void launch_skinny_e4m3(const LinearArgs&, int, int64_t, hipStream_t);
-void launch_skinny_e5m2(const LinearArgs&, int, int64_t, hipStream_t);
-void launch_skinny_mapped(const LinearArgs&, int, int64_t, hipStream_t);
-void launch_skinny_pairs(const LinearArgs&, int, int64_t, hipStream_t);
+void launch_skinny_e4m3(const LinearArgs&, int64_t, hipStream_t);
+void launch_skinny_e5m2(const LinearArgs&, int64_t, hipStream_t);
+void launch_skinny_mapped(const LinearArgs&, int64_t, hipStream_t);
+void launch_skinny_pairs(const LinearArgs&, int64_t, hipStream_t);
 void launch_tile_e4m3(const TileArgs&, const TilePlan&, hipStream_t);
 void launch_tile_e5m2(const TileArgs&, const TilePlan&, hipStream_t);
 void launch_tile_mapped(const TileArgs&, const TilePlan&, hipStream_t);
@@ -19,25 +19,24 @@ namespace {
 
 // What k_linear_tile's direct loads cannot take as it lies is laid out first, by one launch.
 //   x: bfloat16 planes of kp values, one after another along a row, zeros past K: each plane the leading bits of what the
-//      ones before leave, so that their sum is the value.  Eight values a thread.
-//   codes: rows of whole 128 columns, zeros past K.  16 bytes a thread.
-//   scales: rows of whole words.  Four bytes a thread.
+//      ones before leave, so that their sum is the value.
+//   codes: rows of whole 128 columns, zeros past K.
+//   scales: rows of whole words.
 // Experts without rows are left out.
 struct PrepareArgs {
   LinearArgs l;
-  int64_t kp, x_rows, w_rows;          // columns a plane, rows of x, rows of one weight
+  int64_t kp, x_rows, w_rows;          // columns a plane, rows of x (0: stays), rows of one weight
   int32_t planes;
-  int64_t x_items, code_items, items;  // threads of x, of x and codes, of all
   uint16_t* x;
-  uint8_t *codes, *scales;
+  uint8_t *codes, *scales;             // NULL: stay
 };
+// A workgroup a row of x, then a row of the weight.
 __global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
   const LinearArgs& a = p.l;
   const bool pairs = a.sp.format == MXQ_FMT_E2M1_PAIRS;
-  auto used = [&](int64_t e) { return !a.offsets || a.offsets[e + 1] > a.offsets[e]; };
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.items; i += (int64_t)gridDim.x * 256) {
-    if (i < p.x_items) {
-      const int64_t groups = p.kp / 8, row = i / groups, k = (i - row * groups) * 8;
+  if (blockIdx.x < p.x_rows) {
+    const int64_t row = blockIdx.x;
+    for (int64_t k = threadIdx.x * 8; k < p.kp; k += 256 * 8) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.0f;
@@ -59,35 +58,37 @@ __global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
           v[e] = v[e] == hi ? 0.0f : v[e] - hi;                          // infinities leave nothing
         }
       }
-    } else if (i < p.code_items) {
-      const int64_t bytes = pairs ? p.kp / 2 : p.kp, chunks = bytes / 16, all = (i - p.x_items) / chunks, e = all / p.w_rows;
-      if (!used(e)) continue;
-      const int64_t at = (i - p.x_items - all * chunks) * 16, have = pairs ? (a.K + 1) / 2 : a.K, left = have - at;
-      const uint8_t* from = a.codes + e * a.sp.batch_codes + (all - e * p.w_rows) * a.sp.ld_codes + at;
+    }
+    return;
+  }
+  const int64_t all = (int64_t)blockIdx.x - p.x_rows, e = all / p.w_rows, row = all - e * p.w_rows;
+  if (a.offsets && a.offsets[e + 1] <= a.offsets[e]) return;
+  const int64_t bytes = pairs ? p.kp / 2 : p.kp, have = pairs ? (a.K + 1) / 2 : a.K;
+  const uint8_t* codes = a.codes + e * a.sp.batch_codes + row * a.sp.ld_codes;
+  if (p.codes)
+    for (int64_t at = threadIdx.x * 16; at < bytes; at += 256 * 16) {
+      const int64_t left = have - at;
       u32x4 v;
-      if (left >= 16) v = *(const u32x4_any*)from;
-      else v = load_part(from, left < 0 ? 0 : (int)left);
+      if (left >= 16) v = *(const u32x4_any*)(codes + at);
+      else v = load_part(codes + at, left < 0 ? 0 : (int)left);
       if (pairs && (a.K & 1) && left > 0 && left <= 16) clear_odd(v, (int)left * 2 - 1);
       *(u32x4*)(p.codes + all * bytes + at) = v;
-    } else {
-      const int64_t words = p.kp / 128, all = (i - p.code_items) / words, e = all / p.w_rows;
-      if (!used(e)) continue;
-      const int64_t at = (i - p.code_items - all * words) * 4, left = (a.K + 31) / 32 - at;
-      const uint8_t* from = a.scales + e * a.sp.batch_scales + (all - e * p.w_rows) * a.sp.ld_scales + at;
+    }
+  const uint8_t* scales = a.scales + e * a.sp.batch_scales + row * a.sp.ld_scales;
+  if (p.scales)
+    for (int64_t at = threadIdx.x * 4; at < p.kp / 32; at += 256 * 4) {
       uint32_t v = 0;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        if (b < left) v |= (uint32_t)from[b] << 8 * b;
-      *(uint32_t*)(p.scales + (all * words) * 4 + at) = v;
+        if (at + b < (a.K + 31) / 32) v |= (uint32_t)scales[at + b] << 8 * b;
+      *(uint32_t*)(p.scales + all * (p.kp / 32) + at) = v;
     }
-  }
 }
 
 // The splits' sums in their order, and the epilogue: eight outputs a thread.
 __global__ __launch_bounds__(256) void k_linear_finish(LinearArgs a, const float* partial, int split) {
-  const int64_t groups = (a.N + 7) / 8, width = a.sp.gated ? 2 * a.N : a.N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.M * groups; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / groups, n = i % groups * 8;
+  const int64_t row = blockIdx.x, width = a.sp.gated ? 2 * a.N : a.N;
+  for (int64_t n = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8; n < a.N; n += (int64_t)gridDim.y * 256 * 8) {
     const RowTile t{0, 0, 0, false};
     const float* p = partial + row * width + n;
     if (n + 8 > a.N) {
@@ -130,7 +131,7 @@ int family(int format) {
 }
 
 struct Plan {
-  int mt;                      // rows of a k_linear_skinny workgroup / 16, or 0: k_linear_tile
+  bool few;                    // k_linear_skinny, 16 rows a workgroup; k_linear_tile otherwise
   TilePlan tile;
   int64_t tiles_m, tiles_n;    // of either
   int steps, planes;
@@ -153,8 +154,8 @@ Plan plan_of(const LinearArgs& a) {
   p.lay_scales = K % 128 || (uintptr_t)a.scales % 4 || sp.ld_scales % 4 || sp.batch_scales % 4;
   // by the sizes alone: strides and addresses do not change a result's bits
   if (each <= 16) {
-    p.mt = 1;
-    p.tiles_m = row_tiles(16 * p.mt);
+    p.few = true;
+    p.tiles_m = row_tiles(16);
     return p;
   }
   p.steps = (int)(2 * ceil_div(K, 128));
@@ -168,7 +169,7 @@ Plan plan_of(const LinearArgs& a) {
   p.tile.split = 1;
   if (!E) {
     const int64_t have = p.tiles_m * p.tiles_n, all = (int64_t)p.steps * p.planes;
-    while (p.tile.split < 8 && have * p.tile.split * 2 <= 320 && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
+    while (p.tile.split < 8 && have * p.tile.split * 2 <= 512 && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
   }
   p.lay_x = sp.x_dtype != MXQ_DT_BF16 || K % 8 || sp.ld_x % 8 || (uintptr_t)a.x % 16;
   p.x_rows = E && sp.top_k ? ceil_div(M, sp.top_k) : M;
@@ -186,9 +187,9 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
   const Plan p = plan_of(a);
   if (p.bytes && !workspace) return invalid(std::string(who) + ": NULL workspace");
   const int fam = family(a.sp.format);
-  if (p.mt) {
+  if (p.few) {
     (fam == kE4M3 ? launch_skinny_e4m3 : fam == kE5M2 ? launch_skinny_e5m2 : fam == kPairs ? launch_skinny_pairs : launch_skinny_mapped)(
-        a, p.mt, p.tiles_m, st);
+        a, p.tiles_m, st);
     return check_launch(who);
   }
   if (p.tiles_m * p.tiles_n > 0x7fffffff) return invalid(std::string(who) + ": too many outputs");
@@ -198,13 +199,12 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
   TileArgs t{a, (const uint16_t*)a.x, a.sp.ld_x, p.steps, p.planes, (int32_t)a.K, (int32_t)a.K, (int32_t)p.tiles_m, (int32_t)p.tiles_n,
              p.tile.split, (float*)(work + p.at_partial), code_map(a.sp.format)};
   if (kp && (p.lay_x || p.lay_codes || p.lay_scales)) {
-    PrepareArgs q{a, kp, p.x_rows, p.w_rows, p.planes, 0, 0, 0, (uint16_t*)work, work + p.at_codes, work + p.at_scales};
-    q.x_items = p.lay_x ? p.x_rows * (kp / 8) : 0;
-    q.code_items = q.x_items + (p.lay_codes ? matrices * (kp / (pairs ? 32 : 16)) : 0);
-    q.items = q.code_items + (p.lay_scales ? matrices * (kp / 128) : 0);
-    const int64_t blocks = ceil_div(q.items, 256);
+    const int64_t x_rows = p.lay_x ? p.x_rows : 0, w_rows = p.lay_codes || p.lay_scales ? matrices : 0;
+    if (x_rows + w_rows > 0x7fffffff) return invalid(std::string(who) + ": too many rows");
+    const PrepareArgs q{a, kp, x_rows, p.w_rows, p.planes, (uint16_t*)work, p.lay_codes ? work + p.at_codes : nullptr,
+                        p.lay_scales ? work + p.at_scales : nullptr};
     KernelTimer timer("k_prepare", st);
-    k_prepare<<<dim3((unsigned)(blocks < 32768 ? blocks : 32768)), 256, 0, st>>>(q);
+    k_prepare<<<dim3((unsigned)(x_rows + w_rows)), 256, 0, st>>>(q);
     if (p.lay_x) t.x = q.x, t.ld_x = kp * p.planes, t.x_columns = (int32_t)kp;
     if (p.lay_codes) {
       t.l.codes = q.codes, t.l.sp.ld_codes = pairs ? kp / 2 : kp, t.l.sp.batch_codes = t.l.sp.ld_codes * p.w_rows;
@@ -215,8 +215,8 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
   (fam == kE4M3 ? launch_tile_e4m3 : fam == kE5M2 ? launch_tile_e5m2 : fam == kPairs ? launch_tile_pairs : launch_tile_mapped)(t, p.tile, st);
   if (p.tile.split > 1) {
     KernelTimer timer("k_linear_finish", st);
-    const int64_t blocks = ceil_div(a.M * ceil_div(a.N, 8), 256);
-    k_linear_finish<<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), 256, 0, st>>>(a, t.partial, p.tile.split);
+    const int64_t blocks = ceil_div(a.N, 256 * 8);
+    k_linear_finish<<<dim3((unsigned)a.M, (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, st>>>(a, t.partial, p.tile.split);
   }
   return check_launch(who);
 }
