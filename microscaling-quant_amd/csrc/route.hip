@@ -32,6 +32,7 @@ template <int DT> __device__ __forceinline__ void store_from_float(void* p, int6
 
 // Rotation by N within each row of 16 lanes.
 template <int N> __device__ __forceinline__ int rotate(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x120 + N, 0xF, 0xF, false); }
+template <int N> __device__ __forceinline__ float rotate(float v) { return __int_as_float(rotate<N>(__float_as_int(v))); }
 template <int N> __device__ __forceinline__ double rotate(double v) {
   const uint64_t b = __double_as_longlong(v);
   const uint32_t lo = rotate<N>((int)(uint32_t)b), hi = rotate<N>((int)(uint32_t)(b >> 32));
@@ -64,27 +65,33 @@ template <int L> __device__ __forceinline__ bool lanes_any(bool b) {
   return (all >> (threadIdx.x & 48) & 0xFFFF) != 0;
 }
 
-// e^x for x <= 709.78, zero below -746: x = n ln 2 + r with |r| <= ln(2) / 2, Taylor's series of e^r to r^13 (the next term
-// is below 4e-18), times 2^n.
-__device__ __forceinline__ double exp64(double x) {
-  x = fmax(x, -746.0);
-  const double n = rint(x * 1.4426950408889634);
-  const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994531, x));
-  double p = 1.0 / 6227020800.0;
-  p = fma(p, r, 1.0 / 479001600.0);
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __builtin_ldexp(p, (int)n);
+// x[i] = e^x[i] for x <= 709, zero below -746: x = n ln 2 + r with |r| <= ln(2) / 2, Taylor's series of e^r to r^13 (the
+// next term is below 4e-18), times 2^n.  Up to eight at a time, so that a coefficient is put into registers once for them.
+template <int V> __device__ __forceinline__ void exp64(double (&x)[V]) {
+  constexpr int G = V < 8 ? V : 8;
+  constexpr double kFactorials[14] = {1.0, 1.0, 2.0, 6.0, 24.0, 120.0, 720.0, 5040.0, 40320.0, 362880.0, 3628800.0, 39916800.0, 479001600.0,
+                                      6227020800.0};
+#pragma unroll
+  for (int v = 0; v < V; v += G) {
+    double r[G], p[G];
+    int n[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const double y = fmin(fmax(x[v + i], -746.0), 709.0), whole = rint(y * 1.4426950408889634);
+      r[i] = fma(whole, -2.3190468138462996e-17, fma(whole, -0.69314718055994531, y));
+      n[i] = (int)whole;
+      p[i] = 1.0 / kFactorials[13];
+    }
+#pragma unroll
+    for (int c = 12; c >= 0; --c) {
+      double coefficient = 1.0 / kFactorials[c];
+      asm("" : "+v"(coefficient));                                // once for all, not once an element
+#pragma unroll
+      for (int i = 0; i < G; ++i) p[i] = fma(p[i], r[i], coefficient);
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) x[v + i] = __builtin_ldexp(p[i], n[i]);
+  }
 }
 
 // 1 / d for 1 <= d < 2^1000: the hardware's estimate and two steps of Newton's iteration.
@@ -99,48 +106,55 @@ struct Norm {
   double top, inverse;
 };
 
-__device__ __forceinline__ double score_of(float l, int softmax, const Norm& n) {
-  if (softmax) return exp64((double)l - n.top) * n.inverse;
-  return -l > 709.0f ? 0.0 : inverse(1.0 + exp64(-(double)l));
+// s[i]: the scores of the logits l[i].
+template <int V> __device__ __forceinline__ void scores_of(const float (&l)[V], int softmax, const Norm& n, double (&s)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = softmax ? (double)l[v] - n.top : -(double)l[v];
+  exp64(s);
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = softmax ? s[v] * n.inverse : -l[v] > 709.0f ? 0.0 : inverse(1.0 + s[v]);
 }
 
 // l[]: the lane's logits, s[]: their scores; true if the row holds a NaN, or +inf under softmax, which has no score.
-template <int DT, int L, int V> __device__ __forceinline__ bool scores_of(const void* logits, int64_t row, int E, int softmax, float (&l)[V],
-                                                                          double (&s)[V], Norm& n) {
+template <int DT, int L, int V> __device__ __forceinline__ bool row_scores(const void* logits, int64_t row, int E, int softmax, float (&l)[V],
+                                                                           double (&s)[V], Norm& n) {
   const int lane = threadIdx.x & (L - 1);
   bool bad = false;
-  double top = -INFINITY;
-#pragma unroll
-  for (int v = 0; v < V; ++v) l[v] = v * L + lane < E ? load_as_float<DT>(logits, row * E + v * L + lane) : -INFINITY;
+  float top = -INFINITY;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
+    const int e = v * L + lane;
+    l[v] = load_as_float<DT>(logits, row * E + (e < E ? e : E - 1));
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (v * L + lane >= E) l[v] = -INFINITY;
     bad |= l[v] != l[v] || (softmax && l[v] == INFINITY);
-    top = fmax(top, (double)l[v]);
+    top = fmaxf(top, l[v]);
   }
   bad = lanes_any<L>(bad);
   n = Norm{0.0, 1.0};
   if (softmax) {
-    top = lanes_max<L>(top);
-    n.top = top == -INFINITY ? 0.0 : top;
+    top = over_lanes<L>(top, [](float a, float b) { return fmaxf(a, b); });
+    n.top = top == -INFINITY ? 0.0 : (double)top;
+  }
+  scores_of(l, softmax, n, s);
+  if (softmax) {
     double sum = 0.0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum += s[v] = l[v] == -INFINITY ? 0.0 : exp64((double)l[v] - n.top);
+    for (int v = 0; v < V; ++v) sum += s[v];
     sum = lanes_sum<L>(sum);
     n.inverse = sum < 1.0 ? 1.0 : inverse(sum);                   // an open row's sum is at least 1
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] *= n.inverse;
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = score_of(l[v], 0, n);
   }
   return bad;
 }
 
-template <int DT, int L, int V>
+template <int DT, int L, int V, int SLOTS>
 __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const float* bias, int64_t T, int E,
                                                        mxq_route_spec sp, DivU31 per, float* weights, int32_t* experts) {
   extern __shared__ double shared[];                              // groups > 1: E ranks and 64 scores a token
-  constexpr int kSlots = kMaxTopK / L;
   const int lane = threadIdx.x & (L - 1), token = threadIdx.x / L;
   const int64_t at = (int64_t)blockIdx.x * (blockDim.x / L) + token, row = at < T ? at : T - 1;
   const bool softmax = sp.score == MXQ_SCORE_SOFTMAX, out = at < T;     // lanes past the end go along: the row's lanes work together
@@ -148,7 +162,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
   float l[V];
   double r[V];
   Norm norm;
-  bool bad = scores_of<DT, L, V>(logits, row, E, softmax, l, r, norm);
+  bool bad = row_scores<DT, L, V>(logits, row, E, softmax, l, r, norm);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = v * L + lane;
@@ -158,13 +172,19 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
   }
   bad = lanes_any<L>(bad);
   if (sp.groups > 1) {
-    volatile double* ranks = shared + (size_t)token * (E + kMaxGroups);
-    volatile double* scores = ranks + E;
+    double* ranks = shared + (size_t)token * (E + kMaxGroups);
+    double* scores = ranks + E;
+    auto in_order = [&]() {                                       // the wave's own LDS writes before its reads
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (v * L + lane < E) ranks[v * L + lane] = r[v];
+    in_order();
     for (int g = lane; g < sp.groups; g += L) {
       double a = -INFINITY, b = -INFINITY;
+#pragma unroll 4
       for (int j = 0; j < (int)per.d; ++j) {
         const double x = ranks[g * per.d + j];
         b = fmax(b, fmin(a, x));
@@ -172,12 +192,14 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
       }
       scores[g] = b == -INFINITY ? a : a + b;
     }
+    in_order();
     // a group is kept if fewer than top_groups come before it
     uint64_t kept = 0;
     for (int g0 = 0; g0 < sp.groups; g0 += L) {
       const int g = g0 + lane;
       const double mine = g < sp.groups ? scores[g] : 0.0;
       int before = 0;
+#pragma unroll 4
       for (int h = 0; h < sp.groups; ++h) {
         const double x = scores[h];
         before += x > mine || (x == mine && h < g);
@@ -191,9 +213,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
       if (!(kept >> (g & 63) & 1)) r[v] = -INFINITY;
     }
   }
-  int pick[kSlots];
+  int pick[SLOTS];
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q) {
+  for (int q = 0; q < SLOTS; ++q) {
     pick[q] = -1;
     for (int j = q * L; j < k && j < (q + 1) * L; ++j) {
       double best = r[0];
@@ -211,17 +233,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
         if (i == v * L + lane) r[v] = -INFINITY;
     }
   }
-  double own[kSlots], total = 0.0;
+  double total = 0.0;
+  float chosen[SLOTS];
+  double own[SLOTS];
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q) {
-    own[q] = 0.0;
-    if (pick[q] >= 0 && !bad) own[q] = score_of(load_as_float<DT>(logits, row * E + pick[q]), softmax, norm);
+  for (int q = 0; q < SLOTS; ++q) chosen[q] = load_as_float<DT>(logits, row * E + (pick[q] >= 0 && !bad ? pick[q] : 0));
+  scores_of(chosen, softmax, norm, own);                          // the bits they were chosen by
+#pragma unroll
+  for (int q = 0; q < SLOTS; ++q) {
+    if (pick[q] < 0 || bad) own[q] = 0.0;
     total += own[q];
   }
   total = lanes_sum<L>(total);
   if (!sp.renormalize || total == 0.0) total = 1.0;
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q) {
+  for (int q = 0; q < SLOTS; ++q) {
     const int j = q * L + lane;
     if (j >= k || !out) continue;
     weights[row * k + j] = bad ? NAN : (float)(own[q] / total * (double)sp.scale);
@@ -231,10 +257,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_route(const void* logits, const
 
 // The gradient of the logits: with u_j the chosen scores and U their sum, du_j = scale (g_j - sum_i g_i u_i / U) / U
 // where renormalized, scale g_j otherwise; softmax: dl_e = s_e (du_e - sum_j du_j u_j); sigmoid: dl_e = du_e s_e (1 - s_e).
-template <int DT, int L, int V>
+template <int DT, int L, int V, int SLOTS>
 __global__ __launch_bounds__(64 * kWaves) void k_route_grad(const void* logits, const int32_t* experts, const float* grad,
                                                             int64_t T, int E, mxq_route_spec sp, void* out) {
-  constexpr int kSlots = kMaxTopK / L;
   const int lane = threadIdx.x & (L - 1), first = threadIdx.x & 63 & ~(L - 1);
   const int64_t at = (int64_t)blockIdx.x * (64 * kWaves / L) + threadIdx.x / L, row = at < T ? at : T - 1;
   const bool softmax = sp.score == MXQ_SCORE_SOFTMAX;
@@ -242,15 +267,22 @@ __global__ __launch_bounds__(64 * kWaves) void k_route_grad(const void* logits, 
   float l[V];
   double s[V], d[V];
   Norm norm;
-  const bool bad = scores_of<DT, L, V>(logits, row, E, softmax, l, s, norm);
-  int pick[kSlots];
-  double u[kSlots], du[kSlots], U = 0.0, gu = 0.0;
+  const bool bad = row_scores<DT, L, V>(logits, row, E, softmax, l, s, norm);
+  int pick[SLOTS];
+  float chosen[SLOTS];
+  double u[SLOTS], du[SLOTS], U = 0.0, gu = 0.0;
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q) {
+  for (int q = 0; q < SLOTS; ++q) {
     const int j = q * L + lane;
     const int e = j < k ? experts[row * k + j] : -1;
     pick[q] = e < E ? e : -1;
-    u[q] = pick[q] >= 0 ? score_of(load_as_float<DT>(logits, row * E + pick[q]), softmax, norm) : 0.0;
+    chosen[q] = load_as_float<DT>(logits, row * E + (pick[q] >= 0 ? pick[q] : 0));
+  }
+  scores_of(chosen, softmax, norm, u);
+#pragma unroll
+  for (int q = 0; q < SLOTS; ++q) {
+    const int j = q * L + lane;
+    if (pick[q] < 0) u[q] = 0.0;
     du[q] = pick[q] >= 0 ? (double)grad[row * k + j] * (double)sp.scale : 0.0;
     U += u[q];
     gu += du[q] * u[q];
@@ -261,16 +293,16 @@ __global__ __launch_bounds__(64 * kWaves) void k_route_grad(const void* logits, 
     if (U == 0.0) U = 1.0;
     const double mean = gu / U;
 #pragma unroll
-    for (int q = 0; q < kSlots; ++q) du[q] = pick[q] >= 0 ? (du[q] - mean) / U : 0.0;
+    for (int q = 0; q < SLOTS; ++q) du[q] = pick[q] >= 0 ? (du[q] - mean) / U : 0.0;
   }
   double dot = 0.0;
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q) dot += du[q] * u[q];
+  for (int q = 0; q < SLOTS; ++q) dot += du[q] * u[q];
   dot = softmax ? lanes_sum<L>(dot) : 0.0;
 #pragma unroll
   for (int v = 0; v < V; ++v) d[v] = 0.0;
 #pragma unroll
-  for (int q = 0; q < kSlots; ++q)
+  for (int q = 0; q < SLOTS; ++q)
     for (int j = q * L; j < k && j < (q + 1) * L; ++j) {
       const int e = __shfl(pick[q], first + j - q * L);
       const double x = __shfl(du[q], first + j - q * L);
@@ -300,17 +332,21 @@ int check_spec(const char* who, int32_t dtype, int64_t T, int64_t E, const mxq_r
   return MXQ_OK;
 }
 
-// f(DT, L, V): the dtype, the lanes of a token and the registers of a lane, as compile-time constants.
-template <typename F> void with_shape(int32_t dtype, int64_t E, F f) {
-  auto by_experts = [&](auto dt) {
+// f(DT, L, V, SLOTS): the dtype, the lanes of a token, the registers and the choices of a lane, as compile-time constants.
+template <typename F> void with_shape(int32_t dtype, int64_t E, int k, F f) {
+  auto by_choices = [&](auto dt, auto v) {
     std::integral_constant<int, 16> row;
-    if (E <= 16) f(dt, row, std::integral_constant<int, 1>());
-    else if (E <= 32) f(dt, row, std::integral_constant<int, 2>());
-    else if (E <= 64) f(dt, row, std::integral_constant<int, 4>());
-    else if (E <= 128) f(dt, row, std::integral_constant<int, 8>());
-    else if (E <= 256) f(dt, row, std::integral_constant<int, 16>());
-    else if (E <= 512) f(dt, row, std::integral_constant<int, 32>());
-    else f(dt, std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+    if (k <= 16) f(dt, row, v, std::integral_constant<int, 1>());
+    else f(dt, row, v, std::integral_constant<int, 4>());
+  };
+  auto by_experts = [&](auto dt) {
+    if (E <= 16) f(dt, std::integral_constant<int, 16>(), std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+    else if (E <= 32) by_choices(dt, std::integral_constant<int, 2>());
+    else if (E <= 64) by_choices(dt, std::integral_constant<int, 4>());
+    else if (E <= 128) by_choices(dt, std::integral_constant<int, 8>());
+    else if (E <= 256) by_choices(dt, std::integral_constant<int, 16>());
+    else if (E <= 512) by_choices(dt, std::integral_constant<int, 32>());
+    else f(dt, std::integral_constant<int, 64>(), std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
   };
   if (dtype == MXQ_DT_F32) by_experts(std::integral_constant<int, MXQ_DT_F32>());
   else if (dtype == MXQ_DT_BF16) by_experts(std::integral_constant<int, MXQ_DT_BF16>());
@@ -327,12 +363,12 @@ extern "C" int mxq_route(const void* logits, int32_t dtype, const float* bias, i
   if (int rc = check_spec("mxq_route", dtype, T, E, spec)) return rc;
   if (T == 0) return MXQ_OK;
   if (!logits || !weights || !experts) return invalid("mxq_route: NULL argument");
-  with_shape(dtype, E, [&](auto dt, auto lanes, auto v) {
+  with_shape(dtype, E, spec->top_k, [&](auto dt, auto lanes, auto v, auto slots) {
     constexpr int L = decltype(lanes)::value;
     const int threads = spec->groups > 1 && E > 256 ? 32 * kWaves : 64 * kWaves, tokens = threads / L;   // below 64 KB of LDS
     const size_t lds = spec->groups > 1 ? tokens * (size_t)(E + kMaxGroups) * sizeof(double) : 0;
     KernelTimer timer("k_route", as_stream(stream));
-    k_route<decltype(dt)::value, L, decltype(v)::value><<<dim3((unsigned)ceil_div(T, tokens)), threads, lds, as_stream(stream)>>>(
+    k_route<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(T, tokens)), threads, lds, as_stream(stream)>>>(
         logits, bias, T, (int)E, *spec, make_divu31((uint32_t)(E / spec->groups)), weights, experts);
   });
   return check_launch("mxq_route");
@@ -343,10 +379,10 @@ extern "C" int mxq_route_grad(const void* logits, int32_t dtype, const int32_t* 
   if (int rc = check_spec("mxq_route_grad", dtype, T, E, spec)) return rc;
   if (T == 0) return MXQ_OK;
   if (!logits || !experts || !grad || !out) return invalid("mxq_route_grad: NULL argument");
-  with_shape(dtype, E, [&](auto dt, auto lanes, auto v) {
+  with_shape(dtype, E, spec->top_k, [&](auto dt, auto lanes, auto v, auto slots) {
     constexpr int L = decltype(lanes)::value, kTokens = 64 * kWaves / L;
     KernelTimer timer("k_route_grad", as_stream(stream));
-    k_route_grad<decltype(dt)::value, L, decltype(v)::value><<<dim3((unsigned)ceil_div(T, kTokens)), 64 * kWaves, 0, as_stream(stream)>>>(
+    k_route_grad<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(T, kTokens)), 64 * kWaves, 0, as_stream(stream)>>>(
         logits, experts, grad, T, (int)E, *spec, out);
   });
   return check_launch("mxq_route_grad");

@@ -35,6 +35,15 @@ def _whole(value, who: str, what: str, low: int, high: int) -> int:
     return value
 
 
+def _once(backward):
+    """once_differentiable, without its context where no graph of the gradient is asked for."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 @_lib.memo_spec
 def _route_spec(E, top_k, score, groups, top_groups, renormalize, scale):
     _whole(E, "route", "the number of experts", 1, MAX_EXPERTS)
@@ -66,11 +75,14 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, experts)
         ctx.spec = spec
         ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)               # the experts' would be a tensor of zeros
         return weights, experts
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad, _):
+        if grad is None:
+            return None, None, None
         logits, experts = ctx.saved_tensors
         dev = logits.device
         grad = grad.to(torch.float32).contiguous()
@@ -183,7 +195,7 @@ class _Combine(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         y, weights, positions = ctx.saved_tensors
         T, k = positions.shape

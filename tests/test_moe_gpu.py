@@ -286,3 +286,48 @@ def test_route_to_combine_captured_in_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, step())
+
+
+def test_second_derivatives_are_refused(cuda):
+    """Not taken for zero: a graph of the gradient can be asked for, a derivative through it cannot."""
+    l = torch.randn(4, 8, device="cuda", requires_grad=True)
+    w, _ = nn.route(l, 2)
+    g = torch.autograd.grad(w.square().sum(), l, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    y = torch.randn(8, 5, device="cuda", requires_grad=True)
+    out = nn.combine(y, torch.rand(4, 2, device="cuda"), nn.dispatch(torch.zeros(4, 2, dtype=torch.int32, device="cuda"), 1))
+    g = torch.autograd.grad(out.square().sum(), y, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_forward_and_backward_captured_in_a_graph(cuda):
+    """A step with its gradients captured with no eager graph of its leaves alive; each replay equals an eager step."""
+    rng = np.random.default_rng(6)
+    l = _logits(rng, 40, 16, torch.float32).cuda().requires_grad_()
+    y = torch.randn(80, 24, device="cuda", requires_grad=True)
+    g = torch.randn(40, 24, device="cuda")
+
+    def step():
+        w, e = nn.route(l, 2)
+        out = nn.combine(y, w, nn.dispatch(e, 16))
+        return (out.detach(), *torch.autograd.grad(out, (l, y), g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(4):
+        with torch.no_grad():
+            l.normal_()
+            y.normal_()
+            g.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
