@@ -169,7 +169,7 @@ Plan plan_of(const LinearArgs& a) {
   p.tile.split = 1;
   if (!E) {
     const int64_t have = p.tiles_m * p.tiles_n, all = (int64_t)p.steps * p.planes;
-    while (p.tile.split < 8 && have * p.tile.split * 2 <= 512 && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
+    while (p.tile.split < 8 && have * p.tile.split * 2 <= (p.tile.shape == 0 ? 256 : 512) && all / (p.tile.split * 2) >= 8) p.tile.split *= 2;
   }
   p.lay_x = sp.x_dtype != MXQ_DT_BF16 || K % 8 || sp.ld_x % 8 || (uintptr_t)a.x % 16;
   p.x_rows = E && sp.top_k ? ceil_div(M, sp.top_k) : M;
