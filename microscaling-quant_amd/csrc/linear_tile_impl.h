@@ -11,6 +11,8 @@
 // goes through the weight once a plane.
 #pragma once
 
+#include <type_traits>
+
 #include "packed_linear_common.h"
 
 namespace mxq {
@@ -24,6 +26,9 @@ __device__ __forceinline__ void dma16(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(p) : "memory");
 }
 
+__device__ __forceinline__ void dma16(uint32_t to, const void* base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
 __device__ __forceinline__ void dma4(uint32_t base, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(base), "v"(p) : "memory");
 }
@@ -31,8 +36,9 @@ __device__ __forceinline__ void dma4(uint32_t base, const void* p) {
 // What a chunk past the last column is loaded from.
 static __device__ const u32x4 kNothing = {0, 0, 0, 0};
 
-// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; STAGES of 64 columns in LDS.
-template <int FAM, int BM, int BN, int WM, int WN, int STAGES>
+// FAM: code family; BM x BN rows; WM x WN of 32 x 32 tiles a wave; STAGES of 64 columns in LDS; FAR: a tile's rows lie 2^32
+// bytes apart or more.
+template <int FAM, int BM, int BN, int WM, int WN, int STAGES, bool FAR>
 __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k_linear_tile(TileArgs ta) {
   constexpr int WAVES_N = BN / (32 * WN), WAVES = BM / (32 * WM) * WAVES_N, THREADS = 64 * WAVES;
   constexpr int WB = 2 * kBlockBytes<FAM>, CH = WB / 16;                 // a weight row's bytes and chunks of one stage
@@ -92,21 +98,28 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
   const int first = (int)blockIdx.y * per, last = first + per < all ? first + per : all;
 
   if (!t.zeros && first < last) {
-    const uint8_t *xp[XL], *wp[WL], *sp[SC];
-    const uint8_t* codes = a.codes + t.expert * a.sp.batch_codes;
-    const uint8_t* scales = a.scales + t.expert * a.sp.batch_scales;
+    // A row's place from a scalar base, 32 bits of offset a lane where they suffice: a step then costs scalar additions only.
+    typedef typename std::conditional<FAR, int64_t, uint32_t>::type Offset;
+    Offset xo[XL], wo[WL], so[SC];
+    const uint8_t* x = (const uint8_t*)(ta.x + (a.sp.top_k ? 0 : t.row0 * ta.ld_x));
+    const uint8_t* codes = a.codes + t.expert * a.sp.batch_codes + n0 * a.sp.ld_codes;
+    const uint8_t* scales = a.scales + t.expert * a.sp.batch_scales + n0 * a.sp.ld_scales;
     const int xc = (tid & 7) ^ (tid >> 4 & 7);                           // this thread's chunk of a row, the same in all its rows
     const int wc = (tid % CH) ^ (CH == 4 ? tid >> 4 & 3 : tid >> 4 & 1);
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-      const int row = (i * THREADS + tid) >> 3;
-      xp[i] = (const uint8_t*)(ta.x + x_row(a, t.row0 + (row < t.rows ? row : t.rows - 1)) * ta.ld_x) + xc * 16;
+      const int row = (i * THREADS + tid) >> 3, r = row < t.rows ? row : t.rows - 1;
+      xo[i] = (Offset)((a.sp.top_k ? x_row(a, t.row0 + r) : r) * ta.ld_x * 2 + xc * 16);
     }
 #pragma unroll
-    for (int i = 0; i < WL; ++i) wp[i] = codes + weight_row((i * THREADS + tid) / CH) * a.sp.ld_codes + wc * 16;
+    for (int i = 0; i < WL; ++i) wo[i] = (Offset)((weight_row((i * THREADS + tid) / CH) - n0) * a.sp.ld_codes + wc * 16);
 #pragma unroll
-    for (int i = 0; i < SC; ++i) sp[i] = scales + weight_row((i * THREADS + tid) >> 2) * a.sp.ld_scales;
+    for (int i = 0; i < SC; ++i) so[i] = (Offset)((weight_row((i * THREADS + tid) >> 2) - n0) * a.sp.ld_scales);
 
+    auto load = [&](uint32_t to, const uint8_t* base, Offset offset) {
+      if constexpr (FAR) dma16(to, base + offset);
+      else dma16(to, base, offset);
+    };
     // A third of the next step's loads into stage b, in the order codes and scales, x, x: loads of a step issued at once
     // would keep the wave from its multiplications while the memory pipeline takes them.  The last step again after it, so
     // that every step waits for as many loads.
@@ -114,23 +127,35 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
     auto issue = [&](int b, int part) {
       const uint8_t* nothing = (const uint8_t*)&kNothing;
       if (part == 1 || part == 2) {
-        const uint32_t xo = lds_offset(stage[b].x) + wave * 1024;
-        const bool past = k * 64 + xc * 8 >= ta.x_columns;
+        const uint32_t to = lds_offset(stage[b].x) + wave * 1024;
+        const uint8_t* from = x + (int64_t)st * 128;
+        if (k * 64 + 64 <= ta.x_columns) {
 #pragma unroll
-        for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) dma16(xo + i * THREADS * 16, past ? nothing : xp[i] + (int64_t)st * 128);
+          for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) load(to + i * THREADS * 16, from, xo[i]);
+        } else {
+          const bool past = k * 64 + xc * 8 >= ta.x_columns;
+#pragma unroll
+          for (int i = (part - 1) * (XL / 2); i < part * (XL / 2); ++i) dma16(to + i * THREADS * 16, past ? nothing : from + xo[i]);
+        }
         return;
       }
       const int chunk = st - first;
       if ((chunk & 7) == 0) {
-        const uint32_t so = lds_offset(scale_ring) + (chunk >> 3 & 1) * BN * 16 + wave * 256;
+        const uint32_t to = lds_offset(scale_ring) + (chunk >> 3 & 1) * BN * 16 + wave * 256;
         const int two = (k + 2 * (tid & 3)) % ta.steps;
 #pragma unroll
-        for (int i = 0; i < SC; ++i) dma4(so + i * THREADS * 4, sp[i] + two * 2);
+        for (int i = 0; i < SC; ++i) dma4(to + i * THREADS * 4, scales + so[i] + two * 2);
       }
-      const uint32_t wo = lds_offset(stage[b].w) + wave * 1024;
-      const bool past = k * 64 + wc * (FAM == kPairs ? 32 : 16) >= ta.w_columns;
+      const uint32_t to = lds_offset(stage[b].w) + wave * 1024;
+      const uint8_t* from = codes + (int64_t)k * WB;
+      if (k * 64 + 64 <= ta.w_columns) {
 #pragma unroll
-      for (int i = 0; i < WL; ++i) dma16(wo + i * THREADS * 16, past ? nothing : wp[i] + (int64_t)k * WB);
+        for (int i = 0; i < WL; ++i) load(to + i * THREADS * 16, from, wo[i]);
+      } else {
+        const bool past = k * 64 + wc * (FAM == kPairs ? 32 : 16) >= ta.w_columns;
+#pragma unroll
+        for (int i = 0; i < WL; ++i) dma16(to + i * THREADS * 16, past ? nothing : from + wo[i]);
+      }
     };
     auto advance = [&]() {
       if (st + 1 < last) ++st, k = k + 1 == ta.steps ? 0 : k + 1;
@@ -367,9 +392,10 @@ __global__ __launch_bounds__(64 * (BM / (32 * WM)) * (BN / (32 * WN)), 2) void k
 template <int FAM> void launch_tile_family(const TileArgs& ta, const TilePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)(ta.tiles_m * ta.tiles_n), (unsigned)p.split);
   KernelTimer timer("k_linear_tile", st);
-  if (p.shape == 0) k_linear_tile<FAM, 256, 256, 4, 2, 3><<<grid, 512, 0, st>>>(ta);
-  else if (p.shape == 1) k_linear_tile<FAM, 128, 128, 2, 2, 3><<<grid, 256, 0, st>>>(ta);
-  else k_linear_tile<FAM, 64, 128, 1, 2, 3><<<grid, 256, 0, st>>>(ta);
+  if (p.shape == 0) k_linear_tile<FAM, 256, 256, 4, 2, 3, false><<<grid, 512, 0, st>>>(ta);
+  else if (p.shape == 1) k_linear_tile<FAM, 128, 128, 2, 2, 3, false><<<grid, 256, 0, st>>>(ta);
+  else if (p.shape == 2) k_linear_tile<FAM, 64, 128, 1, 2, 3, false><<<grid, 256, 0, st>>>(ta);
+  else k_linear_tile<FAM, 64, 128, 1, 2, 3, true><<<grid, 256, 0, st>>>(ta);
 }
 
 }  // namespace mxq

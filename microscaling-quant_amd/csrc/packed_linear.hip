@@ -140,7 +140,7 @@ struct Plan {
   int64_t at_codes, at_scales, at_partial, bytes;     // workspace: x, codes, scales, partial sums
 };
 
-constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128};
+constexpr int kTileM[4] = {256, 128, 64, 64}, kTileN[4] = {256, 128, 128, 128};
 
 // a.E = 0: one matrix.
 Plan plan_of(const LinearArgs& a) {
@@ -176,6 +176,15 @@ Plan plan_of(const LinearArgs& a) {
   p.w_rows = width;
   auto whole = [](int64_t bytes) { return ceil_div(bytes, 256) * 256; };
   const int64_t kp = (int64_t)p.steps * 64, matrices = (E ? E : 1) * width;
+  // a tile's rows from its first one (x's of experts: from the first of all)
+  const int64_t x_row = 2 * (p.lay_x ? kp * p.planes : sp.ld_x), w_row = p.lay_codes ? (pairs ? kp / 2 : kp) : sp.ld_codes;
+  const int64_t s_row = p.lay_scales ? kp / 32 : sp.ld_scales, apart = sp.gated ? N + 256 : 256;
+  const int64_t far = 0xFFFF0000;
+  if (x_row > far / (E && sp.top_k ? p.x_rows : 256) || w_row > far / apart || s_row > far / apart) {
+    p.tile.shape = 3;                                                    // the same sums: a split and its order are the others'
+    p.tiles_m = row_tiles(kTileM[3]);
+    p.tiles_n = ceil_div(width, kTileN[3]);
+  }
   p.at_codes = p.lay_x ? whole(p.x_rows * p.planes * kp * 2) : 0;
   p.at_scales = p.at_codes + (p.lay_codes ? whole(matrices * (pairs ? kp / 2 : kp)) : 0);
   p.at_partial = p.at_scales + (p.lay_scales ? whole(matrices * (kp / 32)) : 0);

@@ -78,7 +78,7 @@ __device__ __forceinline__ RowTile row_tile(const LinearArgs& a, int BM, int ind
     rows = offset(e + 1) - row0;
     if (rows > BM) rows = BM;
   }
-  e = __shfl(e, owner), row0 = __shfl(row0, owner), rows = __shfl(rows, owner);
+  e = __builtin_amdgcn_readlane(e, owner), row0 = __builtin_amdgcn_readlane(row0, owner), rows = __builtin_amdgcn_readlane(rows, owner);
   return RowTile{e == a.E ? 0 : e, rows, row0, e == a.E};
 }
 
@@ -176,7 +176,7 @@ struct TileArgs {
 };
 
 struct TilePlan {
-  int shape;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128
+  int shape;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128, 3: as 2, for rows 2^32 bytes apart
   int split;
 };
 
