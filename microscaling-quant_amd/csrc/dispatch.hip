@@ -27,20 +27,39 @@ __global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* expert
   if (wave < used)
     for (int e = lane; e <= E; e += 64) mine[e] = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += kSortThreads * kAhead) {
-    int e[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) e[u] = i + u * kSortThreads < n ? experts[i + u * kSortThreads] : 0;
+  const int own = first + lane < last ? experts[first + lane] : 0;
+  typedef int int4_any __attribute__((ext_vector_type(4), aligned(4)));
+  // 16 slots a thread asked for at once; a single workgroup's runs are the whole array
+  for (int i = gridDim.x > 1 ? tid * 4 : n; i < n; i += kSortThreads * 4 * kAhead) {
+    int4_any e[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int at = i + u * kSortThreads;
-      if (at < n) atomicAdd(at < begin ? &before_me[key_of(e[u])] : &others[key_of(e[u])], 1);
+      const int at = i + u * kSortThreads * 4;
+      if (at + 4 <= n) {
+        e[u] = *(const int4_any*)(experts + at);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) e[u][c] = at + c < n ? experts[at + c] : 0;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int at = i + u * kSortThreads * 4 + c;
+        if (at < n) atomicAdd(at < begin ? &before_me[key_of(e[u][c])] : &others[key_of(e[u][c])], 1);
+      }
   }
-  for (int i = first + lane; i < last; i += 64) atomicAdd(&place[wave][key_of(experts[i])], 1);
+  if (first + lane < last) atomicAdd(&place[wave][key_of(own)], 1);
+  for (int i = first + lane + 64; i < last; i += 64) atomicAdd(&place[wave][key_of(experts[i])], 1);
   __syncthreads();
   // one expert a thread: its count, the prefix over the experts, then the runs' places; slots of none follow all others
-  const int c = tid < E ? before_me[tid] + others[tid] : 0;
+  int c = 0;
+  if (tid < E) {
+    c = before_me[tid] + others[tid];
+    if (gridDim.x == 1)
+      for (int w = 0; w < used; ++w) c += place[w][tid];
+  }
   int p = c;
   for (int o = 1; o < 64; o <<= 1) {
     const int q = __shfl_up(p, o);
@@ -258,7 +277,7 @@ using namespace mxq;
 
 extern "C" int mxq_dispatch(const int32_t* experts, int64_t n, int64_t E, int32_t* order, int32_t* offsets,
                             int32_t* positions, mxq_stream_t stream) {
-  if (n < 0 || n > 0x7fffffff - 2 * kSortThreads * kAhead) return invalid("mxq_dispatch: n out of range");
+  if (n < 0 || n > 0x7fffffff - 8 * kSortThreads * kAhead) return invalid("mxq_dispatch: n out of range");
   if (E < 1 || E > kMaxExperts) return invalid("mxq_dispatch: 1 to 1024 experts");
   if (!offsets || (n && (!experts || !order || !positions))) return invalid("mxq_dispatch: NULL argument");
   int bits = 0;
