@@ -13,6 +13,7 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kAhead = 4;
 // launch and a workspace), and each wave its own run's; prefix sums over the experts and the waves turn the counts into the
 // places where each wave's slots go.  A slot's rank among its wave's equal ones is a population count of the lanes with
 // the same key, which ballots over the key's bits find.  Integer sums throughout: the same order whatever the timing.
+// 16384 slots of 32 experts 8.6 us, 32 slots 3.7: round trips to memory.
 __global__ __launch_bounds__(kSortThreads) void k_dispatch(const int32_t* experts, int n, int E, int bits, int run,
                                                            int32_t* order, int32_t* offsets, int32_t* positions) {
   __shared__ int place[kSortWaves][kMaxExperts + 1];
@@ -146,7 +147,7 @@ template <int DT> struct Pack {
 constexpr int kRows = 4;                                          // experts' rows in flight
 
 // out[t] = residual[t] + sum_j w[t, j] y[position[t, j]] in float32, j in order, rounded once.  Reading y bounds it: 16
-// bytes a thread, four rows' loads in flight before the first is added.
+// bytes a thread, four rows' loads in flight before the first is added.  4096 tokens x 4 x 2048 bfloat16 22.4 us, 4.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y_, const float* weights, const int32_t* positions,
                                                                    const void* residual_, void* out_, int64_t T, int k, int64_t D) {
   typedef Pack<DT> P;
@@ -196,7 +197,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y
 }
 
 // dy[position] = w g[t] (zeros for a slot of no expert), dw = <g[t], y[position]>: a workgroup a token, the gradient's row
-// read once for four slots, their rows' loads in flight together.
+// read once for four slots, their rows' loads in flight together.  4096 tokens x 4 x 2048 bfloat16 29.8 us, 5.1 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void k_combine_grad(const void* grad_, const void* y_, const float* weights,
                                                                         const int32_t* positions, void* dy_, float* dw, int64_t T,
                                                                         int k, int64_t D) {

@@ -8,8 +8,8 @@
 // of two and three bfloat16, also exact, one product each.  The waves' sums meet in LDS, in the order of the waves; biases
 // and residual are asked for at the start.
 //
-// Measured, us: 4096 x 4096 in E4M3 with one row 7.7 (2.2 TB/s; a launch and two trips to memory are what is left), 8
-// experts of 4096 x 4096 35 (3.8 TB/s).  Eight waves a workgroup, or four where there are workgroups enough to fill the
+// Measured, us: 4096 x 4096 in E4M3 with one row 7.2 (2.4 TB/s; a launch and two trips to memory are what is left), 8
+// experts of 4096 x 4096 36 (3.8 TB/s).  Eight waves a workgroup, or four where there are workgroups enough to fill the
 // card four times: 37 against 40 there, 9.0 against 8.3 for the one row.
 #pragma once
 

@@ -9,7 +9,8 @@
 //
 // Up to 512 experts a token has 16 lanes, so that a maximum over its lanes is four rotations within a row of lanes and a
 // wave chooses for four tokens at once; beyond, a whole wave.  Expert e is register e / L of lane e % L.  What bounds it is
-// instructions: about 25 for a score and seven a register and choice.
+// instructions: about 25 for a score and seven a register and choice (16384 tokens of 256 experts in 8
+// groups, 8 choices: 23.9 us; reading the logits would take 4).
 #include "mxq_common.h"
 
 namespace mxq {
