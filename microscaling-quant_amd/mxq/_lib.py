@@ -290,18 +290,19 @@ def numel(shape: Sequence[int]) -> int:
     return n
 
 
+def _function(name: str):
+    load()
+    return _FN[name] if name in _FN else getattr(load(), name)
+
+
 def call(name: str, *args):
     """Call entry point `name` with args; its result."""
-    fn = _FN.get(name)
-    if fn is None:
-        load()
-        fn = _FN[name] if name in _FN else getattr(load(), name)
-    return fn(*args)
+    return (_FN.get(name) or _function(name))(*args)
 
 
 def run(name: str, *args) -> None:
     """Call entry point `name` with args; raise RuntimeError on a nonzero status."""
-    rc = call(name, *args)
+    rc = (_FN.get(name) or _function(name))(*args)
     if rc != 0:
         check(rc, name)
 

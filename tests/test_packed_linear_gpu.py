@@ -321,3 +321,26 @@ def test_layer_captured_in_a_graph(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, layer())
+
+
+def _far(t, stride):
+    """t's rows `stride` elements apart."""
+    there = torch.empty((t.shape[0] - 1) * stride + t.shape[1], dtype=t.dtype, device="cuda").as_strided(t.shape, (stride, 1))
+    return there.copy_(t)
+
+
+def test_rows_2_32_bytes_apart(cuda):
+    """Tiles whose rows' offsets need more than 32 bits: the same bits as of neighbouring rows."""
+    rng = np.random.default_rng(30)
+    for K in (256, 200):
+        codes, scales = (t.cuda() for t in _weight(rng, (150, K), "MXFP8_E4M3"))
+        x = torch.from_numpy(rng.standard_normal((130, K))).to(torch.bfloat16).cuda()
+        want = nn.packed_linear(x, codes, scales, "MXFP8_E4M3")
+        assert torch.equal(nn.packed_linear(x, _far(codes, 1 << 25), scales, "MXFP8_E4M3"), want)
+        assert torch.equal(nn.packed_linear(_far(x, 1 << 24), codes, scales, "MXFP8_E4M3"), want)
+        gated = nn.packed_linear(x, codes, scales, "MXFP8_E4M3", activation="silu", gated=True)
+        assert torch.equal(nn.packed_linear(x, _far(codes, 1 << 25), scales, "MXFP8_E4M3", activation="silu", gated=True), gated)
+        experts, es = (t.cuda() for t in _weight(rng, (3, 96, K), "MXFP8_E4M3"))
+        plan = nn.dispatch(torch.from_numpy(rng.integers(0, 3, (130, 2))).cuda(), 3)
+        want = nn.expert_linear(x, experts, es, "MXFP8_E4M3", plan)
+        assert torch.equal(nn.expert_linear(_far(x, 1 << 24), experts, es, "MXFP8_E4M3", plan), want)
