@@ -12,6 +12,7 @@ built library, every computing call raises RuntimeError.
 import contextlib
 import ctypes
 import functools
+import numbers
 import os
 import threading
 from typing import Optional, Sequence
@@ -210,18 +211,36 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     return _lib
 
 
+def _is_value(a) -> bool:
+    """Whether a stays what it is and compares by it: not so a tensor, which is equal to itself after a change."""
+    if isinstance(a, tuple):
+        return all(map(_is_value, a))
+    frozen = getattr(type(a), "__dataclass_params__", None)
+    return isinstance(a, (numbers.Number, str, type(None), torch.dtype)) or (frozen is not None and frozen.frozen)
+
+
+class _Afresh(Exception):
+    pass
+
+
 def memo_spec(make):
     """make, remembered per positional arguments (their types included): a spec struct is only read once built,
     and building one, with the reference's argument checks, costs about a microsecond of every call.  Arguments
-    that cannot be hashed are built afresh; errors are raised as make raises them."""
-    cached = functools.lru_cache(maxsize=512, typed=True)(make)
+    that are no plain values (_is_value; looked at only where nothing is remembered) are built afresh; errors are
+    raised as make raises them."""
+    @functools.lru_cache(maxsize=512, typed=True)
+    def cached(*args):
+        if not _is_value(args):
+            raise _Afresh                      # an exception is not remembered
+        return make(*args)
 
     @functools.wraps(make)
     def spec(*args):
         try:
             return cached(*args)
-        except TypeError:
-            return make(*args)
+        except (TypeError, _Afresh):
+            pass
+        return make(*args)
     return spec
 
 

@@ -152,3 +152,20 @@ def test_c_entries_refuse():
     refused("NULL", "mxq_expert_linear", buf, buf, buf, 0, buf, 4, 8, 64, 2, buf, 0, lin, 0, 0)
     lin.top_k = 65
     refused("top_k", "mxq_expert_linear", buf, buf, buf, 0, buf, 4, 8, 64, 2, buf, buf, lin, 0, 0)
+
+
+def test_specs_are_remembered_by_value():
+    """A scale held in a tensor is read in every call: a tensor's hash is its identity, which a change in place keeps."""
+    from mxq.nn._moe import _route_spec
+    scale = torch.tensor(2.5)
+    assert _route_spec(8, 2, "softmax", 1, 1, True, scale).scale == 2.5
+    scale.mul_(2)
+    assert _route_spec(8, 2, "softmax", 1, 1, True, scale).scale == 5.0
+    assert _route_spec(8, 2, "softmax", 1, 1, True, 2.5) is _route_spec(8, 2, "softmax", 1, 1, True, 2.5)
+    from mxq.block import mxgemmini
+    from mxq.element_quant.formats import get
+    f, floor = get("MXFP8_E4M3"), torch.tensor(0.5)
+    assert mxgemmini.spec(f, "ties_away", floor, None).scale_floor == 0.5
+    floor.fill_(0.25)
+    assert mxgemmini.spec(f, "ties_away", floor, None).scale_floor == 0.25
+    assert mxgemmini.spec(f, "ties_away", 0.5, None) is mxgemmini.spec(f, "ties_away", 0.5, None)
