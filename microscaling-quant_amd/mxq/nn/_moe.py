@@ -6,11 +6,12 @@ are the layer between two attention cores of a mixture-of-experts model.
     y = expert_linear(x, codes, scales, fmt, plan)        a row a slot, in the experts' order
     out = combine(y, weights, plan, residual=shared)      T x D
 
-route and combine are differentiable, in the logits, and in y, the weights and the residual.
+route and combine are differentiable once and in reverse mode, in the logits, and in y, the weights and the residual.
 """
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -27,6 +28,15 @@ def _dtype(t: torch.Tensor, who: str, what: str) -> int:
     if code is None:
         raise TypeError(f"mxq.nn.{who}: {what} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
+
+
+def _no_tangent(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses inputs of forward-mode differentiation, which do not ask for a gradient and whose tangent a kernel on
+    raw pointers would drop."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"mxq.nn.{who}: no forward-mode derivative")
 
 
 def _whole(value, who: str, what: str, low: int, high: int) -> int:
@@ -111,6 +121,7 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
         raise ValueError("mxq.nn.route: logits must have an experts axis")
     E = logits.shape[-1]
     spec = _route_spec(E, top_k, score, groups, top_groups, renormalize, scale)
+    _no_tangent("route", logits)
     if bias is not None and tuple(bias.shape) != (E,):
         raise ValueError(f"mxq.nn.route: bias must hold {E} values, got shape {tuple(bias.shape)}")
     dev = _lib.compute_device(logits)
@@ -226,6 +237,7 @@ def combine(y: torch.Tensor, weights: torch.Tensor, plan: Dispatch,
     if residual is not None and (tuple(residual.shape) != (T, y.shape[1]) or residual.dtype != y.dtype):
         raise ValueError(f"mxq.nn.combine: residual must be {T} x {y.shape[1]} {y.dtype}, got "
                          f"{tuple(residual.shape)} {residual.dtype}")
+    _no_tangent("combine", y, weights, residual)
     dev = _lib.compute_device(y, weights)
     yd = _lib.to_device(y, dev).contiguous()
     wd = _lib.to_device(weights, dev).to(torch.float32).contiguous()

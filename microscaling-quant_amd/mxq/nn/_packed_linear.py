@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from ..element_quant.formats import Format, get
-from ._moe import MAX_EXPERTS, Dispatch, _check_plan, _dtype
+from ._moe import MAX_EXPERTS, Dispatch, _check_plan, _dtype, _no_tangent
 
 __all__ = ["packed_linear", "expert_linear", "ACTIVATIONS"]
 
@@ -47,6 +47,7 @@ def _weight(fmt, codes_shape, codes_dtype, scales_shape, scales_dtype, K, ndim, 
 
 
 def _no_grad(who: str, *tensors) -> None:
+    _no_tangent(who, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

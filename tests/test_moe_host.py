@@ -169,3 +169,26 @@ def test_specs_are_remembered_by_value():
     floor.fill_(0.25)
     assert mxgemmini.spec(f, "ties_away", floor, None).scale_floor == 0.25
     assert mxgemmini.spec(f, "ties_away", 0.5, None) is mxgemmini.spec(f, "ties_away", 0.5, None)
+
+
+def test_forward_mode_tangents_are_refused():
+    """An input of forward-mode differentiation does not ask for a gradient; its tangent must not be taken for zero."""
+    from torch.autograd import forward_ad
+
+    dual = lambda *shape: forward_ad.make_dual(torch.zeros(shape), torch.ones(shape))
+    packed = dict(codes=_u8(6, 64), scales=_u8(6, 2), fmt="MXFP8_E4M3")
+    experts = dict(codes=_u8(4, 6, 64), scales=_u8(4, 6, 2), fmt="MXFP8_E4M3", plan=_plan())
+    plain = torch.zeros
+    with forward_ad.dual_level():
+        for call in (lambda: nn.route(dual(3, 8), 2),
+                     lambda: nn.combine(dual(6, 4), plain(3, 2), _plan()),
+                     lambda: nn.combine(plain(6, 4), dual(3, 2), _plan()),
+                     lambda: nn.combine(plain(6, 4), plain(3, 2), _plan(), residual=dual(3, 4)),
+                     lambda: nn.packed_linear(dual(5, 64), **packed),
+                     lambda: nn.packed_linear(plain(5, 64), **packed, bias=dual(6)),
+                     lambda: nn.packed_linear(plain(5, 64), **packed, residual=dual(5, 6)),
+                     lambda: nn.expert_linear(dual(3, 64), **experts),
+                     lambda: nn.expert_linear(plain(3, 64), **experts, bias=dual(4, 6))):
+            for grad in (True, False):                 # torch.no_grad does not end forward mode
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
