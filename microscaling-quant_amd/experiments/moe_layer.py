@@ -33,15 +33,13 @@ class MoELayer:
         return cls(router, pack(gate_up), pack(down), pack(shared_up), pack(shared_down), fmt=fmt, **more)
 
     def _experts(self, x, experts):
-        with torch.no_grad():
-            x = x.detach()
-            plan = nn.dispatch(experts, self.router.shape[0])
-            h = nn.expert_linear(x, *self.gate_up, self.fmt, plan, activation="silu", gated=True)
-            y = nn.expert_linear(h, *self.down, self.fmt, plan, sorted_rows=True)
-            shared = None
-            if self.shared_up is not None:
-                s = nn.packed_linear(x, *self.shared_up, self.fmt, activation="silu", gated=True)
-                shared = nn.packed_linear(s, *self.shared_down, self.fmt)
+        plan = nn.dispatch(experts, self.router.shape[0])
+        h = nn.expert_linear(x, *self.gate_up, self.fmt, plan, activation="silu", gated=True)
+        y = nn.expert_linear(h, *self.down, self.fmt, plan, sorted_rows=True)
+        shared = None
+        if self.shared_up is not None:
+            s = nn.packed_linear(x, *self.shared_up, self.fmt, activation="silu", gated=True)
+            shared = nn.packed_linear(s, *self.shared_down, self.fmt)
         return plan, y, shared
 
     def __call__(self, x):
@@ -50,8 +48,9 @@ class MoELayer:
         return nn.combine(y, weights, plan, residual=shared)
 
     def router_gradient(self, x, grad_y):
-        """The gradient of the router's weight; the experts' weights are bytes and have none."""
-        router = self.router.detach().requires_grad_()
+        """The gradient of the router's weight; the experts' weights are bytes and have none, nor do their
+        products have one of x, so that a call refuses an x that asks for it."""
+        router, x = self.router.detach().requires_grad_(), x.detach()
         weights, experts = nn.route((x @ router.t()).float(), self.top_k, **self.routing)
         plan, y, shared = self._experts(x, experts)
         return torch.autograd.grad(nn.combine(y, weights, plan, residual=shared), router, grad_y)[0]

@@ -192,3 +192,13 @@ def test_forward_mode_tangents_are_refused():
             for grad in (True, False):                 # torch.no_grad does not end forward mode
                 with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                     call()
+
+
+def test_layer_refuses_an_input_that_asks_for_a_gradient(monkeypatch):
+    """The experts' products have no gradient of x: the router's share of it alone must not pass for the whole."""
+    from experiments import moe_layer
+    monkeypatch.setattr(moe_layer.nn, "route", lambda l, k: (torch.zeros(3, k), torch.zeros(3, k, dtype=torch.int32)))
+    monkeypatch.setattr(moe_layer.nn, "dispatch", lambda e, n: _plan(3, 2, n))
+    layer = moe_layer.MoELayer(torch.zeros(4, 64), (_u8(4, 12, 64), _u8(4, 12, 2)), (_u8(4, 64, 6), _u8(4, 64, 1)))
+    with pytest.raises(RuntimeError, match="torch.no_grad"):
+        layer(torch.zeros(3, 64, requires_grad=True))
