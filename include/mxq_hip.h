@@ -508,7 +508,9 @@ int mxq_dispatch(const int32_t* experts, int64_t n, int64_t E, int32_t* order, i
 
 /* out (T x D) = residual (NULL: none) + sum over j of weights[t, j] y[positions[t, j]], summed in float32 in the order
  * of j and rounded once; y (T k x D), residual and out of one dtype.  A slot of no expert adds nothing, unless its
- * weight is NaN.  mxq_combine_grad: dy (T k x D, zeros for slots of no expert) and dw (T x k float32), either NULL. */
+ * weight is NaN; so does a position past the last row, which mxq_dispatch does not write.  mxq_combine_grad: dy
+ * (T k x D, zeros for slots of no expert; rows that no position names are left as they are) and dw (T x k float32),
+ * either NULL. */
 int mxq_combine(const void* y, int32_t dtype, const float* weights, const int32_t* positions, const void* residual,
                 void* out, int64_t T, int64_t k, int64_t D, mxq_stream_t stream);
 int mxq_combine_grad(const void* grad, int32_t dtype, const void* y, const float* weights, const int32_t* positions,

@@ -146,6 +146,10 @@ template <int DT> struct Pack {
 
 constexpr int kRows = 4;                                          // experts' rows in flight
 
+// The row of y at a slot's position, -1 for a slot of none: a position past the rows is the caller's mistake, which must
+// not reach memory.
+__device__ __forceinline__ int row_of(int position, int rows) { return position < rows ? position : -1; }
+
 // out[t] = residual[t] + sum_j w[t, j] y[position[t, j]] in float32, j in order, rounded once.  Reading y bounds it: 16
 // bytes a thread, four rows' loads in flight before the first is added.  4096 tokens x 4 x 2048 bfloat16 22.4 us, 4.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y_, const float* weights, const int32_t* positions,
@@ -169,7 +173,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y
       for (int j = 0; j < kRows; ++j) {
         const bool in = j0 + j < k;
         w[j] = in ? weights[t * k + j0 + j] : 0.0f;
-        p[j] = in ? positions[t * k + j0 + j] : -1;
+        p[j] = in ? row_of(positions[t * k + j0 + j], (int)(T * k)) : -1;
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
@@ -212,12 +216,13 @@ template <int DT> __global__ __launch_bounds__(256) void k_combine_grad(const vo
     for (int j0 = 0; j0 < k; j0 += kRows, turn ^= 1) {
       float w[kRows], dot[kRows];
       int64_t at[kRows];
-      bool live[kRows];
+      bool there[kRows], live[kRows];                             // a row of dy, one of y
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int p = j0 + j < k ? positions[t * k + j0 + j] : 0;
-        live[j] = j0 + j < k && p >= 0;
-        at[j] = (p >= 0 ? p : -1 - (int64_t)p) * D;
+        const int p = j0 + j < k ? positions[t * k + j0 + j] : 0, row = p < 0 ? -1 - p : p;
+        there[j] = j0 + j < k && row < T * k;
+        live[j] = there[j] && p >= 0;
+        at[j] = (int64_t)row * D;
         w[j] = live[j] ? weights[t * k + j0 + j] : 0.0f;
         dot[j] = 0.0f;
       }
@@ -234,7 +239,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_combine_grad(const vo
 #pragma unroll
             for (int e = 0; e < P::N; ++e) dot[j] = __builtin_fmaf((float)g.v[e], (float)row[j].v[e], dot[j]);
           }
-          if (dy && j0 + j < k) {
+          if (dy && there[j]) {
             P o;
 #pragma unroll
             for (int e = 0; e < P::N; ++e) o.v[e] = (E)(live[j] ? w[j] * (float)g.v[e] : 0.0f);

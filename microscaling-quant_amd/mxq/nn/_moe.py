@@ -225,7 +225,8 @@ def combine(y: torch.Tensor, weights: torch.Tensor, plan: Dispatch,
     """residual + sum_j weights[t, j] * (the row of y that token t's j-th slot has in plan): tokens x D in y's dtype.
 
     y: n x D in the experts' order.  The sum is float32, in the order of j, and rounded once.  A slot of no expert adds
-    nothing, unless its weight is NaN, which the token's output then is."""
+    nothing, unless its weight is NaN, which the token's output then is; a position past y's rows, which no plan of
+    dispatch's holds, is taken as one of no expert."""
     _check_plan(plan, "combine")
     _dtype(y, "combine", "y")
     T, k = plan.positions.shape

@@ -331,3 +331,37 @@ def test_forward_and_backward_captured_in_a_graph(cuda):
         torch.cuda.synchronize()
         for a, b in zip(captured, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("T, k, D", [(3, 2, 40), (5, 7, 33)])
+def test_combine_holds_positions_to_the_rows(cuda, T, k, D, dtype):
+    """Positions past the last row, in a plan that is not dispatch's: as slots of no expert, and nothing outside y and dy is
+    read or written."""
+    from mxq import _lib
+    rng = np.random.default_rng(D)
+    n, dt = T * k, _lib.DTYPE_CODE[DTYPES[dtype]]
+    place = torch.from_numpy(rng.permutation(n).astype(np.int32)).reshape(T, k)
+    far = torch.from_numpy(rng.integers(0, 3, (T, k))) == 0
+    far[0, 0], far[0, 1] = True, False
+    held = torch.where(far, torch.tensor(-1, dtype=torch.int32), place).cuda()
+    wild = torch.tensor([n, n + 1, 2 ** 31 - 1, n + 5], dtype=torch.int32)[torch.from_numpy(rng.integers(0, 4, (T, k)))]
+    place = torch.where(far, wild, place)
+    place[far & (torch.from_numpy(rng.integers(0, 2, (T, k))) == 0)] = -2 ** 31          # a slot of none, its row far away too
+    around = torch.full((n + 8, D), float("nan"), dtype=DTYPES[dtype], device="cuda")
+    around[:n].normal_()
+    y, g = around[:n], torch.randn(T, D, device="cuda").to(DTYPES[dtype])
+    w = torch.rand(T, k, device="cuda")
+    offsets = torch.zeros(2, dtype=torch.int32, device="cuda")
+    plan = nn.Dispatch(torch.zeros(n, dtype=torch.int32, device="cuda"), offsets, place.cuda())
+    assert torch.equal(nn.combine(y, w, plan), nn.combine(y, w, plan._replace(positions=held)))
+    dy, dw = torch.full_like(around, 7), torch.empty(T, k, device="cuda")
+    _lib.run("mxq_combine_grad", g.data_ptr(), dt, y.data_ptr(), w.data_ptr(), plan.positions.data_ptr(), dy.data_ptr(), dw.data_ptr(), T, k, D,
+             _lib.stream(torch.device("cuda", 0)))
+    named = torch.zeros(n + 8, dtype=torch.bool)
+    named[place[~far].long()] = True
+    assert (dy[~named.cuda()] == 7).all()
+    _, want = torch.autograd.grad(nn.combine(y.requires_grad_(), w.requires_grad_(), plan._replace(positions=held)), (y, w), g)
+    assert torch.equal(dw, want) and (dw.cpu()[far] == 0).all() and (dw.cpu()[~far] != 0).all()
+    for t, j in torch.nonzero(~far).tolist():
+        assert torch.equal(dy[place[t, j].item()], (w[t, j].detach() * g[t].float()).to(DTYPES[dtype]))
