@@ -161,20 +161,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_linear_skinny(LinearArgs a, C
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          uint32_t left, f[kWords<FAM>];
-          const float scale = scale_of<FAM>(s[u][i], map, left);
-          if constexpr (P > 1 && FAM == kE5M2) {                       // an infinite weight meets no zero of a lower plane
-#pragma unroll
-            for (int c = 0; c < 8; ++c) f[c] = without_infinities(w[u][i][c], ~0u);
-          }
+          uint32_t left;
+          const float scale = scale_of<FAM>(s[u][i], w[u][i], map, left, P > 1);
+          const bool seldom = (FAM == kMapped || P > 1) && __builtin_expect(__any(left), 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             bf16x8 wv = eight<FAM>(w[u][i], scale, j, map), xv[P];
-            if (FAM == kMapped && __builtin_expect(__any(left), 0)) apply_left(wv, left);
+            if (FAM == kMapped && seldom) apply_left(wv, left);
             x[u].planes(j, xv);
             acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[0], acc[i], 0, 0, 0);
             if constexpr (P > 1) {
-              if constexpr (FAM == kE5M2) wv = eight<FAM>(f, scale, j, map);
+              if (seldom) finite_only(wv);
 #pragma unroll
               for (int p = 1; p < P; ++p) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[p], acc[i], 0, 0, 0);
             }

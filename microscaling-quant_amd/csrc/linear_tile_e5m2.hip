@@ -1,8 +1,5 @@
 #include "linear_tile_impl.h"
 
 namespace mxq {
-void launch_tile_e5m2(const TileArgs& a, const TilePlan& p, hipStream_t st) {
-  if (a.planes > 1) launch_tile_family<kE5M2Wide>(a, p, st);
-  else launch_tile_family<kE5M2>(a, p, st);
-}
+void launch_tile_e5m2(const TileArgs& a, const TilePlan& p, hipStream_t st) { launch_tile_family<kE5M2>(a, p, st); }
 }  // namespace mxq

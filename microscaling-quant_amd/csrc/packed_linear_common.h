@@ -98,8 +98,7 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));       // at any address
 
 // How a format's bytes become bfloat16.  kMapped: the formats of 4 and 6 bits a byte, put into E4M3's fields first.
-// kE5M2Wide: E5M2 under activations of several planes, whose lower ones see zeros in the place of infinities.
-enum Family { kE4M3 = 0, kE5M2 = 1, kMapped = 2, kPairs = 3, kE5M2Wide = 4 };
+enum Family { kE4M3 = 0, kE5M2 = 1, kMapped = 2, kPairs = 3 };
 
 // 32 codes of one row with one scale: eight words, four of MXFP4's pairs.
 template <int FAM> constexpr int kWords = FAM == kPairs ? 4 : 8;
@@ -118,21 +117,46 @@ inline CodeMap code_map(int format) {
   return CodeMap{0x07070707u, 2, 4, 6};
 }
 
-// The E8M0 byte as the conversions take it: a float's exponent field, 0 standing for 2^-127 and 255 for NaN.  kMapped: a
-// scale past 2^127 with the map's power leaves the excess in `left` for apply_left.
-template <int FAM> __device__ __forceinline__ float scale_of(uint32_t s, const CodeMap& map, uint32_t& left) {
+// Activations of several planes meet an infinite weight in the first one; the lower ones, which are zero where an activation
+// has no more bits, see the largest finite value in its place (finite_only), or zero times infinity would make a NaN.  From
+// this scale byte on a code's largest value is 2^128 or more, infinite in bfloat16 as in float32; a value of a code's few
+// bits below 2^128 is finite in both.
+template <int FAM> constexpr uint32_t kPastFloat = FAM == kE4M3 ? 247 : FAM == kE5M2 ? 240 : FAM == kMapped ? 251 : 253;
+constexpr uint32_t kFinite = 0x80000000u;
+
+// The E8M0 byte as the conversions take it: a float's exponent field, 0 standing for 2^-127 and 255 for NaN.  `left` holds
+// what a block seldom needs besides.  kMapped: the excess of a scale past 2^127 with the map's power, for apply_left.
+// lower, the block's codes for a lower plane: a bit above the lowest eight where one of them may be an infinity.
+template <int FAM> __device__ __forceinline__ float scale_of(uint32_t s, const uint32_t (&codes)[kWords<FAM>], const CodeMap& map,
+                                                             uint32_t& left, bool lower) {
   left = 0;
+  uint32_t infinite = s >= kPastFloat<FAM> ? kFinite : 0;
   if constexpr (FAM == kMapped) {
     const uint32_t t = s + map.power;
     left = s != 255 && t > 254 ? t - 254 : 0;
     s = s == 255 ? 255 : t < 254 ? t : 254;
   }
+  if constexpr (FAM == kE5M2) {
+    uint32_t none = ~0u;                                           // a byte's highest bit: no code 0x7C or 0xFC there
+#pragma unroll
+    for (int i = 0; i < kWords<FAM>; ++i) none &= ((codes[i] & 0x7F7F7F7Fu) ^ 0x7C7C7C7Cu) + 0x7F7F7F7Fu;
+    infinite |= (~none & 0x80808000u) | (~none & 0x80u) << 1;
+  }
+  if (lower) left |= infinite;
   return __uint_as_float(s << 23);
 }
 __device__ __forceinline__ void apply_left(bf16x8& w, uint32_t left) {
-  const float more = __uint_as_float((127 + left) << 23);
+  const float more = __uint_as_float((127 + (left & 255)) << 23);
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = (__bf16)((float)w[i] * more);
+}
+// Magnitudes past bfloat16's largest become it, NaN too, which the first plane has shown.
+__device__ __forceinline__ void finite_only(bf16x8& w) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 u;
+  __builtin_memcpy(&u, &w, 16);
+  u = __builtin_elementwise_min(u & (uint16_t)0x7FFF, (u16x8)(uint16_t)0x7F7F) | (u & (uint16_t)0x8000);
+  __builtin_memcpy(&w, &u, 16);
 }
 
 // The j-th eight of the 32 codes as bfloat16, times the scale: exact (a code has at most 4 significant bits), but for
@@ -148,7 +172,7 @@ template <int FAM> __device__ __forceinline__ bf16x8 eight(const uint32_t (&w)[k
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       uint32_t c = w[2 * j + i];
-      if constexpr (FAM == kE5M2 || FAM == kE5M2Wide) {
+      if constexpr (FAM == kE5M2) {
         v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(c, scale, false);
         v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(c, scale, true);
       } else {
@@ -179,12 +203,6 @@ struct TilePlan {
   int shape;              // 0: 256 x 256, 1: 128 x 128, 2: 64 x 128, 3: as 2, for rows 2^32 bytes apart
   int split;
 };
-
-// E5M2's codes, the infinities' bits under `drop` cleared.
-__device__ __forceinline__ uint32_t without_infinities(uint32_t w, uint32_t drop) {
-  const uint32_t z = ~(((w & 0x7F7F7F7Fu) ^ 0x7C7C7C7Cu) + 0x7F7F7F7Fu) & 0x80808080u;     // 0x80 in the bytes that hold one
-  return w & ~(((z << 1) - (z >> 7)) & drop);
-}
 
 // 16 bytes of which the first `valid` exist; zeros for the others.
 __device__ __forceinline__ u32x4 load_part(const uint8_t* p, int valid) {
