@@ -301,7 +301,7 @@ extern "C" int mxq_combine(const void* y, int32_t dtype, const float* weights, c
   if (T == 0 || D == 0) return MXQ_OK;
   if (!y || !weights || !positions || !out) return invalid("mxq_combine: NULL argument");
   const int64_t blocks = ceil_div(T * ceil_div(D, dtype == MXQ_DT_F32 ? 4 : 8), 256);
-  const dim3 grid((unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff));
+  const dim3 grid(blocks_for(blocks));
   with_dtype(dtype, [&](auto dt) {
     KernelTimer timer("k_combine", as_stream(stream));
     k_combine<decltype(dt)::value><<<grid, 256, 0, as_stream(stream)>>>(y, weights, positions, residual, out, T, (int)k, D);
@@ -316,7 +316,7 @@ extern "C" int mxq_combine_grad(const void* grad, int32_t dtype, const void* y, 
   if (!positions || (D && (!grad || !y || !weights))) return invalid("mxq_combine_grad: NULL argument");
   with_dtype(dtype, [&](auto dt) {
     KernelTimer timer("k_combine_grad", as_stream(stream));
-    k_combine_grad<decltype(dt)::value><<<dim3((unsigned)T), 256, 0, as_stream(stream)>>>(grad, y, weights, positions, dy, dw, T,
+    k_combine_grad<decltype(dt)::value><<<dim3(blocks_for(T)), 256, 0, as_stream(stream)>>>(grad, y, weights, positions, dy, dw, T,
                                                                                          (int)k, D);
   });
   return check_launch("mxq_combine_grad");

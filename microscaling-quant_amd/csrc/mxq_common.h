@@ -25,6 +25,11 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // One-dimensional grid of `threads` threads in blocks of `block`; grid.x caps at 2^31 - 1 blocks.
 inline dim3 grid_for(int64_t threads, int block) { return dim3((unsigned)ceil_div(threads, block)); }
 
+// A launch of 2^32 threads or more along an axis runs a part of them, with no error: what one axis of a launch may have, and
+// the workgroups, of 512 threads at most, that kernels going on in strides of their grid are given.
+constexpr int64_t kMaxThreads = 0xFFFFFFFF, kMaxBlocks = 1 << 22;
+inline unsigned blocks_for(int64_t blocks) { return (unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks); }
+
 // Division of n < 2^31 by a divisor d >= 1 fixed at launch, as one multiply-high, an add and a shift
 // (Granlund and Montgomery's round-up method): with l = ceil(log2 d) and mul = floor(2^32 (2^l - d) / d) + 1
 // (below 2^32, since 2^l - d < d), n / d = (umulhi(n, mul) + n) >> l, and the sum stays below 2^32 because

@@ -25,17 +25,15 @@ namespace {
 // Experts without rows are left out.
 struct PrepareArgs {
   LinearArgs l;
-  int64_t kp, x_rows, w_rows;          // columns a plane, rows of x (0: stays), rows of one weight
+  int64_t kp, x_rows, w_rows, rows;    // columns a plane, rows of x (0: stays), rows of one weight, rows in all
   int32_t planes;
   uint16_t* x;
   uint8_t *codes, *scales;             // NULL: stay
 };
-// A workgroup a row of x, then a row of the weight.
-__global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
+__device__ __forceinline__ void prepare_row(const PrepareArgs& p, int64_t row) {
   const LinearArgs& a = p.l;
   const bool pairs = a.sp.format == MXQ_FMT_E2M1_PAIRS;
-  if (blockIdx.x < p.x_rows) {
-    const int64_t row = blockIdx.x;
+  if (row < p.x_rows) {
     for (int64_t k = threadIdx.x * 8; k < p.kp; k += 256 * 8) {
       float v[8];
 #pragma unroll
@@ -61,7 +59,8 @@ __global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
     }
     return;
   }
-  const int64_t all = (int64_t)blockIdx.x - p.x_rows, e = all / p.w_rows, row = all - e * p.w_rows;
+  const int64_t all = row - p.x_rows, e = all / p.w_rows;
+  row = all - e * p.w_rows;
   if (a.offsets && a.offsets[e + 1] <= a.offsets[e]) return;
   const int64_t bytes = pairs ? p.kp / 2 : p.kp, have = pairs ? (a.K + 1) / 2 : a.K;
   const uint8_t* codes = a.codes + e * a.sp.batch_codes + row * a.sp.ld_codes;
@@ -83,6 +82,10 @@ __global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
         if (at + b < (a.K + 31) / 32) v |= (uint32_t)scales[at + b] << 8 * b;
       *(uint32_t*)(p.scales + all * (p.kp / 32) + at) = v;
     }
+}
+// A workgroup a row of x, then a row of the weight.
+__global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) prepare_row(p, row);
 }
 
 // The splits' sums in their order, and the epilogue: eight outputs a thread.
@@ -196,12 +199,14 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
   const Plan p = plan_of(a);
   if (p.bytes && !workspace) return invalid(std::string(who) + ": NULL workspace");
   const int fam = family(a.sp.format);
+  const int64_t threads = p.few ? (ceil_div(a.N, 16) * p.tiles_m >= 1024 ? 256 : 512) * ceil_div(a.N, 16)
+                                : (p.tile.shape == 0 ? 512 : 256) * p.tiles_m * p.tiles_n;
+  if (threads > kMaxThreads) return invalid(std::string(who) + ": too many outputs");
   if (p.few) {
     (fam == kE4M3 ? launch_skinny_e4m3 : fam == kE5M2 ? launch_skinny_e5m2 : fam == kPairs ? launch_skinny_pairs : launch_skinny_mapped)(
         a, p.tiles_m, st);
     return check_launch(who);
   }
-  if (p.tiles_m * p.tiles_n > 0x7fffffff) return invalid(std::string(who) + ": too many outputs");
   uint8_t* work = (uint8_t*)workspace;
   const bool pairs = fam == kPairs;
   const int64_t kp = (int64_t)p.steps * 64, matrices = (a.E ? a.E : 1) * p.w_rows;
@@ -209,11 +214,10 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
              p.tile.split, (float*)(work + p.at_partial), code_map(a.sp.format)};
   if (kp && (p.lay_x || p.lay_codes || p.lay_scales)) {
     const int64_t x_rows = p.lay_x ? p.x_rows : 0, w_rows = p.lay_codes || p.lay_scales ? matrices : 0;
-    if (x_rows + w_rows > 0x7fffffff) return invalid(std::string(who) + ": too many rows");
-    const PrepareArgs q{a, kp, x_rows, p.w_rows, p.planes, (uint16_t*)work, p.lay_codes ? work + p.at_codes : nullptr,
+    const PrepareArgs q{a, kp, x_rows, p.w_rows, x_rows + w_rows, p.planes, (uint16_t*)work, p.lay_codes ? work + p.at_codes : nullptr,
                         p.lay_scales ? work + p.at_scales : nullptr};
     KernelTimer timer("k_prepare", st);
-    k_prepare<<<dim3((unsigned)(x_rows + w_rows)), 256, 0, st>>>(q);
+    k_prepare<<<dim3(blocks_for(x_rows + w_rows)), 256, 0, st>>>(q);
     if (p.lay_x) t.x = q.x, t.ld_x = kp * p.planes, t.x_columns = (int32_t)kp;
     if (p.lay_codes) {
       t.l.codes = q.codes, t.l.sp.ld_codes = pairs ? kp / 2 : kp, t.l.sp.batch_codes = t.l.sp.ld_codes * p.w_rows;

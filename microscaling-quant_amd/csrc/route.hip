@@ -367,10 +367,15 @@ extern "C" int mxq_route(const void* logits, int32_t dtype, const float* bias, i
   with_shape(dtype, E, spec->top_k, [&](auto dt, auto lanes, auto v, auto slots) {
     constexpr int L = decltype(lanes)::value;
     const int threads = spec->groups > 1 && E > 256 ? 32 * kWaves : 64 * kWaves, tokens = threads / L;   // below 64 KB of LDS
+    constexpr size_t size = decltype(dt)::value == MXQ_DT_F32 ? 4 : 2;
     const size_t lds = spec->groups > 1 ? tokens * (size_t)(E + kMaxGroups) * sizeof(double) : 0;
-    KernelTimer timer("k_route", as_stream(stream));
-    k_route<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(T, tokens)), threads, lds, as_stream(stream)>>>(
-        logits, bias, T, (int)E, *spec, make_divu31((uint32_t)(E / spec->groups)), weights, experts);
+    for (int64_t t = 0, n; t < T; t += n) {
+      n = T - t < kMaxBlocks * tokens ? T - t : kMaxBlocks * tokens;
+      KernelTimer timer("k_route", as_stream(stream));
+      k_route<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(n, tokens)), threads, lds, as_stream(stream)>>>(
+          (const char*)logits + t * E * size, bias, n, (int)E, *spec, make_divu31((uint32_t)(E / spec->groups)), weights + t * spec->top_k,
+          experts + t * spec->top_k);
+    }
   });
   return check_launch("mxq_route");
 }
@@ -382,9 +387,13 @@ extern "C" int mxq_route_grad(const void* logits, int32_t dtype, const int32_t* 
   if (!logits || !experts || !grad || !out) return invalid("mxq_route_grad: NULL argument");
   with_shape(dtype, E, spec->top_k, [&](auto dt, auto lanes, auto v, auto slots) {
     constexpr int L = decltype(lanes)::value, kTokens = 64 * kWaves / L;
-    KernelTimer timer("k_route_grad", as_stream(stream));
-    k_route_grad<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(T, kTokens)), 64 * kWaves, 0, as_stream(stream)>>>(
-        logits, experts, grad, T, (int)E, *spec, out);
+    constexpr size_t size = decltype(dt)::value == MXQ_DT_F32 ? 4 : 2;
+    for (int64_t t = 0, n; t < T; t += n) {
+      n = T - t < kMaxBlocks * kTokens ? T - t : kMaxBlocks * kTokens;
+      KernelTimer timer("k_route_grad", as_stream(stream));
+      k_route_grad<decltype(dt)::value, L, decltype(v)::value, decltype(slots)::value><<<dim3((unsigned)ceil_div(n, kTokens)), 64 * kWaves, 0, as_stream(stream)>>>(
+          (const char*)logits + t * E * size, experts + t * spec->top_k, grad + t * spec->top_k, n, (int)E, *spec, (char*)out + t * E * size);
+    }
   });
   return check_launch("mxq_route_grad");
 }
