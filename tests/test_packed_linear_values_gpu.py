@@ -1,5 +1,5 @@
 """Which values the products with packed weights take, on the kernel of few rows and on every tile: every code under every
-scale byte, weights past float32's range."""
+scale byte, weights past float32's range, float16's products bit for bit."""
 import numpy as np
 import pytest
 import torch
@@ -98,3 +98,23 @@ def test_weights_past_float32(cuda, fmt, pairs, dtype):
         near = finite & (size < 2.0 ** 127)                          # no partial sum leaves float32
         assert ((y - want).abs()[near] <= ((K + 2) * HALF * size)[near]).all(), M
         assert near[:, ::2].all()
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+def test_float16_products_are_exact(cuda, fmt):
+    """One product an output: 11 bits by 4 fit float32, and so do two sums of an 8-bit part and the rest."""
+    rng = np.random.default_rng(3)
+    e, m = FORMATS[fmt]
+    codes = torch.from_numpy(rng.integers(0, 2 ** (e + m) - (4 if e > 3 else 0), (80, 128)).astype(np.uint8))
+    codes |= torch.from_numpy((rng.integers(0, 2, (80, 128)) << (e + m)).astype(np.uint8))
+    scales = torch.from_numpy(rng.integers(112, 130, (80, 4)).astype(np.uint8))
+    W = torch.from_numpy(om.weight(codes.numpy(), scales.numpy(), fmt, 128))
+    lost = 0
+    for M in ROWS:
+        x = torch.zeros(M, 128, dtype=torch.float16)
+        at = torch.from_numpy(rng.integers(0, 128, M))
+        x[torch.arange(M), at] = torch.from_numpy(rng.standard_normal(M) * np.exp2(rng.integers(-20, 10, M))).half()
+        y = nn.packed_linear(x.cuda(), codes.cuda(), scales.cuda(), fmt, out_dtype=torch.float32).double().cpu()
+        assert torch.equal(y, x.double() @ W.t())
+        lost += int((x.bfloat16().double() @ W.t() != y).sum())
+    assert lost > 1000                                               # one plane alone would not pass
