@@ -530,8 +530,9 @@ typedef struct mxq_linear_spec {
 /* y (M x N) = act(x W^T + bias) [* (x U^T + bias of U)] + residual, W's rows packed codes (K of them a row) with one
  * E8M0 byte for 32 columns; bias and residual NULL for none.  Products are exact, sums float32, y is rounded once.  A
  * weight below 2^-126 is rounded to bfloat16's subnormals, one of 2^128 or more is infinite, as it is in float32; scale
- * byte 255 makes its block NaN.  `workspace`: device memory of mxq_packed_linear_workspace bytes, 256-byte aligned (NULL
- * where that is 0, as it is for M <= 16, n <= 16 E).
+ * byte 255 makes its block NaN.  The part of a float32 activation below 2^-133 is left out (only one below 2^-110 has any).
+ * `workspace`: device memory of mxq_packed_linear_workspace bytes, 256-byte aligned (NULL where that is 0, as it is for
+ * M <= 16, n <= 16 E).
  * mxq_expert_linear: n rows sorted by expert (mxq_dispatch's order and offsets; order is read where top_k > 0), row r
  * of expert e multiplied by matrix e; rows past the last expert's become zeros. */
 int64_t mxq_packed_linear_workspace(const void* x, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t N,

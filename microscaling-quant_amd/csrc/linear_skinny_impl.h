@@ -5,8 +5,8 @@
 // a row's bytes are read in whole 128-byte lines, the next ones asked for before these are multiplied.  Lane (r, g) of a
 // wave holds block g of row r: 32 codes, one scale, four operands of mfma_f32_16x16x32_bf16 (whose order of the contraction
 // is free, as long as x's follows).  Weights become bfloat16 exactly; float16 and float32 activations are taken as the sum
-// of two and three bfloat16, also exact, one product each.  The waves' sums meet in LDS, in the order of the waves; biases
-// and residual are asked for at the start.
+// of two and three bfloat16, one product each, also exact but for what a float32 has below 2^-133, bfloat16's smallest step.
+// The waves' sums meet in LDS, in the order of the waves; biases and residual are asked for at the start.
 //
 // Measured, us: 4096 x 4096 in E4M3 with one row 7.2 (2.4 TB/s; a launch and two trips to memory are what is left), 8
 // experts of 4096 x 4096 36 (3.8 TB/s).  Eight waves a workgroup, or four where there are workgroups enough to fill the

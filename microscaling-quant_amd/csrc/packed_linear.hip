@@ -19,7 +19,7 @@ namespace {
 
 // What k_linear_tile's direct loads cannot take as it lies is laid out first, by one launch.
 //   x: bfloat16 planes of kp values, one after another along a row, zeros past K: each plane the leading bits of what the
-//      ones before leave, so that their sum is the value.
+//      ones before leave, so that their sum is the value (of a float32, down to bfloat16's smallest step of 2^-133).
 //   codes: rows of whole 128 columns, zeros past K.
 //   scales: rows of whole words.
 // Experts without rows are left out.

@@ -8,7 +8,8 @@ own dtype.  Not in the reference, whose products take float32 codes of both oper
 y = act(x W^T + bias) + residual; gated: act(x G^T + b) * (x U^T + c) + residual, where the weight's first half of rows
 is G and the second U (bias likewise).  Each product of an activation and a weight is exact, sums are float32, and y
 is rounded once.  A weight is its code times its scale; below 2^-126 it is rounded to bfloat16's subnormals, from 2^128 on
-it is infinite, as in packed.dequantize's float32.
+it is infinite, as in packed.dequantize's float32.  The part of a float32 activation below 2^-133 is left out (only
+one below 2^-110 has any).
 
 For inference: codes have no gradient, and an input that asks for one is refused.
 """

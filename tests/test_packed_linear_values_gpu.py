@@ -1,5 +1,6 @@
 """Which values the products with packed weights take, on the kernel of few rows and on every tile: every code under every
-scale byte, weights past float32's range, float16's products bit for bit."""
+scale byte, weights past float32's range, float16's products bit for bit, activations
+below bfloat16's smallest step."""
 import numpy as np
 import pytest
 import torch
@@ -118,3 +119,20 @@ def test_float16_products_are_exact(cuda, fmt):
         assert torch.equal(y, x.double() @ W.t())
         lost += int((x.bfloat16().double() @ W.t() != y).sum())
     assert lost > 1000                                               # one plane alone would not pass
+
+
+@pytest.mark.parametrize("M", ROWS)
+def test_small_float32_activations(cuda, M):
+    """The part of a float32 activation below 2^-133, bfloat16's smallest step, is left out; above 2^-110 there is none."""
+    rng = np.random.default_rng(11)
+    codes = torch.from_numpy((rng.integers(0, 0x7F, (64, 128)) | rng.integers(0, 2, (64, 128)) << 7).astype(np.uint8))
+    scales = torch.from_numpy(rng.integers(200, 220, (64, 4)).astype(np.uint8))
+    W = torch.from_numpy(om.weight(codes.numpy(), scales.numpy(), "MXFP8_E4M3", 128))
+    for low, high, part in ((-149, -109, 2.0 ** -133), (-110, -90, 0.0)):
+        x = torch.from_numpy(rng.standard_normal((M, 128)) * np.exp2(rng.integers(low, high, (M, 128)))).float()
+        if not part:
+            x = torch.where(x.abs() < 2.0 ** -110, 0.0, x)
+        y = nn.packed_linear(x.cuda(), codes.cuda(), scales.cuda(), "MXFP8_E4M3").double().cpu()
+        size = x.double().abs() @ W.abs().t()
+        bound = 130 * HALF * size + part * W.abs().sum(1) + 2.0 ** -126
+        assert ((y - x.double() @ W.t()).abs() <= bound).all()
