@@ -146,14 +146,15 @@ template <int DT> struct Pack {
 
 constexpr int kRows = 4;                                          // experts' rows in flight
 
-// The row of y at a slot's position, -1 for a slot of none: a position past the rows is the caller's mistake, which must
-// not reach memory.
-__device__ __forceinline__ int row_of(int position, int rows) { return position < rows ? position : -1; }
+// Whether a slot's position is a row of y's, and not that of a slot of none, below zero, or past the rows, the caller's
+// mistake, which must not reach memory.
+__device__ __forceinline__ bool is_row(int position, int rows) { return (uint32_t)position < (uint32_t)rows; }
 
 // out[t] = residual[t] + sum_j w[t, j] y[position[t, j]] in float32, j in order, rounded once.  Reading y bounds it: 16
 // bytes a thread, four rows' loads in flight before the first is added.  4096 tokens x 4 x 2048 bfloat16 22.4 us, 4.5 TB/s.
 template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y_, const float* weights, const int32_t* positions,
-                                                                   const void* residual_, void* out_, int64_t T, int k, int64_t D) {
+                                                                   const void* residual_, void* out_, int64_t T, int k, int rows,
+                                                                   int64_t D) {
   typedef Pack<DT> P;
   typedef typename P::E E;
   const E *y = (const E*)y_, *residual = (const E*)residual_;
@@ -173,18 +174,18 @@ template <int DT> __global__ __launch_bounds__(256) void k_combine(const void* y
       for (int j = 0; j < kRows; ++j) {
         const bool in = j0 + j < k;
         w[j] = in ? weights[t * k + j0 + j] : 0.0f;
-        p[j] = in ? row_of(positions[t * k + j0 + j], (int)(T * k)) : -1;
+        p[j] = in ? positions[t * k + j0 + j] : -1;
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (p[j] >= 0) row[j].load(y + p[j] * D + d, left);
+        if (is_row(p[j], rows)) row[j].load(y + p[j] * D + d, left);
       if (residual && j0 == 0) {
 #pragma unroll
         for (int e = 0; e < P::N; ++e) sum[e] = (float)res.v[e];
       }
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        if (p[j] >= 0) {
+        if (is_row(p[j], rows)) {
 #pragma unroll
           for (int e = 0; e < P::N; ++e) sum[e] = __builtin_fmaf(w[j], (float)row[j].v[e], sum[e]);
         } else if (w[j] != w[j]) {                                // a NaN weight of no expert stays visible
@@ -304,7 +305,7 @@ extern "C" int mxq_combine(const void* y, int32_t dtype, const float* weights, c
   const dim3 grid(blocks_for(blocks));
   with_dtype(dtype, [&](auto dt) {
     KernelTimer timer("k_combine", as_stream(stream));
-    k_combine<decltype(dt)::value><<<grid, 256, 0, as_stream(stream)>>>(y, weights, positions, residual, out, T, (int)k, D);
+    k_combine<decltype(dt)::value><<<grid, 256, 0, as_stream(stream)>>>(y, weights, positions, residual, out, T, (int)k, (int)(T * k), D);
   });
   return check_launch("mxq_combine");
 }
