@@ -26,7 +26,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline dim3 grid_for(int64_t threads, int block) { return dim3((unsigned)ceil_div(threads, block)); }
 
 // A launch of 2^32 threads or more along an axis runs a part of them, with no error: what one axis of a launch may have, and
-// the workgroups, of 512 threads at most, that kernels going on in strides of their grid are given.
+// the workgroups, of 512 threads at most, of a launch whose kernel goes on in strides of its grid, or which others follow.
 constexpr int64_t kMaxThreads = 0xFFFFFFFF, kMaxBlocks = 1 << 22;
 inline unsigned blocks_for(int64_t blocks) { return (unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks); }
 

@@ -25,13 +25,15 @@ namespace {
 // Experts without rows are left out.
 struct PrepareArgs {
   LinearArgs l;
-  int64_t kp, x_rows, w_rows, rows;    // columns a plane, rows of x (0: stays), rows of one weight, rows in all
+  int64_t kp, x_rows, w_rows, first;   // columns a plane, rows of x (0: stays), rows of one weight, this launch's first row
   int32_t planes;
   uint16_t* x;
   uint8_t *codes, *scales;             // NULL: stay
 };
-__device__ __forceinline__ void prepare_row(const PrepareArgs& p, int64_t row) {
+// A workgroup a row of x, then a row of the weight.
+__global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
   const LinearArgs& a = p.l;
+  int64_t row = p.first + blockIdx.x;
   const bool pairs = a.sp.format == MXQ_FMT_E2M1_PAIRS;
   if (row < p.x_rows) {
     for (int64_t k = threadIdx.x * 8; k < p.kp; k += 256 * 8) {
@@ -82,10 +84,6 @@ __device__ __forceinline__ void prepare_row(const PrepareArgs& p, int64_t row) {
         if (at + b < (a.K + 31) / 32) v |= (uint32_t)scales[at + b] << 8 * b;
       *(uint32_t*)(p.scales + all * (p.kp / 32) + at) = v;
     }
-}
-// A workgroup a row of x, then a row of the weight.
-__global__ __launch_bounds__(256) void k_prepare(PrepareArgs p) {
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) prepare_row(p, row);
 }
 
 // The splits' sums in their order, and the epilogue: eight outputs a thread.
@@ -214,10 +212,12 @@ int launch(const char* who, const LinearArgs& a, void* workspace, hipStream_t st
              p.tile.split, (float*)(work + p.at_partial), code_map(a.sp.format)};
   if (kp && (p.lay_x || p.lay_codes || p.lay_scales)) {
     const int64_t x_rows = p.lay_x ? p.x_rows : 0, w_rows = p.lay_codes || p.lay_scales ? matrices : 0;
-    const PrepareArgs q{a, kp, x_rows, p.w_rows, x_rows + w_rows, p.planes, (uint16_t*)work, p.lay_codes ? work + p.at_codes : nullptr,
+    PrepareArgs q{a, kp, x_rows, p.w_rows, 0, p.planes, (uint16_t*)work, p.lay_codes ? work + p.at_codes : nullptr,
                         p.lay_scales ? work + p.at_scales : nullptr};
-    KernelTimer timer("k_prepare", st);
-    k_prepare<<<dim3(blocks_for(x_rows + w_rows)), 256, 0, st>>>(q);
+    for (; q.first < x_rows + w_rows; q.first += kMaxBlocks) {
+      KernelTimer timer("k_prepare", st);
+      k_prepare<<<dim3(blocks_for(x_rows + w_rows - q.first)), 256, 0, st>>>(q);
+    }
     if (p.lay_x) t.x = q.x, t.ld_x = kp * p.planes, t.x_columns = (int32_t)kp;
     if (p.lay_codes) {
       t.l.codes = q.codes, t.l.sp.ld_codes = pairs ? kp / 2 : kp, t.l.sp.batch_codes = t.l.sp.ld_codes * p.w_rows;
