@@ -8,9 +8,9 @@
 // of two and three bfloat16, one product each, also exact but for what a float32 has below 2^-133, bfloat16's smallest step.
 // The waves' sums meet in LDS, in the order of the waves; biases and residual are asked for at the start.
 //
-// Measured, us: 4096 x 4096 in E4M3 with one row 7.2 (2.4 TB/s; a launch and two trips to memory are what is left), 8
+// Measured, us: 4096 x 4096 in E4M3 with one row 7.5 (2.3 TB/s; a launch and two trips to memory are what is left), 8
 // experts of 4096 x 4096 36 (3.8 TB/s).  Eight waves a workgroup, or four where there are workgroups enough to fill the
-// card four times: 37 against 40 there, 9.0 against 8.3 for the one row.
+// card four times: four take 36.3 there, eight 39.0, and for the one row 8.2 and 7.5.
 #pragma once
 
 #include "packed_linear_common.h"

@@ -162,7 +162,7 @@ Plan plan_of(const LinearArgs& a) {
   p.steps = (int)(2 * ceil_div(K, 128));
   p.planes = sp.x_dtype == MXQ_DT_BF16 ? 1 : sp.x_dtype == MXQ_DT_F16 ? 2 : 3;
   auto tiles = [&](int s) { return ceil_div(each, kTileM[s]) * (E ? E : 1) * ceil_div(width, kTileN[s]); };
-  // Measured at 4096 columns and 8192 rows of the weight, us on 256 x 256, 128 x 128, 64 x 128: 200 rows 39, 32, 31; 500
+  // By rows alone, measured with one weight of 4096 columns and 8192 rows, us on 256 x 256, 128 x 128, 64 x 128: 200 rows 39, 32, 31; 500
   // rows 54, 49, 46; 1000 rows 80, 72, 90; 2000 rows 114, 138, 166; 512 rows an expert 228, 206, 212, 1024 346, 351, 377.
   p.tile.shape = tiles(0) >= 192 && each > 1000 ? 0 : each > 500 ? 1 : 2;
   p.tiles_m = row_tiles(kTileM[p.tile.shape]);

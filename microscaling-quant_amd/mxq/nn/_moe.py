@@ -114,7 +114,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Opt
     their sum.  scale multiplies the weights.
 
     A logit of -inf closes its expert.  Where fewer than top_k are open the rest is expert -1 with weight 0, which
-    dispatch leaves out.  A row with a NaN (for softmax also +inf) gets NaN weights and experts -1.  Scores are taken
+    dispatch leaves out.  A row with a NaN (for softmax also +inf) gets NaN weights and experts -1, and a gradient of
+    NaN; a NaN of the bias does the same to the weights, and leaves no gradient, as all slots of no expert.  Scores are taken
     in 64 bits, so that the choice does not depend on float32's rounding of exp."""
     _dtype(logits, "route", "logits")
     if logits.ndim < 1:
