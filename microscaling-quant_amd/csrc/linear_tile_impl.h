@@ -11,7 +11,7 @@
 // goes through the weight, and converts it, once a plane.
 //
 // Measured, 8192 x 8192 x 4096 in E4M3 on 256 x 256: 436 us without an epilogue (1.26 PFLOP/s, what the library's product of
-// bfloat16 weights reaches here), 480 with bias, gelu and residual.  The matrix pipes are busy for 524 K of 905 K cycles at
+// bfloat16 weights reaches here), 488 with bias, gelu and residual.  The matrix pipes are busy for 524 K of 905 K cycles at
 // 1.7 GHz; alone, the products of a 64-column step take 1.0 us, its loads 0.9 (0.4 where they hit the first cache), both
 // together 1.5.  4096 x 4096 x 4096, a call, in E4M3, E5M2, E3M2 and MXFP4's pairs: bfloat16 114 and 116 (E4M3, pairs),
 // float16 234, 236, 245, 221, float32 348, 358, 370, 336.  Tried and slower: four waves of 128 x 128 (no second wave to fill a wait), two halves of waves taking turns
