@@ -22,13 +22,17 @@ inline hipStream_t as_stream(mxq_stream_t s) { return reinterpret_cast<hipStream
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// One-dimensional grid of `threads` threads in blocks of `block`; grid.x caps at 2^31 - 1 blocks.
-inline dim3 grid_for(int64_t threads, int block) { return dim3((unsigned)ceil_div(threads, block)); }
-
 // A launch of 2^32 threads or more along an axis runs a part of them, with no error: what one axis of a launch may have, and
 // the workgroups, of 512 threads at most, of a launch whose kernel goes on in strides of its grid, or which others follow.
 constexpr int64_t kMaxThreads = 0xFFFFFFFF, kMaxBlocks = 1 << 22;
 inline unsigned blocks_for(int64_t blocks) { return (unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks); }
+
+// One-dimensional grid of `threads` threads in blocks of `block`, for kernels that have a thread for each of their items: past
+// a launch's threads the empty grid, which HIP refuses and check_launch reports.
+inline dim3 grid_for(int64_t threads, int block) {
+  const int64_t blocks = ceil_div(threads, block);
+  return dim3(blocks * block > kMaxThreads ? 0u : (unsigned)blocks);
+}
 
 // Division of n < 2^31 by a divisor d >= 1 fixed at launch, as one multiply-high, an add and a shift
 // (Granlund and Montgomery's round-up method): with l = ceil(log2 d) and mul = floor(2^32 (2^l - d) / d) + 1

@@ -285,3 +285,14 @@ def test_dequantize_narrow_rows(cuda, shape, axis, bs):
     want = P * X.repeat_interleave(bs, dim=axis).narrow(axis, 0, P.shape[axis])
     assert torch.equal(got, want)
     assert torch.equal(mxq.block.dequantize(P, X, axis=axis, block_size=bs), want)
+
+
+def test_launches_past_2_32_threads_fail_loudly(cuda):
+    """A block an element: more threads than a launch has, of which a part would run."""
+    import mxq
+    n = 2 ** 32 + 1024
+    P, X = torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    with pytest.raises(RuntimeError, match="mxq_pack"):
+        mxq.packed.pack(P, X, "MXFP8_E4M3", axis=0, block_size=1)
+    codes, scales = mxq.packed.pack(P[:1 << 20], X[:1 << 20], "MXFP8_E4M3", axis=0, block_size=1)
+    assert not codes.any() and (scales == 127).all()
