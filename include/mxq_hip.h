@@ -36,8 +36,9 @@ typedef void* mxq_stream_t;
  *   4  mxq_attend_windows writes one flag word per call and 64 query rows, each whole (was one per call, zeroed
  *      by the caller).
  *   5  mxq_systolic_plan_of.
- *   6  mxq_route, mxq_dispatch, mxq_combine, mxq_packed_linear, mxq_expert_linear and their specs. */
-#define MXQ_ABI_VERSION 6
+ *   6  mxq_route, mxq_dispatch, mxq_combine, mxq_packed_linear, mxq_expert_linear and their specs.
+ *   7  mxq_cache_write, mxq_cache_read, mxq_cache_attend and their specs. */
+#define MXQ_ABI_VERSION 7
 
 enum { MXQ_OK = 0, MXQ_EINVAL = 1, MXQ_EHIP = 2, MXQ_EBUSY = 3 };
 
@@ -545,6 +546,58 @@ int64_t mxq_expert_linear_workspace(const void* x, const uint8_t* codes, const u
 int mxq_expert_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const void* bias, void* y, int64_t n,
                       int64_t N, int64_t K, int64_t E, const int32_t* order, const int32_t* offsets,
                       const mxq_linear_spec* spec, void* workspace, mxq_stream_t stream);
+
+/* ---- a key and value cache in MX formats, and the attention that reads it (no counterpart in the reference) ---- */
+
+/* Keys and values of `pages` pages of `page_size` rows for each of kv_heads heads.  A row is a vector of head_dim columns
+ * in ceil(head_dim / 32) blocks, the last filled up with zeros: codes (32 bytes a block, MXQ_FMT_E2M1_PAIRS 16) and one
+ * E8M0 byte a block, each row's next to each other.  Strides in bytes between pages, heads and rows, of keys' codes, keys'
+ * scales, values' codes, values' scales.  Slot s is row s % page_size of page s / page_size. */
+typedef struct mxq_cache_spec {
+  int32_t format;       /* MXQ_FMT_E4M3, MXQ_FMT_E5M2 or MXQ_FMT_E2M1_PAIRS */
+  int32_t head_dim;     /* 1 to 256 */
+  int64_t pages, page_size, kv_heads;
+  int64_t page_stride[4], head_stride[4], row_stride[4];
+} mxq_cache_spec;
+
+/* k and v (T x kv_heads x head_dim of dtype MXQ_DT_*; strides in elements between tokens and heads, columns next to each
+ * other) quantized into the slots' rows (T of them, int64 where slots_wide, else int32) as mxq_block_quantize_packed does
+ * under MXQ_SCALE_OCP at nearest even: the bytes are the same for finite blocks.  A block with an infinity or a NaN gets
+ * scale byte 255 and codes of zero.  A token whose slot is not in the cache is left out; of tokens with one slot the last
+ * one's row stays.  No other row is touched. */
+int mxq_cache_write(const void* k, const void* v, int32_t dtype, int64_t T, int64_t k_token, int64_t k_head,
+                    int64_t v_token, int64_t v_head, const void* slots, int32_t slots_wide, uint8_t* k_codes,
+                    uint8_t* k_scales, uint8_t* v_codes, uint8_t* v_scales, const mxq_cache_spec* cache,
+                    mxq_stream_t stream);
+
+/* The slots' rows as values: k and v, T x kv_heads x head_dim of dtype, code times scale rounded once; zeros for a slot
+ * that is not in the cache. */
+int mxq_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales,
+                   const mxq_cache_spec* cache, const void* slots, int32_t slots_wide, int64_t T, void* k, void* v,
+                   int32_t dtype, mxq_stream_t stream);
+
+typedef struct mxq_attend_spec {
+  int32_t dtype;        /* of q and out, MXQ_DT_* */
+  int32_t causal;
+  float scale;          /* positive, of q k^T */
+  int64_t T, B, heads;  /* queries, sequences, heads of q (a multiple of kv_heads) */
+  int64_t q_token, q_head;          /* q's strides in elements; columns next to each other */
+  int64_t table_pages, table_row;   /* pages a sequence may have, and elements between the table's rows */
+  int64_t window;       /* keys a query sees back from its own position; 0: all */
+} mxq_attend_spec;
+
+/* out (T x heads x head_dim) = softmax(scale q k^T) v over the keys that a query sees, and lse (T x heads float32, or
+ * NULL) the logarithm of the sum of exp(scale q k^T).  Sequence b has its first lengths[b] keys in the pages that row b of
+ * table (int32) names, and the queries [starts[b], starts[b + 1]) (starts NULL: T / B each), whose last one is at the last
+ * key: query j of n is at p = lengths[b] - n + j and sees keys up to p where causal, from p - window + 1 on where there is
+ * a window.  Lengths are held to the table's pages, starts to T; a key on a page that does not exist is not there.  A
+ * query that sees no key, or belongs to no sequence, gets zeros and an lse of -inf.
+ * `workspace`: device memory of mxq_cache_attend_workspace bytes, 256-byte aligned (NULL where that is 0). */
+int64_t mxq_cache_attend_workspace(const mxq_cache_spec* cache, const mxq_attend_spec* spec, int32_t ragged);
+int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
+                     const uint8_t* v_scales, const mxq_cache_spec* cache, const int32_t* table, const int32_t* lengths,
+                     const int32_t* starts, void* out, float* lse, const mxq_attend_spec* spec, void* workspace,
+                     mxq_stream_t stream);
 
 /* ---- elementwise primitives over flat arrays of n elements (the caller broadcasts) ---------------------- */
 

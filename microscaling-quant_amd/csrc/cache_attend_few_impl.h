@@ -1,0 +1,306 @@
+// Attention of few queries over a cache in MX formats: reading the cache is what it costs.
+//
+//   s = scale q k^T;  out = sum_i 2^(s_i log2 e - m) v_i / sum_i 2^(s_i log2 e - m),  m the running maximum
+//
+// A workgroup takes 16 rows (queries of the heads that share a head of keys) and a run of keys, its four waves 32 keys in
+// turn.  No wave waits for another before the end and nothing passes through LDS on the way: the scores are computed
+// transposed, S^T = K Q^T by mfma_f32_16x16x32_bf16, so that the lane that has four keys' scores of a query is the one whose
+// operand of out^T = V^T P^T they are.  Orders of keys and columns are free as long as both products agree on them: key
+// 16 t + 4 r + g is row 4 g + r of tile t, so that four neighbouring rows of the cache are read by one load, lane (g, c) has
+// the g-th share of a row of keys (whole blocks, 128 columns and more) and the c-th sixteenth of four rows of values,
+// whose pairs of keys v_perm puts next to each other.
+// Codes become bfloat16 exactly by the scaled conversions; float16 and float32 queries and their weights are taken as the
+// sum of two and three bfloat16.
+#pragma once
+
+#include "cache_common.h"
+
+namespace mxq {
+
+constexpr int kFewRows = 16, kFewWaves = 4;
+
+template <int FAM, int DT, int NB>
+__global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int least) {
+  constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
+  constexpr int KW = NB * BB / 16;                        // words of keys' codes a lane and tile of 16 keys
+  constexpr int EW = FAM == kPairs ? 1 : 2;               // words of eight codes
+  constexpr int VB = NB * BB / 16, VW = VB / 4 < EW ? EW : VB / 4;   // bytes and words of values' codes a lane and key
+  constexpr int OT = 2 * NB, DP = 32 * NB;                // tiles of out^T, columns
+  __shared__ float sums[kFewWaves][16][DP + 4];
+  __shared__ float tops[kFewWaves][16], weights[kFewWaves][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+
+  const int quota = quota_of(a, kFewRows, least);
+  const Unit u = unit_of(a, kFewRows, quota, blockIdx.x);
+  if (u.b < 0) return;
+  const Sequence s = sequence(a, u.b);
+  const int rows = s.n * a.group, row0 = u.tile * kFewRows;
+  const int D = a.c.head_dim;
+
+  // this lane's query, and the keys it sees: [lo, hi]
+  const int row = row0 + c, token = (int)divu31(row < rows ? row : rows - 1, a.by_group), last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
+  const int head = u.head * a.group + (row < rows ? row : rows - 1) - token * a.group;
+  auto first_key = [&](int t) {
+    const int64_t f = (int64_t)s.length - s.n + t + 1 - a.a.window;
+    return a.a.window && f > 0 ? (f < s.length ? (int)f : s.length) : 0;
+  };
+  auto last_key = [&](int t) { return a.a.causal ? s.length - s.n + t : s.length - 1; };
+  const int lo = row < rows ? first_key(token) : 1, hi = row < rows ? last_key(token) : 0;
+  const int t_first = (int)divu31(row0, a.by_group), t_last = (int)divu31(last_row, a.by_group);
+  const int from = first_key(t_first), to = last_key(t_last) + 1;   // some row sees them
+  const int all_from = first_key(t_last), all_to = last_key(t_first) + 1;   // every row does
+
+  bf16x8 q[P][NB];
+  {
+    const int64_t at = (int64_t)(s.start + token) * a.a.q_token + head * a.a.q_head;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int d = NB == 2 ? 16 * g + 8 * i : 32 * (g + 4 * (i >> 2)) + 8 * (i & 3);
+      bf16x8 p[P];
+      load_query<DT>(a.q, at + d, row < rows ? D - d : 0, p);
+#pragma unroll
+      for (int j = 0; j < P; ++j) q[j][i] = p[j];
+    }
+  }
+
+  f32x4 o[OT];
+#pragma unroll
+  for (int t = 0; t < OT; ++t) o[t] = f32x4{0, 0, 0, 0};
+  float top = -__builtin_inff(), total = 0.0f;
+
+  // this unit's steps, of which every kFewWaves-th is this wave's
+  const int base = from & ~(kStep - 1), steps = to > from ? (to - base + kStep - 1) / kStep : 0;
+  const int begin = (int)((int64_t)steps * u.run / u.runs), end = (int)((int64_t)steps * (u.run + 1) / u.runs);
+
+  // where a lane reads within a row: its share of a row of keys, and of values
+  const int kblock = NB == 2 ? g >> 1 : g, kbyte = NB == 2 ? g * (BB / 2) : g * BB;
+  const int vblock = c * NB / 16;
+  const bool kthere = kblock < a.blocks, kthere2 = NB == 8 && g + 4 < a.blocks, vthere = vblock < a.blocks;
+  const uint8_t *kc = a.kc + u.head * a.c.head_stride[0], *ks = a.ks + u.head * a.c.head_stride[1];
+  const uint8_t *vc = a.vc + u.head * a.c.head_stride[2], *vs = a.vs + u.head * a.c.head_stride[3];
+  const int32_t* table = a.table + (int64_t)u.b * a.a.table_row;
+  // The page and row of a key that the cache has; false: there is none.
+  auto locate = [&](int key, int& page, int& at) {
+    const int k = key < s.length ? key : s.length - 1;
+    const int i = (int)divu31(k, a.by_page);
+    at = k - i * (int)a.c.page_size;
+    page = table[i];
+    const bool there = key < s.length && page >= 0 && page < a.c.pages;
+    if (!there) page = 0, at = 0;
+    return there;
+  };
+
+  uint32_t kw[2][KW], ksc[2][NB == 8 ? 2 : 1], vw[8][VW], vsc[8];
+  uint32_t there = 0;                                     // bit i: key i of this lane's eight
+  auto load_keys = [&](int step) {
+    const int k0 = base + step * kStep;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int page, at;
+      locate(k0 + 16 * t + 4 * (c & 3) + (c >> 2), page, at);
+      const uint8_t* p = kc + page * a.c.page_stride[0] + at * a.c.row_stride[0] + kbyte;
+      const uint8_t* f = ks + page * a.c.page_stride[1] + at * a.c.row_stride[1] + kblock;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) kw[t][i] = 0;
+      ksc[t][0] = 0;
+      constexpr int first = NB == 8 ? KW / 2 : KW;
+      if (kthere) {
+        __builtin_memcpy(&kw[t][0], p, 4 * first);
+        ksc[t][0] = *f;
+      }
+      if constexpr (NB == 8) {
+        ksc[t][1] = 0;
+        if (kthere2) {
+          __builtin_memcpy(&kw[t][first], p + 4 * BB, 4 * first);
+          ksc[t][1] = f[4];
+        }
+      }
+    }
+  };
+  auto load_values = [&](int step) {
+    const int k0 = base + step * kStep;
+    there = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      int page, at;
+      const bool yes = locate(k0 + 16 * (i >> 2) + 4 * (i & 3) + g, page, at);
+      there |= yes ? 1u << i : 0u;
+      const uint8_t* p = vc + page * a.c.page_stride[2] + at * a.c.row_stride[2] + c * VB;
+#pragma unroll
+      for (int w = 0; w < VW; ++w) vw[i][w] = 0;
+      vsc[i] = 0;
+      if (yes && vthere) {
+        __builtin_memcpy(&vw[i][0], p, VB);
+        vsc[i] = vs[page * a.c.page_stride[3] + at * a.c.row_stride[3] + vblock];
+      }
+    }
+  };
+
+  int step = begin + wave;
+  if (step < end) {
+    load_keys(step);
+    load_values(step);
+  }
+  for (; step < end; step += kFewWaves) {
+    const int k0 = base + step * kStep;
+    f32x4 z[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      z[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const bf16x8 k = eight_codes<FAM>(&kw[t][i * EW], scale_field(ksc[t][NB == 8 ? i >> 2 : 0]));
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) z[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[p][i], z[t], 0, 0, 0);
+      }
+    }
+    if (step + kFewWaves < end) load_keys(step + kFewWaves);
+
+    const bool part = k0 < all_from || k0 + kStep > all_to || __any(there != 0xFF);
+    uint32_t seen = 0xFF;
+    if (part) {
+      seen = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = k0 + 16 * (i >> 2) + 4 * (i & 3) + g;
+        const bool yes = key >= lo && key <= hi && (there >> i & 1);
+        seen |= yes ? 1u << i : 0u;
+        z[i >> 2][i & 3] = yes ? z[i >> 2][i & 3] : -__builtin_inff();
+      }
+    }
+    float most = z[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = __builtin_fmaxf(most, z[i >> 2][i & 3]);
+    most *= a.scale2;
+    // The maximum follows only when a weight would pass 2^8: until then weights and sums are relative to an old one.
+    if (__any(most > top + 8.0f)) {
+      most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      const float now = __builtin_fmaxf(top, most);
+      const float factor = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      total *= factor;
+#pragma unroll
+      for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[t][r] *= factor;
+    }
+    const float less = top == -__builtin_inff() ? 0.0f : -top;
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i >> 2][i & 3], a.scale2, less));
+      total += w[i];
+    }
+    bf16x8 pw[P];
+    planes_of(w, pw);
+
+    // two neighbouring columns at a time: pairs of columns of a key become pairs of keys of a column
+    bool odd = false;                                     // an infinity or a NaN among the values
+#pragma unroll
+    for (int t8 = 0; t8 < (OT < 8 ? 1 : OT / 8); ++t8) {
+      constexpr int pairs = OT < 8 ? OT / 2 : 4;
+      uint32_t col[8][pairs];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = scale_field(vsc[i]);
+        const bf16x8 e = eight_codes<FAM>(&vw[i][t8 * EW], f);      // of a row of 64 columns only the first four are there
+        uint32_t x[4];
+        __builtin_memcpy(x, &e, 16);
+#pragma unroll
+        for (int j = 0; j < pairs; ++j) col[i][j] = x[j];
+      }
+#pragma unroll
+      for (int j = 0; j < pairs; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(col[2 * i + 1][j], col[2 * i][j], half ? 0x07060302u : 0x05040100u);
+          bf16x8 v;
+          __builtin_memcpy(&v, x, 16);
+          const int t = t8 * 8 + 2 * j + half;
+          if (part) {
+            odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= (x[i] & 0x7F80u) == 0x7F80u || (x[i] & 0x7F800000u) == 0x7F800000u;
+            if (__any(odd)) {
+              // zero times infinity is no zero: the product with each query's own keys alone, its column kept
+              for (int n = 0; n < 16; ++n) {
+                const int l = __builtin_amdgcn_readlane(lo, n), h = __builtin_amdgcn_readlane(hi, n);
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int key = k0 + 16 * (i >> 2) + 4 * (i & 3) + g;
+                  const uint32_t keep = key >= l && key <= h ? 0xFFFFu : 0u;
+                  if (i & 1) y[i >> 1] |= x[i >> 1] & keep << 16;
+                  else y[i >> 1] = x[i >> 1] & keep;
+                }
+                bf16x8 m;
+                __builtin_memcpy(&m, y, 16);
+                f32x4 sum = o[t];
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, pw[p], sum, 0, 0, 0);
+                if (c == n) o[t] = sum;
+              }
+              continue;
+            }
+          }
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw[p], o[t], 0, 0, 0);
+        }
+      }
+    }
+    if (step + kFewWaves < end) load_values(step + kFewWaves);
+  }
+
+  // the waves' sums, relative to the largest of their maxima, in the order of the waves
+  total += __shfl_xor(total, 16);
+  total += __shfl_xor(total, 32);
+  if (g == 0) tops[wave][c] = top, weights[wave][c] = total;
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sums[wave][c][OT * (4 * g + r) + t] = o[t][r];
+  __syncthreads();
+  const int r = threadIdx.x >> 4, d0 = threadIdx.x & 15;
+  if (row0 + r >= rows) return;
+  float best = tops[0][r], all = 0.0f, factor[kFewWaves];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) best = __builtin_fmaxf(best, tops[w][r]);
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) {
+    factor[w] = tops[w][r] == -__builtin_inff() ? (weights[w][r] == 0.0f ? 0.0f : weights[w][r]) : __builtin_amdgcn_exp2f(tops[w][r] - best);
+    all += tops[w][r] == -__builtin_inff() ? weights[w][r] : factor[w] * weights[w][r];
+  }
+  const bool whole = u.runs == 1;
+  const int t = (int)divu31(row0 + r, a.by_group), h = u.head * a.group + row0 + r - t * a.group;
+  const int64_t out_row = (int64_t)(s.start + t) * a.a.heads + h;
+  float* part = a.partial + ((int64_t)blockIdx.x * kFewRows + r) * (DP + 2);
+  const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+  for (int d = d0; d < D; d += 16) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) v += factor[w] == 0.0f ? 0.0f : factor[w] * sums[w][r][d];
+    if (whole) store_elem(a.out, DT, out_row * D + d, v * inv);
+    else part[d] = v;
+  }
+  if (d0 == 0) {
+    if (!whole) part[DP] = best, part[DP + 1] = all;
+    else if (a.lse) a.lse[out_row] = all == 0.0f ? -__builtin_inff() : (best == -__builtin_inff() ? all : (best + __builtin_amdgcn_logf(all)) * 0.693147180559945309f);
+  }
+}
+
+template <int FAM, int DT> void launch_attend_few_of(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
+  const dim3 grid((unsigned)units), block(64 * kFewWaves);
+  if (a.blocks <= 2) k_attend_few<FAM, DT, 2><<<grid, block, 0, st>>>(a, least);
+  else if (a.blocks <= 4) k_attend_few<FAM, DT, 4><<<grid, block, 0, st>>>(a, least);
+  else k_attend_few<FAM, DT, 8><<<grid, block, 0, st>>>(a, least);
+}
+template <int FAM> void launch_attend_few(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
+  if (a.a.dtype == MXQ_DT_F32) launch_attend_few_of<FAM, MXQ_DT_F32>(a, units, least, st);
+  else if (a.a.dtype == MXQ_DT_BF16) launch_attend_few_of<FAM, MXQ_DT_BF16>(a, units, least, st);
+  else launch_attend_few_of<FAM, MXQ_DT_F16>(a, units, least, st);
+}
+
+}  // namespace mxq

@@ -27,7 +27,7 @@ _lib: Optional[ctypes.CDLL] = None
 _FN = {}            # entry point name -> its ctypes function, filled by load()
 
 #: the MXQ_ABI_VERSION of include/mxq_hip.h these signatures follow; a library reporting another is refused
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 c_i32, c_i64, c_f32, c_f64, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
 
@@ -92,6 +92,18 @@ class LinearSpec(ctypes.Structure):
                                      "gated", "top_k")] + \
                [(n, c_i64) for n in ("ld_x", "ld_residual", "ld_y", "ld_codes", "ld_scales", "batch_codes",
                                      "batch_scales", "batch_bias")]
+
+
+class CacheSpec(ctypes.Structure):
+    """mxq_cache_spec (include/mxq_hip.h)."""
+    _fields_ = [("format", c_i32), ("head_dim", c_i32), ("pages", c_i64), ("page_size", c_i64), ("kv_heads", c_i64),
+                ("page_stride", c_i64 * 4), ("head_stride", c_i64 * 4), ("row_stride", c_i64 * 4)]
+
+
+class AttendSpec(ctypes.Structure):
+    """mxq_attend_spec (include/mxq_hip.h)."""
+    _fields_ = [("dtype", c_i32), ("causal", c_i32), ("scale", c_f32)] + \
+               [(n, c_i64) for n in ("T", "B", "heads", "q_token", "q_head", "table_pages", "table_row", "window")]
 
 
 # exported symbol -> (restype, argtypes); every symbol include/mxq_hip.h declares
@@ -174,6 +186,13 @@ SIGNATURES = {
     "mxq_expert_linear_workspace": (c_i64, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(LinearSpec)]),
     "mxq_expert_linear": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr,
                                   ctypes.POINTER(LinearSpec), c_ptr, c_ptr]),
+    "mxq_cache_write": (c_i32, [c_ptr, c_ptr, c_i32, c_i64, c_i64, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr, c_ptr,
+                                c_ptr, c_ptr, ctypes.POINTER(CacheSpec), c_ptr]),
+    "mxq_cache_read": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, ctypes.POINTER(CacheSpec), c_ptr, c_i32, c_i64, c_ptr,
+                               c_ptr, c_i32, c_ptr]),
+    "mxq_cache_attend_workspace": (c_i64, [ctypes.POINTER(CacheSpec), ctypes.POINTER(AttendSpec), c_i32]),
+    "mxq_cache_attend": (c_i32, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, ctypes.POINTER(CacheSpec), c_ptr, c_ptr, c_ptr,
+                                 c_ptr, c_ptr, ctypes.POINTER(AttendSpec), c_ptr, c_ptr]),
 }
 
 # MXQ_DT_* codes
