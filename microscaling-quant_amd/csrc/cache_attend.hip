@@ -136,6 +136,8 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   a.by_page = make_divu31((uint32_t)cache->page_size), a.by_group = make_divu31((uint32_t)group);
   a.group = (int)group, a.blocks = (cache->head_dim + 31) / 32;
   a.wanted = kFewWanted;
+  a.aligned = cache->page_size % 16 == 0;
+  for (int64_t r : cache->row_stride) a.aligned = a.aligned && r >= 0 && r < 1 << 26;
   a.scale2 = spec->scale * 1.44269504088896341f;
   hipStream_t st = as_stream(stream);
   if (spec->B) {

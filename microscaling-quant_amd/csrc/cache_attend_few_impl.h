@@ -19,8 +19,9 @@ namespace mxq {
 
 constexpr int kFewRows = 16, kFewWaves = 4;
 
-template <int FAM, int DT, int NB>
-__global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int least) {
+// PAGES16: pages of whole 16 rows less than 2^26 bytes apart.
+template <int FAM, int DT, int NB, bool PAGES16>
+__global__ __launch_bounds__(64 * kFewWaves, (NB == 2 ? 3 : NB == 4 ? 2 : 1) + (DT == MXQ_DT_BF16)) void k_attend_few(AttendArgs a, int least) {
   constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
   constexpr int KW = NB * BB / 16;                        // words of keys' codes a lane and tile of 16 keys
   constexpr int EW = FAM == kPairs ? 1 : 2;               // words of eight codes
@@ -30,10 +31,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
   __shared__ float tops[kFewWaves][16], weights[kFewWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
 
-  const int quota = quota_of(a, kFewRows, least);
+  const int quota = same(quota_of(a, kFewRows, least));
   const Unit u = unit_of(a, kFewRows, quota, blockIdx.x);
   if (u.b < 0) return;
-  const Sequence s = sequence(a, u.b);
+  const Sequence s = same(sequence(a, u.b));
   const int rows = s.n * a.group, row0 = u.tile * kFewRows;
   const int D = a.c.head_dim;
 
@@ -69,8 +70,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
   float top = -__builtin_inff(), total = 0.0f;
 
   // this unit's steps, of which every kFewWaves-th is this wave's
-  const int base = from & ~(kStep - 1), steps = to > from ? (to - base + kStep - 1) / kStep : 0;
-  const int begin = (int)((int64_t)steps * u.run / u.runs), end = (int)((int64_t)steps * (u.run + 1) / u.runs);
+  const int base = same(from & ~(kStep - 1)), steps = to > from ? (to - base + kStep - 1) / kStep : 0;
+  const int begin = same((int)((int64_t)steps * u.run / u.runs)), end = same((int)((int64_t)steps * (u.run + 1) / u.runs));
 
   // where a lane reads within a row: its share of a row of keys, and of values
   const int kblock = NB == 2 ? g >> 1 : g, kbyte = NB == 2 ? g * (BB / 2) : g * BB;
@@ -79,67 +80,95 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
   const uint8_t *kc = a.kc + u.head * a.c.head_stride[0], *ks = a.ks + u.head * a.c.head_stride[1];
   const uint8_t *vc = a.vc + u.head * a.c.head_stride[2], *vs = a.vs + u.head * a.c.head_stride[3];
   const int32_t* table = a.table + (int64_t)u.b * a.a.table_row;
-  // The page and row of a key that the cache has; false: there is none.
-  auto locate = [&](int key, int& page, int& at) {
-    const int k = key < s.length ? key : s.length - 1;
-    const int i = (int)divu31(k, a.by_page);
-    at = k - i * (int)a.c.page_size;
-    page = table[i];
-    const bool there = key < s.length && page >= 0 && page < a.c.pages;
-    if (!there) page = 0, at = 0;
-    return there;
-  };
-
   uint32_t kw[2][KW], ksc[2][NB == 8 ? 2 : 1], vw[8][VW], vsc[8];
   uint32_t there = 0;                                     // bit i: key i of this lane's eight
-  auto load_keys = [&](int step) {
-    const int k0 = base + step * kStep;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      int page, at;
-      locate(k0 + 16 * t + 4 * (c & 3) + (c >> 2), page, at);
-      const uint8_t* p = kc + page * a.c.page_stride[0] + at * a.c.row_stride[0] + kbyte;
-      const uint8_t* f = ks + page * a.c.page_stride[1] + at * a.c.row_stride[1] + kblock;
+  constexpr int first = NB == 8 ? KW / 2 : KW;            // words of keys' codes in one piece
+  auto read_keys = [&](int t, const uint8_t* p, const uint8_t* f, uint32_t code, uint32_t scale) {
+    if (a.blocks < NB) {
 #pragma unroll
       for (int i = 0; i < KW; ++i) kw[t][i] = 0;
       ksc[t][0] = 0;
-      constexpr int first = NB == 8 ? KW / 2 : KW;
-      if (kthere) {
-        __builtin_memcpy(&kw[t][0], p, 4 * first);
-        ksc[t][0] = *f;
+      if constexpr (NB == 8) ksc[t][1] = 0;
+    }
+    if (a.blocks == NB || kthere) {
+      __builtin_memcpy(&kw[t][0], p + code, 4 * first);
+      ksc[t][0] = f[scale];
+    }
+    if constexpr (NB == 8) {
+      if (a.blocks == NB || kthere2) {
+        __builtin_memcpy(&kw[t][first], p + code + 4 * BB, 4 * first);
+        ksc[t][1] = f[scale + 4];
       }
-      if constexpr (NB == 8) {
-        ksc[t][1] = 0;
-        if (kthere2) {
-          __builtin_memcpy(&kw[t][first], p + 4 * BB, 4 * first);
-          ksc[t][1] = f[4];
+    }
+  };
+  const uint32_t krow = 4 * (c & 3) + (c >> 2);
+  // Where the 32 keys of a step lie.  PAGES16: each tile of 16 has a page, found by scalar loads a step ahead, and a lane's
+  // place within a tile is the same in every step; rows past the length are read as they are, and masked.  Otherwise lane l
+  // finds key l % 32, and the others ask it.
+  struct Places {
+    int page[2], at[2];
+    uint32_t there;                                       // bit t: tile t's page; otherwise bit 0: this lane's key
+  };
+  auto places_of = [&](int step) {
+    Places p;
+    p.there = 0;
+#pragma unroll
+    for (int t = 0; t < (PAGES16 ? 2 : 1); ++t) {
+      const int key = base + step * kStep + (PAGES16 ? 16 * t : lane & 31), k = key < s.length ? key : s.length - 1;
+      const int i = (int)divu31(k, a.by_page), page = PAGES16 ? same(table[i]) : table[i];
+      const bool yes = key < s.length && (uint32_t)page < (uint32_t)a.c.pages;
+      p.page[t] = yes ? page : 0;
+      p.at[t] = yes ? k - i * (int)a.c.page_size : 0;
+      p.there |= yes ? 1u << t : 0u;
+    }
+    return p;
+  };
+  const uint32_t kcode = PAGES16 ? krow * (uint32_t)a.c.row_stride[0] + kbyte : kbyte, kscale = PAGES16 ? krow * (uint32_t)a.c.row_stride[1] + kblock : kblock;
+  // columns of blocks that a row does not have are not stored: the first block does for them
+  const uint32_t vcode = (PAGES16 ? g * (uint32_t)a.c.row_stride[2] : 0) + (vthere ? c * VB : 0);
+  const uint32_t vscale = (PAGES16 ? g * (uint32_t)a.c.row_stride[3] : 0) + (vthere ? vblock : 0);
+  auto load_keys = [&](const Places& p) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int page = PAGES16 ? p.page[t] : __shfl(p.page[0], 16 * t + krow), at = PAGES16 ? p.at[t] : __shfl(p.at[0], 16 * t + krow);
+      read_keys(t, kc + page * a.c.page_stride[0] + at * a.c.row_stride[0], ks + page * a.c.page_stride[1] + at * a.c.row_stride[1], kcode, kscale);
+    }
+  };
+  auto load_values = [&](const Places& p) {
+    there = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (PAGES16) {
+        there |= p.there >> t & 1 ? 0xFu << 4 * t : 0u;
+        const uint8_t* code = vc + p.page[t] * a.c.page_stride[2] + p.at[t] * a.c.row_stride[2];
+        const uint8_t* scale = vs + p.page[t] * a.c.page_stride[3] + p.at[t] * a.c.row_stride[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          __builtin_memcpy(&vw[4 * t + r][0], code + 4 * r * a.c.row_stride[2] + vcode, VB);
+          vsc[4 * t + r] = (scale + 4 * r * a.c.row_stride[3])[vscale];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int from = 16 * t + 4 * r + g, page = __shfl(p.page[0], from), at = __shfl(p.at[0], from);
+          there |= (uint32_t)__shfl((int)p.there, from) << (4 * t + r);
+          __builtin_memcpy(&vw[4 * t + r][0], vc + page * a.c.page_stride[2] + at * a.c.row_stride[2] + vcode, VB);
+          vsc[4 * t + r] = (vs + page * a.c.page_stride[3] + at * a.c.row_stride[3])[vscale];
         }
       }
     }
   };
-  auto load_values = [&](int step) {
-    const int k0 = base + step * kStep;
-    there = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      int page, at;
-      const bool yes = locate(k0 + 16 * (i >> 2) + 4 * (i & 3) + g, page, at);
-      there |= yes ? 1u << i : 0u;
-      const uint8_t* p = vc + page * a.c.page_stride[2] + at * a.c.row_stride[2] + c * VB;
-#pragma unroll
-      for (int w = 0; w < VW; ++w) vw[i][w] = 0;
-      vsc[i] = 0;
-      if (yes && vthere) {
-        __builtin_memcpy(&vw[i][0], p, VB);
-        vsc[i] = vs[page * a.c.page_stride[3] + at * a.c.row_stride[3] + vblock];
-      }
-    }
-  };
 
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int w = 0; w < VW; ++w) vw[i][w] = 0;
   int step = begin + wave;
+  Places next = step < end ? places_of(step) : Places{};
   if (step < end) {
-    load_keys(step);
-    load_values(step);
+    load_keys(next);
+    load_values(next);
+    next = places_of(step + kFewWaves);
   }
   for (; step < end; step += kFewWaves) {
     const int k0 = base + step * kStep;
@@ -154,9 +183,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
         for (int p = P - 1; p >= 0; --p) z[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[p][i], z[t], 0, 0, 0);
       }
     }
-    if (step + kFewWaves < end) load_keys(step + kFewWaves);
+    if (step + kFewWaves < end) load_keys(next);
 
-    const bool part = k0 < all_from || k0 + kStep > all_to || __any(there != 0xFF);
+    const bool part = k0 < all_from || k0 + kStep > all_to || (PAGES16 ? there != 0xFF : __any(there != 0xFF));
     uint32_t seen = 0xFF;
     if (part) {
       seen = 0;
@@ -195,63 +224,52 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
     bf16x8 pw[P];
     planes_of(w, pw);
 
-    // two neighbouring columns at a time: pairs of columns of a key become pairs of keys of a column
-    bool odd = false;                                     // an infinity or a NaN among the values
+    // Zero times infinity is no zero.  Where a key is hidden from some query, values that are no finite number are taken out,
+    // and the sums of the queries that see one of them become NaN.
+    if (part) {
+      bool odd = false;
 #pragma unroll
-    for (int t8 = 0; t8 < (OT < 8 ? 1 : OT / 8); ++t8) {
-      constexpr int pairs = OT < 8 ? OT / 2 : 4;
-      uint32_t col[8][pairs];
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = scale_field(vsc[i]);
-        const bf16x8 e = eight_codes<FAM>(&vw[i][t8 * EW], f);      // of a row of 64 columns only the first four are there
-        uint32_t x[4];
-        __builtin_memcpy(x, &e, 16);
+        for (int w = 0; w < VW; ++w) odd |= may_be_odd<FAM>(vw[i][w], vsc[i]);
+      if (__any(odd)) {
+        uint32_t sees[4];
 #pragma unroll
-        for (int j = 0; j < pairs; ++j) col[i][j] = x[j];
-      }
+        for (int i = 0; i < 4; ++i) sees[i] = (seen >> 2 * i & 1 ? 0x3F80u : 0u) | (seen >> 2 * i & 2 ? 0x3F800000u : 0u);
+        bf16x8 sw;
+        __builtin_memcpy(&sw, sees, 16);
 #pragma unroll
-      for (int j = 0; j < pairs; ++j) {
+        for (int j = 0; j < OT / 2; ++j) {
+          uint32_t x[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t x[4];
+          for (int i = 0; i < 8; ++i) x[i] = take_odd<FAM>(&vw[i][0], j, scale_field(vsc[i]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(col[2 * i + 1][j], col[2 * i][j], half ? 0x07060302u : 0x05040100u);
-          bf16x8 v;
-          __builtin_memcpy(&v, x, 16);
-          const int t = t8 * 8 + 2 * j + half;
-          if (part) {
-            odd = false;
+          for (int half = 0; half < 2; ++half) {
+            const f32x4 found = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys_of_column(x, half), sw, f32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) odd |= (x[i] & 0x7F80u) == 0x7F80u || (x[i] & 0x7F800000u) == 0x7F800000u;
-            if (__any(odd)) {
-              // zero times infinity is no zero: the product with each query's own keys alone, its column kept
-              for (int n = 0; n < 16; ++n) {
-                const int l = __builtin_amdgcn_readlane(lo, n), h = __builtin_amdgcn_readlane(hi, n);
-                uint32_t y[4];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const int key = k0 + 16 * (i >> 2) + 4 * (i & 3) + g;
-                  const uint32_t keep = key >= l && key <= h ? 0xFFFFu : 0u;
-                  if (i & 1) y[i >> 1] |= x[i >> 1] & keep << 16;
-                  else y[i >> 1] = x[i >> 1] & keep;
-                }
-                bf16x8 m;
-                __builtin_memcpy(&m, y, 16);
-                f32x4 sum = o[t];
-#pragma unroll
-                for (int p = P - 1; p >= 0; --p) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(m, pw[p], sum, 0, 0, 0);
-                if (c == n) o[t] = sum;
-              }
-              continue;
-            }
+            for (int r = 0; r < 4; ++r) o[2 * j + half][r] = found[r] > 0.0f ? __builtin_nanf("") : o[2 * j + half][r];
           }
-#pragma unroll
-          for (int p = P - 1; p >= 0; --p) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw[p], o[t], 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vsc[i] = vsc[i] == 255 ? 127 : vsc[i];        // whose codes are zeros now
       }
     }
-    if (step + kFewWaves < end) load_values(step + kFewWaves);
+#pragma unroll
+    for (int j = 0; j < OT / 2; ++j) {
+      uint32_t x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = two_codes<FAM>(&vw[i][0], j, scale_field(vsc[i]));
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const bf16x8 v = keys_of_column(x, half);
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) o[2 * j + half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw[p], o[2 * j + half], 0, 0, 0);
+      }
+    }
+    if (step + kFewWaves < end) {
+      load_values(next);
+      next = places_of(step + 2 * kFewWaves);
+    }
   }
 
   // the waves' sums, relative to the largest of their maxima, in the order of the waves
@@ -291,16 +309,20 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attend_few(AttendArgs a, int
   }
 }
 
-template <int FAM, int DT> void launch_attend_few_of(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
+template <int FAM, int DT, int NB> void launch_attend_few_of(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
   const dim3 grid((unsigned)units), block(64 * kFewWaves);
-  if (a.blocks <= 2) k_attend_few<FAM, DT, 2><<<grid, block, 0, st>>>(a, least);
-  else if (a.blocks <= 4) k_attend_few<FAM, DT, 4><<<grid, block, 0, st>>>(a, least);
-  else k_attend_few<FAM, DT, 8><<<grid, block, 0, st>>>(a, least);
+  if (a.aligned) k_attend_few<FAM, DT, NB, true><<<grid, block, 0, st>>>(a, least);
+  else k_attend_few<FAM, DT, NB, false><<<grid, block, 0, st>>>(a, least);
+}
+template <int FAM, int DT> void launch_attend_few_by(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
+  if (a.blocks <= 2) launch_attend_few_of<FAM, DT, 2>(a, units, least, st);
+  else if (a.blocks <= 4) launch_attend_few_of<FAM, DT, 4>(a, units, least, st);
+  else launch_attend_few_of<FAM, DT, 8>(a, units, least, st);
 }
 template <int FAM> void launch_attend_few(const AttendArgs& a, int64_t units, int least, hipStream_t st) {
-  if (a.a.dtype == MXQ_DT_F32) launch_attend_few_of<FAM, MXQ_DT_F32>(a, units, least, st);
-  else if (a.a.dtype == MXQ_DT_BF16) launch_attend_few_of<FAM, MXQ_DT_BF16>(a, units, least, st);
-  else launch_attend_few_of<FAM, MXQ_DT_F16>(a, units, least, st);
+  if (a.a.dtype == MXQ_DT_F32) launch_attend_few_by<FAM, MXQ_DT_F32>(a, units, least, st);
+  else if (a.a.dtype == MXQ_DT_BF16) launch_attend_few_by<FAM, MXQ_DT_BF16>(a, units, least, st);
+  else launch_attend_few_by<FAM, MXQ_DT_F16>(a, units, least, st);
 }
 
 }  // namespace mxq

@@ -10,32 +10,66 @@ namespace mxq {
 // A row's block of 32 codes: 32 bytes, 16 of MXFP4's pairs.  FAM: kE4M3, kE5M2 or kPairs.
 constexpr int kCacheBlock = 32;
 
-// Eight codes (two words, one of pairs) times the scale as bfloat16: exact (a code has at most 4 significant bits) but for
+// Codes 2 j and 2 j + 1 of some words times the scale as two bfloat16: exact (a code has at most 4 significant bits) but for
 // values below 2^-126, rounded to bfloat16's subnormals.  scale: 2^(byte - 127) as the conversions take it, the byte in a
 // float's exponent field.
-template <int FAM> __device__ __forceinline__ bf16x8 eight_codes(const uint32_t* w, float scale) {
-  bf16x2 v[4];
+template <int FAM> __device__ __forceinline__ uint32_t two_codes(const uint32_t* w, int j, float scale) {
+  bf16x2 v;
   if constexpr (FAM == kPairs) {
-    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 0);
-    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 1);
-    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 2);
-    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 3);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (FAM == kE5M2) {
-        v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[i], scale, false);
-        v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[i], scale, true);
-      } else {
-        v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, false);
-        v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], scale, true);
-      }
+    switch (j & 3) {
+      case 0: v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j >> 2], scale, 0); break;
+      case 1: v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j >> 2], scale, 1); break;
+      case 2: v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j >> 2], scale, 2); break;
+      default: v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j >> 2], scale, 3); break;
     }
+  } else if constexpr (FAM == kE5M2) {
+    v = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[j >> 1], scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w[j >> 1], scale, false);
+  } else {
+    v = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], scale, false);
   }
+  uint32_t u;
+  __builtin_memcpy(&u, &v, 4);
+  return u;
+}
+template <int FAM> __device__ __forceinline__ bf16x8 eight_codes(const uint32_t* w, float scale) {
+  uint32_t v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = two_codes<FAM>(w, j, scale);
   bf16x8 r;
   __builtin_memcpy(&r, v, 16);
   return r;
 }
+
+// Whether some value of a word of codes under this scale byte is, or may be, an infinity or a NaN in bfloat16.
+template <int FAM> __device__ __forceinline__ bool may_be_odd(uint32_t w, uint32_t scale) {
+  if (scale >= kPastFloat<FAM>) return true;
+  if constexpr (FAM == kPairs) return false;
+  constexpr uint32_t special = FAM == kE4M3 ? 0x7F7F7F7Fu : 0x7C7C7C7Cu;
+  const uint32_t x = (w & special) ^ special;               // a byte of zeros: E4M3's NaN, E5M2's infinities and NaNs
+  return (x - 0x01010101u & ~x & 0x80808080u) != 0;
+}
+// Ones in the place of those of codes 2 j and 2 j + 1 whose value is no finite number, zeros in that of others; the codes
+// become zeros.
+template <int FAM> __device__ __forceinline__ uint32_t take_odd(uint32_t* w, int j, float scale) {
+  const uint32_t x = two_codes<FAM>(w, j, scale);
+  const bool low = (x & 0x7F80u) == 0x7F80u, high = (x & 0x7F800000u) == 0x7F800000u;
+  constexpr int bits = FAM == kPairs ? 4 : 8, each = 32 / bits;
+  const uint32_t code = (1u << bits) - 1, at = 2 * j % each * bits;
+  w[2 * j / each] &= ~((low ? code << at : 0u) | (high ? code << (at + bits) : 0u));
+  return (low ? 0x3F80u : 0u) | (high ? 0x3F800000u : 0u);
+}
+
+// Of pairs of neighbouring columns, a pair a key of eight keys, the keys of the first or the second column: an operand of
+// the product with values.
+__device__ __forceinline__ bf16x8 keys_of_column(const uint32_t (&x)[8], int second) {
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], second ? 0x07060302u : 0x05040100u);
+  bf16x8 v;
+  __builtin_memcpy(&v, y, 16);
+  return v;
+}
+
 __device__ __forceinline__ float scale_field(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 struct AttendArgs {
@@ -86,6 +120,8 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
 // keys; a sequence's keys are cut into runs of whole `steps` of 32, as many as make the units about fill the card, however
 // its sequences' lengths differ.  Every wave finds its unit by itself from the lengths.
 constexpr int kStep = 32;
+__device__ __forceinline__ int same(int v) { return __builtin_amdgcn_readfirstlane(v); }   // of a wave's lanes, as it is in all of them
+__device__ __forceinline__ Sequence same(const Sequence& s) { return Sequence{same(s.start), same(s.n), same(s.length), same(s.lo), same(s.hi)}; }
 struct Cut {
   int tiles, runs;       // tiles of rows, runs of keys of each
 };
@@ -136,7 +172,7 @@ __device__ __forceinline__ Unit unit_of(const AttendArgs& a, int rows, int quota
       const int owner = __builtin_ctzll(at);
       const int within = which - before - __builtin_amdgcn_readlane(upto - mine, owner);
       const int runs = __builtin_amdgcn_readlane(c.runs, owner), tile = within / runs;
-      return Unit{b0 + owner, tile, within - tile * runs, runs, head};
+      return Unit{same(b0 + owner), same(tile), same(within - tile * runs), same(runs), head};
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
