@@ -10,66 +10,71 @@ void launch_attend_few_pairs(const AttendArgs&, int64_t, int, hipStream_t);
 
 namespace {
 
-constexpr int kFewRows = 16, kFewLeast = 8, kFewWanted = 1024;
+constexpr int kFewRows = 16, kFewLeast = 8, kUnits = 256;   // rows a tile, steps a workgroup at least, CUs
 
-// The rows of sequences that were cut, from their units' sums in the order of the runs, and zeros for rows of no sequence.
-// A wave a row.
-__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, int unit_rows, int least, int columns) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, H = (int)a.a.heads, D = a.c.head_dim;
-  if (row >= a.a.T * H) return;
-  const int t = (int)(row / H), h = (int)(row - (int64_t)t * H);
-  int b;
+// The rows of tiles that were cut, from their parts' sums, and zeros for rows of no sequence.  A workgroup takes every
+// gridDim.y-th row of a tile of rows, its waves the runs in turn, then the waves' sums in their order.
+template <int COLUMNS>
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, int unit_rows, int least) {
+  constexpr int V = COLUMNS / 64;
+  __shared__ float sums[4][COLUMNS];
+  __shared__ float weights[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim;
   if (a.starts) {
-    int low = -1, high = (int)a.a.B;                        // the last sequence that starts at t or before
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (a.starts[mid] <= t) low = mid;
-      else high = mid;
+    // queries [0, starts[0]) and [starts[B], T) are no sequence's
+    const int T = (int)a.a.T, x = a.a.B ? a.starts[0] : T, y = a.a.B ? a.starts[a.a.B] : T;
+    const int64_t head = (int64_t)(x < 0 ? 0 : x > T ? T : x) * a.a.heads, tail = (int64_t)(y < 0 ? 0 : y > T ? T : y) * a.a.heads;
+    const int64_t from = tail < head ? head : tail, all = head + (a.a.T * a.a.heads - from);
+    const int64_t groups = (int64_t)gridDim.x * gridDim.y, me = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    for (int64_t i = me * 4 + wave; i < all; i += groups * 4) {
+      const int64_t row = i < head ? i : from + i - head;
+      for (int d = lane; d < D; d += 64) store_elem(a.out, a.a.dtype, row * D + d, 0.0f);
+      if (a.lse && lane == 0) a.lse[row] = -__builtin_inff();
     }
-    b = low;
-  } else {
-    b = t / (int)(a.a.T / a.a.B);
-  }
-  const Sequence s = b < 0 ? Sequence{0, 0, 0, 0, 0} : sequence(a, b);
-  if (t < s.start || t >= s.start + s.n) {
-    for (int d = lane; d < D; d += 64) store_elem(a.out, a.a.dtype, row * D + d, 0.0f);
-    if (a.lse && lane == 0) a.lse[row] = -__builtin_inff();
-    return;
   }
   if (!a.partial) return;
-  const int quota = quota_of(a, unit_rows, least);
-  const Cut c = cut(a, s, unit_rows, quota);
-  if (c.runs == 1) return;
-  int first = 0;
-  for (int i = lane; i < b; i += 64) {
-    const Cut o = cut(a, sequence(a, i), unit_rows, quota);
-    first += o.tiles * o.runs;
-  }
-  first = wave_sum(first);
-  const int head = h / a.group, r = (t - s.start) * a.group + h - head * a.group, tile = r / unit_rows;
-  const int64_t stride = (int64_t)a.c.kv_heads * unit_rows * (columns + 2);
-  const float* part = a.partial + (((int64_t)(first + tile * c.runs) * a.c.kv_heads + head) * unit_rows + r - tile * unit_rows) * (columns + 2);
-  float best = -__builtin_inff(), all = 0.0f;
-  for (int i = lane; i < c.runs; i += 64) best = __builtin_fmaxf(best, part[i * stride + columns]);
-  for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = 0; i < c.runs; ++i) {
-    const float top = part[i * stride + columns], sum = part[i * stride + columns + 1];
-    // a run without a maximum has seen no key, or only scores of NaN
-    const float factor = top == -__builtin_inff() ? sum : __builtin_amdgcn_exp2f(top - best);
-    if (factor == 0.0f) continue;
-    all += top == -__builtin_inff() ? sum : factor * sum;
+  const Tile u = tile_of(a, unit_rows, blockIdx.x, true);
+  if (u.b < 0) return;
+  const Line line = line_of(a, unit_rows, least);
+  const int g0 = same(line.group_at(u.first)), runs = same(line.group_at(u.first + u.steps - 1)) - g0 + 1;
+  if (runs == 1) return;
+  const bool at_begin = line.begin(g0) == u.first;          // of the first group's piece the tile is the first
+  const Sequence s = same(sequence(a, u.b));
+  const int rows = s.n * a.group, row_tiles = (rows + unit_rows - 1) / unit_rows, kv_head = u.index / row_tiles;
+  const int row0 = (u.index - kv_head * row_tiles) * unit_rows, last = rows - row0 < unit_rows ? rows - row0 : unit_rows;
+  for (int r = blockIdx.y; r < last; r += gridDim.y) {
+    auto part_of = [&](int i) { return a.partial + (part_slot(g0 + i, i || at_begin) * unit_rows + r) * (COLUMNS + 2); };
+    float best = -__builtin_inff(), all = 0.0f, v[V];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 64 * k < D) v[k] += factor * part[i * stride + lane + 64 * k];
-  }
-  const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+    for (int i = lane; i < runs; i += 64) best = __builtin_fmaxf(best, part_of(i)[COLUMNS]);
+    for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
+#pragma unroll 4
+    for (int i = wave; i < runs; i += 4) {
+      const float* part = part_of(i);
+      const float top = part[COLUMNS], sum = part[COLUMNS + 1];
+      // a run without a maximum has seen no key, or only scores of NaN, which its sum is then
+      const float factor = top == -__builtin_inff() ? sum : __builtin_amdgcn_exp2f(top - best);
+      float x[V];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 64 * k < D) store_elem(a.out, a.a.dtype, row * D + lane + 64 * k, v[k] * inv);
-  if (a.lse && lane == 0)
-    a.lse[row] = all == 0.0f ? -__builtin_inff() : best == -__builtin_inff() ? all : (best + __builtin_amdgcn_logf(all)) * 0.693147180559945309f;
+      for (int k = 0; k < V; ++k) x[k] = part[lane * V + k];
+      all += top == -__builtin_inff() ? sum : factor * sum;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
+    }
+    if (lane == 0) weights[wave] = all;
+#pragma unroll
+    for (int k = 0; k < V; ++k) sums[wave][lane * V + k] = v[k];
+    __syncthreads();
+    const int t = (int)divu31(row0 + r, a.by_group), h = kv_head * a.group + row0 + r - t * a.group;
+    const int64_t row = (int64_t)(s.start + t) * a.a.heads + h;
+    all = ((weights[0] + weights[1]) + weights[2]) + weights[3];
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+    for (int d = threadIdx.x; d < D; d += 256)
+      store_elem(a.out, a.a.dtype, row * D + d, (((sums[0][d] + sums[1][d]) + sums[2][d]) + sums[3][d]) * inv);
+    if (a.lse && threadIdx.x == 0) a.lse[row] = log_sum(best, all);
+    __syncthreads();
+  }
 }
 
 int check(const mxq_cache_spec* c, const mxq_attend_spec* a) {
@@ -90,20 +95,18 @@ int check(const mxq_cache_spec* c, const mxq_attend_spec* a) {
   return MXQ_OK;
 }
 
-// Units of `rows` rows that a call may have: tiles of rows, and with runs of keys as many as are wanted besides.
+// Tiles of `rows` rows that a call may have, and whether they may be cut: not where no sequence has keys for it.
 struct Plan {
-  int64_t units;
+  int64_t tiles;
   bool split;
 };
-Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged, int rows, int least, int wanted) {
+Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged, int rows, int least) {
   const int64_t group = a.heads / c.kv_heads;
   int64_t tiles;
   if (ragged) tiles = a.T * group / rows + (a.B < a.T ? a.B : a.T);
   else tiles = a.B * ceil_div(a.T / a.B * group, rows);
   const int64_t keys = a.table_pages * c.page_size, seen = a.window && a.window < keys ? a.window + (ragged ? a.T : a.T / a.B) : keys;
-  const bool split = (keys < seen ? keys : seen) > (int64_t)(least - 1) * kStep;
-  // the quota is a float32 sum's, a part of 2^-16 too small at worst
-  return Plan{tiles * c.kv_heads + (split ? wanted + wanted / 64 : 0), split};
+  return Plan{tiles * c.kv_heads, (keys < seen ? keys : seen) > (int64_t)(least - 1) * kStep};
 }
 int columns_of(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
@@ -113,8 +116,9 @@ int columns_of(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 12
 extern "C" int64_t mxq_cache_attend_workspace(const mxq_cache_spec* cache, const mxq_attend_spec* spec, int32_t ragged) {
   using namespace mxq;
   if (check(cache, spec) || spec->T == 0 || spec->B == 0) return 0;
-  const Plan p = plan_of(*cache, *spec, ragged, kFewRows, kFewLeast, kFewWanted);
-  return p.split ? p.units * kFewRows * (columns_of(cache->head_dim) + 2) * (int64_t)sizeof(float) : 0;
+  const Plan p = plan_of(*cache, *spec, ragged, kFewRows, kFewLeast);
+  const int64_t groups = kUnits * few_groups(spec->dtype, (cache->head_dim + 31) / 32);
+  return p.split ? 2 * groups * kFewRows * (columns_of(cache->head_dim) + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
@@ -135,22 +139,28 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   a.c = *cache, a.a = *spec;
   a.by_page = make_divu31((uint32_t)cache->page_size), a.by_group = make_divu31((uint32_t)group);
   a.group = (int)group, a.blocks = (cache->head_dim + 31) / 32;
-  a.wanted = kFewWanted;
+  a.wanted = kUnits * few_groups(spec->dtype, a.blocks);
   a.aligned = cache->page_size % 16 == 0;
   for (int64_t r : cache->row_stride) a.aligned = a.aligned && r >= 0 && r < 1 << 26;
   a.scale2 = spec->scale * 1.44269504088896341f;
   hipStream_t st = as_stream(stream);
+  Plan p = {};
   if (spec->B) {
-    const Plan p = plan_of(*cache, *spec, starts != nullptr, kFewRows, kFewLeast, kFewWanted);
+    p = plan_of(*cache, *spec, starts != nullptr, kFewRows, kFewLeast);
     if (p.split && !workspace) return invalid("mxq_cache_attend: NULL workspace");
-    if (p.units * 256 > kMaxThreads) return invalid("mxq_cache_attend: too many units for a launch");
+    if (p.tiles * 256 > kMaxThreads) return invalid("mxq_cache_attend: too many tiles for a launch");
     a.partial = p.split ? (float*)workspace : nullptr;
     auto launch = cache->format == MXQ_FMT_E4M3 ? launch_attend_few_e4m3 : cache->format == MXQ_FMT_E5M2 ? launch_attend_few_e5m2 : launch_attend_few_pairs;
-    launch(a, p.units, kFewLeast, st);
+    launch(a, p.tiles, kFewLeast, st);
     if (int rc = check_launch("mxq_cache_attend")) return rc;
   }
   if (a.partial || starts) {
-    k_attend_join<<<dim3((unsigned)ceil_div(spec->T * spec->heads, 4)), 256, 0, st>>>(a, kFewRows, kFewLeast, columns);
+    // few tiles: a workgroup for each of their rows
+    const int64_t tiles = a.partial ? p.tiles : blocks_for(ceil_div(spec->T * spec->heads, 64));
+    const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 2048 ? 1 : tiles >= 512 ? 4 : 16));
+    if (columns == 64) k_attend_join<64><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
+    else if (columns == 128) k_attend_join<128><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
+    else k_attend_join<256><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
     return check_launch("mxq_cache_attend");
   }
   return MXQ_OK;

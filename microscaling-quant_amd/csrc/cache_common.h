@@ -78,7 +78,7 @@ struct AttendArgs {
   const int32_t *table, *lengths, *starts;
   void* out;
   float* lse;
-  float* partial;        // a unit's unnormalised sums, maxima and sums of weights; NULL: no sequence is split
+  float* partial;        // sums, maxima and sums of weights of parts of tiles; NULL: a workgroup has one whole tile
   mxq_cache_spec c;
   mxq_attend_spec a;
   DivU31 by_page, by_group;
@@ -116,67 +116,83 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
   return s;
 }
 
-// How the work is cut.  A unit is `rows` rows (a head of keys' queries, token by token, its heads within) and a run of
-// keys; a sequence's keys are cut into runs of whole `steps` of 32, as many as make the units about fill the card, however
-// its sequences' lengths differ.  Every wave finds its unit by itself from the lengths.
+// How the work of few queries is cut.  A tile is `rows` rows of one head of keys (queries token by token, the heads that
+// share it within) and its steps of 32 keys, one at least.  The batch's tiles, a sequence's with equal numbers of steps, lie
+// one behind another on a line of steps, and every workgroup takes an equal piece of it, however lengths differ: a number of
+// whole tiles, and a part of one before and behind them, whose sums are joined later.  Every wave finds its way by itself from
+// the lengths.
 constexpr int kStep = 32;
 __device__ __forceinline__ int same(int v) { return __builtin_amdgcn_readfirstlane(v); }   // of a wave's lanes, as it is in all of them
+__device__ __forceinline__ int64_t same(int64_t v) { return (int64_t)((uint64_t)(uint32_t)same((int)(v >> 32)) << 32 | (uint32_t)same((int)v)); }
 __device__ __forceinline__ Sequence same(const Sequence& s) { return Sequence{same(s.start), same(s.n), same(s.length), same(s.lo), same(s.hi)}; }
-struct Cut {
-  int tiles, runs;       // tiles of rows, runs of keys of each
+
+struct Share {
+  int tiles, steps;      // of a sequence: its tiles (of all heads), steps of each
 };
-__device__ __forceinline__ int steps_of(const Sequence& s) { return s.hi > s.lo ? (s.hi - (s.lo & ~(kStep - 1)) + kStep - 1) / kStep : 0; }
-__device__ __forceinline__ Cut cut(const AttendArgs& a, const Sequence& s, int rows, int quota) {
-  Cut c;
-  c.tiles = (int)(((int64_t)s.n * a.group + rows - 1) / rows);
-  const int steps = steps_of(s);
-  c.runs = a.partial && steps > quota ? (steps + quota - 1) / quota : 1;
-  return c;
+__device__ __forceinline__ Share share_of(const AttendArgs& a, const Sequence& s, int rows) {
+  const int tiles = (int)(((int64_t)s.n * a.group + rows - 1) / rows) * (int)a.c.kv_heads;
+  return Share{tiles, s.hi > s.lo ? (s.hi - (s.lo & ~(kStep - 1)) + kStep - 1) / kStep : 1};
 }
-__device__ __forceinline__ int wave_sum(int v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-// Steps a unit should take: the batch's steps over the units wanted, `least` at least.
-__device__ __forceinline__ int quota_of(const AttendArgs& a, int rows, int least) {
-  if (!a.partial) return least;
-  const int lane = threadIdx.x & 63;
-  float total = 0.0f;                                       // a number of the batch's steps, not a sum that results depend on
-  for (int b = lane; b < a.a.B; b += 64) {
-    const Sequence s = sequence(a, b);
-    total += (float)cut(a, s, rows, 1 << 30).tiles * (float)steps_of(s);
+struct Line {
+  int64_t total;         // steps
+  int groups;            // workgroups that have a piece
+  __device__ int64_t begin(int i) const { return total * i / groups; }
+  __device__ int group_at(int64_t step) const { return (int)(((step + 1) * groups - 1) / total); }
+};
+__device__ __forceinline__ Line line_of(const AttendArgs& a, int rows, int least) {
+  int64_t total = 0;
+  for (int b = threadIdx.x & 63; b < a.a.B; b += 64) {
+    const Share h = share_of(a, sequence(a, b), rows);
+    total += (int64_t)h.tiles * h.steps;
   }
   for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-  const float each = total * (float)a.c.kv_heads / (float)a.wanted;
-  const int quota = each < 1e9f ? (int)__builtin_ceilf(each) : 1000000000;
-  return quota < least ? least : quota;
+  total = same(total);
+  const int64_t most = (total + least - 1) / least;
+  return Line{total, most < a.wanted ? (int)most : a.wanted};
 }
-struct Unit {
-  int b, tile, run, runs, head;   // b < 0: there is none
+// A tile: of sequence b (-1: there is none) the index-th, and the place of its first step on the line.
+struct Tile {
+  int b, index, steps;
+  int64_t first;
 };
-__device__ __forceinline__ Unit unit_of(const AttendArgs& a, int rows, int quota, int index) {
-  const int lane = threadIdx.x & 63, heads = (int)a.c.kv_heads;
-  const int which = index / heads, head = index - which * heads;
-  int before = 0;
+// The tile at a step of the line, or the one with this number.
+__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int rows, int64_t at, bool number) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0, steps_before = 0;
   for (int b0 = 0; b0 < a.a.B; b0 += 64) {
-    Cut c{0, 1};
-    if (b0 + lane < a.a.B) c = cut(a, sequence(a, b0 + lane), rows, quota);
-    const int mine = c.tiles * c.runs;
-    int upto = mine;
+    Share h{0, 1};
+    if (b0 + lane < a.a.B) h = share_of(a, sequence(a, b0 + lane), rows);
+    const int64_t steps = (int64_t)h.tiles * h.steps, mine = number ? h.tiles : steps;
+    int64_t upto = mine, steps_upto = steps;
     for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
+      const int64_t v = __shfl_up(upto, o), w = __shfl_up(steps_upto, o);
+      if (lane >= o) upto += v, steps_upto += w;
     }
-    const uint64_t at = __ballot(which < before + upto && which >= before + upto - mine);
-    if (at) {
-      const int owner = __builtin_ctzll(at);
-      const int within = which - before - __builtin_amdgcn_readlane(upto - mine, owner);
-      const int runs = __builtin_amdgcn_readlane(c.runs, owner), tile = within / runs;
-      return Unit{same(b0 + owner), same(tile), same(within - tile * runs), same(runs), head};
+    upto += before, steps_upto += steps_before;
+    const uint64_t found = __ballot(at < upto && at >= upto - mine);
+    if (found) {
+      const int owner = __builtin_ctzll(found);
+      const int each = __shfl(h.steps, owner);
+      const int64_t first = __shfl(steps_upto - steps, owner), within = at - __shfl(upto - mine, owner);
+      const int index = same((int)(number ? within : within / each));
+      return Tile{same(b0 + owner), index, same(each), same(first + (int64_t)index * each)};
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before = __shfl(upto, 63), steps_before = __shfl(steps_upto, 63);
   }
-  return Unit{-1, 0, 0, 1, 0};
+  return Tile{-1, 0, 1, 0};
+}
+// Workgroups a CU (of a wave for each of its SIMDs) that the registers of the kernel of few queries are held to, and the
+// steps that it asks for ahead.
+constexpr int few_groups(int dtype, int blocks) { return blocks <= 2 ? 3 : blocks <= 4 || dtype == MXQ_DT_BF16 ? 2 : 1; }
+constexpr int few_depth(int dtype, int blocks) { return blocks <= 4 ? 2 : 1; }
+
+// Where the sums of a piece's parts of tiles lie: of the tile that its first step is in, and of its last one.
+__device__ __forceinline__ int64_t part_slot(int group, bool first) { return 2 * (int64_t)group + !first; }
+
+// The logarithm of a sum of weights relative to 2^top; of no weights -inf.
+__device__ __forceinline__ float log_sum(float top, float sum) {
+  if (sum == 0.0f) return -__builtin_inff();
+  return top == -__builtin_inff() ? sum : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
 }
 
 template <int DT> constexpr int kAttendPlanes = DT == MXQ_DT_BF16 ? 1 : DT == MXQ_DT_F16 ? 2 : 3;

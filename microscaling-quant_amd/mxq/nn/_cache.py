@@ -11,14 +11,14 @@ Slot s is row s % page_size of page s // page_size.  Rows are quantized in block
 2^(floor(log2 amax) - emax), elements to the nearest: the bytes of mxq.packed.quantize(x, fmt, "ocp", axis=-1), MXFP4's codes
 two to a byte.  For inference: codes have no gradient, and an input that asks for one is refused.
 """
-import math
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
 from .. import _lib
 from ..element_quant.formats import Format, get
-from ._moe import _dtype, _no_tangent, _whole
+from ._moe import _no_tangent, _whole
 from ._packed_linear import BLOCK
 
 __all__ = ["PackedCache", "packed_cache", "cache_write", "cache_read", "cache_attend"]
@@ -70,12 +70,22 @@ def packed_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, fmt: 
     return PackedCache(new(blocks * each), new(blocks), new(blocks * each), new(blocks), fmt, head_dim)
 
 
-@_lib.memo_spec
-def _spec(fmt, head_dim, shapes, strides, who):
-    """The cache's spec, its shapes checked."""
+def _remembered(make):
+    """make, remembered per its arguments: shapes, strides, types and numbers, all plain values.  What a call's checks and
+    its spec depend on costs it one lookup; errors are raised as make raises them."""
+    return functools.lru_cache(maxsize=512, typed=True)(make)
+
+
+def _spec(key, who):
+    """The spec of a cache with these (fmt, head_dim, shapes, strides, types), checked."""
+    fmt, head_dim, shapes, strides, dtypes = key
+    for t in dtypes:
+        if t != torch.uint8:
+            raise TypeError(f"mxq.nn.{who}: a cache's codes and scales must be uint8, got {t}")
     code, each = _format(fmt, who)
     _whole(head_dim, who, "the cache's head_dim", 1, MAX_HEAD_DIM)
     blocks = -(-head_dim // BLOCK)
+    shapes = tuple(map(tuple, shapes))
     if any(len(s) != 4 for s in shapes):
         raise ValueError(f"mxq.nn.{who}: a cache's tensors must be pages x kv_heads x page_size x bytes, got {shapes}")
     lead = shapes[0][:3]
@@ -95,20 +105,26 @@ def _spec(fmt, head_dim, shapes, strides, who):
     return spec
 
 
-def _parts(cache, who) -> Tuple[torch.Tensor, ...]:
+def _key(cache, who):
+    """What _spec takes of a cache."""
     if not isinstance(cache, PackedCache):
         raise TypeError(f"mxq.nn.{who}: cache must be a PackedCache, got {type(cache).__name__}")
-    parts = cache[:4]
-    for t in parts:
-        if t.dtype != torch.uint8:
-            raise TypeError(f"mxq.nn.{who}: a cache's codes and scales must be uint8, got {t.dtype}")
-        if t.device != parts[0].device:
-            raise ValueError(f"mxq.nn.{who}: a cache's tensors must be on one device, got {[p.device for p in parts]}")
-    return parts
+    a, b, c, d, fmt, head_dim = cache
+    return (fmt, head_dim, (a.shape, b.shape, c.shape, d.shape), (a.stride(), b.stride(), c.stride(), d.stride()),
+            (a.dtype, b.dtype, c.dtype, d.dtype))
 
 
-def _checked(cache, parts, who):
-    return _spec(cache.fmt, cache.head_dim, tuple(tuple(t.shape) for t in parts), tuple(t.stride() for t in parts), who)
+def _device(cache, who, *others):
+    """The GPU that a call on this cache runs on."""
+    dev = cache.k_codes.device
+    if cache.k_scales.device != dev or cache.v_codes.device != dev or cache.v_scales.device != dev:
+        raise ValueError(f"mxq.nn.{who}: a cache's tensors must be on one device, got {[t.device for t in cache[:4]]}")
+    return dev if dev.type == "cuda" else _lib.compute_device(*others)
+
+
+def _there(cache, dev):
+    """A copy of a cache in host memory on dev, its rows next to each other."""
+    return PackedCache(*(t.to(dev).contiguous() for t in cache[:4]), cache.fmt, cache.head_dim)
 
 
 def _no_grad(who: str, *tensors) -> None:
@@ -117,12 +133,11 @@ def _no_grad(who: str, *tensors) -> None:
         raise RuntimeError(f"mxq.nn.{who}: a cache's bytes have no gradient; call it under torch.no_grad()")
 
 
-def _slots(slots, who):
-    if slots.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"mxq.nn.{who}: slots must be int32 or int64, got {slots.dtype}")
-    if slots.ndim != 1 or slots.shape[0] > _MOST:
-        raise ValueError(f"mxq.nn.{who}: slots must have one axis, got shape {tuple(slots.shape)}")
-    return slots.shape[0]
+def _check_slots(shape, dtype, who):
+    if dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"mxq.nn.{who}: slots must be int32 or int64, got {dtype}")
+    if len(shape) != 1 or shape[0] > _MOST:
+        raise ValueError(f"mxq.nn.{who}: slots must have one axis, got shape {tuple(shape)}")
 
 
 def _columns(t, dev):
@@ -131,36 +146,54 @@ def _columns(t, dev):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+@_remembered
+def _write_spec(key, k_shape, k_dtype, v_shape, v_dtype, slots_shape, slots_dtype):
+    who = "cache_write"
+    spec = _spec(key, who)
+    _check_slots(slots_shape, slots_dtype, who)
+    shape = (slots_shape[0], spec.kv_heads, spec.head_dim)
+    for what, s, dtype in (("k", k_shape, k_dtype), ("v", v_shape, v_dtype)):
+        if dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"mxq.nn.cache_write: {what} must be float32, bfloat16 or float16, got {dtype}")
+        if tuple(s) != shape:
+            raise ValueError(f"mxq.nn.cache_write: {what} must have shape {shape}, got {tuple(s)}")
+    if k_dtype != v_dtype:
+        raise TypeError(f"mxq.nn.cache_write: k and v must have one dtype, got {k_dtype} and {v_dtype}")
+    return spec, _lib.DTYPE_CODE[k_dtype]
+
+
 def cache_write(k: torch.Tensor, v: torch.Tensor, cache: PackedCache, slots: torch.Tensor) -> None:
     """Quantizes k and v (T x kv_heads x head_dim; float32, bfloat16 or float16) into the rows of `slots` (T whole numbers).
 
     A token whose slot is not in the cache (-1, say) is left out; where several have one slot the last one's row stays.  A
     block with an infinity or a NaN reads back as NaN."""
     who = "cache_write"
-    parts = _parts(cache, who)
-    spec = _checked(cache, parts, who)
-    T = _slots(slots, who)
-    shape = (T, parts[0].shape[1], cache.head_dim)
-    for what, t in (("k", k), ("v", v)):
-        _dtype(t, who, what)
-        if tuple(t.shape) != shape:
-            raise ValueError(f"mxq.nn.cache_write: {what} must have shape {shape}, got {tuple(t.shape)}")
-    if k.dtype != v.dtype:
-        raise TypeError(f"mxq.nn.cache_write: k and v must have one dtype, got {k.dtype} and {v.dtype}")
+    spec, code = _write_spec(_key(cache, who), k.shape, k.dtype, v.shape, v.dtype, slots.shape, slots.dtype)
     _no_grad(who, k, v)
-    dev = _lib.compute_device(parts[0], k)
-    if parts[0].device != dev:                                   # a cache in host memory: written on the GPU, copied back
-        there = PackedCache(*(t.to(dev).contiguous() for t in parts), cache.fmt, cache.head_dim)
+    dev = _device(cache, who, k)
+    if cache.k_codes.device != dev:                             # a cache in host memory: written on the GPU, copied back
+        there = _there(cache, dev)
         cache_write(k, v, there, slots)
-        for t, new in zip(parts, there):
+        for t, new in zip(cache[:4], there):
             t.copy_(new)
         return
     kd, vd = _columns(k, dev), _columns(v, dev)
     sd = _lib.to_device(slots, dev).contiguous()
+    kt, kh, _ = kd.stride()
+    vt, vh, _ = vd.stride()
     with _lib.on(dev):
-        _lib.run("mxq_cache_write", kd.data_ptr(), vd.data_ptr(), _lib.DTYPE_CODE[k.dtype], T, kd.stride(0), kd.stride(1),
-                 vd.stride(0), vd.stride(1), sd.data_ptr(), int(sd.dtype == torch.int64), *(t.data_ptr() for t in parts),
-                 spec, _lib.stream(dev))
+        _lib.run("mxq_cache_write", kd.data_ptr(), vd.data_ptr(), code, sd.shape[0], kt, kh, vt, vh, sd.data_ptr(),
+                 sd.dtype == torch.int64, cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+                 cache.v_scales.data_ptr(), spec, _lib.stream(dev))
+
+
+@_remembered
+def _read_spec(key, slots_shape, slots_dtype, dtype):
+    spec = _spec(key, "cache_read")
+    _check_slots(slots_shape, slots_dtype, "cache_read")
+    if dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"mxq.nn.cache_read: dtype must be float32, bfloat16 or float16, got {dtype}")
+    return spec, (slots_shape[0], spec.kv_heads, spec.head_dim), _lib.DTYPE_CODE[dtype]
 
 
 def cache_read(cache: PackedCache, slots: torch.Tensor,
@@ -168,30 +201,58 @@ def cache_read(cache: PackedCache, slots: torch.Tensor,
     """(k, v), T x kv_heads x head_dim each, of the rows of `slots`: code times scale, rounded once to dtype (float32,
     bfloat16 or float16); zeros for a slot that is not in the cache."""
     who = "cache_read"
-    parts = _parts(cache, who)
-    spec = _checked(cache, parts, who)
-    T = _slots(slots, who)
-    code = _lib.DTYPE_CODE.get(dtype)
-    if code is None:
-        raise TypeError(f"mxq.nn.cache_read: dtype must be float32, bfloat16 or float16, got {dtype}")
-    dev = _lib.compute_device(parts[0], slots)
-    if parts[0].device != dev:
-        parts = tuple(t.to(dev).contiguous() for t in parts)
-        spec = _checked(cache, parts, who)
+    spec, shape, code = _read_spec(_key(cache, who), slots.shape, slots.dtype, dtype)
+    dev = _device(cache, who, slots)
+    if cache.k_codes.device != dev:
+        k, v = cache_read(_there(cache, dev), slots, dtype)
+        return _lib.back(k, cache.k_codes), _lib.back(v, cache.k_codes)
     sd = _lib.to_device(slots, dev).contiguous()
-    k = torch.empty((T, parts[0].shape[1], cache.head_dim), dtype=dtype, device=dev)
-    v = torch.empty_like(k)
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     with _lib.on(dev):
-        _lib.run("mxq_cache_read", *(t.data_ptr() for t in parts), spec, sd.data_ptr(), int(sd.dtype == torch.int64), T,
-                 k.data_ptr(), v.data_ptr(), code, _lib.stream(dev))
-    return _lib.back(k, cache.k_codes), _lib.back(v, cache.k_codes)
+        _lib.run("mxq_cache_read", cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+                 cache.v_scales.data_ptr(), spec, sd.data_ptr(), sd.dtype == torch.int64, shape[0], k.data_ptr(),
+                 v.data_ptr(), code, _lib.stream(dev))
+    return k, v
 
 
-def _indices(t, who, what, shape):
-    if t.dtype != torch.int32:
-        raise TypeError(f"mxq.nn.{who}: {what} must be int32, got {t.dtype}")
-    if len(t.shape) != len(shape) or any(n is not None and m != n for m, n in zip(t.shape, shape)):
-        raise ValueError(f"mxq.nn.{who}: {what} must have shape {shape}, got {tuple(t.shape)}")
+def _check_indices(t, who, what, shape):
+    if t[1] != torch.int32:
+        raise TypeError(f"mxq.nn.{who}: {what} must be int32, got {t[1]}")
+    if len(t[0]) != len(shape) or any(n is not None and m != n for m, n in zip(t[0], shape)):
+        raise ValueError(f"mxq.nn.{who}: {what} must have shape {shape}, got {tuple(t[0])}")
+
+
+@_remembered
+def _attend_spec(key, q_shape, q_dtype, q_strides, table, table_row, lengths, starts, scale, causal, window):
+    """(cache spec, attention spec, bytes of workspace); table, lengths and starts as (shape, dtype)."""
+    who = "cache_attend"
+    spec = _spec(key, who)
+    code = _lib.DTYPE_CODE.get(q_dtype)
+    if code is None:
+        raise TypeError(f"mxq.nn.cache_attend: q must be float32, bfloat16 or float16, got {q_dtype}")
+    G, D = spec.kv_heads, spec.head_dim
+    if len(q_shape) != (4 if starts is None else 3):
+        raise ValueError(f"mxq.nn.cache_attend: q must be B x n x heads x head_dim, or T x heads x head_dim with starts, got "
+                         f"shape {tuple(q_shape)}")
+    H = q_shape[-2]
+    if q_shape[-1] != D or H % G or not H:
+        raise ValueError(f"mxq.nn.cache_attend: q must have a multiple of {G} heads of {D} columns, got shape {tuple(q_shape)}")
+    _check_indices(table, who, "table", (None, None))
+    B, pages = table[0]
+    _check_indices(lengths, who, "lengths", (B,))
+    if starts is not None:
+        _check_indices(starts, who, "starts", (B + 1,))
+    elif q_shape[0] != B:
+        raise ValueError(f"mxq.nn.cache_attend: q must have {B} sequences, as table has, got shape {tuple(q_shape)}")
+    if window is not None:
+        _whole(window, who, "window", 1, _MOST)
+    if not 0.0 < scale <= torch.finfo(torch.float32).max:
+        raise ValueError(f"mxq.nn.cache_attend: scale must be positive and finite, got {scale}")
+    T = q_shape[0] if starts is not None else q_shape[0] * q_shape[1]
+    if T * H > _MOST // 2:
+        raise ValueError(f"mxq.nn.cache_attend: {T} queries of {H} heads are too many")
+    att = _lib.AttendSpec(code, causal, scale, T, B, H, *q_strides, pages, table_row, 0 if window is None else window)
+    return spec, att, _lib.call("mxq_cache_attend_workspace", spec, att, int(starts is not None))
 
 
 def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengths: torch.Tensor,
@@ -209,54 +270,38 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
 
     Lengths are held to the table's pages and starts to T.  A key on a page that the cache does not have (-1, say) is not
     there.  A query that sees no key, or that belongs to no sequence, gets zeros and an lse of -inf; so does one whose every
-    score is -inf.  Sums are float32, and the weights exp(scale q k^T - max) of bfloat16 queries are rounded to bfloat16."""
+    score is -inf.  A query that sees a value that is no finite number gets no finite number in its column.  Sums are float32,
+    and the weights exp(scale q k^T - max) of bfloat16 queries are rounded to bfloat16."""
     who = "cache_attend"
-    parts = _parts(cache, who)
-    spec = _checked(cache, parts, who)
-    _dtype(q, who, "q")
+    qd = q
+    if qd.ndim and qd.stride(-1) != 1 and qd.shape[-1] > 1:
+        qd = qd.contiguous()
+    if qd.ndim == 4:
+        S, n, h, _ = qd.stride()
+        if S != n * qd.shape[1] and qd.shape[0] > 1 and qd.shape[1] > 1:       # a token's stride is one number
+            qd = qd.contiguous()
+    strides = qd.stride()[-3:-1]
+    if qd.ndim == 4 and qd.shape[1] == 1:
+        strides = (qd.stride(0), strides[1])
+    td = table if table.ndim != 2 or table.shape[1] < 2 or table.stride(1) == 1 else table.contiguous()
+    spec, att, size = _attend_spec(
+        _key(cache, who), q.shape, q.dtype, strides, (table.shape, table.dtype), td.stride(0) if td.ndim == 2 else 0,
+        (lengths.shape, lengths.dtype), None if starts is None else (starts.shape, starts.dtype),
+        cache.head_dim ** -0.5 if scale is None else float(scale), bool(causal), window)
     _no_grad(who, q)
-    G, D = parts[0].shape[1], cache.head_dim
-    if q.ndim != (4 if starts is None else 3):
-        raise ValueError(f"mxq.nn.cache_attend: q must be B x n x heads x head_dim, or T x heads x head_dim with starts, got "
-                         f"shape {tuple(q.shape)}")
-    H = q.shape[-2]
-    if q.shape[-1] != D or H % G or not H:
-        raise ValueError(f"mxq.nn.cache_attend: q must have a multiple of {G} heads of {D} columns, got shape {tuple(q.shape)}")
-    _indices(table, who, "table", (None, None))
-    B = table.shape[0]
-    _indices(lengths, who, "lengths", (B,))
-    if starts is not None:
-        _indices(starts, who, "starts", (B + 1,))
-    elif q.shape[0] != B:
-        raise ValueError(f"mxq.nn.cache_attend: q must have {B} sequences, as table has, got shape {tuple(q.shape)}")
-    if window is not None:
-        _whole(window, who, "window", 1, _MOST)
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"mxq.nn.cache_attend: scale must be positive and finite, got {scale}")
-    T = q.shape[0] if starts is not None else q.shape[0] * q.shape[1]
-    if T * H > _MOST // 2:
-        raise ValueError(f"mxq.nn.cache_attend: {T} queries of {H} heads are too many")
-    dev = _lib.compute_device(parts[0], q)
-    if parts[0].device != dev:
-        parts = tuple(t.to(dev).contiguous() for t in parts)
-        spec = _checked(cache, parts, who)
-    qd = _columns(q if q.ndim == 3 else q.reshape(T, H, D), dev)
-    td, ld = _lib.to_device(table, dev), _lib.to_device(lengths, dev).contiguous()
-    if td.stride(1) != 1 and td.shape[1] > 1:
-        td = td.contiguous()
+    dev = _device(cache, who, q)
+    if cache.k_codes.device != dev:                             # a cache in host memory
+        return cache_attend(q, _there(cache, dev), table, lengths, starts, scale=scale, causal=causal, window=window,
+                            return_lse=return_lse)
+    qd, td, ld = _lib.to_device(qd, dev), _lib.to_device(td, dev), _lib.to_device(lengths, dev).contiguous()
     sd = None if starts is None else _lib.to_device(starts, dev).contiguous()
-    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-    att = _lib.AttendSpec(_lib.DTYPE_CODE[q.dtype], int(bool(causal)), scale, T, B, H, qd.stride(0), qd.stride(1),
-                          td.shape[1], td.stride(0), 0 if window is None else window)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
     with _lib.on(dev):
-        size = _lib.call("mxq_cache_attend_workspace", spec, att, int(sd is not None))
         work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _lib.run("mxq_cache_attend", qd.data_ptr(), *(t.data_ptr() for t in parts), spec, td.data_ptr(), ld.data_ptr(),
-                 _lib.ptr(sd), out.data_ptr(), _lib.ptr(lse), att, _lib.ptr(work), _lib.stream(dev))
-    if q.ndim == 4:
-        out = out.reshape(q.shape)
-        lse = None if lse is None else lse.reshape(q.shape[:-1])
-    out = _lib.back(out, q)
-    return (out, _lib.back(lse, q)) if return_lse else out
+        _lib.run("mxq_cache_attend", qd.data_ptr(), cache.k_codes.data_ptr(), cache.k_scales.data_ptr(),
+                 cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), spec, td.data_ptr(), ld.data_ptr(), _lib.ptr(sd),
+                 out.data_ptr(), _lib.ptr(lse), att, _lib.ptr(work), _lib.stream(dev))
+    if out.device != q.device:
+        out, lse = _lib.back(out, q), None if lse is None else _lib.back(lse, q)
+    return (out, lse) if return_lse else out

@@ -168,34 +168,11 @@ def test_c_entries_refuse():
     refused("workspace", "mxq_cache_attend", *run(cache(pages=1 << 12), attend(table_pages=1 << 12)))
 
 
-def test_workspace_covers_every_cut():
-    """The units that the workspace and the launch have room for are no fewer than a batch can make, whatever its lengths
-    and starts: as the device cuts it, counted here."""
-    import random
-    rng = random.Random(0)
+def test_workspace():
+    """None where no sequence can have more keys than a workgroup takes; else one size for any number of sequences."""
     lib = _lib.load()
-    for _ in range(300):
-        ragged = rng.random() < 0.5
-        G, group, B = rng.randint(1, 8), rng.choice((1, 2, 7, 16, 40)), rng.randint(1, 9)
-        page, pages, D = rng.choice((1, 16, 100)), rng.randint(1, 3000), rng.choice((64, 128, 256))
-        n = [rng.randint(0, 40) for _ in range(B)] if ragged else [rng.randint(1, 40)] * B
-        window = rng.choice((0, 0, 1, 500))
-        cache = _lib.CacheSpec(5, D, 1 << 14, page, G)
-        att = _lib.AttendSpec(1, 1, 1.0, sum(n), B, G * group, 0, 0, pages, pages, window)
-        room = lib.mxq_cache_attend_workspace(cache, att, int(ragged))
-        assert room % 4 == 0
-        if not sum(n):
-            assert room == 0
-            continue
-        lengths = [rng.choice((0, 1, rng.randint(0, pages * page), pages * page)) for _ in range(B)]
-        for rows, least, wanted in ((16, 8, 1024),):
-            def steps(length, m):
-                lo = max(0, length - m + 1 - window) if window else 0
-                hi = length if m else 0
-                return -(-(hi - lo // 32 * 32) // 32) if hi > lo else 0
-            tiles = [-(-m * group // rows) for m in n]
-            work = sum(t * steps(l, m) for t, l, m in zip(tiles, lengths, n))
-            quota = max(least, -(-work * G // wanted))
-            units = sum(t * max(1, -(-steps(l, m) // quota)) for t, l, m in zip(tiles, lengths, n)) * G
-            if any(steps(l, m) > quota for l, m in zip(lengths, n)):
-                assert room >= units * rows * (D + 2) * 4, (units, room)
+    cache = _lib.CacheSpec(5, 128, 4096, 16, 2)
+    size = lambda ragged=0, **change: lib.mxq_cache_attend_workspace(cache, _lib.AttendSpec(**{**dict(      # noqa: E731
+        dtype=1, causal=1, scale=1.0, T=4, B=4, heads=8, table_pages=1000, table_row=1000), **change}), ragged)
+    assert size(table_pages=14) == 0 and size(T=0) == 0 and size(window=200) == 0
+    assert 0 < size() == size(T=8) == size(T=40, B=40) <= 64 << 20
