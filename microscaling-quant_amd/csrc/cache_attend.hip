@@ -4,76 +4,127 @@
 
 namespace mxq {
 
-void launch_attend_few_e4m3(const AttendArgs&, int64_t, int, hipStream_t);
-void launch_attend_few_e5m2(const AttendArgs&, int64_t, int, hipStream_t);
-void launch_attend_few_pairs(const AttendArgs&, int64_t, int, hipStream_t);
+#define MXQ_LAUNCH(NAME) void NAME(const AttendArgs&, bool many, bool wide, int64_t groups, hipStream_t);
+MXQ_LAUNCH(launch_attend_e4m3_f32)
+MXQ_LAUNCH(launch_attend_e4m3_bf16)
+MXQ_LAUNCH(launch_attend_e4m3_f16)
+MXQ_LAUNCH(launch_attend_e5m2_f32)
+MXQ_LAUNCH(launch_attend_e5m2_bf16)
+MXQ_LAUNCH(launch_attend_e5m2_f16)
+MXQ_LAUNCH(launch_attend_pairs_f32)
+MXQ_LAUNCH(launch_attend_pairs_bf16)
+MXQ_LAUNCH(launch_attend_pairs_f16)
+#undef MXQ_LAUNCH
 
 namespace {
 
-constexpr int kFewRows = 16, kFewLeast = 8, kUnits = 256;   // rows a tile, steps a workgroup at least, CUs
+constexpr int kUnits = 256, kLeast = 8;       // CUs; steps of 32 keys that a workgroup takes at least
+constexpr int kFewRows = 64;                  // rows a sequence up to which its keys are what a call costs
 
-// The rows of tiles that were cut, from their parts' sums, and zeros for rows of no sequence.  A workgroup takes every
-// gridDim.y-th row of a tile of rows, its waves the runs in turn, then the waves' sums in their order.
+constexpr int kWholeTiles = 3;                // tiles of many rows a workgroup from which on none is cut
+
+int wanted_of(int dtype, int blocks, int rows, bool many) { return kUnits * attend_groups(dtype, blocks, rows / 16 / (many ? kWaves : 1), many); }
+
+// What differs between the two ways that a call's sequences are taken.
+struct JoinWay {
+  float* partial;
+  int32_t above, upto, wanted, size;
+  int32_t places, shares;    // workgroups: tiles, or pieces of the line where they are fewer, and what shares one's rows
+  bool by_tile;
+};
+struct JoinWays {
+  JoinWay way[2];
+};
+// The rows of tiles that lie in two pieces of the line and more, from their parts' sums in the pieces' order, and zeros for
+// rows of no sequence.  A workgroup takes rows of a tile, or of the tile that a piece ends in, if that is the tile's first end
+// of a piece: sixteen lanes a row, or, of many parts, the workgroup a row, its sixteens of lanes the parts in turn.
+constexpr int kManyParts = 8;
 template <int COLUMNS>
-__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, int unit_rows, int least) {
-  constexpr int V = COLUMNS / 64;
-  __shared__ float sums[4][COLUMNS];
-  __shared__ float weights[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim;
-  if (a.starts) {
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways, bool empty_rows) {
+  constexpr int V = COLUMNS / 16;
+  __shared__ float sums[16][COLUMNS];
+  __shared__ float weights[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim, c = lane & 15, sixteen = threadIdx.x >> 4;
+  if (empty_rows) {
     // queries [0, starts[0]) and [starts[B], T) are no sequence's
     const int T = (int)a.a.T, x = a.a.B ? a.starts[0] : T, y = a.a.B ? a.starts[a.a.B] : T;
     const int64_t head = (int64_t)(x < 0 ? 0 : x > T ? T : x) * a.a.heads, tail = (int64_t)(y < 0 ? 0 : y > T ? T : y) * a.a.heads;
     const int64_t from = tail < head ? head : tail, all = head + (a.a.T * a.a.heads - from);
-    const int64_t groups = (int64_t)gridDim.x * gridDim.y, me = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    for (int64_t i = me * 4 + wave; i < all; i += groups * 4) {
+    for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < all; i += (int64_t)gridDim.x * 4) {
       const int64_t row = i < head ? i : from + i - head;
       for (int d = lane; d < D; d += 64) store_elem(a.out, a.a.dtype, row * D + d, 0.0f);
       if (a.lse && lane == 0) a.lse[row] = -__builtin_inff();
     }
   }
-  if (!a.partial) return;
-  const Tile u = tile_of(a, unit_rows, blockIdx.x, true);
+  const int first_way = ways.way[0].places * ways.way[0].shares, which = (int)blockIdx.x >= first_way;
+  const JoinWay& w = ways.way[which];
+  const int index = (int)blockIdx.x - (which ? first_way : 0);
+  if (index >= w.places * w.shares) return;
+  const int share = index / w.places, place = index - share * w.places, size = w.size;
+  a.above = w.above, a.upto = w.upto, a.wanted = w.wanted;
+  const Member own = member(a, lane, size);
+  const Line line = line_of(a, size, own);
+  if (!w.by_tile && place + 1 >= line.groups) return;
+  const Tile u = tile_of(a, size, own, w.by_tile ? place : line.begin(place + 1), w.by_tile);
   if (u.b < 0) return;
-  const Line line = line_of(a, unit_rows, least);
-  const int g0 = same(line.group_at(u.first)), runs = same(line.group_at(u.first + u.steps - 1)) - g0 + 1;
+  if (!w.by_tile && (u.first == line.begin(place + 1) || u.first < line.begin(place))) return;
+  const int g0 = w.by_tile ? same(line.group_at(u.first)) : place;
+  const int runs = same(line.group_at(u.first + u.weight - 1)) - g0 + 1;
   if (runs == 1) return;
-  const bool at_begin = line.begin(g0) == u.first;          // of the first group's piece the tile is the first
-  const Sequence s = same(sequence(a, u.b));
-  const int rows = s.n * a.group, row_tiles = (rows + unit_rows - 1) / unit_rows, kv_head = u.index / row_tiles;
-  const int row0 = (u.index - kv_head * row_tiles) * unit_rows, last = rows - row0 < unit_rows ? rows - row0 : unit_rows;
-  for (int r = blockIdx.y; r < last; r += gridDim.y) {
-    auto part_of = [&](int i) { return a.partial + (part_slot(g0 + i, i || at_begin) * unit_rows + r) * (COLUMNS + 2); };
+  const bool at_begin = line.begin(g0) == u.first;          // of the first piece it is the first tile
+  const int rows = u.s.n * a.group, row0 = u.row * size, last = rows - row0 < size ? rows - row0 : size;
+  const bool many = runs > kManyParts;
+  for (int r = many ? share : share * 16 + sixteen; r < last; r += many ? w.shares : w.shares * 16) {
+    auto part_of = [&](int i) { return w.partial + (part_slot(g0 + i, i || at_begin) * size + r) * (COLUMNS + 2); };
     float best = -__builtin_inff(), all = 0.0f, v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.0f;
-    for (int i = lane; i < runs; i += 64) best = __builtin_fmaxf(best, part_of(i)[COLUMNS]);
-    for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
+    for (int i = c; i < runs; i += 16) best = __builtin_fmaxf(best, part_of(i)[COLUMNS]);
+    for (int o = 8; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
 #pragma unroll 4
-    for (int i = wave; i < runs; i += 4) {
+    for (int i = many ? sixteen : 0; i < runs; i += many ? 16 : 1) {
       const float* part = part_of(i);
       const float top = part[COLUMNS], sum = part[COLUMNS + 1];
-      // a run without a maximum has seen no key, or only scores of NaN, which its sum is then
+      // a part without a maximum has seen no key, or only scores of NaN, which its sum is then
       const float factor = top == -__builtin_inff() ? sum : __builtin_amdgcn_exp2f(top - best);
       float x[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) x[k] = part[lane * V + k];
+      for (int k = 0; k < V; k += 4) __builtin_memcpy(x + k, part + k * 16 + c * 4, 16);
       all += top == -__builtin_inff() ? sum : factor * sum;
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
     }
-    if (lane == 0) weights[wave] = all;
+    if (many) {
+      if (c == 0) weights[sixteen] = all;
 #pragma unroll
-    for (int k = 0; k < V; ++k) sums[wave][lane * V + k] = v[k];
-    __syncthreads();
-    const int t = (int)divu31(row0 + r, a.by_group), h = kv_head * a.group + row0 + r - t * a.group;
-    const int64_t row = (int64_t)(s.start + t) * a.a.heads + h;
-    all = ((weights[0] + weights[1]) + weights[2]) + weights[3];
+      for (int k = 0; k < V; ++k) sums[sixteen][k / 4 * 64 + c * 4 + k % 4] = v[k];
+      __syncthreads();
+      all = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) all += weights[j];
+      if (sixteen == 0) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          v[k] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[k] += sums[j][k / 4 * 64 + c * 4 + k % 4];
+        }
+      }
+      __syncthreads();
+      if (sixteen) continue;
+    }
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-    for (int d = threadIdx.x; d < D; d += 256)
-      store_elem(a.out, a.a.dtype, row * D + d, (((sums[0][d] + sums[1][d]) + sums[2][d]) + sums[3][d]) * inv);
-    if (a.lse && threadIdx.x == 0) a.lse[row] = log_sum(best, all);
-    __syncthreads();
+    const int t = (int)divu31(row0 + r, a.by_group), h = u.head * a.group + row0 + r - t * a.group;
+    const int64_t row = (int64_t)(u.s.start + t) * a.a.heads + h;
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const int d = k * 16 + c * 4;
+      const float y[4] = {v[k] * inv, v[k + 1] * inv, v[k + 2] * inv, v[k + 3] * inv};
+      if (a.a.dtype == MXQ_DT_F32) store_four<MXQ_DT_F32>(a.out, row * D + d, D - d, y);
+      else if (a.a.dtype == MXQ_DT_BF16) store_four<MXQ_DT_BF16>(a.out, row * D + d, D - d, y);
+      else store_four<MXQ_DT_F16>(a.out, row * D + d, D - d, y);
+    }
+    if (a.lse && c == 0) a.lse[row] = log_sum(best, all);
   }
 }
 
@@ -95,20 +146,37 @@ int check(const mxq_cache_spec* c, const mxq_attend_spec* a) {
   return MXQ_OK;
 }
 
-// Tiles of `rows` rows that a call may have, and whether they may be cut: not where no sequence has keys for it.
-struct Plan {
-  int64_t tiles;
-  bool split;
+// How a call is taken: sequences of few rows (queries times the heads that share one of keys) by tiles whose keys the waves
+// share, others by tiles whose waves have rows of their own.  Without starts every sequence has as many, so that one of the
+// two does it.
+struct Way {
+  int rows;                  // of a tile; 0: nothing goes this way
+  int64_t tiles, groups;     // as many as there may be, of all heads; workgroups
+  int64_t bytes;             // workspace; 0: no tile is cut
 };
-Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged, int rows, int least) {
-  const int64_t group = a.heads / c.kv_heads;
-  int64_t tiles;
-  if (ragged) tiles = a.T * group / rows + (a.B < a.T ? a.B : a.T);
-  else tiles = a.B * ceil_div(a.T / a.B * group, rows);
-  const int64_t keys = a.table_pages * c.page_size, seen = a.window && a.window < keys ? a.window + (ragged ? a.T : a.T / a.B) : keys;
-  return Plan{tiles * c.kv_heads, (keys < seen ? keys : seen) > (int64_t)(least - 1) * kStep};
+struct Plan {
+  int limit;                 // rows a sequence that are few
+  Way way[2];
+};
+Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
+  const int64_t group = a.heads / c.kv_heads, n = ragged ? a.T : a.T / a.B, rows = n * group, least = ragged ? group : rows;
+  const int blocks = blocks_class((c.head_dim + 31) / 32);
+  Plan p = {};
+  if (least <= kFewRows) p.limit = kFewRows, p.way[0].rows = least <= 16 || blocks == 8 ? 16 : 32;
+  if (rows > p.limit) p.way[1].rows = 16 * kWaves * attend_rows(a.dtype, blocks);
+  const int64_t keys = a.table_pages * c.page_size, seen = a.window && a.window < keys ? a.window + n : keys;
+  const bool split = (keys < seen ? keys : seen) > (int64_t)(kLeast - 1) * kStep;    // a sequence may have keys for it
+  for (int many = 0; many < 2; ++many) {
+    Way& w = p.way[many];
+    if (!w.rows) continue;
+    w.tiles = (ragged ? rows / w.rows + (a.B < a.T ? a.B : a.T) : a.B * ceil_div(rows, w.rows)) * c.kv_heads;
+    w.groups = w.tiles;
+    if (!split || (many && w.tiles >= kWholeTiles * wanted_of(a.dtype, blocks, w.rows, many))) continue;
+    w.groups = wanted_of(a.dtype, blocks, w.rows, many);
+    w.bytes = 2 * w.groups * w.rows * (32 * blocks + 2) * (int64_t)sizeof(float);
+  }
+  return p;
 }
-int columns_of(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 }  // namespace
 }  // namespace mxq
@@ -116,9 +184,8 @@ int columns_of(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 12
 extern "C" int64_t mxq_cache_attend_workspace(const mxq_cache_spec* cache, const mxq_attend_spec* spec, int32_t ragged) {
   using namespace mxq;
   if (check(cache, spec) || spec->T == 0 || spec->B == 0) return 0;
-  const Plan p = plan_of(*cache, *spec, ragged, kFewRows, kFewLeast);
-  const int64_t groups = kUnits * few_groups(spec->dtype, (cache->head_dim + 31) / 32);
-  return p.split ? 2 * groups * kFewRows * (columns_of(cache->head_dim) + 2) * (int64_t)sizeof(float) : 0;
+  const Plan p = plan_of(*cache, *spec, ragged);
+  return p.way[0].bytes + p.way[1].bytes;
 }
 
 extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,
@@ -131,7 +198,6 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   if (!starts && (spec->B == 0 || spec->T % spec->B)) return invalid("mxq_cache_attend: T must be a multiple of B without starts");
   if (!q || !k_codes || !k_scales || !v_codes || !v_scales || !out || (spec->B && (!lengths || (spec->table_pages && !table))))
     return invalid("mxq_cache_attend: NULL pointer");
-  const int columns = columns_of(cache->head_dim);
   const int64_t group = spec->heads / cache->kv_heads;
   AttendArgs a = {};
   a.q = q, a.kc = k_codes, a.ks = k_scales, a.vc = v_codes, a.vs = v_scales;
@@ -139,28 +205,42 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   a.c = *cache, a.a = *spec;
   a.by_page = make_divu31((uint32_t)cache->page_size), a.by_group = make_divu31((uint32_t)group);
   a.group = (int)group, a.blocks = (cache->head_dim + 31) / 32;
-  a.wanted = kUnits * few_groups(spec->dtype, a.blocks);
   a.aligned = cache->page_size % 16 == 0;
   for (int64_t r : cache->row_stride) a.aligned = a.aligned && r >= 0 && r < 1 << 26;
   a.scale2 = spec->scale * 1.44269504088896341f;
   hipStream_t st = as_stream(stream);
-  Plan p = {};
-  if (spec->B) {
-    p = plan_of(*cache, *spec, starts != nullptr, kFewRows, kFewLeast);
-    if (p.split && !workspace) return invalid("mxq_cache_attend: NULL workspace");
-    if (p.tiles * 256 > kMaxThreads) return invalid("mxq_cache_attend: too many tiles for a launch");
-    a.partial = p.split ? (float*)workspace : nullptr;
-    auto launch = cache->format == MXQ_FMT_E4M3 ? launch_attend_few_e4m3 : cache->format == MXQ_FMT_E5M2 ? launch_attend_few_e5m2 : launch_attend_few_pairs;
-    launch(a, p.tiles, kFewLeast, st);
+  a.least = kLeast;
+  const Plan p = spec->B ? plan_of(*cache, *spec, starts != nullptr) : Plan{};
+  if (p.way[0].bytes + p.way[1].bytes && !workspace) return invalid("mxq_cache_attend: NULL workspace");
+  for (const Way& w : p.way)
+    if (w.tiles * 64 * kWaves > kMaxThreads) return invalid("mxq_cache_attend: too many tiles for a launch");
+  const int blocks = blocks_class(a.blocks);
+  constexpr decltype(&launch_attend_e4m3_f32) launches[3][3] = {{launch_attend_e4m3_f32, launch_attend_e4m3_bf16, launch_attend_e4m3_f16},
+                                                                {launch_attend_e5m2_f32, launch_attend_e5m2_bf16, launch_attend_e5m2_f16},
+                                                                {launch_attend_pairs_f32, launch_attend_pairs_bf16, launch_attend_pairs_f16}};
+  const auto launch = launches[cache->format == MXQ_FMT_E4M3 ? 0 : cache->format == MXQ_FMT_E5M2 ? 1 : 2][spec->dtype];
+  JoinWays ways = {};
+  int64_t joins = 0;
+  char* work = (char*)workspace;
+  for (int many = 0; many < 2; ++many) {
+    const Way& w = p.way[many];
+    if (!w.rows) continue;
+    a.partial = w.bytes ? (float*)work : nullptr;
+    work += w.bytes;
+    a.above = many ? p.limit : 0, a.upto = many ? 0x7fffffff : p.limit;
+    a.wanted = wanted_of(spec->dtype, blocks, w.rows, many);
+    launch(a, many, w.rows == 32, w.groups, st);
     if (int rc = check_launch("mxq_cache_attend")) return rc;
+    if (!a.partial) continue;
+    const bool by_tile = w.tiles <= a.wanted;
+    const int places = by_tile ? (int)w.tiles : a.wanted, shares = w.rows > 32 ? w.rows / 16 : places > 128 ? 1 : places > 32 ? 4 : 16;
+    ways.way[many] = JoinWay{a.partial, a.above, a.upto, a.wanted, w.rows, places, shares, by_tile};
+    joins += places * shares;
   }
-  if (a.partial || starts) {
-    // few tiles: a workgroup for each of their rows
-    const int64_t tiles = a.partial ? p.tiles : blocks_for(ceil_div(spec->T * spec->heads, 64));
-    const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 2048 ? 1 : tiles >= 512 ? 4 : 16));
-    if (columns == 64) k_attend_join<64><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
-    else if (columns == 128) k_attend_join<128><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
-    else k_attend_join<256><<<grid, 256, 0, st>>>(a, kFewRows, kFewLeast);
+  if (joins || starts) {
+    const unsigned groups = joins ? (unsigned)joins : blocks_for(ceil_div(spec->T * spec->heads, 64));
+    const auto join = blocks == 2 ? k_attend_join<64> : blocks == 4 ? k_attend_join<128> : k_attend_join<256>;
+    join<<<dim3(groups), 256, 0, st>>>(a, ways, starts != nullptr);
     return check_launch("mxq_cache_attend");
   }
   return MXQ_OK;

@@ -1,0 +1,5 @@
+#include "cache_attend_impl.h"
+
+namespace mxq {
+void launch_attend_pairs_bf16(const AttendArgs& a, bool many, bool wide, int64_t groups, hipStream_t st) { launch_attend<kPairs, MXQ_DT_BF16>(a, many, wide, groups, st); }
+}  // namespace mxq

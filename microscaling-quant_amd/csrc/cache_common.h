@@ -84,7 +84,8 @@ struct AttendArgs {
   DivU31 by_page, by_group;
   int32_t group, blocks; // heads of q a head of keys; blocks a row
   int32_t aligned;       // pages of whole 16 rows, whose rows are less than 2^26 bytes apart
-  int32_t wanted;        // workgroups that fill the card
+  int32_t wanted, least; // workgroups that fill the card, and steps that one takes at least
+  int32_t above, upto;   // the numbers of rows a sequence that this launch takes: (above, upto]
   float scale2;          // scale times log2 e
 };
 
@@ -116,78 +117,160 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
   return s;
 }
 
-// How the work of few queries is cut.  A tile is `rows` rows of one head of keys (queries token by token, the heads that
-// share it within) and its steps of 32 keys, one at least.  The batch's tiles, a sequence's with equal numbers of steps, lie
-// one behind another on a line of steps, and every workgroup takes an equal piece of it, however lengths differ: a number of
-// whole tiles, and a part of one before and behind them, whose sums are joined later.  Every wave finds its way by itself from
-// the lengths.
+// How the work is cut.  A tile is `size` rows of one head of keys (queries token by token, the heads that share it within).  A
+// tile's weight is about the keys that its queries see, times the heads that share one, and what starting it costs.  The
+// batch's tiles lie one behind another on a line, and every workgroup takes an equal piece of it, however lengths differ: a
+// number of whole tiles, and a part of one before and behind them, whose sums are joined later.   Where there are
+// tiles enough, a workgroup takes one whole tile instead, a sequence's last ones, which see most, first, and heads in turn, so
+// that with eight of them each part of the card reads one head's keys.  Every wave finds its way by itself from the
+// lengths, by the same arithmetic, so that all agree.
 constexpr int kStep = 32;
 __device__ __forceinline__ int same(int v) { return __builtin_amdgcn_readfirstlane(v); }   // of a wave's lanes, as it is in all of them
 __device__ __forceinline__ int64_t same(int64_t v) { return (int64_t)((uint64_t)(uint32_t)same((int)(v >> 32)) << 32 | (uint32_t)same((int)v)); }
-__device__ __forceinline__ Sequence same(const Sequence& s) { return Sequence{same(s.start), same(s.n), same(s.length), same(s.lo), same(s.hi)}; }
 
-struct Share {
-  int tiles, steps;      // of a sequence: its tiles (of all heads), steps of each
+// The weights of a sequence's tiles of one head: `base` and 2^shift more for each tile before and itself, `most` at most.
+struct Weights {
+  int tiles, shift;      // shift < 0: all of weight `base`
+  int64_t base, most, start;
+  __device__ __forceinline__ int64_t of(int j) const {
+    const int64_t w = shift < 0 ? base : base + ((int64_t)(j + 1) << shift);
+    return (w < most ? w : most) + start;
+  }
+  __device__ __forceinline__ int64_t before(int j) const {          // of the first j together
+    int64_t grow = shift < 0 ? 0 : (most - base) >> shift;          // tiles whose weight still grows
+    grow = grow < 0 ? 0 : grow < j ? grow : j;
+    return grow * base + (grow * (grow + 1) / 2 << (shift & 63)) + (j - grow) * most + j * start;
+  }
 };
-__device__ __forceinline__ Share share_of(const AttendArgs& a, const Sequence& s, int rows) {
-  const int tiles = (int)(((int64_t)s.n * a.group + rows - 1) / rows) * (int)a.c.kv_heads;
-  return Share{tiles, s.hi > s.lo ? (s.hi - (s.lo & ~(kStep - 1)) + kStep - 1) / kStep : 1};
+// Of this lane: a sequence and its weights.
+struct Member {
+  Sequence s;
+  Weights w;
+};
+__device__ __forceinline__ Member member(const AttendArgs& a, int b, int size) {
+  constexpr int64_t kMost = (int64_t)1 << 34;                       // so that no sum of weights passes 63 bits
+  auto hold = [](int64_t v) { return v < kMost ? v : kMost; };
+  Member m{};
+  if (b >= a.a.B) return m;
+  m.s = sequence(a, b);
+  const Sequence& s = m.s;
+  Weights& w = m.w;
+  const int rows = s.n * a.group;
+  w.tiles = rows > a.above && rows <= a.upto ? (rows + size - 1) / size : 0;
+  w.start = hold((int64_t)4 * kStep * a.group);
+  if (a.a.causal) {
+    w.shift = __builtin_ctz(size);
+    w.base = s.length > s.n ? hold((int64_t)(s.length - s.n) * a.group) : 0;
+    w.most = a.a.window ? hold(a.a.window * a.group + size) : 2 * kMost;
+  } else {
+    const int64_t keys = a.a.window && a.a.window < s.length - s.n ? a.a.window + s.n : s.length;
+    w.shift = -1, w.base = w.most = hold(keys * a.group);
+  }
+  return m;
 }
 struct Line {
-  int64_t total;         // steps
-  int groups;            // workgroups that have a piece
-  __device__ int64_t begin(int i) const { return total * i / groups; }
-  __device__ int group_at(int64_t step) const { return (int)(((step + 1) * groups - 1) / total); }
-};
-__device__ __forceinline__ Line line_of(const AttendArgs& a, int rows, int least) {
-  int64_t total = 0;
-  for (int b = threadIdx.x & 63; b < a.a.B; b += 64) {
-    const Share h = share_of(a, sequence(a, b), rows);
-    total += (int64_t)h.tiles * h.steps;
+  int64_t total;
+  double each;           // weight of a piece
+  int groups;            // workgroups that have one
+  __device__ __forceinline__ int64_t begin(int i) const { return (int64_t)(each * i + 0.5); }
+  __device__ __forceinline__ int group_at(int64_t at) const {
+    int i = (int)((double)at / each);
+    i = i < groups ? i : groups - 1;
+    while (i > 0 && begin(i) > at) --i;
+    while (i + 1 < groups && begin(i + 1) <= at) ++i;
+    return i;
   }
-  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-  total = same(total);
-  const int64_t most = (total + least - 1) / least;
-  return Line{total, most < a.wanted ? (int)most : a.wanted};
-}
-// A tile: of sequence b (-1: there is none) the index-th, and the place of its first step on the line.
-struct Tile {
-  int b, index, steps;
-  int64_t first;
 };
-// The tile at a step of the line, or the one with this number.
-__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int rows, int64_t at, bool number) {
+// own: of lane l sequence l.
+__device__ __forceinline__ Line line_of(const AttendArgs& a, int size, const Member& own) {
   const int lane = threadIdx.x & 63;
-  int64_t before = 0, steps_before = 0;
+  int64_t total = own.w.before(own.w.tiles) * a.c.kv_heads;
+  int tiles = own.w.tiles;
+  for (int b = 64 + lane; b < a.a.B; b += 64) {
+    const Member m = member(a, b, size);
+    total += m.w.before(m.w.tiles) * a.c.kv_heads, tiles += m.w.tiles;
+  }
+  for (int o = 1; o < 64 && o < a.a.B; o <<= 1) total += __shfl_xor(total, o), tiles += __shfl_xor(tiles, o);
+  total = same(total);
+  const int64_t all = (int64_t)same(tiles) * a.c.kv_heads;
+  const double most = (double)total / ((double)a.least * kStep * a.group) + 1.0;
+  int n = most < a.wanted ? (int)most : a.wanted;
+  // less work than fills the card: a whole number of pieces a tile, so that equal tiles' ends are pieces' ends
+  if (n < a.wanted && all <= a.wanted) n = all ? (int)all * (n > all ? n / (int)all : 1) : 1;
+  return Line{total, (double)total / n, n};
+}
+// A tile: of sequence b (-1: there is none) and a head of keys, and its place on the line.
+struct Tile {
+  int b, head, row;
+  int64_t first, weight;
+  Sequence s;
+};
+// The tile at a point of the line or, `number`, the one with this number.
+__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int size, const Member& own, int64_t at, bool number) {
+  const int lane = threadIdx.x & 63, heads = (int)a.c.kv_heads;
+  int64_t before = 0, weight_before = 0;
   for (int b0 = 0; b0 < a.a.B; b0 += 64) {
-    Share h{0, 1};
-    if (b0 + lane < a.a.B) h = share_of(a, sequence(a, b0 + lane), rows);
-    const int64_t steps = (int64_t)h.tiles * h.steps, mine = number ? h.tiles : steps;
-    int64_t upto = mine, steps_upto = steps;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(upto, o), w = __shfl_up(steps_upto, o);
-      if (lane >= o) upto += v, steps_upto += w;
+    const Member m = b0 ? member(a, b0 + lane, size) : own;
+    const Weights& w = m.w;
+    const int64_t of_head = w.before(w.tiles), weight = of_head * heads, mine = number ? (int64_t)w.tiles * heads : weight;
+    int64_t upto = mine, weight_upto = weight;
+    for (int o = 1; o < 64 && o < a.a.B; o <<= 1) {
+      const int64_t v = __shfl_up(upto, o), x = __shfl_up(weight_upto, o);
+      if (lane >= o) upto += v, weight_upto += x;
     }
-    upto += before, steps_upto += steps_before;
+    upto += before, weight_upto += weight_before;
     const uint64_t found = __ballot(at < upto && at >= upto - mine);
     if (found) {
       const int owner = __builtin_ctzll(found);
-      const int each = __shfl(h.steps, owner);
-      const int64_t first = __shfl(steps_upto - steps, owner), within = at - __shfl(upto - mine, owner);
-      const int index = same((int)(number ? within : within / each));
-      return Tile{same(b0 + owner), index, same(each), same(first + (int64_t)index * each)};
+      int head = 0, row = 0;
+      int64_t first = 0, its = 0;
+      if (lane == owner) {
+        int64_t in = at - (upto - mine);
+        if (number) {
+          row = (int)((uint32_t)in / (uint32_t)heads), head = (int)in - row * heads, row = w.tiles - 1 - row;
+        } else {
+          head = (int)((double)in / (double)of_head);
+          while (head > 0 && head * of_head > in) --head;
+          while ((head + 1) * of_head <= in) ++head;
+          in -= head * of_head;
+          int low = 0, high = w.tiles;                              // the last tile that begins at `in` or before
+          while (high - low > 1) {
+            const int mid = (low + high) >> 1;
+            if (w.before(mid) <= in) low = mid;
+            else high = mid;
+          }
+          row = low;
+        }
+        first = weight_upto - weight + head * of_head + w.before(row), its = w.of(row);
+      }
+      auto its_own = [&](int v) { return __builtin_amdgcn_readlane(v, owner); };
+      auto its_own64 = [&](int64_t v) { return (int64_t)((uint64_t)(uint32_t)its_own((int)(v >> 32)) << 32 | (uint32_t)its_own((int)v)); };
+      return Tile{same(b0 + owner), its_own(head), its_own(row), its_own64(first), its_own64(its),
+                  Sequence{its_own(m.s.start), its_own(m.s.n), its_own(m.s.length), its_own(m.s.lo), its_own(m.s.hi)}};
     }
-    before = __shfl(upto, 63), steps_before = __shfl(steps_upto, 63);
+    before = __shfl(upto, 63), weight_before = __shfl(weight_upto, 63);
   }
-  return Tile{-1, 0, 1, 0};
+  return Tile{-1, 0, 0, 0, 1, {}};
 }
-// Workgroups a CU (of a wave for each of its SIMDs) that the registers of the kernel of few queries are held to, and the
-// steps that it asks for ahead.
-constexpr int few_groups(int dtype, int blocks) { return blocks <= 2 ? 3 : blocks <= 4 || dtype == MXQ_DT_BF16 ? 2 : 1; }
-constexpr int few_depth(int dtype, int blocks) { return blocks <= 4 ? 2 : 1; }
-
-// Where the sums of a piece's parts of tiles lie: of the tile that its first step is in, and of its last one.
+// Of `steps` those before a share of a tile's weight.
+__device__ __forceinline__ int steps_before(int steps, int64_t share, int64_t weight) {
+  if (share >= weight) return steps;
+  const int n = (int)((float)steps * ((float)share * __builtin_amdgcn_rcpf((float)weight)));
+  return n < steps ? n : steps;
+}
+// Where the sums of a piece's parts of tiles lie: of the tile that its first point is in, and of its last one.
 __device__ __forceinline__ int64_t part_slot(int group, bool first) { return 2 * (int64_t)group + !first; }
+
+constexpr int kWaves = 4;
+// Sixteens of rows that a wave of many queries has: as many as let two waves share a SIMD's registers (of float32's three
+// planes half as many).
+constexpr int attend_rows(int dtype, int blocks) { return blocks == 8 ? 1 : dtype == MXQ_DT_F32 ? 4 / blocks : 8 / blocks; }
+// Workgroups a CU (of a wave for each of its SIMDs) that the registers are held to.
+constexpr int attend_groups(int dtype, int blocks, int tiles, bool many) {
+  if (!many && tiles == 1 && blocks == 2) return 3;
+  return dtype == MXQ_DT_BF16 || tiles * blocks < 8 ? 2 : 1;
+}
+constexpr int blocks_class(int blocks) { return blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8; }
 
 // The logarithm of a sum of weights relative to 2^top; of no weights -inf.
 __device__ __forceinline__ float log_sum(float top, float sum) {
@@ -237,6 +320,25 @@ template <int DT> __device__ __forceinline__ void load_query(const void* q, int6
       if (i < valid) f[i] = load_elem(q, DT, at + i);
   }
   planes_of(f, out);
+}
+
+// Four neighbouring columns of a row of the output, the first `valid` of them there.
+template <int DT> __device__ __forceinline__ void store_four(void* p, int64_t at, int valid, const float (&v)[4]) {
+  if (valid >= 4) {
+    if constexpr (DT == MXQ_DT_F32) {
+      __builtin_memcpy((float*)p + at, v, 16);
+    } else if constexpr (DT == MXQ_DT_BF16) {
+      const bf16x2 w[2] = {{(__bf16)v[0], (__bf16)v[1]}, {(__bf16)v[2], (__bf16)v[3]}};
+      __builtin_memcpy((uint16_t*)p + at, w, 8);
+    } else {
+      const f16x2 w[2] = {{(_Float16)v[0], (_Float16)v[1]}, {(_Float16)v[2], (_Float16)v[3]}};
+      __builtin_memcpy((uint16_t*)p + at, w, 8);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < valid) store_elem(p, DT, at + i, v[i]);
+  }
 }
 
 }  // namespace mxq
