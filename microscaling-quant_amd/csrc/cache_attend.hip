@@ -233,7 +233,7 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
     if (int rc = check_launch("mxq_cache_attend")) return rc;
     if (!a.partial) continue;
     const bool by_tile = w.tiles <= a.wanted;
-    const int places = by_tile ? (int)w.tiles : a.wanted, shares = w.rows > 32 ? w.rows / 16 : places > 128 ? 1 : places > 32 ? 4 : 16;
+    const int places = by_tile ? (int)w.tiles : a.wanted, shares = w.rows > 32 ? w.rows / 16 : places > 128 ? 1 : 16;
     ways.way[many] = JoinWay{a.partial, a.above, a.upto, a.wanted, w.rows, places, shares, by_tile};
     joins += places * shares;
   }

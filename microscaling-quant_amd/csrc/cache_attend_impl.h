@@ -19,7 +19,7 @@ namespace mxq {
 
 // PAGES16: pages of whole 16 rows that are less than 2^26 bytes apart.
 
-template <int FAM, int DT, int NB, bool PAGES16, int RT, int WR>
+template <int FAM, int DT, int NB, bool PAGES16, int RT, int WR, bool LINE>
 __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) void k_attend(AttendArgs a) {
   constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
   constexpr int KW = NB * BB / 16;                        // words of keys' codes a lane and tile of 16 keys
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   // this workgroup's piece of the line
   int piece = blockIdx.x;
   int64_t at = blockIdx.x, end_at = 0;
-  if (a.partial) {
+  if constexpr (LINE) {
     const Line line = line_of(a, ROWS, member(a, lane, ROWS));
     if ((int)blockIdx.x >= line.groups) return;
     // neighbouring pieces, which may share keys, on one of the card's eight parts
@@ -44,11 +44,11 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
     at = line.begin(piece), end_at = line.begin(piece + 1);
   }
   for (bool first_part = true;; first_part = false) {
-  const Tile u = tile_of(a, ROWS, member(a, lane, ROWS), at, !a.partial);
+  const Tile u = tile_of(a, ROWS, member(a, lane, ROWS), at, !LINE);
   if (u.b < 0) return;
   // this piece's share of the tile's weight
-  const int64_t share_from = a.partial ? at - u.first : 0, share_to = a.partial && end_at - u.first < u.weight ? end_at - u.first : u.weight;
-  const bool whole = share_from == 0 && share_to == u.weight;
+  const int64_t share_from = LINE ? at - u.first : 0, share_to = LINE && end_at - u.first < u.weight ? end_at - u.first : u.weight;
+  const bool whole = !LINE || (share_from == 0 && share_to == u.weight);
   const int kv_head = u.head;
   const Sequence& s = u.s;
   const int rows = s.n * a.group, row0 = u.row * ROWS + (WR > 1 ? wave * 16 * RT : 0);   // of this wave
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
       }
     }
   }
-  if (!a.partial) return;
+  if constexpr (!LINE) return;
   at = u.first + u.weight;
   if (at >= end_at) return;
   }
@@ -472,8 +472,10 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
 
 template <int FAM, int DT, int NB, int RT, int WR> void launch_attend_of(const AttendArgs& a, int64_t groups, hipStream_t st) {
   const dim3 grid((unsigned)groups), block(64 * kWaves);
-  if (a.aligned) k_attend<FAM, DT, NB, true, RT, WR><<<grid, block, 0, st>>>(a);
-  else k_attend<FAM, DT, NB, false, RT, WR><<<grid, block, 0, st>>>(a);
+  if (a.aligned && a.partial) k_attend<FAM, DT, NB, true, RT, WR, true><<<grid, block, 0, st>>>(a);
+  else if (a.aligned) k_attend<FAM, DT, NB, true, RT, WR, false><<<grid, block, 0, st>>>(a);
+  else if (a.partial) k_attend<FAM, DT, NB, false, RT, WR, true><<<grid, block, 0, st>>>(a);
+  else k_attend<FAM, DT, NB, false, RT, WR, false><<<grid, block, 0, st>>>(a);
 }
 // many: tiles of many rows; wide: few queries' rows are 32.
 template <int FAM, int DT, int NB> void launch_attend_by(const AttendArgs& a, bool many, bool wide, int64_t groups, hipStream_t st) {
