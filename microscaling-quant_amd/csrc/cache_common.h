@@ -172,6 +172,7 @@ struct Line {
   int64_t total;
   double each;           // weight of a piece
   int groups;            // workgroups that have one
+  // begin(groups) is the total exactly while that is below 2^51 steps, which no call lives to see the end of.
   __device__ __forceinline__ int64_t begin(int i) const { return (int64_t)(each * i + 0.5); }
   __device__ __forceinline__ int group_at(int64_t at) const {
     int i = (int)((double)at / each);
