@@ -39,11 +39,30 @@ struct JoinWays {
 // rows of no sequence.  A workgroup takes rows of a tile, or of the tile that a piece ends in, if that is the tile's first end
 // of a piece: sixteen lanes a row, or, of many parts, the workgroup a row, its sixteens of lanes the parts in turn.
 constexpr int kManyParts = 8;
+// Workgroups that share what there is to join, twice as many of tiles of many rows: 64 sequences' 512 tiles of 4 to 8 rows took
+// 128 us with 512 of them, 131 with 1024 and 139 with 2048 (most find nothing), prompts of 128 rows a tile 198, 193 and 198.
+constexpr int kJoins = 512;
+constexpr int kAtOnce = 4;                    // parts asked for together
+// Sums of weights and of values relative to 2^best, and those of a part relative to its own maximum, `best` at most.
+template <int V> __device__ __forceinline__ void add_part(float& all, float (&v)[V], float top, float weight, float best, const float (&x)[V]) {
+  // a part without a maximum has seen no key, or only scores of NaN, which its sum is then
+  const bool none = top == -__builtin_inff();
+  const float factor = none ? weight : __builtin_amdgcn_exp2f(top - best);
+  all += none ? weight : factor * weight;
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
+}
 template <int COLUMNS>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways, bool empty_rows) {
   constexpr int V = COLUMNS / 16;
   __shared__ float sums[16][COLUMNS];
-  __shared__ float weights[16];
+  __shared__ float weights[16], maxima[16];
+  struct Found {
+    Tile u;
+    int group, runs;           // its first piece, and in how many it lies
+    bool at_begin;
+  };
+  __shared__ Found found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim, c = lane & 15, sixteen = threadIdx.x >> 4;
   if (empty_rows) {
     // queries [0, starts[0]) and [starts[B], T) are no sequence's
@@ -62,16 +81,26 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
   if (index >= w.places * w.shares) return;
   const int share = index / w.places, place = index - share * w.places, size = w.size;
   a.above = w.above, a.upto = w.upto, a.wanted = w.wanted;
-  const Member own = member(a, lane, size);
-  const Line line = line_of(a, size, own);
-  if (!w.by_tile && place + 1 >= line.groups) return;
-  const Tile u = tile_of(a, size, own, w.by_tile ? place : line.begin(place + 1), w.by_tile);
-  if (u.b < 0) return;
-  if (!w.by_tile && (u.first == line.begin(place + 1) || u.first < line.begin(place))) return;
-  const int g0 = w.by_tile ? same(line.group_at(u.first)) : place;
-  const int runs = same(line.group_at(u.first + u.weight - 1)) - g0 + 1;
-  if (runs == 1) return;
-  const bool at_begin = line.begin(g0) == u.first;          // of the first piece it is the first tile
+  // one wave finds the tile: what it takes to find it is most of what a workgroup computes
+  if (wave == 0) {
+    Member own = member(a, lane, size, 0.0);
+    const Line line = line_of(a, size, own);
+    Found f{};
+    if (w.by_tile || place + 1 < line.groups) {
+      f.u = tile_of(a, size, own, line.unit, w.by_tile ? place : line.begin(place + 1), w.by_tile);
+      if (f.u.b >= 0 && (w.by_tile || (f.u.first != line.begin(place + 1) && f.u.first >= line.begin(place)))) {
+        f.group = w.by_tile ? line.group_at(f.u.first) : place;
+        f.runs = line.group_at(f.u.first + f.u.weight - 1) - f.group + 1;
+        f.at_begin = line.begin(f.group) == f.u.first;          // of the first piece it is the first tile
+      }
+    }
+    if (lane == 0) found = f;
+  }
+  __syncthreads();
+  const Tile u = found.u;
+  const int g0 = same(found.group), runs = same(found.runs);
+  if (runs < 2) return;
+  const bool at_begin = found.at_begin;
   const int rows = u.s.n * a.group, row0 = u.row * size, last = rows - row0 < size ? rows - row0 : size;
   const bool many = runs > kManyParts;
   for (int r = many ? share : share * 16 + sixteen; r < last; r += many ? w.shares : w.shares * 16) {
@@ -79,35 +108,44 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
     float best = -__builtin_inff(), all = 0.0f, v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.0f;
-    for (int i = c; i < runs; i += 16) best = __builtin_fmaxf(best, part_of(i)[COLUMNS]);
-    for (int o = 8; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
-#pragma unroll 4
-    for (int i = many ? sixteen : 0; i < runs; i += many ? 16 : 1) {
-      const float* part = part_of(i);
-      const float top = part[COLUMNS], sum = part[COLUMNS + 1];
-      // a part without a maximum has seen no key, or only scores of NaN, which its sum is then
-      const float factor = top == -__builtin_inff() ? sum : __builtin_amdgcn_exp2f(top - best);
-      float x[V];
+    const int by = many ? 16 : 1;
+    for (int i0 = many ? sixteen : 0; i0 < runs; i0 += kAtOnce * by) {
+      float x[kAtOnce][V], tops[kAtOnce], weight[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < V; k += 4) __builtin_memcpy(x + k, part + k * 16 + c * 4, 16);
-      all += top == -__builtin_inff() ? sum : factor * sum;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = i0 + u * by;
+        const float* part = part_of(i < runs ? i : i0);
+        tops[u] = i < runs ? part[COLUMNS] : -__builtin_inff(), weight[u] = i < runs ? part[COLUMNS + 1] : 0.0f;
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
+        for (int k = 0; k < V; k += 4) __builtin_memcpy(x[u] + k, part + k * 16 + c * 4, 16);
+      }
+      float now = best;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) now = __builtin_fmaxf(now, tops[u]);
+      const float keep = best == now ? 1.0f : __builtin_amdgcn_exp2f(best - now);
+      all *= keep;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = keep == 0.0f ? 0.0f : keep * v[k];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) add_part(all, v, tops[u], weight[u], now, x[u]);
+      best = now;
     }
     if (many) {
-      if (c == 0) weights[sixteen] = all;
+      if (c == 0) weights[sixteen] = all, maxima[sixteen] = best;
 #pragma unroll
       for (int k = 0; k < V; ++k) sums[sixteen][k / 4 * 64 + c * 4 + k % 4] = v[k];
       __syncthreads();
-      all = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) all += weights[j];
       if (sixteen == 0) {
+        best = maxima[0], all = 0.0f;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          v[k] = 0.0f;
+        for (int j = 1; j < 16; ++j) best = __builtin_fmaxf(best, maxima[j]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[k] += sums[j][k / 4 * 64 + c * 4 + k % 4];
+        for (int k = 0; k < V; ++k) v[k] = 0.0f;
+        for (int j = 0; j < 16; ++j) {
+          float x[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) x[k] = sums[j][k / 4 * 64 + c * 4 + k % 4];
+          add_part(all, v, maxima[j], weights[j], best, x);
         }
       }
       __syncthreads();
@@ -233,7 +271,8 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
     if (int rc = check_launch("mxq_cache_attend")) return rc;
     if (!a.partial) continue;
     const bool by_tile = w.tiles <= a.wanted;
-    const int places = by_tile ? (int)w.tiles : a.wanted, shares = w.rows > 32 ? w.rows / 16 : places > 128 ? 1 : 16;
+    const int places = by_tile ? (int)w.tiles : a.wanted, most = many ? w.rows / 16 : 16, spare = (many ? 2 : 1) * kJoins / places;
+    const int shares = spare < 1 ? 1 : spare < most ? spare : most;
     ways.way[many] = JoinWay{a.partial, a.above, a.upto, a.wanted, w.rows, places, shares, by_tile};
     joins += places * shares;
   }

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   constexpr int SW = NB == 8 ? 2 : 1;                     // words of a row's scales
   constexpr int OT = 2 * NB, DP = 32 * NB;                // tiles of out^T, columns
   constexpr int WK = kWaves / WR, ROWS = 16 * RT * WR;    // waves that share a row's keys; rows of a workgroup
-  __shared__ float sums[WK > 1 ? WK : 1][WK > 1 ? 16 : 1][WK > 1 ? DP + 4 : 1];
+  __shared__ __attribute__((aligned(16))) float sums[WK > 1 ? WK : 1][WK > 1 ? 16 : 1][WK > 1 ? DP + 4 : 1];
   __shared__ float tops[kWaves][16], weights[kWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int D = a.c.head_dim;
@@ -36,15 +36,17 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   // this workgroup's piece of the line
   int piece = blockIdx.x;
   int64_t at = blockIdx.x, end_at = 0;
+  double unit = 0.0;
   if constexpr (LINE) {
-    const Line line = line_of(a, ROWS, member(a, lane, ROWS));
+    Member own = member(a, lane, ROWS, 0.0);
+    const Line line = line_of(a, ROWS, own);
     if ((int)blockIdx.x >= line.groups) return;
     // neighbouring pieces, which may share keys, on one of the card's eight parts
     if (line.groups == a.wanted) piece = (int)(blockIdx.x & 7) * (a.wanted >> 3) + (int)(blockIdx.x >> 3);
-    at = line.begin(piece), end_at = line.begin(piece + 1);
+    at = line.begin(piece), end_at = line.begin(piece + 1), unit = line.unit;
   }
   for (bool first_part = true;; first_part = false) {
-  const Tile u = tile_of(a, ROWS, member(a, lane, ROWS), at, !LINE);
+  const Tile u = tile_of(a, ROWS, member(a, lane, ROWS, unit), unit, at, !LINE);
   if (u.b < 0) return;
   // this piece's share of the tile's weight
   const int64_t share_from = LINE ? at - u.first : 0, share_to = LINE && end_at - u.first < u.weight ? end_at - u.first : u.weight;
@@ -61,20 +63,47 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   auto last_key = [&](int t) { return a.a.causal ? s.length - s.n + t : s.length - 1; };
   int lo[RT], hi[RT];
   bf16x8 q[RT][P][NB];
+  int64_t q_at[RT];
 #pragma unroll
   for (int m = 0; m < RT; ++m) {
     const int row = row0 + 16 * m + c, held = row < rows ? row : rows - 1;
     const int token = (int)divu31(held, a.by_group), head = kv_head * a.group + held - token * a.group;
     lo[m] = row < rows ? first_key(token) : 1, hi[m] = row < rows ? last_key(token) : 0;
-    const int64_t at = (int64_t)(s.start + token) * a.a.q_token + head * a.a.q_head;
+    q_at[m] = (int64_t)(s.start + token) * a.a.q_token + head * a.a.q_head;
+  }
+  auto q_column = [&](int i) { return NB == 2 ? 16 * g + 8 * i : 32 * (g + 4 * (i >> 2)) + 8 * (i & 3); };
+  if (D & 7) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int d = NB == 2 ? 16 * g + 8 * i : 32 * (g + 4 * (i >> 2)) + 8 * (i & 3);
-      bf16x8 p[P];
-      load_query<DT>(a.q, at + d, row < rows ? D - d : 0, p);
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int j = 0; j < P; ++j) q[m][j][i] = p[j];
-    }
+      for (int i = 0; i < NB; ++i) {
+        bf16x8 p[P];
+        load_query<DT>(a.q, q_at[m] + q_column(i), D - q_column(i), p);
+#pragma unroll
+        for (int j = 0; j < P; ++j) q[m][j][i] = p[j];
+      }
+  } else {
+    // all on their way before the first is looked at
+    Eight x[RT][NB];
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) x[m][i] = load_eight(a.q, DT, q_at[m] + (q_column(i) < D ? q_column(i) : 0));
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = 0.0f;
+        add_eight(f, x[m][i], DT);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = q_column(i) < D ? f[k] : 0.0f;
+        bf16x8 p[P];
+        planes_of(f, p);
+#pragma unroll
+        for (int j = 0; j < P; ++j) q[m][j][i] = p[j];
+      }
   }
   const int end_row = row0 + 16 * RT < rows ? row0 + 16 * RT : rows;       // no row is this wave's where it is not past row0
   const int t_first = (int)divu31(row0 < rows ? row0 : rows - 1, a.by_group), t_last = (int)divu31((row0 < end_row ? end_row : rows) - 1, a.by_group);
@@ -437,7 +466,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
 #pragma unroll
         for (int r = 0; r < 4; ++r) sums[wave][c][OT * (4 * g + r) + t] = o[m][t][r];
       __syncthreads();
-      const int r = threadIdx.x >> 4, d0 = threadIdx.x & 15;
+      const int r = threadIdx.x >> 4, d0 = 4 * (threadIdx.x & 15);
       if (tile0 + r >= rows) continue;
       float best = tops[0][r], all = 0.0f, factor[WK];
 #pragma unroll
@@ -451,12 +480,20 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
       const float inv = all == 0.0f ? 0.0f : 1.0f / all;
       const int64_t row = out_row(r);
       float* part = part_row(r);
-      for (int d = d0; d < D; d += 16) {
-        float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WK; ++w) v += factor[w] == 0.0f ? 0.0f : factor[w] * sums[w][r][d];
-        if (whole) store_elem(a.out, DT, row * D + d, v * inv);
-        else part[d] = v;
+      for (int d = d0; d < DP; d += 64) {
+        float v[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WK; ++w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] += factor[w] == 0.0f ? 0.0f : factor[w] * sums[w][r][d + k];
+        if (!whole) {
+          __builtin_memcpy(part + d, v, 16);
+        } else if (d < D) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] *= inv;
+          store_four<DT>(a.out, row * D + d, D - d, v);
+        }
       }
       if (d0 == 0) {
         if (!whole) part[DP] = best, part[DP + 1] = all;

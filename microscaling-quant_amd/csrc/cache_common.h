@@ -142,12 +142,17 @@ struct Weights {
     return grow * base + (grow * (grow + 1) / 2 << (shift & 63)) + (j - grow) * most + j * start;
   }
 };
-// Of this lane: a sequence and its weights.
+// Of this lane: a sequence and its weights.  unit: 0, or what the tiles of a sequence, all as heavy as its last one, are cut
+// into: a tile's weight is then its pieces.
 struct Member {
   Sequence s;
   Weights w;
 };
-__device__ __forceinline__ Member member(const AttendArgs& a, int b, int size) {
+__device__ __forceinline__ Weights in_pieces(const Weights& w, double unit) {
+  const int64_t pieces = w.tiles ? (int64_t)((double)w.of(w.tiles - 1) / unit) + 1 : 0;
+  return Weights{w.tiles, -1, pieces, pieces, 0};
+}
+__device__ __forceinline__ Member member(const AttendArgs& a, int b, int size, double unit) {
   constexpr int64_t kMost = (int64_t)1 << 34;                       // so that no sum of weights passes 63 bits
   auto hold = [](int64_t v) { return v < kMost ? v : kMost; };
   Member m{};
@@ -166,12 +171,14 @@ __device__ __forceinline__ Member member(const AttendArgs& a, int b, int size) {
     const int64_t keys = a.a.window && a.a.window < s.length - s.n ? a.a.window + s.n : s.length;
     w.shift = -1, w.base = w.most = hold(keys * a.group);
   }
+  if (unit != 0.0) w = in_pieces(w, unit);
   return m;
 }
 struct Line {
   int64_t total;
   double each;           // weight of a piece
   int groups;            // workgroups that have one
+  double unit;           // weight that a piece is of, where no piece is of two tiles; else 0
   // begin(groups) is the total exactly while that is below 2^51 steps, which no call lives to see the end of.
   __device__ __forceinline__ int64_t begin(int i) const { return (int64_t)(each * i + 0.5); }
   __device__ __forceinline__ int group_at(int64_t at) const {
@@ -182,23 +189,38 @@ struct Line {
     return i;
   }
 };
-// own: of lane l sequence l.
-__device__ __forceinline__ Line line_of(const AttendArgs& a, int size, const Member& own) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = own.w.before(own.w.tiles) * a.c.kv_heads;
-  int tiles = own.w.tiles;
+// own: of lane l sequence l; its weights become the line's.
+__device__ __forceinline__ Line line_of(const AttendArgs& a, int size, Member& own) {
+  const int lane = threadIdx.x & 63, heads = (int)a.c.kv_heads;
+  auto sum = [&](int64_t v) {
+    for (int o = 1; o < 64 && o < a.a.B; o <<= 1) v += __shfl_xor(v, o);
+    return same(v) * heads;
+  };
+  auto even_weight = [](const Weights& w) { return w.tiles ? w.tiles * w.of(w.tiles - 1) : 0; };
+  int64_t total = own.w.before(own.w.tiles), even = even_weight(own.w), all = own.w.tiles;
   for (int b = 64 + lane; b < a.a.B; b += 64) {
-    const Member m = member(a, b, size);
-    total += m.w.before(m.w.tiles) * a.c.kv_heads, tiles += m.w.tiles;
+    const Weights w = member(a, b, size, 0.0).w;
+    total += w.before(w.tiles), even += even_weight(w), all += w.tiles;
   }
-  for (int o = 1; o < 64 && o < a.a.B; o <<= 1) total += __shfl_xor(total, o), tiles += __shfl_xor(tiles, o);
-  total = same(total);
-  const int64_t all = (int64_t)same(tiles) * a.c.kv_heads;
-  const double most = (double)total / ((double)a.least * kStep * a.group) + 1.0;
+  total = sum(total), even = sum(even), all = sum(all);
+  const double least = (double)a.least * kStep * a.group;
+  if (2 * all <= a.wanted && even <= total + total / 4) {
+    // w / unit + 1 pieces of each tile are `wanted` together
+    const double share = (double)even / (double)(a.wanted - all), unit = share < least ? least : share;
+    own.w = in_pieces(own.w, unit);
+    int64_t pieces = own.w.before(own.w.tiles);
+    for (int b = 64 + lane; b < a.a.B; b += 64) {
+      const Weights w = member(a, b, size, unit).w;
+      pieces += w.before(w.tiles);
+    }
+    pieces = sum(pieces);
+    return Line{pieces, 1.0, (int)pieces, unit};
+  }
+  const double most = (double)total / least + 1.0;
   int n = most < a.wanted ? (int)most : a.wanted;
   // less work than fills the card: a whole number of pieces a tile, so that equal tiles' ends are pieces' ends
   if (n < a.wanted && all <= a.wanted) n = all ? (int)all * (n > all ? n / (int)all : 1) : 1;
-  return Line{total, (double)total / n, n};
+  return Line{total, (double)total / n, n, 0.0};
 }
 // A tile: of sequence b (-1: there is none) and a head of keys, and its place on the line.
 struct Tile {
@@ -207,11 +229,11 @@ struct Tile {
   Sequence s;
 };
 // The tile at a point of the line or, `number`, the one with this number.
-__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int size, const Member& own, int64_t at, bool number) {
+__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int size, const Member& own, double unit, int64_t at, bool number) {
   const int lane = threadIdx.x & 63, heads = (int)a.c.kv_heads;
   int64_t before = 0, weight_before = 0;
   for (int b0 = 0; b0 < a.a.B; b0 += 64) {
-    const Member m = b0 ? member(a, b0 + lane, size) : own;
+    const Member m = b0 ? member(a, b0 + lane, size, unit) : own;
     const Weights& w = m.w;
     const int64_t of_head = w.before(w.tiles), weight = of_head * heads, mine = number ? (int64_t)w.tiles * heads : weight;
     int64_t upto = mine, weight_upto = weight;
