@@ -18,6 +18,7 @@ MXQ_LAUNCH(launch_attend_pairs_f16)
 
 namespace {
 
+constexpr int64_t kMostKeys = 0x7fff0000;     // of a sequence, as its table has room for them
 constexpr int kUnits = 256, kLeast = 8;       // CUs; steps of 32 keys that a workgroup takes at least
 constexpr int kFewRows = 64;                  // rows a sequence up to which its keys are what a call costs
 
@@ -178,9 +179,10 @@ int check(const mxq_cache_spec* c, const mxq_attend_spec* a) {
   if (a->T < 0 || a->B < 0 || a->heads < 1 || a->T > 0x3fffffff || a->B > 0x3fffffff || a->heads > 0x3fffffff || a->T * a->heads > 0x3fffffff)
     return invalid(who + ": size out of range");
   if (a->heads % c->kv_heads) return invalid(who + ": heads must be a multiple of kv_heads");
-  if (!(a->scale > 0.0f) || a->scale > 3.4e38f) return invalid(who + ": scale must be positive and finite");
+  if (!(a->scale > 0.0f) || a->scale > 0x1p127f) return invalid(who + ": scale must be positive, and 2^127 at most");
   if (a->window < 0 || a->window > 0x7fffffff) return invalid(who + ": window out of range");
-  if (a->table_pages < 0 || a->table_pages > 0x7fffffff) return invalid(who + ": table out of range");
+  // keys are counted in 32 bits, also those that a wave looks for ahead of its last one
+  if (a->table_pages < 0 || a->table_pages > 0x7fffffff || a->table_pages * c->page_size > kMostKeys) return invalid(who + ": table out of range");
   return MXQ_OK;
 }
 

@@ -26,6 +26,7 @@ __all__ = ["PackedCache", "packed_cache", "cache_write", "cache_read", "cache_at
 _FORMATS = {"MXFP8_E4M3": (0, 32), "MXFP8_E5M2": (1, 32), "MXFP4": (5, 16)}      # MXQ_FMT_* and a block's bytes
 MAX_HEAD_DIM = 256
 _MOST = 2 ** 31 - 1
+_MOST_KEYS = 2 ** 31 - 2 ** 16
 
 
 class PackedCache(NamedTuple):
@@ -246,8 +247,10 @@ def _attend_spec(key, q_shape, q_dtype, q_strides, table, table_row, lengths, st
         raise ValueError(f"mxq.nn.cache_attend: q must have {B} sequences, as table has, got shape {tuple(q_shape)}")
     if window is not None:
         _whole(window, who, "window", 1, _MOST)
-    if not 0.0 < scale <= torch.finfo(torch.float32).max:
-        raise ValueError(f"mxq.nn.cache_attend: scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= 2.0 ** 127:
+        raise ValueError(f"mxq.nn.cache_attend: scale must be positive, and 2^127 at most, got {scale}")
+    if pages * spec.page_size > _MOST_KEYS:
+        raise ValueError(f"mxq.nn.cache_attend: {pages} pages of {spec.page_size} keys a sequence are more than {_MOST_KEYS}")
     T = q_shape[0] if starts is not None else q_shape[0] * q_shape[1]
     if T * H > _MOST // 2:
         raise ValueError(f"mxq.nn.cache_attend: {T} queries of {H} heads are too many")
@@ -263,10 +266,10 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
 
     q: B x n x heads x head_dim, or with starts (B + 1 ascending int32) T x heads x head_dim, sequence b's queries being
     [starts[b], starts[b + 1]); float32, bfloat16 or float16.  heads is a multiple of the cache's; neighbouring heads share
-    one.  table (B x pages, int32) names each sequence's pages and lengths (B, int32) says how many keys it has, its newest
+    one.  table (B x pages, at most 2^31 - 2^16 keys; int32) names each sequence's pages and lengths (B, int32) says how many keys it has, its newest
     tokens', written before, among them.  The last query is at the last key; query j of n is at position
     p = lengths[b] - n + j.  causal: it sees keys up to p; window: from p - window + 1 on.  scale (head_dim ** -0.5 by default)
-    must be positive.
+    must be positive, and 2^127 at most.
 
     Lengths are held to the table's pages and starts to T.  A key on a page that the cache does not have (-1, say) is not
     there.  A query that sees no key, or that belongs to no sequence, gets zeros and an lse of -inf; so does one whose every

@@ -97,6 +97,9 @@ def test_cache_read_refuses(change, error, text):
     (dict(scale=0.0), ValueError, "scale must be positive"),
     (dict(scale=float("nan")), ValueError, "scale must be positive"),
     (dict(scale=float("inf")), ValueError, "scale must be positive"),
+    (dict(scale=1.8e38), ValueError, "scale must be positive"),
+    (dict(table=_i32(1, 1).expand(3, 2 ** 27)), ValueError, "keys a sequence"),
+    (dict(table=_i32(1, 1).expand(3, 2 ** 27 - 2 ** 12 + 1)), ValueError, "keys a sequence"),
 ])
 def test_cache_attend_refuses(change, error, text):
     args = {**dict(q=torch.zeros(3, 1, 6, 40), cache=_cache(), table=_i32(3, 2), lengths=_i32(3)), **change}
@@ -161,6 +164,7 @@ def test_c_entries_refuse():
     for change, text in ((dict(dtype=3), "dtype"), (dict(heads=3), "multiple"), (dict(heads=0), "out of range"), (dict(T=-1), "out of range"),
                          (dict(T=1 << 29, heads=4), "out of range"), (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"),
                          (dict(scale=float("nan")), "scale"), (dict(window=-1), "window"), (dict(table_pages=-1), "table"),
+                         (dict(scale=1.8e38), "scale"), (dict(table_pages=1 << 27), "table"), (dict(table_pages=(1 << 27) - (1 << 12) + 1), "table"),
                          (dict(T=5), "multiple of B"), (dict(B=0), "multiple of B")):
         refused(text, "mxq_cache_attend", *run(cache(), attend(**change)))
     refused("NULL", "mxq_cache_attend", *run(cache(), attend(), q=0))
