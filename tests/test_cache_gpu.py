@@ -179,6 +179,54 @@ def test_write_same_slot_again(cuda, T):
     assert torch.equal(k, want) and torch.equal(v, -want)
 
 
+@pytest.mark.parametrize("T", [1, 1023, 1024, 1025, 1500])
+@pytest.mark.parametrize("fmt, dtype, dim, heads, page", [("MXFP8_E4M3", "bf16", 256, 40, 3), ("MXFP4", "f16", 40, 3, 16), ("MXFP8_E5M2", "f32", 100, 33, 7)])
+def test_write_and_read_few_and_many_tokens(cuda, fmt, dtype, dim, heads, page, T):
+    """One token a workgroup and several, rows of more items than a workgroup has threads, tokens and heads apart."""
+    gen = _gen(T + dim)
+    pages = -(-T // page) + 2
+    cache = nn.packed_cache(pages, page, heads, dim, fmt)
+    for t in cache[:4]:
+        t.fill_(0x5A)
+    wide = torch.randn(T, 2 * heads, dim + 3, generator=gen, device="cuda").to(DTYPES[dtype])
+    x = (wide[:, 1::2, 3:], wide[:, ::2, :dim])
+    slots = torch.randperm(pages * page, generator=gen, device="cuda")[:T]
+    slots[1::11] = pages * page
+    nn.cache_write(*x, cache, slots)
+    kept = slots < pages * page
+    page_of, at = slots[kept] // page, slots[kept] % page
+    free = torch.ones(pages, page, dtype=torch.bool, device="cuda")
+    free[page_of, at] = False
+    for t, codes, scales in ((x[0], cache.k_codes, cache.k_scales), (x[1], cache.v_codes, cache.v_scales)):
+        want_codes, want_scales = packed.quantize(torch.nn.functional.pad(t, (0, scales.shape[-1] * 32 - dim)), fmt, "ocp", axis=-1)
+        assert torch.equal(codes[page_of, :, at], _pairs(want_codes, fmt)[kept])
+        assert torch.equal(scales[page_of, :, at], want_scales[kept])
+        assert (codes.transpose(1, 2)[free] == 0x5A).all() and (scales.transpose(1, 2)[free] == 0x5A).all()
+    for out in DTYPES.values():
+        for got, want in zip(nn.cache_read(cache, slots.int(), out), oc.rows(cache, slots)):
+            assert torch.equal(got, want.to(out))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_read_every_code_and_scale(cuda, fmt):
+    """Each code under each scale byte, rounded once: subnormal, overflowing and NaN ones too."""
+    codes = torch.arange(16 if fmt == "MXFP4" else 256, device="cuda").repeat_interleave(2 if fmt == "MXFP4" else 1)
+    dim = 32 if fmt == "MXFP4" else 256
+    cache = nn.packed_cache(256, 1, 1, dim, fmt)
+    bytes_ = codes.to(torch.uint8)
+    cache.k_codes.copy_(bytes_[0::2] | bytes_[1::2] << 4 if fmt == "MXFP4" else bytes_)
+    cache.v_codes.copy_(cache.k_codes.flip(-1))
+    for scales in (cache.k_scales, cache.v_scales):
+        scales.copy_(torch.arange(256, device="cuda").to(torch.uint8)[:, None, None, None])
+    slots = torch.arange(256, device="cuda")
+    for T in (256, 2560):
+        for out in DTYPES.values():
+            for got, want in zip(nn.cache_read(cache, slots.repeat(T // 256), out), oc.rows(cache, slots)):
+                want = want.to(out).repeat(T // 256, 1, 1)
+                assert torch.equal(got.nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf),
+                                   want.nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf)), out
+
+
 def test_slots_of_64_bits_and_none(cuda):
     cache = _filled(_gen(1), 4, 8, 2, 64, "MXFP4")
     before = [t.clone() for t in cache[:4]]
@@ -294,6 +342,36 @@ def test_attend_many_sequences(cuda):
     lengths = [(37 * i) % 91 for i in range(300)]
     _case(0, lengths, 1, 2, 1, 64, 16, "MXFP4", torch.bfloat16)
     _case(0, lengths, [i % 3 for i in range(300)], 2, 1, 64, 16, "MXFP4", torch.bfloat16, ragged=True)
+
+
+@pytest.mark.parametrize("fmt, dtype, dim, n, heads", [("MXFP4", "bf16", 130, 260, 128), ("MXFP8_E4M3", "f32", 256, 260, 64)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attend_tiles_enough_to_stay_whole(cuda, fmt, dtype, dim, n, heads, ragged):
+    """So many rows that no tile is cut, the last one of a sequence not full."""
+    for page in (16, 24):
+        _case(n, [n + 40, n - 10, 300], [n, n, n] if ragged else n, heads, 1, dim, page, fmt, DTYPES[dtype], ragged=ragged)
+
+
+@pytest.mark.parametrize("lengths, n, heads, kv_heads", [
+    ([(61 * i) % 997 for i in range(100)], 1, 2, 1),              # tiles of their own pieces, more sequences than a wave has lanes
+    ([(61 * i) % 997 for i in range(100)], 3, 8, 4),              # equal pieces of the line, parts of two tiles and more each
+    ([(61 * i) % 997 for i in range(330)], 1, 2, 2),
+    ([2500], 700, 1, 1), ([1100, 700], 350, 6, 3)])               # prompts: tiles that weigh more and more
+def test_attend_pieces(cuda, lengths, n, heads, kv_heads):
+    for fmt, dim, page, dtype in (("MXFP4", 64, 16, torch.bfloat16), ("MXFP8_E4M3", 128, 20, torch.float16)):
+        _case(len(lengths), lengths, n, heads, kv_heads, dim, page, fmt, dtype)
+
+
+def test_attend_tiny_and_large_scale_bytes(cuda):
+    """Values of about 2^-100 and 2^110: no sum passes float32, and products below its smallest normal number, taken as
+    zeros, would be less than half a step of bfloat16."""
+    for n in (1, 60):
+        for fmt, low in (("MXFP4", 26), ("MXFP4", 200), ("MXFP8_E4M3", 32), ("MXFP8_E5M2", 32), ("MXFP8_E4M3", 240)):
+            gen = _gen(low)
+            cache = _filled(gen, 9, 16, 2, 96, fmt, low, low + 3)
+            cache.k_scales.copy_(torch.randint(118, 126, cache.k_scales.shape, generator=gen, device="cuda"))
+            q = torch.randn(1, n, 4, 96, generator=gen, device="cuda").bfloat16()
+            _attend(q, cache, torch.arange(9, dtype=torch.int32, device="cuda")[None], _i32([140]))
 
 
 @pytest.mark.parametrize("size", [1e-3, 30.0, 3000.0])
@@ -442,6 +520,47 @@ def test_attend_same_bits_again(cuda):
     for _ in range(5):
         again = nn.cache_attend(q, cache, table, _i32(lengths), return_lse=True)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("fmt, page", [("MXFP4", 16), ("MXFP8_E4M3", 20)])
+def test_attention_layer(cuda, fmt, page):
+    """Projections on packed weights around the cache and its attention: prompts in pieces, then token by token, several
+    sequences at once, their queries, keys and values views of one product.  Each step's attention is held to the oracle on
+    the cache as it is, whose rows are the step's keys and values quantized; the layer's output is close to the same layer
+    on float64."""
+    gen = _gen(20)
+    width, H, G, D, B, pages = 256, 8, 2, 64, 3, 40
+    pack = lambda w: packed.quantize(w, "MXFP8_E4M3", axis=-1)                                # noqa: E731
+    w_in = torch.randn((H + 2 * G) * D, width, generator=gen, device="cuda") / 16
+    w_out = torch.randn(width, H * D, generator=gen, device="cuda") / 23
+    w_in, w_out = pack(w_in), pack(w_out)
+    plain = [packed.dequantize(*w, "MXFP8_E4M3", axis=-1).double() for w in (w_in, w_out)]
+    cache = nn.packed_cache(pages, page, G, D, fmt)
+    lengths = [0] * B
+    table = torch.randperm(pages, generator=gen, device="cuda")[:B * 12].view(B, 12).int()
+    for tokens in ([50, 7, 1], [64, 1, 0], [1, 1, 1], [1, 1, 1], [3, 0, 40]):
+        starts = [0] + list(np.cumsum(tokens))
+        x = torch.randn(starts[-1], width, generator=gen, device="cuda").bfloat16()
+        at = torch.tensor([l + j for l, n in zip(lengths, tokens) for j in range(n)], device="cuda")
+        which = torch.tensor([b for b, n in enumerate(tokens) for _ in range(n)], device="cuda")
+        lengths = [l + n for l, n in zip(lengths, tokens)]
+        slots = table[which, at // page].long() * page + at % page
+        y = nn.packed_linear(x, *w_in, "MXFP8_E4M3").view(-1, H + 2 * G, D)
+        q, k, v = y[:, :H], y[:, H:H + G], y[:, H + G:]
+        nn.cache_write(k, v, cache, slots)
+        for got, t in zip(nn.cache_read(cache, slots, torch.float32), (k, v)):
+            codes, scales = packed.quantize(t, fmt, "ocp", axis=-1)
+            assert torch.equal(got, packed.dequantize(codes, scales, fmt, axis=-1).float())
+        if tokens == [1] * B:
+            _attend(q[:, None], cache, table, _i32(lengths))
+        out, _ = _attend(q, cache, table, _i32(lengths), _i32(starts))
+        got = nn.packed_linear(out.reshape(-1, H * D), *w_out, "MXFP8_E4M3", residual=x)
+        full = (x.double() @ plain[0].t()).view(-1, H + 2 * G, D)
+        assert ((y.double() - full).abs() <= 2.0 ** -8 * full.abs() + 256 * 2.0 ** -23 * (x.double().abs() @ plain[0].abs().t()).view_as(full)).all()
+        full = out.reshape(-1, H * D).double() @ plain[1].t()
+        size = out.reshape(-1, H * D).double().abs() @ plain[1].abs().t() + x.double().abs()
+        full = full + x.double()
+        assert ((got.double() - full).abs() <= 2.0 ** -8 * full.abs() + 512 * 2.0 ** -23 * size).all()
 
 
 def test_generation_captured_in_a_graph(cuda):
