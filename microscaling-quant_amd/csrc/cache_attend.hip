@@ -22,7 +22,16 @@ constexpr int64_t kMostKeys = 0x7fff0000;     // of a sequence, as its table has
 constexpr int kUnits = 256, kLeast = 8;       // CUs; steps of 32 keys that a workgroup takes at least
 constexpr int kFewRows = 64;                  // rows a sequence up to which its keys are what a call costs
 
-constexpr int kWholeTiles = 3;                // tiles of many rows a workgroup from which on none is cut
+// Whether tiles of many rows stay whole, `steps` of keys each at most.  Workgroups that take equal pieces end together, however
+// unlike the tiles are, but parts and their join cost about kCutCost steps.  Four prompts of 512, 1024 and 2048 tokens (one,
+// two and four tiles of 128 rows a workgroup; 32 heads of 128 columns, 8 of MXFP4 keys): 39, 87 and 242 us whole, 67, 116 and
+// 291 cut.  With fewer tiles than workgroups: one prompt of 1024, half a tile each, 43 us whole and 60 cut; four of 256 that
+// end contexts of 8192, 295 and 240.  Sequences of unlike lengths and numbers of queries, 2.5 tiles a workgroup: 237 and 214.
+constexpr int kWholeTiles = 3, kCutCost = 24;
+bool stay_whole(int64_t tiles, int64_t wanted, int64_t steps, bool unlike) {
+  if (tiles >= wanted) return !unlike || tiles >= kWholeTiles * wanted;
+  return steps * (wanted - tiles) <= kCutCost * wanted;
+}
 
 int wanted_of(int dtype, int blocks, int rows, bool many) { return kUnits * attend_groups(dtype, blocks, rows / 16 / (many ? kWaves : 1), many); }
 
@@ -211,8 +220,9 @@ Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
     if (!w.rows) continue;
     w.tiles = (ragged ? rows / w.rows + (a.B < a.T ? a.B : a.T) : a.B * ceil_div(rows, w.rows)) * c.kv_heads;
     w.groups = w.tiles;
-    if (!split || (many && w.tiles >= kWholeTiles * wanted_of(a.dtype, blocks, w.rows, many))) continue;
-    w.groups = wanted_of(a.dtype, blocks, w.rows, many);
+    const int64_t wanted = wanted_of(a.dtype, blocks, w.rows, many);
+    if (!split || (many && stay_whole(w.tiles, wanted, ceil_div(keys < seen ? keys : seen, kStep), ragged && a.B > 1))) continue;
+    w.groups = wanted;
     w.bytes = 2 * w.groups * w.rows * (32 * blocks + 2) * (int64_t)sizeof(float);
   }
   return p;

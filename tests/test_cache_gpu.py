@@ -362,6 +362,14 @@ def test_attend_pieces(cuda, lengths, n, heads, kv_heads):
         _case(len(lengths), lengths, n, heads, kv_heads, dim, page, fmt, dtype)
 
 
+@pytest.mark.parametrize("lengths", [[300, 900, 40], [31, 2000, 500]])
+@pytest.mark.parametrize("fmt, dtype, dim, window", [("MXFP4", "f32", 256, None), ("MXFP8_E4M3", "bf16", 200, 333)])
+def test_attend_many_tiles_of_unlike_sequences(cuda, fmt, dtype, dim, window, lengths):
+    """Tiles between one and three times the workgroups that take equal pieces of them."""
+    for page in (16, 12):
+        _case(lengths[1], lengths, [70, 160, 30], 256, 2, dim, page, fmt, DTYPES[dtype], ragged=True, window=window)
+
+
 def test_attend_tiny_and_large_scale_bytes(cuda):
     """Values of about 2^-100 and 2^110: no sum passes float32, and products below its smallest normal number, taken as
     zeros, would be less than half a step of bfloat16."""
