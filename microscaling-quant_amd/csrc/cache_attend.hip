@@ -19,8 +19,13 @@ MXQ_LAUNCH(launch_attend_pairs_f16)
 namespace {
 
 constexpr int64_t kMostKeys = 0x7fff0000;     // of a sequence, as its table has room for them
-constexpr int kUnits = 256, kLeast = 8;       // CUs; steps of 32 keys that a workgroup takes at least
-constexpr int kFewRows = 64;                  // rows a sequence up to which its keys are what a call costs
+constexpr int kUnits = 256;                   // CUs
+// Steps of 32 keys that a workgroup takes at least: one token's 8000 keys 19.1 us, with 4 steps 20.4, with 16 21.0.
+constexpr int kLeast = 8;
+// Rows a sequence up to which its keys are what a call costs, and tiles of few rows take them.  Eight sequences of 4096 keys
+// with 32, 64 and 128 rows of each head: 37, 43 and 58 us by tiles of few rows, 42, 52 and 62 by tiles of many; past 64 rows
+// each 32 of them read the keys again.
+constexpr int kFewRows = 64;
 
 // Whether tiles of many rows stay whole, `steps` of keys each at most.  Workgroups that take equal pieces end together, however
 // unlike the tiles are, but parts and their join cost about kCutCost steps.  Four prompts of 512, 1024 and 2048 tokens (one,
@@ -47,8 +52,11 @@ struct JoinWays {
 };
 // The rows of tiles that lie in two pieces of the line and more, from their parts' sums in the pieces' order, and zeros for
 // rows of no sequence.  A workgroup takes rows of a tile, or of the tile that a piece ends in, if that is the tile's first end
-// of a piece: sixteen lanes a row, or, of many parts, the workgroup a row, its sixteens of lanes the parts in turn.
-constexpr int kManyParts = 8;
+// of a piece: sixteen lanes a row, or the workgroup a row, its sixteens of lanes the parts in turn, whichever waits less often
+// for loads.  One token's 131072 keys of 8 heads, in 64 parts a head, take 44 us by workgroups and 55 by sixteens; prompts in
+// two to four parts a tile 67 by sixteens and 219 by workgroups.
+// It is bound by its parts' bytes where they are many (23 sequences of up to 512 tokens, 1000 parts of 128 rows of 128 columns:
+// 67 MB in 30 us) and by four loads one behind another else: 6 to 9 us.
 // Workgroups that share what there is to join, twice as many of tiles of many rows: 64 sequences' 512 tiles of 4 to 8 rows took
 // 128 us with 512 of them, 131 with 1024 and 139 with 2048 (most find nothing), prompts of 128 rows a tile 198, 193 and 198.
 constexpr int kJoins = 512;
@@ -112,8 +120,9 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
   if (runs < 2) return;
   const bool at_begin = found.at_begin;
   const int rows = u.s.n * a.group, row0 = u.row * size, last = rows - row0 < size ? rows - row0 : size;
-  const bool many = runs > kManyParts;
-  for (int r = many ? share : share * 16 + sixteen; r < last; r += many ? w.shares : w.shares * 16) {
+  const int shares = w.shares, by_rows = (last + 16 * shares - 1) / (16 * shares) * (runs / kAtOnce + 1);
+  const bool many = (last + shares - 1) / shares * (runs / (16 * kAtOnce) + 2) < by_rows;
+  for (int r = many ? share : share * 16 + sixteen; r < last; r += many ? shares : shares * 16) {
     auto part_of = [&](int i) { return w.partial + (part_slot(g0 + i, i || at_begin) * size + r) * (COLUMNS + 2); };
     float best = -__builtin_inff(), all = 0.0f, v[V];
 #pragma unroll

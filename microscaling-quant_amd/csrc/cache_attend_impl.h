@@ -1,24 +1,37 @@
-// Attention of few queries over a cache in MX formats: reading the cache is what it costs.
+// Attention over a cache in MX formats.
 //
 //   s = scale q k^T;  out = sum_i 2^(s_i log2 e - m) v_i / sum_i 2^(s_i log2 e - m),  m the running maximum
 //
-// A workgroup takes 16 rows (queries of the heads that share a head of keys) and a run of keys, its four waves 32 keys in
-// turn.  No wave waits for another before the end and nothing passes through LDS on the way: the scores are computed
-// transposed, S^T = K Q^T by mfma_f32_16x16x32_bf16, so that the lane that has four keys' scores of a query is the one whose
-// operand of out^T = V^T P^T they are.  Orders of keys and columns are free as long as both products agree on them: key
-// 16 t + 4 r + g is row 4 g + r of tile t, so that four neighbouring rows of the cache are read by one load, lane (g, c) has
-// the g-th share of a row of keys (whole blocks, 128 columns and more) and the c-th sixteenth of four rows of values,
-// whose pairs of keys v_perm puts next to each other.
+// A tile is some rows (queries, token by token, of the heads that share a head of keys) and the keys that they see, taken 32 a
+// step.  Of few rows (16 or 32 a tile) reading the cache is the cost, and the tile's four waves take its steps in turn, all with
+// the same rows, and add their sums at the end; of many (64 to 256) the matrix cores' rate and what feeds them is, and each wave
+// has rows of its own.  No wave waits for another before the end and nothing but what lanes hand each other passes through
+// LDS on the way: the scores are computed transposed, S^T = K Q^T by mfma_f32_16x16x32_bf16, so that the lane that has four
+// keys' scores of a query is the one whose operand of out^T = V^T P^T they are.  Orders of keys and columns are free as long
+// as both products agree on them: key 16 t + 4 r + g is row 4 g + r of tile t, so that four neighbouring rows of the cache are
+// read by one load, lane (g, c) has the g-th share of a row of keys (whole blocks, 128 columns and more) and the c-th sixteenth
+// of four rows of values, whose pairs of keys v_perm puts next to each other.
 // Codes become bfloat16 exactly by the scaled conversions; float16 and float32 queries and their weights are taken as the
-// sum of two and three bfloat16.
+// sum of two and three bfloat16, so that nothing of them is rounded; bfloat16 queries' weights are rounded to bfloat16, as
+// precise as their output, while their sum is of the unrounded ones.
+//
+// Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 117 us, 3.7 TB/s of the 5.2 that
+// a copy reaches, and 9 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead
+// (two and three steps ahead gained nothing), which two workgroups a CU do not keep up with the memory's latency.
+// Many rows: a prompt of 8192 tokens (32 heads on 8, 128 columns, MXFP8): 785 us, 700 TFLOP/s, of the 1350 of a large library
+// product.  Of its cycles 78% issue vector instructions (285 a step of a wave's 32 rows: 96 make bfloat16 of the codes, 16 are
+// exponentials at a quarter of the rate) and 28% the matrix cores'.  Rows that share a step's conversions are as many as
+// registers let two waves a SIMD have: twice the rows with one wave took 2450 us.  Keys and values converted once for the four
+// waves, in LDS, a barrier a step, were fewer instructions (223) and slower, 860 us, the waves waiting for each other.
 #pragma once
 
 #include "cache_common.h"
 
 namespace mxq {
 
-// PAGES16: pages of whole 16 rows that are less than 2^26 bytes apart.
-
+// PAGES16: pages of whole 16 rows that are less than 2^26 bytes apart: one page a tile of 16 keys, and a lane's place within it
+// the same in every step.  64 sequences of 4096 keys take 73 us in pages of 16 and 89 in pages of 24.
+// RT: sixteens of rows a wave; WR: waves with rows of their own; LINE: a piece of the line of tiles, not a tile by its number.
 template <int FAM, int DT, int NB, bool PAGES16, int RT, int WR, bool LINE>
 __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) void k_attend(AttendArgs a) {
   constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
