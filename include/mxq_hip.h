@@ -579,10 +579,10 @@ int mxq_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_
 typedef struct mxq_attend_spec {
   int32_t dtype;        /* of q and out, MXQ_DT_* */
   int32_t causal;
-  float scale;          /* positive, of q k^T */
+  float scale;          /* positive and 2^127 at most, of q k^T */
   int64_t T, B, heads;  /* queries, sequences, heads of q (a multiple of kv_heads) */
   int64_t q_token, q_head;          /* q's strides in elements; columns next to each other */
-  int64_t table_pages, table_row;   /* pages a sequence may have, and elements between the table's rows */
+  int64_t table_pages, table_row;   /* pages a sequence may have (2^31 - 2^16 keys), elements between the table's rows */
   int64_t window;       /* keys a query sees back from its own position; 0: all */
 } mxq_attend_spec;
 

@@ -29,9 +29,9 @@ constexpr int kFewRows = 64;
 
 // Whether tiles of many rows stay whole, `steps` of keys each at most.  Workgroups that take equal pieces end together, however
 // unlike the tiles are, but parts and their join cost about kCutCost steps.  Four prompts of 512, 1024 and 2048 tokens (one,
-// two and four tiles of 128 rows a workgroup; 32 heads of 128 columns, 8 of MXFP4 keys): 39, 87 and 242 us whole, 67, 116 and
-// 291 cut.  With fewer tiles than workgroups: one prompt of 1024, half a tile each, 43 us whole and 60 cut; four of 256 that
-// end contexts of 8192, 295 and 240.  Sequences of unlike lengths and numbers of queries, 2.5 tiles a workgroup: 237 and 214.
+// two and four tiles of 128 rows a workgroup; 32 heads of 128 columns, 8 of MXFP4 keys): 39, 86 and 242 us whole, 68, 116 and
+// 292 cut.  With fewer tiles than workgroups: one prompt of 1024, half a tile each, 43 us whole and 60 cut; four of 256 that
+// end contexts of 8192, 295 and 240.  Sequences of unlike lengths and numbers of queries, 2.5 tiles a workgroup: 198 and 182.
 constexpr int kWholeTiles = 3, kCutCost = 24;
 bool stay_whole(int64_t tiles, int64_t wanted, int64_t steps, bool unlike) {
   if (tiles >= wanted) return !unlike || tiles >= kWholeTiles * wanted;
@@ -56,7 +56,7 @@ struct JoinWays {
 // for loads.  One token's 131072 keys of 8 heads, in 64 parts a head, take 44 us by workgroups and 55 by sixteens; prompts in
 // two to four parts a tile 67 by sixteens and 219 by workgroups.
 // It is bound by its parts' bytes where they are many (23 sequences of up to 512 tokens, 1000 parts of 128 rows of 128 columns:
-// 67 MB in 30 us) and by four loads one behind another else: 6 to 9 us.
+// 67 MB in 20 us) and by four loads one behind another else: 6 to 9 us.
 // Workgroups that share what there is to join, twice as many of tiles of many rows: 64 sequences' 512 tiles of 4 to 8 rows took
 // 128 us with 512 of them, 131 with 1024 and 139 with 2048 (most find nothing), prompts of 128 rows a tile 198, 193 and 198.
 constexpr int kJoins = 512;
