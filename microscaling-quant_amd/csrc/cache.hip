@@ -317,7 +317,7 @@ RowsArgs rows_args(const mxq_cache_spec* c, const void* slots, int32_t wide, uin
    : a.c.format == MXQ_FMT_E5M2 ? MXQ_EACH_TYPE(KERNEL, kE5M2, FEW)           \
                                 : MXQ_EACH_TYPE(KERNEL, kPairs, FEW))
 
-// Tokens in launches of at most `most`, one behind another.
+// Tokens in launches of at most `most` (2^26: 2^31 threads, half of what a launch can have), one behind another.
 template <typename Kernel> int launch_rows(RowsArgs a, Kernel one, Kernel many, int64_t T, int64_t most, hipStream_t st, const char* who) {
   for (int64_t first = 0; first < T; first += most) {
     a.first = first, a.T = T - first < most ? T : first + most;
@@ -354,5 +354,5 @@ extern "C" int mxq_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, c
   RowsArgs a = rows_args(cache, slots, slots_wide, const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(k_scales), const_cast<uint8_t*>(v_codes),
                          const_cast<uint8_t*>(v_scales));
   a.k_out = k, a.v_out = v;
-  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_read, true), MXQ_EACH_FORMAT(k_cache_read, false), T, 1 << 27, as_stream(stream), "mxq_cache_read");
+  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_read, true), MXQ_EACH_FORMAT(k_cache_read, false), T, 1 << 26, as_stream(stream), "mxq_cache_read");
 }

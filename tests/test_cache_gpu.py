@@ -227,6 +227,18 @@ def test_read_every_code_and_scale(cuda, fmt):
                                    want.nan_to_num(nan=12345.0, posinf=math.inf, neginf=-math.inf)), out
 
 
+def test_read_more_rows_than_a_launch(cuda):
+    """2^27 rows of one column and some more: several launches of as many threads as one may have."""
+    gen = _gen(5)
+    cache = _filled(gen, 8, 16, 1, 1, "MXFP8_E4M3")
+    T = 2 ** 27 + 5
+    slots = torch.randint(0, 128, (T,), dtype=torch.int32, device="cuda", generator=gen)
+    slots[-1] = 128
+    for got, want in zip(nn.cache_read(cache, slots, torch.bfloat16), oc.rows(cache, torch.arange(128, device="cuda"))):
+        want = torch.cat([want.bfloat16().flatten(), torch.zeros(1, dtype=torch.bfloat16, device="cuda")])
+        assert torch.equal(got.flatten(), want[slots])
+
+
 def test_slots_of_64_bits_and_none(cuda):
     cache = _filled(_gen(1), 4, 8, 2, 64, "MXFP4")
     before = [t.clone() for t in cache[:4]]
