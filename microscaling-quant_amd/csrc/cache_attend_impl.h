@@ -58,8 +58,8 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
     if (line.groups == a.wanted) piece = (int)(blockIdx.x & 7) * (a.wanted >> 3) + (int)(blockIdx.x >> 3);
     at = line.begin(piece), end_at = line.begin(piece + 1), unit = line.unit;
   }
+  Tile u = tile_of(a, ROWS, member(a, lane, ROWS, unit), unit, at, !LINE);
   for (bool first_part = true;; first_part = false) {
-  const Tile u = tile_of(a, ROWS, member(a, lane, ROWS, unit), unit, at, !LINE);
   if (u.b < 0) return;
   // this piece's share of the tile's weight
   const int64_t share_from = LINE ? at - u.first : 0, share_to = LINE && end_at - u.first < u.weight ? end_at - u.first : u.weight;
@@ -517,6 +517,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   if constexpr (!LINE) return;
   at = u.first + u.weight;
   if (at >= end_at) return;
+  u = next_tile(a, ROWS, unit, u);
   }
 }
 

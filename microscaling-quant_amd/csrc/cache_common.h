@@ -278,6 +278,30 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int size, const Mem
   }
   return Tile{-1, 0, 0, 0, 1, {}};
 }
+// The tile behind a tile on the line.
+__device__ __forceinline__ Tile next_tile(const AttendArgs& a, int size, double unit, const Tile& u) {
+  const int lane = threadIdx.x & 63, B = (int)a.a.B;
+  Tile v = u;
+  v.first = u.first + u.weight;
+  Weights w = member(a, u.b, size, unit).w;
+  if (u.row + 1 < w.tiles) {
+    ++v.row;
+  } else if (u.head + 1 < (int)a.c.kv_heads) {
+    ++v.head, v.row = 0;
+  } else {
+    v.b = -1, v.head = v.row = 0;
+    for (int b0 = u.b + 1; b0 < B && v.b < 0; b0 += 64) {
+      const uint64_t found = __ballot(member(a, b0 + lane, size, unit).w.tiles > 0);
+      if (found) v.b = b0 + __builtin_ctzll(found);
+    }
+    if (v.b < 0) return v;
+    const Member m = member(a, v.b, size, unit);
+    v.s = Sequence{same(m.s.start), same(m.s.n), same(m.s.length), same(m.s.lo), same(m.s.hi)};
+    w = m.w;
+  }
+  v.weight = same(w.of(v.row));
+  return v;
+}
 // Of `steps` those before a share of a tile's weight.
 __device__ __forceinline__ int steps_before(int steps, int64_t share, int64_t weight) {
   if (share >= weight) return steps;
