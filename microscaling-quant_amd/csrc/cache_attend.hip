@@ -33,6 +33,10 @@ constexpr int kFewRows = 64;
 // 292 cut.  With fewer tiles than workgroups: one prompt of 1024, half a tile each, 43 us whole and 60 cut; four of 256 that
 // end contexts of 8192, 295 and 240.  Sequences of unlike lengths and numbers of queries, 2.5 tiles a workgroup: 198 and 182.
 constexpr int kWholeTiles = 3, kCutCost = 24;
+// Sequences up to which each workgroup of a whole tile looks for it among all of them, 64 at once; with more, workgroups take
+// pieces of the line, and find the tile behind one where it is.  2048 sequences of 128 tokens: 2.0 ms, and 8.6 of whole tiles;
+// 128 of 128: 0.17 and 0.18; 4096 sequences' tokens over 200 keys: 0.75 and 2.3; but 128 of them 34 us and 21 of whole tiles.
+constexpr int kLookFew = 256, kLookMany = 64;
 bool stay_whole(int64_t tiles, int64_t wanted, int64_t steps, bool unlike) {
   if (tiles >= wanted) return !unlike || tiles >= kWholeTiles * wanted;
   return steps * (wanted - tiles) <= kCutCost * wanted;
@@ -227,10 +231,14 @@ Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
   for (int many = 0; many < 2; ++many) {
     Way& w = p.way[many];
     if (!w.rows) continue;
-    w.tiles = (ragged ? rows / w.rows + (a.B < a.T ? a.B : a.T) : a.B * ceil_div(rows, w.rows)) * c.kv_heads;
+    // of sequences that may go this way, each with a tile that is not full
+    const int64_t most = many ? rows / (p.limit + 1) : a.T, sequences = most < a.B ? most : a.B;
+    w.tiles = ragged ? rows / w.rows + sequences : a.B * ceil_div(rows, w.rows);
+    if (ragged && !many && w.tiles > a.B * ceil_div(p.limit, w.rows)) w.tiles = a.B * ceil_div(p.limit, w.rows);
+    w.tiles *= c.kv_heads;
     w.groups = w.tiles;
     const int64_t wanted = wanted_of(a.dtype, blocks, w.rows, many);
-    if (!split || (many && stay_whole(w.tiles, wanted, ceil_div(keys < seen ? keys : seen, kStep), ragged && a.B > 1))) continue;
+    if (a.B <= (many ? kLookMany : kLookFew) && (!split || (many && stay_whole(w.tiles, wanted, ceil_div(keys < seen ? keys : seen, kStep), ragged && a.B > 1)))) continue;
     w.groups = wanted;
     w.bytes = 2 * w.groups * w.rows * (32 * blocks + 2) * (int64_t)sizeof(float);
   }

@@ -394,6 +394,15 @@ def test_attend_tiny_and_large_scale_bytes(cuda):
             _attend(q, cache, torch.arange(9, dtype=torch.int32, device="cuda")[None], _i32([140]))
 
 
+@pytest.mark.parametrize("B, n", [(64, 3), (65, 3), (70, 20), (256, 1), (257, 1), (600, 2)])
+def test_attend_sequences_of_short_contexts(cuda, B, n):
+    """Contexts too short to be cut, of as many sequences as are looked through for a tile and of more; ragged ones of one
+    query and of many in turn."""
+    lengths = [(29 * i) % 100 for i in range(B)]
+    _case(B, lengths, n, 8, 2, 64, 16, "MXFP4", torch.bfloat16)
+    _case(B, lengths, [1 if i % 5 else 17 * (i % 3) for i in range(B)], 8, 2, 96, 24, "MXFP8_E4M3", torch.float16, ragged=True)
+
+
 @pytest.mark.parametrize("size", [1e-3, 30.0, 3000.0])
 def test_attend_score_sizes(cuda, size):
     """Nearly even weights, and scores so far apart that one key has all the weight."""
