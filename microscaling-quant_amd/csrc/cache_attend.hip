@@ -27,20 +27,25 @@ constexpr int kLeast = 8;
 // each 32 of them read the keys again.
 constexpr int kFewRows = 64;
 
-// Whether tiles of many rows stay whole, `steps` of keys each at most.  Workgroups that take equal pieces end together, however
-// unlike the tiles are, but parts and their join cost about kCutCost steps.  Four prompts of 512, 1024 and 2048 tokens (one,
-// two and four tiles of 128 rows a workgroup; 32 heads of 128 columns, 8 of MXFP4 keys): 39, 86 and 242 us whole, 68, 116 and
-// 292 cut.  With fewer tiles than workgroups: one prompt of 1024, half a tile each, 43 us whole and 60 cut; four of 256 that
-// end contexts of 8192, 295 and 240.  Sequences of unlike lengths and numbers of queries, 2.5 tiles a workgroup: 198 and 182.
-constexpr int kWholeTiles = 3, kCutCost = 24;
+// Whether tiles stay whole, `steps` of keys each at most.  Workgroups that take equal pieces end together, however unlike the
+// tiles are, but parts and their join cost about as long as kCutFew or kCutMany steps.
+// Many rows: four prompts of 512, 1024 and 2048 tokens (one, two and four tiles of 128 rows a workgroup; 32 heads of 128
+// columns, 8 of MXFP4 keys): 39, 86 and 242 us whole, 68, 116 and 292 cut.  With fewer tiles than workgroups: one prompt of
+// 1024, half a tile each, 43 us whole and 60 cut; four of 256 that end contexts of 8192, 295 and 240.  Sequences of unlike
+// lengths and numbers of queries, 2.5 tiles a workgroup: 198 and 182.
+// Few rows, one token of each sequence, the same heads: one sequence of 500, 1500 and 3000 keys 11, 18 and 29 us whole, 18, 19
+// and 20 cut; 16 of 1000, 2000 and 3000 15, 25 and 33, and 24, 27 and 30; 48 of 2000 and 3000 30 and 40, and 43 and 51.  Past
+// twice that many steps one sequence's length could make whole tiles the slower ones by more than cutting costs.
+constexpr int kWholeTiles = 3, kCutMany = 24, kCutFew = 56;
+bool stay_whole(bool many, int64_t tiles, int64_t wanted, int64_t steps, bool unlike) {
+  if (!many) return steps <= 2 * kCutFew && steps * (wanted - (unlike ? 0 : tiles)) <= kCutFew * wanted;
+  if (tiles >= wanted) return !unlike || tiles >= kWholeTiles * wanted;
+  return steps * (wanted - tiles) <= kCutMany * wanted;
+}
 // Sequences up to which each workgroup of a whole tile looks for it among all of them, 64 at once; with more, workgroups take
 // pieces of the line, and find the tile behind one where it is.  2048 sequences of 128 tokens: 2.0 ms, and 8.6 of whole tiles;
 // 128 of 128: 0.17 and 0.18; 4096 sequences' tokens over 200 keys: 0.75 and 2.3; but 128 of them 34 us and 21 of whole tiles.
 constexpr int kLookFew = 256, kLookMany = 64;
-bool stay_whole(int64_t tiles, int64_t wanted, int64_t steps, bool unlike) {
-  if (tiles >= wanted) return !unlike || tiles >= kWholeTiles * wanted;
-  return steps * (wanted - tiles) <= kCutCost * wanted;
-}
 
 int wanted_of(int dtype, int blocks, int rows, bool many) { return kUnits * attend_groups(dtype, blocks, rows / 16 / (many ? kWaves : 1), many); }
 
@@ -227,7 +232,6 @@ Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
   if (least <= kFewRows) p.limit = kFewRows, p.way[0].rows = least <= 16 || blocks == 8 ? 16 : 32;
   if (rows > p.limit) p.way[1].rows = 16 * kWaves * attend_rows(a.dtype, blocks);
   const int64_t keys = a.table_pages * c.page_size, seen = a.window && a.window < keys ? a.window + n : keys;
-  const bool split = (keys < seen ? keys : seen) > (int64_t)(kLeast - 1) * kStep;    // a sequence may have keys for it
   for (int many = 0; many < 2; ++many) {
     Way& w = p.way[many];
     if (!w.rows) continue;
@@ -238,7 +242,7 @@ Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
     w.tiles *= c.kv_heads;
     w.groups = w.tiles;
     const int64_t wanted = wanted_of(a.dtype, blocks, w.rows, many);
-    if (a.B <= (many ? kLookMany : kLookFew) && (!split || (many && stay_whole(w.tiles, wanted, ceil_div(keys < seen ? keys : seen, kStep), ragged && a.B > 1)))) continue;
+    if (a.B <= (many ? kLookMany : kLookFew) && stay_whole(many, w.tiles, wanted, ceil_div(keys < seen ? keys : seen, kStep), ragged && a.B > 1)) continue;
     w.groups = wanted;
     w.bytes = 2 * w.groups * w.rows * (32 * blocks + 2) * (int64_t)sizeof(float);
   }

@@ -365,9 +365,10 @@ def test_attend_tiles_enough_to_stay_whole(cuda, fmt, dtype, dim, n, heads, ragg
 
 
 @pytest.mark.parametrize("lengths, n, heads, kv_heads", [
-    ([(61 * i) % 997 for i in range(100)], 1, 2, 1),              # tiles of their own pieces, more sequences than a wave has lanes
-    ([(61 * i) % 997 for i in range(100)], 3, 8, 4),              # equal pieces of the line, parts of two tiles and more each
+    ([(61 * i) % 997 for i in range(100)], 1, 2, 1),              # more sequences than a wave has lanes
+    ([(61 * i) % 997 for i in range(100)], 3, 8, 4),
     ([(61 * i) % 997 for i in range(330)], 1, 2, 2),
+    ([(331 * i) % 3700 + 300 for i in range(40)], 1, 16, 8), ([(331 * i) % 3900 for i in range(100)], 2, 8, 4),    # longer, the same
     ([2500], 700, 1, 1), ([1100, 700], 350, 6, 3)])               # prompts: tiles that weigh more and more
 def test_attend_pieces(cuda, lengths, n, heads, kv_heads):
     for fmt, dim, page, dtype in (("MXFP4", 64, 16, torch.bfloat16), ("MXFP8_E4M3", 128, 20, torch.float16)):
