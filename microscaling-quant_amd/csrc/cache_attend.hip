@@ -47,7 +47,7 @@ bool stay_whole(bool many, int64_t tiles, int64_t wanted, int64_t steps, bool un
 // 128 of 128: 0.17 and 0.18; 4096 sequences' tokens over 200 keys: 0.75 and 2.3; but 128 of them 34 us and 21 of whole tiles.
 constexpr int kLookFew = 256, kLookMany = 64;
 
-int wanted_of(int dtype, int blocks, int rows, bool many) { return kUnits * attend_groups(dtype, blocks, rows / 16 / (many ? kWaves : 1), many); }
+int wanted_of(int dtype, int blocks, int rows, bool many) { return kUnits * attend_groups(dtype, blocks, rows / 16 / (many ? kWaves : 1)); }
 
 // What differs between the two ways that a call's sequences are taken.
 struct JoinWay {
@@ -59,8 +59,7 @@ struct JoinWay {
 struct JoinWays {
   JoinWay way[2];
 };
-// The rows of tiles that lie in two pieces of the line and more, from their parts' sums in the pieces' order, and zeros for
-// rows of no sequence.  A workgroup takes rows of a tile, or of the tile that a piece ends in, if that is the tile's first end
+// The rows of tiles that lie in two pieces of the line and more, from their parts' sums in the pieces' order.  A workgroup takes rows of a tile, or of the tile that a piece ends in, if that is the tile's first end
 // of a piece: sixteen lanes a row, or the workgroup a row, its sixteens of lanes the parts in turn, whichever waits less often
 // for loads.  One token's 131072 keys of 8 heads, in 64 parts a head, take 44 us by workgroups and 55 by sixteens; prompts in
 // two to four parts a tile 67 by sixteens and 219 by workgroups.
@@ -80,7 +79,7 @@ template <int V> __device__ __forceinline__ void add_part(float& all, float (&v)
   for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
 }
 template <int COLUMNS>
-__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways, bool empty_rows) {
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways) {
   constexpr int V = COLUMNS / 16;
   __shared__ float sums[16][COLUMNS];
   __shared__ float weights[16], maxima[16];
@@ -91,23 +90,13 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
   };
   __shared__ Found found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim, c = lane & 15, sixteen = threadIdx.x >> 4;
-  if (empty_rows) {
-    // queries [0, starts[0]) and [starts[B], T) are no sequence's
-    const int T = (int)a.a.T, x = a.a.B ? a.starts[0] : T, y = a.a.B ? a.starts[a.a.B] : T;
-    const int64_t head = (int64_t)(x < 0 ? 0 : x > T ? T : x) * a.a.heads, tail = (int64_t)(y < 0 ? 0 : y > T ? T : y) * a.a.heads;
-    const int64_t from = tail < head ? head : tail, all = head + (a.a.T * a.a.heads - from);
-    for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < all; i += (int64_t)gridDim.x * 4) {
-      const int64_t row = i < head ? i : from + i - head;
-      for (int d = lane; d < D; d += 64) store_elem(a.out, a.a.dtype, row * D + d, 0.0f);
-      if (a.lse && lane == 0) a.lse[row] = -__builtin_inff();
-    }
-  }
   const int first_way = ways.way[0].places * ways.way[0].shares, which = (int)blockIdx.x >= first_way;
   const JoinWay& w = ways.way[which];
   const int index = (int)blockIdx.x - (which ? first_way : 0);
   if (index >= w.places * w.shares) return;
   const int share = index / w.places, place = index - share * w.places, size = w.size;
   a.above = w.above, a.upto = w.upto, a.wanted = w.wanted;
+  if (a.fill) fill_rows(a);
   // one wave finds the tile: what it takes to find it is most of what a workgroup computes
   if (wave == 0) {
     Member own = member(a, lane, size, 0.0);
@@ -194,6 +183,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
   }
 }
 
+__global__ __launch_bounds__(256) void k_attend_none(AttendArgs a) { fill_rows(a); }
+
 int check(const mxq_cache_spec* c, const mxq_attend_spec* a) {
   const std::string who = "mxq_cache_attend";
   if (!c || !a) return invalid(who + ": NULL spec");
@@ -229,6 +220,8 @@ Plan plan_of(const mxq_cache_spec& c, const mxq_attend_spec& a, bool ragged) {
   const int64_t group = a.heads / c.kv_heads, n = ragged ? a.T : a.T / a.B, rows = n * group, least = ragged ? group : rows;
   const int blocks = blocks_class((c.head_dim + 31) / 32);
   Plan p = {};
+  // 32 rows share a step's conversions and loads: 64 sequences of 4096 keys with 32 rows a head take 91 us so and 126 by 16 rows
+  // a tile, but eight of them, which do not fill the card, 37 and 34.
   if (least <= kFewRows) p.limit = kFewRows, p.way[0].rows = least <= 16 || blocks == 8 ? 16 : 32;
   if (rows > p.limit) p.way[1].rows = 16 * kWaves * attend_rows(a.dtype, blocks);
   const int64_t keys = a.table_pages * c.page_size, seen = a.window && a.window < keys ? a.window + n : keys;
@@ -282,14 +275,20 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   hipStream_t st = as_stream(stream);
   a.least = kLeast;
   const Plan p = spec->B ? plan_of(*cache, *spec, starts != nullptr) : Plan{};
-  if (p.way[0].bytes + p.way[1].bytes && !workspace) return invalid("mxq_cache_attend: NULL workspace");
+  const bool cut = p.way[0].bytes || p.way[1].bytes;
+  if (cut && !workspace) return invalid("mxq_cache_attend: NULL workspace");
   for (const Way& w : p.way)
-    if (w.tiles * 64 * kWaves > kMaxThreads) return invalid("mxq_cache_attend: too many tiles for a launch");
+    if (w.groups * 64 * kWaves > kMaxThreads) return invalid("mxq_cache_attend: too many tiles for a launch");
   const int blocks = blocks_class(a.blocks);
   constexpr decltype(&launch_attend_e4m3_f32) launches[3][3] = {{launch_attend_e4m3_f32, launch_attend_e4m3_bf16, launch_attend_e4m3_f16},
                                                                 {launch_attend_e5m2_f32, launch_attend_e5m2_bf16, launch_attend_e5m2_f16},
                                                                 {launch_attend_pairs_f32, launch_attend_pairs_bf16, launch_attend_pairs_f16}};
   const auto launch = launches[cache->format == MXQ_FMT_E4M3 ? 0 : cache->format == MXQ_FMT_E5M2 ? 1 : 2][spec->dtype];
+  a.fill = starts && !cut;
+  if (!spec->B) {
+    k_attend_none<<<dim3(blocks_for(ceil_div(spec->T * spec->heads, 64))), 256, 0, st>>>(a);
+    return check_launch("mxq_cache_attend");
+  }
   JoinWays ways = {};
   int64_t joins = 0;
   char* work = (char*)workspace;
@@ -302,6 +301,7 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
     a.wanted = wanted_of(spec->dtype, blocks, w.rows, many);
     launch(a, many, w.rows == 32, w.groups, st);
     if (int rc = check_launch("mxq_cache_attend")) return rc;
+    a.fill = 0;
     if (!a.partial) continue;
     const bool by_tile = w.tiles <= a.wanted;
     const int places = by_tile ? (int)w.tiles : a.wanted, most = many ? w.rows / 16 : 16, spare = (many ? 2 : 1) * kJoins / places;
@@ -309,10 +309,10 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
     ways.way[many] = JoinWay{a.partial, a.above, a.upto, a.wanted, w.rows, places, shares, by_tile};
     joins += places * shares;
   }
-  if (joins || starts) {
-    const unsigned groups = joins ? (unsigned)joins : blocks_for(ceil_div(spec->T * spec->heads, 64));
+  if (joins) {
+    a.fill = starts != nullptr;
     const auto join = blocks == 2 ? k_attend_join<64> : blocks == 4 ? k_attend_join<128> : k_attend_join<256>;
-    join<<<dim3(groups), 256, 0, st>>>(a, ways, starts != nullptr);
+    join<<<dim3((unsigned)joins), 256, 0, st>>>(a, ways);
     return check_launch("mxq_cache_attend");
   }
   return MXQ_OK;

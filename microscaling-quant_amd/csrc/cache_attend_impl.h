@@ -15,10 +15,10 @@
 // sum of two and three bfloat16, so that nothing of them is rounded; bfloat16 queries' weights are rounded to bfloat16, as
 // precise as their output, while their sum is of the unrounded ones.
 //
-// Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 117 us, 3.7 TB/s of the 5.2 that
-// a copy reaches, and 9 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead
+// Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 110 us, 3.9 TB/s of the 5.2 that
+// a copy reaches, and 8 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead
 // (two and three steps ahead gained nothing), which two workgroups a CU do not keep up with the memory's latency.
-// Many rows: a prompt of 8192 tokens (32 heads on 8, 128 columns, MXFP8): 785 us, 700 TFLOP/s, of the 1350 of a large library
+// Many rows: a prompt of 8192 tokens (32 heads on 8, 128 columns, MXFP8): 782 us, 700 TFLOP/s, of the 1350 of a large library
 // product.  Of its cycles 78% issue vector instructions (285 a step of a wave's 32 rows: 96 make bfloat16 of the codes, 16 are
 // exponentials at a quarter of the rate) and 28% the matrix cores'.  Rows that share a step's conversions are as many as
 // registers let two waves a SIMD have: twice the rows with one wave took 2450 us.  Keys and values converted once for the four
@@ -30,10 +30,10 @@
 namespace mxq {
 
 // PAGES16: pages of whole 16 rows that are less than 2^26 bytes apart: one page a tile of 16 keys, and a lane's place within it
-// the same in every step.  64 sequences of 4096 keys take 73 us in pages of 16 and 89 in pages of 24.
+// the same in every step.  64 sequences of 4096 keys take 72 us in pages of 16 and 85 in pages of 24.
 // RT: sixteens of rows a wave; WR: waves with rows of their own; LINE: a piece of the line of tiles, not a tile by its number.
 template <int FAM, int DT, int NB, bool PAGES16, int RT, int WR, bool LINE>
-__global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) void k_attend(AttendArgs a) {
+__global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_attend(AttendArgs a) {
   constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
   constexpr int KW = NB * BB / 16;                        // words of keys' codes a lane and tile of 16 keys
   constexpr int EW = FAM == kPairs ? 1 : 2;               // words of eight codes
@@ -45,6 +45,10 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT, (WR > 1))) v
   __shared__ float tops[kWaves][16], weights[kWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int D = a.c.head_dim;
+
+  if constexpr (!LINE) {
+    if (a.fill) fill_rows(a);
+  }
 
   // this workgroup's piece of the line
   int piece = blockIdx.x;

@@ -86,6 +86,7 @@ struct AttendArgs {
   int32_t aligned;       // pages of whole 16 rows, whose rows are less than 2^26 bytes apart
   int32_t wanted, least; // workgroups that fill the card, and steps that one takes at least
   int32_t above, upto;   // the numbers of rows a sequence that this launch takes: (above, upto]
+  int32_t fill;          // whether this launch writes the rows of no sequence
   float scale2;          // scale times log2 e
 };
 
@@ -115,6 +116,19 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
     s.lo = lo <= 0 ? 0 : lo < s.hi ? (int)lo : s.hi;
   }
   return s;
+}
+
+// Zeros for the queries of no sequence: [0, starts[0]) and [starts[B], T).  By all workgroups of a launch together.
+__device__ __forceinline__ void fill_rows(const AttendArgs& a) {
+  const int T = (int)a.a.T, x = a.a.B ? a.starts[0] : T, y = a.a.B ? a.starts[a.a.B] : T, D = a.c.head_dim;
+  const int64_t head = (int64_t)(x < 0 ? 0 : x > T ? T : x) * a.a.heads, tail = (int64_t)(y < 0 ? 0 : y > T ? T : y) * a.a.heads;
+  const int64_t from = tail < head ? head : tail, all = head + (a.a.T * a.a.heads - from);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  for (int64_t i = (int64_t)blockIdx.x * waves + wave; i < all; i += (int64_t)gridDim.x * waves) {
+    const int64_t row = i < head ? i : from + i - head;
+    for (int d = lane; d < D; d += 64) store_elem(a.out, a.a.dtype, row * D + d, 0.0f);
+    if (a.lse && lane == 0) a.lse[row] = -__builtin_inff();
+  }
 }
 
 // How the work is cut.  A tile is `size` rows of one head of keys (queries token by token, the heads that share it within).  A
@@ -315,11 +329,9 @@ constexpr int kWaves = 4;
 // Sixteens of rows that a wave of many queries has: as many as let two waves share a SIMD's registers (of float32's three
 // planes half as many).
 constexpr int attend_rows(int dtype, int blocks) { return blocks == 8 ? 1 : dtype == MXQ_DT_F32 ? 4 / blocks : 8 / blocks; }
-// Workgroups a CU (of a wave for each of its SIMDs) that the registers are held to.
-constexpr int attend_groups(int dtype, int blocks, int tiles, bool many) {
-  if (!many && tiles == 1 && blocks == 2) return 3;
-  return dtype == MXQ_DT_BF16 || tiles * blocks < 8 ? 2 : 1;
-}
+// Workgroups a CU (of a wave for each of its SIMDs) that the registers are held to; with sixteen rows of 64 columns, where three
+// would nearly fit, 64 sequences' 512 and 1024 tiles took 55 and 92 us of three, 51 and 97 of two.
+constexpr int attend_groups(int dtype, int blocks, int tiles) { return dtype == MXQ_DT_BF16 || tiles * blocks < 8 ? 2 : 1; }
 constexpr int blocks_class(int blocks) { return blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8; }
 
 // The logarithm of a sum of weights relative to 2^top; of no weights -inf.

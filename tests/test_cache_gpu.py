@@ -464,6 +464,19 @@ def test_attend_rows_of_no_sequence(cuda):
     assert (out == 0).all() and (lse == -math.inf).all()
 
 
+def test_attend_rows_of_no_sequence_beside_cut_tiles(cuda):
+    """The same where sequences are long enough to be cut and joined."""
+    gen = _gen(18)
+    cache = _filled(gen, 600, 16, 2, 64, "MXFP4")
+    lengths = [8000, 30, 500]
+    table = _table(gen, lengths, 16, 600)
+    q = torch.randn(90, 8, 64, generator=gen, device="cuda").bfloat16()
+    for starts in ([3, 20, 31, 32], [0, 70, 71, 85], [5, 5, 6, 89]):
+        out, lse = _attend(q, cache, table, _i32(lengths), _i32(starts))
+        assert (out[:starts[0]] == 0).all() and (out[starts[3]:] == 0).all()
+        assert (lse[:starts[0]] == -math.inf).all() and (lse[starts[3]:] == -math.inf).all()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("n, group", [(1, 1), (6, 2), (70, 2), (150, 4)])
 def test_attend_nan_and_infinity_behind_the_mask(cuda, n, group, fmt):
