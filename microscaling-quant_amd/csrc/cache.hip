@@ -318,13 +318,17 @@ RowsArgs rows_args(const mxq_cache_spec* c, const void* slots, int32_t wide, uin
                                 : MXQ_EACH_TYPE(KERNEL, kPairs, FEW))
 
 // Tokens in launches of at most `most` (2^26: 2^31 threads, half of what a launch can have), one behind another.
-template <typename Kernel> int launch_rows(RowsArgs a, Kernel one, Kernel many, int64_t T, int64_t most, hipStream_t st, const char* who) {
+template <typename Kernel> int launch_rows(RowsArgs a, Kernel one, Kernel many, int64_t T, int64_t most, hipStream_t st, const char* who,
+                                       const char* name) {
   for (int64_t first = 0; first < T; first += most) {
     a.first = first, a.T = T - first < most ? T : first + most;
     const int64_t n = a.T - first;
     const bool few = n <= kFewTokens;
     a.per_group = few ? 1 : (int)(ceil_div(n, 1024) < kTokens ? ceil_div(n, 1024) : kTokens);
-    (few ? one : many)<<<dim3((unsigned)ceil_div(n, a.per_group)), few ? kThreads<true> : kThreads<false>, 0, st>>>(a);
+    {
+      KernelTimer timer(name, st);
+      (few ? one : many)<<<dim3((unsigned)ceil_div(n, a.per_group)), few ? kThreads<true> : kThreads<false>, 0, st>>>(a);
+    }
     if (int rc = check_launch(who)) return rc;
   }
   return MXQ_OK;
@@ -342,7 +346,8 @@ extern "C" int mxq_cache_write(const void* k, const void* v, int32_t dtype, int6
   a.k = k, a.v = v;
   a.token[0] = k_token, a.token[1] = v_token, a.head[0] = k_head, a.head[1] = v_head;
   // A launch looks through its own later tokens for each of its slots; launches follow one another.
-  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_write, true), MXQ_EACH_FORMAT(k_cache_write, false), T, 1 << 15, as_stream(stream), "mxq_cache_write");
+  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_write, true), MXQ_EACH_FORMAT(k_cache_write, false), T, 1 << 15, as_stream(stream), "mxq_cache_write",
+                     "k_cache_write");
 }
 
 extern "C" int mxq_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes, const uint8_t* v_scales,
@@ -354,5 +359,6 @@ extern "C" int mxq_cache_read(const uint8_t* k_codes, const uint8_t* k_scales, c
   RowsArgs a = rows_args(cache, slots, slots_wide, const_cast<uint8_t*>(k_codes), const_cast<uint8_t*>(k_scales), const_cast<uint8_t*>(v_codes),
                          const_cast<uint8_t*>(v_scales));
   a.k_out = k, a.v_out = v;
-  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_read, true), MXQ_EACH_FORMAT(k_cache_read, false), T, 1 << 26, as_stream(stream), "mxq_cache_read");
+  return launch_rows(a, MXQ_EACH_FORMAT(k_cache_read, true), MXQ_EACH_FORMAT(k_cache_read, false), T, 1 << 26, as_stream(stream), "mxq_cache_read",
+                     "k_cache_read");
 }

@@ -286,6 +286,7 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   const auto launch = launches[cache->format == MXQ_FMT_E4M3 ? 0 : cache->format == MXQ_FMT_E5M2 ? 1 : 2][spec->dtype];
   a.fill = starts && !cut;
   if (!spec->B) {
+    KernelTimer timer("k_attend_none", st);
     k_attend_none<<<dim3(blocks_for(ceil_div(spec->T * spec->heads, 64))), 256, 0, st>>>(a);
     return check_launch("mxq_cache_attend");
   }
@@ -299,7 +300,10 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
     work += w.bytes;
     a.above = many ? p.limit : 0, a.upto = many ? 0x7fffffff : p.limit;
     a.wanted = wanted_of(spec->dtype, blocks, w.rows, many);
-    launch(a, many, w.rows == 32, w.groups, st);
+    {
+      KernelTimer timer("k_attend", st);
+      launch(a, many, w.rows == 32, w.groups, st);
+    }
     if (int rc = check_launch("mxq_cache_attend")) return rc;
     a.fill = 0;
     if (!a.partial) continue;
@@ -312,6 +316,7 @@ extern "C" int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uin
   if (joins) {
     a.fill = starts != nullptr;
     const auto join = blocks == 2 ? k_attend_join<64> : blocks == 4 ? k_attend_join<128> : k_attend_join<256>;
+    KernelTimer timer("k_attend_join", st);
     join<<<dim3((unsigned)joins), 256, 0, st>>>(a, ways);
     return check_launch("mxq_cache_attend");
   }

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from mxq import nn, packed
+from mxq import _lib, nn, packed
 from oracle import cache as oc
 
 pytestmark = pytest.mark.gpu
@@ -652,6 +652,28 @@ def test_generation_captured_in_a_graph(cuda):
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
             for a, b in zip(other, cache[:4]):
                 assert torch.equal(a, b)
+
+
+def test_launches_are_timed(cuda):
+    """The library's timers see a launch for each of a call's kernels: whole tiles in one, cut ones joined."""
+    gen = _gen(19)
+    cache = _filled(gen, 600, 16, 2, 64, "MXFP4")
+    names = ("k_cache_write", "k_cache_read", "k_attend", "k_attend_join", "k_attend_none")
+    q = torch.randn(2, 4, 64, generator=gen, device="cuda").bfloat16()
+    slots = torch.arange(3, device="cuda")
+    _lib.timer_enable(True)
+    try:
+        for name in names:
+            _lib.timer_read(name)
+        nn.cache_write(*nn.cache_read(cache, slots), cache, slots)
+        for length, starts in ((100, None), (9000, None), (100, [0, 1, 1])):
+            nn.cache_attend(q[:, None] if starts is None else q, cache, _table(gen, [length, 1], 16, 600), _i32([length, 1]),
+                            None if starts is None else _i32(starts))
+        nn.cache_attend(q, cache, _i32([]).view(0, 3), _i32([]), _i32([0]))
+        got = {name: _lib.timer_read(name)[1] for name in names}
+    finally:
+        _lib.timer_enable(False)
+    assert got == {"k_cache_write": 1, "k_cache_read": 1, "k_attend": 3, "k_attend_join": 1, "k_attend_none": 1}
 
 
 def test_other_stream(cuda):
