@@ -296,7 +296,11 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
     if cache.k_codes.device != dev:                             # a cache in host memory
         return cache_attend(q, _there(cache, dev), table, lengths, starts, scale=scale, causal=causal, window=window,
                             return_lse=return_lse)
-    qd, td, ld = _lib.to_device(qd, dev), _lib.to_device(td, dev), _lib.to_device(lengths, dev).contiguous()
+    if q.device != dev or table.device != dev:                  # a view's copy has strides of its own: the spec is of the copy
+        got = cache_attend(_lib.to_device(q, dev), cache, _lib.to_device(table, dev), lengths, starts, scale=scale,
+                           causal=causal, window=window, return_lse=return_lse)
+        return tuple(_lib.back(t, q) for t in got) if return_lse else _lib.back(got, q)
+    ld = _lib.to_device(lengths, dev).contiguous()
     sd = None if starts is None else _lib.to_device(starts, dev).contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
@@ -305,6 +309,4 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
         _lib.run("mxq_cache_attend", qd.data_ptr(), cache.k_codes.data_ptr(), cache.k_scales.data_ptr(),
                  cache.v_codes.data_ptr(), cache.v_scales.data_ptr(), spec, td.data_ptr(), ld.data_ptr(), _lib.ptr(sd),
                  out.data_ptr(), _lib.ptr(lse), att, _lib.ptr(work), _lib.stream(dev))
-    if out.device != q.device:
-        out, lse = _lib.back(out, q), None if lse is None else _lib.back(lse, q)
     return (out, lse) if return_lse else out

@@ -297,6 +297,32 @@ def test_host_tensors(cuda):
     assert out.device.type == "cpu" and torch.equal(out, nn.cache_attend(q, here, *args).cpu())
 
 
+@pytest.mark.parametrize("here", [True, False])
+def test_host_views(cuda, here):
+    """Queries and tables that are views of larger tensors in host memory, with a cache on the GPU and one beside them."""
+    gen = _gen(21)
+    cache = _filled(gen, 30, 16, 2, 40, "MXFP8_E4M3")
+    wide = torch.randn(3, 5, 12, 45, generator=gen, device="cuda").bfloat16()
+    tables = torch.randint(0, 30, (6, 40), generator=gen, device="cuda").int()
+    lengths = torch.tensor([160, 9, 77, 3, 50, 33], device="cuda").int()[::2]
+    starts = torch.tensor([0, 9, 1, 9, 4, 9, 5], device="cuda").int()[::2]
+    taken = cache if here else nn.PackedCache(*(t.cpu() for t in cache[:4]), *cache[4:])
+    queries = (lambda w: (w[..., 3:7, 5:], None), lambda w: (w[:, 2:3, :4, :40], None), lambda w: (w[..., :1, :40].expand(3, 5, 4, 40), None),
+               lambda w: (w[0, :, 4:8, :40], True), lambda w: (w[1, :, ::3, 5:], True), lambda w: (w[:, 0, :1, :40].expand(3, 4, 40), True))
+    for cut in queries:
+        for part in (lambda t: t[:3, 4:14], lambda t: t[::2, 20:], lambda t: t[:10, :3].t(), lambda t: t[:1, 7:17].expand(3, 10)):
+            (q, ragged), table, of = cut(wide), part(tables), None
+            host, args = cut(wide.cpu())[0], [taken, part(tables.cpu()), lengths.cpu()]
+            if ragged:
+                of, args = starts, [*args, starts.cpu()]
+            assert table.shape[0] == 3
+            want, want_lse = nn.cache_attend(q.contiguous(), cache, table.contiguous(), lengths, of, return_lse=True)
+            out, lse = nn.cache_attend(host, *args, return_lse=True)
+            assert out.device.type == lse.device.type == "cpu" and torch.equal(out.cuda(), want) and torch.equal(lse.cuda(), want_lse)
+            assert torch.equal(nn.cache_attend(q, *args), want)
+            assert torch.equal(nn.cache_attend(host, cache, table, lengths, of).cuda(), want)
+
+
 # ---------------------------------------------------------------------------------------------------- attention
 
 @pytest.mark.parametrize("fmt", FORMATS)

@@ -180,3 +180,35 @@ def test_workspace():
         dtype=1, causal=1, scale=1.0, T=4, B=4, heads=8, table_pages=1000, table_row=1000), **change}), ragged)
     assert size(table_pages=14) == 0 and size(T=0) == 0 and size(window=200) == 0
     assert 0 < size() == size(T=8) == size(T=40, B=40) <= 64 << 20
+
+
+@pytest.mark.parametrize("here", [False, True])
+def test_strides_are_of_what_the_call_reads(monkeypatch, here):
+    """A view is laid out anew by its copy to the call's device: the spec has the strides of the tensors whose memory the
+    call is given.  The meta device stands for the GPU; nothing runs."""
+    dev, read, called = torch.device("meta"), [], []
+    monkeypatch.setattr(_lib, "compute_device", lambda *tensors: dev)
+    monkeypatch.setattr(_lib, "stream", lambda dev: 0)
+    monkeypatch.setattr(_lib, "back", lambda t, like: t)
+    monkeypatch.setattr(_lib, "run", lambda name, *args: called.append(args))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: read.append(t) or len(read) - 1, raising=False)
+    cache = nn.packed_cache(9, 16, 2, 40, "MXFP4", device="meta" if here else "cpu")
+    wide = torch.zeros(3, 5, 12, 45)
+    queries = ((wide[..., 3:7, 5:], None), (wide[:, 1:3, :4, :40], None), (wide[:, 2:3, :4, :40], None),
+               (wide[:1, :, :2, :40].expand(3, 5, 2, 40), None), (wide[..., :1, :40].expand(3, 5, 4, 40), None),
+               (wide[0, :, 4:8, :40], _i32(4)), (wide[0, ::2, ::3, 5:], _i32(4)), (wide[0, :, :1, :40].expand(5, 4, 40), _i32(4)))
+    tables = (_i32(3, 9)[:, 2:6], _i32(3, 9)[:, ::2], _i32(4, 3).t(), _i32(1, 4).expand(3, 4), _i32(6, 4)[::2], _i32(3, 4))
+    for q, starts in queries:
+        for table in tables:
+            for q_here, table_here in ((False, False), (True, False), (False, True)):
+                read.clear(), called.clear()
+                out = nn.cache_attend(q.to(dev) if q_here else q, cache, table.to(dev) if table_here else table, _i32(3), starts)
+                (args,) = called
+                assert out.shape == q.shape and all(t.device == dev for t in read)
+                qd, td, spec = read[args[0]], read[args[6]], args[11]
+                assert qd.shape == q.shape and td.shape == table.shape
+                assert qd.stride(-1) == 1 and spec.q_head == qd.stride(-2) and td.stride(1) == 1 and spec.table_row == td.stride(0)
+                if starts is not None or q.shape[1] > 1:
+                    assert spec.q_token == qd.stride(-3) and (starts is not None or qd.stride(0) == q.shape[1] * qd.stride(1))
+                else:
+                    assert spec.q_token == qd.stride(0)
