@@ -69,14 +69,15 @@ struct JoinWays {
 // 128 us with 512 of them, 131 with 1024 and 139 with 2048 (most find nothing), prompts of 128 rows a tile 198, 193 and 198.
 constexpr int kJoins = 512;
 constexpr int kAtOnce = 4;                    // parts asked for together
-// Sums of weights and of values relative to 2^best, and those of a part relative to its own maximum, `best` at most.
+// Sums of weights and of values relative to 2^best, and those of a part relative to its own maximum, `best` at most.  A part
+// that has seen no key has sums of zero; any other's are taken with a factor of zero too, so that NaN of a value stays NaN.
 template <int V> __device__ __forceinline__ void add_part(float& all, float (&v)[V], float top, float weight, float best, const float (&x)[V]) {
   // a part without a maximum has seen no key, or only scores of NaN, which its sum is then
   const bool none = top == -__builtin_inff();
   const float factor = none ? weight : __builtin_amdgcn_exp2f(top - best);
   all += none ? weight : factor * weight;
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] += factor == 0.0f ? 0.0f : factor * x[k];
+  for (int k = 0; k < V; ++k) v[k] += factor * x[k];
 }
 template <int COLUMNS>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways) {
@@ -142,9 +143,10 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, JoinWays ways
       const float keep = best == now ? 1.0f : __builtin_amdgcn_exp2f(best - now);
       all *= keep;
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = keep == 0.0f ? 0.0f : keep * v[k];
+      for (int k = 0; k < V; ++k) v[k] = keep * v[k];
 #pragma unroll
-      for (int u = 0; u < kAtOnce; ++u) add_part(all, v, tops[u], weight[u], now, x[u]);
+      for (int u = 0; u < kAtOnce; ++u)
+        if (i0 + u * by < runs) add_part(all, v, tops[u], weight[u], now, x[u]);
       best = now;
     }
     if (many) {

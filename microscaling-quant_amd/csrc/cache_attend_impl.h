@@ -503,7 +503,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
 #pragma unroll
         for (int w = 0; w < WK; ++w)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] += factor[w] == 0.0f ? 0.0f : factor[w] * sums[w][r][d + k];
+          for (int k = 0; k < 4; ++k) v[k] += factor[w] * sums[w][r][d + k];    // a factor of zero too: NaN stays NaN
         if (!whole) {
           __builtin_memcpy(part + d, v, 16);
         } else if (d < D) {

@@ -561,6 +561,46 @@ def test_attend_infinite_values_behind_the_mask(cuda):
         assert (~torch.isfinite(out[0, n - 1])).any(-1).all()
 
 
+@pytest.mark.parametrize("keys, n, heads, joined", [
+    (300, 1, 4, False), (300, 1, 40, False), (300, 70, 4, False),        # tiles that stay whole, of few and of many rows
+    (20000, 1, 4, True), (20000, 4, 12, True), (9000, 100, 4, True)])    # cut ones, joined row by row and all at once
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_attend_nan_and_infinity_of_no_weight(cuda, dtype, keys, n, heads, joined):
+    """A value that is no finite number, under a score so low that its weight is zero: seen all the same, in whichever wave
+    or part of a tile the largest score is.  Other columns are the best key's value exactly, all other weights being zero."""
+    gen = _gen(22)
+    for fmt, dim, page in (("MXFP8_E5M2", 128, 16), ("MXFP4", 64, 24), ("MXFP8_E4M3", 200, 32)):
+        cache = _filled(gen, -(-keys // page), page, 1, dim, fmt)
+        table, slots = torch.arange(cache.k_codes.shape[0], device="cuda").int()[None], torch.arange(keys, device="cuda")
+        q = torch.zeros(1, n, heads, dim, dtype=DTYPES[dtype], device="cuda")
+        q[..., 0] = 1
+        for best, bad in ((0, keys - 1), (keys - 1, 0), (40, 41), (keys // 2, 100), (100, keys // 2), (70, 35), (keys // 3, 2 * keys // 3)):
+            v = nn.cache_read(cache, slots, torch.float32)[1]
+            k = torch.zeros_like(v)
+            k[:, 0, 0] = -192
+            k[best] = 0
+            nn.cache_write(k, v, cache, slots)
+            v = nn.cache_read(cache, slots, torch.float32)[1]
+            where = (bad // page, 0, bad % page)
+            scales, codes = cache.v_scales[where].clone(), cache.v_codes[where].clone()
+            cache.v_scales[where + (1,)] = 255
+            if fmt == "MXFP8_E5M2":
+                cache.v_codes[where + (0,)] = 0x7C
+            _lib.timer_enable(True)
+            try:
+                _lib.timer_read("k_attend_join")
+                out, lse = nn.cache_attend(q, cache, table, _i32([keys]), scale=1.0, causal=False, return_lse=True)
+                assert (_lib.timer_read("k_attend_join")[1] > 0) == joined
+            finally:
+                _lib.timer_enable(False)
+            cache.v_scales[where], cache.v_codes[where] = scales, codes
+            finite = torch.ones(dim, dtype=torch.bool, device="cuda")
+            finite[32:64] = False
+            finite[0] = fmt != "MXFP8_E5M2"
+            assert (~torch.isfinite(out[..., ~finite])).all(), (fmt, best, bad)
+            assert (out == v[best, 0].to(q.dtype))[..., finite].all() and (lse == 0).all(), (fmt, best, bad)
+
+
 def test_attend_strides(cuda):
     gen = _gen(12)
     cache = _filled(gen, 9, 16, 2, 72, "MXFP8_E4M3")
