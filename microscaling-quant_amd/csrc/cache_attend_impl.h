@@ -25,6 +25,8 @@
 // waves, in LDS, a barrier a step, were fewer instructions (223) and slower, 860 us, the waves waiting for each other.
 #pragma once
 
+#include <type_traits>
+
 #include "cache_common.h"
 
 namespace mxq {
@@ -308,18 +310,34 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) vsc[i] = scale_from(ahead, 16 * (i >> 2) + 4 * (i & 3) + g, vblock);
+      auto scores = [&](auto lower_finite) {
 #pragma unroll
-      for (int m = 0; m < RT; ++m) z[m][0] = z[m][1] = f32x4{0, 0, 0, 0};
+        for (int m = 0; m < RT; ++m) z[m][0] = z[m][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+        for (int i = 0; i < NB; ++i) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const bf16x8 k = eight_codes<FAM>(&kw[t][i * EW], scale_field(ksc[t][NB == 8 ? i >> 2 : 0]));
+          for (int t = 0; t < 2; ++t) {
+            const bf16x8 k = eight_codes<FAM>(&kw[t][i * EW], scale_field(ksc[t][NB == 8 ? i >> 2 : 0]));
+            bf16x8 lower = k;
+            if constexpr (decltype(lower_finite)::value) finite_only(lower);
 #pragma unroll
-          for (int m = 0; m < RT; ++m)
+            for (int m = 0; m < RT; ++m)
 #pragma unroll
-            for (int p = P - 1; p >= 0; --p) z[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[m][p][i], z[m][t], 0, 0, 0);
+              for (int p = P - 1; p >= 0; --p) z[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p ? lower : k, q[m][p][i], z[m][t], 0, 0, 0);
+          }
         }
+      };
+      scores(std::false_type{});
+      // A query's lower planes are zero where it has no more bits, and zero times an infinite key is NaN: where some score is
+      // one, the scores are taken again with the first plane alone meeting infinities.  (Looking at the scores costs four
+      // comparisons for 16 rows, looking at the keys some four instructions for each word of codes.)
+      if constexpr (P > 1) {
+        bool none = false;
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) none |= __builtin_isunordered(z[m][i >> 2][i & 3], z[m][i >> 2][(i & 3) + 1]);
+        if (__builtin_expect(__any(none), 0)) scores(std::true_type{});
       }
     }
     Places next{};

@@ -601,6 +601,53 @@ def test_attend_nan_and_infinity_of_no_weight(cuda, dtype, keys, n, heads, joine
             assert (out == v[best, 0].to(q.dtype))[..., finite].all() and (lse == 0).all(), (fmt, best, bad)
 
 
+@pytest.mark.parametrize("fmt, code, scale", [("MXFP8_E5M2", 0x7C, 120), ("MXFP8_E5M2", 0x7B, 254), ("MXFP8_E4M3", 0x7E, 247), ("MXFP4", 7, 253)])
+@pytest.mark.parametrize("n, heads", [(1, 4), (5, 12), (100, 4)])
+def test_attend_infinite_keys(cuda, n, heads, fmt, code, scale):
+    """Keys that are infinite, by their code or by their scale, under queries of few bits and of a type's most: scores of -inf
+    have no weight, nothing but them gives zeros, and a score of +inf or of zero times infinity gives no number."""
+    gen = _gen(23)
+    sign = 8 if fmt == "MXFP4" else 0x80
+    for dtype in DTYPES.values():
+        for dim, page, pages in ((64, 16, 6), (128, 24, 4), (200, 16, 320)):
+            cache = _filled(gen, pages, page, 1, dim, fmt)
+            table, lengths = torch.arange(pages, device="cuda").int()[None], _i32([pages * page - 3])
+            q = torch.randn(1, n, heads, dim, generator=gen, device="cuda")
+            q[..., 33], q[..., 1] = q[..., 33].abs() + 1, 0
+            q[:, :, ::2] = q[:, :, ::2].to(torch.float8_e4m3fn).float()
+            q = q.to(dtype)
+
+            def infinite(of, column, negative=False):
+                """The keys of some pages infinite in this column, zero in the rest of its block."""
+                c = torch.zeros(32, dtype=torch.int32, device="cuda")
+                c[column % 32] = code | (sign if negative else 0)
+                c = (c if fmt != "MXFP4" else c[0::2] | c[1::2] << 4).to(torch.uint8)
+                block = column // 32
+                cache.k_codes[of, :, :, block * len(c):(block + 1) * len(c)] = c
+                cache.k_scales[of, :, :, block] = scale
+
+            def call():
+                return nn.cache_attend(q, cache, table, lengths, causal=False, return_lse=True)
+
+            few = torch.tensor([1, pages - 1], device="cuda")
+            others = table.clone()
+            others[0, few] = -1
+            want, want_lse, bound, lse_bound = oc.attend(q, cache, others, lengths, causal=False)
+            infinite(few, 33, negative=True)
+            out, lse = call()
+            _check(out, want, bound, (dtype, dim))
+            _check(lse, want_lse, lse_bound, (dtype, dim))
+            infinite(few[:1], 33)
+            assert torch.isnan(call()[0]).all()
+            cache.k_codes[few[:1]] = 0
+            infinite(few[:1], 1)
+            assert torch.isnan(call()[0]).all()
+            cache.k_codes.zero_()
+            infinite(slice(None), 33, negative=True)
+            out, lse = call()
+            assert (out == 0).all() and (lse == -math.inf).all(), (dtype, dim)
+
+
 def test_attend_strides(cuda):
     gen = _gen(12)
     cache = _filled(gen, 9, 16, 2, 72, "MXFP8_E4M3")
