@@ -11,9 +11,10 @@
 // as both products agree on them: key 16 t + 4 r + g is row 4 g + r of tile t, so that four neighbouring rows of the cache are
 // read by one load, lane (g, c) has the g-th share of a row of keys (whole blocks, 128 columns and more) and the c-th sixteenth
 // of four rows of values, whose pairs of keys v_perm puts next to each other.
-// Codes become bfloat16 exactly by the scaled conversions; float16 and float32 queries and their weights are taken as the
-// sum of two and three bfloat16, so that nothing of them is rounded; bfloat16 queries' weights are rounded to bfloat16, as
-// precise as their output, while their sum is of the unrounded ones.
+// Codes become bfloat16 exactly by the scaled conversions, and float16 and float32 queries are taken as the sum of two and three
+// bfloat16, so that the products are exact.  Weights are taken as the same number of bfloat16: those of float32 queries whole,
+// those of float16 ones to 2^-15, a sixteenth of their output's rounding, and bfloat16 queries' rounded to bfloat16, as
+// precise as their output.  Each goes to the nearest, and their sum is of the unrounded ones.
 //
 // Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 110 us, 3.9 TB/s of the 5.2 that
 // a copy reaches, and 8 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead

@@ -342,31 +342,26 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
 
 template <int DT> constexpr int kAttendPlanes = DT == MXQ_DT_BF16 ? 1 : DT == MXQ_DT_F16 ? 2 : 3;
 
-// Eight float32 as bfloat16 planes, each the leading bits of what the ones before leave: three hold all of a float32 down
-// to 2^-133, two hold a float16.  A single plane is rounded to the nearest.
+// Eight float32 as bfloat16 planes, each the leading bits of what the ones before leave, the last one rounded to the nearest:
+// three hold all of a float32 down to 2^-133, two all of a float16, and all but 2^-15 of a weight.
 template <int P> __device__ __forceinline__ void planes_of(float (&f)[8], bf16x8 (&out)[P]) {
-  if constexpr (P == 1) {
-    bf16x2 w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = bf16x2{(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
-    __builtin_memcpy(&out[0], w, 16);
-  } else {
+  for (int p = 0; p + 1 < P; ++p) {
+    uint32_t w[4];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      uint32_t w[4];
+    for (int i = 0; i < 4; ++i)
+      w[i] = __builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302u);
+    __builtin_memcpy(&out[p], w, 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = __builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302u);
-      __builtin_memcpy(&out[p], w, 16);
-      if (p + 1 < P) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float hi = __uint_as_float(__float_as_uint(f[i]) & 0xFFFF0000u);
-          f[i] = f[i] == hi ? 0.0f : f[i] - hi;                          // infinities leave nothing
-        }
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float hi = __uint_as_float(__float_as_uint(f[i]) & 0xFFFF0000u);
+      f[i] = f[i] == hi ? 0.0f : f[i] - hi;                              // infinities leave nothing
     }
   }
+  bf16x2 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = bf16x2{(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
+  __builtin_memcpy(&out[P - 1], w, 16);
 }
 
 // Eight neighbouring columns of a row of q as planes, the first `valid` of them there.

@@ -34,8 +34,9 @@ def rows(cache, slots):
 
 
 #: how far a weight of bfloat16, float16 and float32 queries may be from exp's value by its rounding alone: half a step of
-#: bfloat16, two bfloat16 of eight bits each cut off, three, which hold all of a float32
-ROUNDED = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -14, torch.float32: 0.0}
+#: bfloat16; two bfloat16, the leading eight bits, which leave less than 2^-7 of the weight, and what they leave to the
+#: nearest; three, which hold all of a float32
+ROUNDED = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -15, torch.float32: 0.0}
 
 
 def attend(q, cache, table, lengths, starts=None, scale=None, causal=True, window=None):

@@ -438,6 +438,25 @@ def test_attend_score_sizes(cuda, size):
         _case(n, [400, 33], n, 4, 2, 64, 16, "MXFP4", torch.float32, size=size, scale=0.3)
 
 
+@pytest.mark.parametrize("B, n, heads", [(1024, 1, 16), (1, 128, 128)])
+def test_attend_float16_weights_are_rounded_to_the_nearest(cuda, B, n, heads):
+    """Values of 1 and -1 under weights of 1 and exp(-t), t to 2^-6, are tanh(t / 2), small enough for float16 to show the
+    weight's own error: that of a weight's two bfloat16 is 2^-17 at most here (a weight in [1/2, 1) is eight bits and a
+    remainder below 2^-8, whose half step is 2^-17 at most), as often up as down, and half of it the output's, beside the output's
+    rounding, 2^-19 at most.  The mean of 16384 errors is then within 6 / 128 of 2^-18 + 2^-19, and 4 units of float32 for
+    exp2, its argument and the quotient, which may lean one way: below 2^-20 together.  Weights cut off instead lean by
+    2/3 2^-17, half of it the output's: 2^-18.6."""
+    t = (torch.rand(B, n, heads, generator=_gen(24), device="cuda") * 2.0 ** -6).half()
+    q = torch.zeros(B, n, heads, 32, dtype=torch.float16, device="cuda")
+    q[..., 0] = t
+    cache = nn.packed_cache(1, 2, 1, 32, "MXFP8_E4M3")
+    k, v = torch.zeros(2, 1, 32, device="cuda"), torch.ones(2, 1, 32, device="cuda")
+    k[1, 0, 0], v[1] = -1, -1
+    nn.cache_write(k, v, cache, torch.arange(2, device="cuda"))
+    out = nn.cache_attend(q, cache, _i32([[0]]).expand(B, 1), _i32([2]).expand(B), scale=1.0, causal=False)
+    assert t.numel() == 16384 and abs(float((out[..., 0].double() - torch.tanh(t.double() / 2)).mean())) <= 2.0 ** -20
+
+
 def test_attend_rising_scores(cuda):
     """Each key larger than the one before: the maximum moves in every step."""
     gen = _gen(7)
