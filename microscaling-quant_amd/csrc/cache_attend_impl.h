@@ -12,9 +12,9 @@
 // read by one load, lane (g, c) has the g-th share of a row of keys (whole blocks, 128 columns and more) and the c-th sixteenth
 // of four rows of values, whose pairs of keys v_perm puts next to each other.
 // Codes become bfloat16 exactly by the scaled conversions, and float16 and float32 queries are taken as the sum of two and three
-// bfloat16, so that the products are exact.  Weights are taken as the same number of bfloat16: those of float32 queries whole,
-// those of float16 ones to 2^-15, a sixteenth of their output's rounding, and bfloat16 queries' rounded to bfloat16, as
-// precise as their output.  Each goes to the nearest, and their sum is of the unrounded ones.
+// bfloat16, so that the products are exact.  Weights are taken as three bfloat16 of float32 queries, which is all of them, and as
+// two, all but 2^-16 of them, of others; of bfloat16 queries in tiles of many rows as one, as precise as their output
+// (weight_planes_of).  The sum of weights is of the unrounded ones.
 //
 // Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 110 us, 3.9 TB/s of the 5.2 that
 // a copy reaches, and 8 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead
@@ -37,7 +37,7 @@ namespace mxq {
 // RT: sixteens of rows a wave; WR: waves with rows of their own; LINE: a piece of the line of tiles, not a tile by its number.
 template <int FAM, int DT, int NB, bool PAGES16, int RT, int WR, bool LINE>
 __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_attend(AttendArgs a) {
-  constexpr int P = kAttendPlanes<DT>, BB = FAM == kPairs ? 16 : 32;
+  constexpr int P = kAttendPlanes<DT>, PW = weight_planes_of(DT, WR > 1), BB = FAM == kPairs ? 16 : 32;
   constexpr int KW = NB * BB / 16;                        // words of keys' codes a lane and tile of 16 keys
   constexpr int EW = FAM == kPairs ? 1 : 2;               // words of eight codes
   constexpr int VB = NB * BB / 16, VW = VB / 4 < EW ? EW : VB / 4;   // bytes and words of values' codes a lane and key
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
           for (int r = 0; r < 4; ++r) o[m][t][r] *= factor;
       }
     }
-    bf16x8 pw[RT][P];
+    bf16x8 pw[RT][PW];
 #pragma unroll
     for (int m = 0; m < RT; ++m) {
       const float less = top[m] == -__builtin_inff() ? 0.0f : -top[m];
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
         w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[m][i >> 2][i & 3], a.scale2, less));
         total[m] += w[i];
       }
-      planes_of(w, pw[m]);
+      weight_planes(w, pw[m]);
     }
 
     // Zero times infinity is no zero.  Where a key is hidden from some query, values that are no finite number are taken out,
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
 #pragma unroll
         for (int m = 0; m < RT; ++m)
 #pragma unroll
-          for (int p = P - 1; p >= 0; --p) o[m][2 * j + half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw[m][p], o[m][2 * j + half], 0, 0, 0);
+          for (int p = PW - 1; p >= 0; --p) o[m][2 * j + half] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pw[m][p], o[m][2 * j + half], 0, 0, 0);
       }
     }
     if (more) load_values(ahead, next);

@@ -340,10 +340,16 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
   return top == -__builtin_inff() ? sum : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
 }
 
-template <int DT> constexpr int kAttendPlanes = DT == MXQ_DT_BF16 ? 1 : DT == MXQ_DT_F16 ? 2 : 3;
+template <int DT> constexpr int kAttendPlanes = DT == MXQ_DT_BF16 ? 1 : DT == MXQ_DT_F16 ? 2 : 3;   // of queries
+// Planes of their weights, of tiles of many rows or of few.  bfloat16 queries' weights in one plane, rounded by 2^-9 on the
+// average of each, add about as much to an output as its own rounding does; a second plane takes that away (an error of 2.6
+// thousandths becomes 1.6, one token's 1000 keys of 64 columns).  Few rows, where the cache's bytes are the cost, have it: 64
+// sequences of 4 to 8 thousand keys 112.7 us, 109.8 without; eight of 4096 with 64 rows a head 43.5 and 40.6.  Many rows, where
+// products are, do not: a prompt of 8192 would take 958 us for 802, for 1.6 thousandths instead of 2.0.
+constexpr int weight_planes_of(int dtype, bool many) { return dtype == MXQ_DT_F32 ? 3 : dtype == MXQ_DT_F16 || !many ? 2 : 1; }
 
 // Eight float32 as bfloat16 planes, each the leading bits of what the ones before leave, the last one rounded to the nearest:
-// three hold all of a float32 down to 2^-133, two all of a float16, and all but 2^-15 of a weight.
+// three hold all of a float32 down to 2^-133, two all of a float16.
 template <int P> __device__ __forceinline__ void planes_of(float (&f)[8], bf16x8 (&out)[P]) {
 #pragma unroll
   for (int p = 0; p + 1 < P; ++p) {
@@ -362,6 +368,26 @@ template <int P> __device__ __forceinline__ void planes_of(float (&f)[8], bf16x8
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = bf16x2{(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
   __builtin_memcpy(&out[P - 1], w, 16);
+}
+
+// Eight weights (finite or NaN) as bfloat16 planes: all of them in three; else each plane to the nearest, all but 2^-16 in two
+// and all but 2^-8 in one.
+template <int P> __device__ __forceinline__ void weight_planes(float (&f)[8], bf16x8 (&out)[P]) {
+  if constexpr (P == 3) {
+    planes_of(f, out);
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x2 two = {(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
+        __builtin_memcpy(&w[i], &two, 4);
+        if (p + 1 < P) f[2 * i] -= __uint_as_float(w[i] << 16), f[2 * i + 1] -= __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+      __builtin_memcpy(&out[p], w, 16);
+    }
+  }
 }
 
 // Eight neighbouring columns of a row of q as planes, the first `valid` of them there.

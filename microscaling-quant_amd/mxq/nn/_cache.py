@@ -273,8 +273,9 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
 
     Lengths are held to the table's pages and starts to T.  A key on a page that the cache does not have (-1, say) is not
     there.  A query that sees no key, or that belongs to no sequence, gets zeros and an lse of -inf; so does one whose every
-    score is -inf.  A query that sees a value that is no finite number gets no finite number in its column.  Sums are float32,
-    and the weights exp(scale q k^T - max) of bfloat16 queries are rounded to bfloat16."""
+    score is -inf.  A query that sees a value that is no finite number gets no finite number in its column.  Sums are float32;
+    the weights exp(scale q k^T - max) are held to 2^-16 (float32 queries' whole), but those of bfloat16 queries are rounded to
+    bfloat16 in a sequence of more than 64 rows (its queries times the heads that share one of keys)."""
     who = "cache_attend"
     qd = q
     if qd.ndim and qd.stride(-1) != 1 and qd.shape[-1] > 1:

@@ -34,19 +34,20 @@ def rows(cache, slots):
 
 
 #: how far a weight of bfloat16, float16 and float32 queries may be from exp's value by its rounding alone: half a step of
-#: bfloat16; two bfloat16, the leading eight bits, which leave less than 2^-7 of the weight, and what they leave to the
-#: nearest; three, which hold all of a float32
-ROUNDED = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -15, torch.float32: 0.0}
+#: bfloat16; two bfloat16, the weight to the nearest and what that leaves, 2^-8 of it at most, to the nearest; three, which
+#: hold all of a float32
+ROUNDED = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16, torch.float32: 0.0}
 
 
-def attend(q, cache, table, lengths, starts=None, scale=None, causal=True, window=None):
+def attend(q, cache, table, lengths, starts=None, scale=None, causal=True, window=None, rounded=None):
     """(out, lse, bound of out, bound of lse), float64, T x heads x D and T x heads.
 
     A score is a float32 sum of D exact products, then scaled: off by (D + 8) half steps of the sum of magnitudes.  Such an
     error e of all scores' exponents is at most 2 e of a normalised weight, beside the weight's own rounding, exp2's unit
     and the sums of L terms of numerator and denominator, joined from 64 parts at most in as many steps.  A weight is taken
     relative to a maximum that is no larger than the scores', so that the weights' sum is 1 or more, and the hardware's exp2
-    makes those below float32's smallest normal zero: 2^-126 of each value at most."""
+    makes those below float32's smallest normal zero: 2^-126 of each value at most.  rounded: the weights' rounding, where it
+    is not ROUNDED's."""
     D, G, S = cache.head_dim, cache.k_codes.shape[1], cache.page_size
     if starts is None:
         starts = [i * q.shape[1] for i in range(q.shape[0] + 1)]
@@ -83,7 +84,7 @@ def attend(q, cache, table, lengths, starts=None, scale=None, causal=True, windo
                 w = torch.exp(s - total)
                 size = scale * (x.abs() @ kk.abs().t()).amax(-1, keepdim=True)
                 e = (D + 8) * half * size + 16 * half
-                each = 2 * e + 2 * ROUNDED[q.dtype] + (2 * min(L, 4096) + 200) * half
+                each = 2 * e + 2 * (ROUNDED[q.dtype] if rounded is None else rounded) + (2 * min(L, 4096) + 200) * half
                 out[t, heads] = w @ vv
                 off[t, heads] = each * (w @ vv.abs()) + 2.0 ** -126 * vv.abs().sum(0)
                 lse[t, heads] = total[:, 0]

@@ -438,6 +438,22 @@ def test_attend_score_sizes(cuda, size):
         _case(n, [400, 33], n, 4, 2, 64, 16, "MXFP4", torch.float32, size=size, scale=0.3)
 
 
+@pytest.mark.parametrize("lengths, n, heads, kv_heads", [([40] * 30, 1, 8, 8), ([33, 60, 7], 1, 40, 4), ([50, 45], 5, 24, 2), ([45, 64], 2, 32, 2),
+                                                         ([100, 5000], 1, 8, 2)])
+@pytest.mark.parametrize("fmt, dim", [("MXFP4", 64), ("MXFP8_E4M3", 128), ("MXFP8_E5M2", 200)])
+def test_attend_weights_of_few_bfloat16_rows(cuda, fmt, dim, lengths, n, heads, kv_heads):
+    """Tiles of few rows take bfloat16 queries' weights as two bfloat16, too: within the oracle's bound for 2^-16, beside which
+    a weight rounded to bfloat16 alone would show, keys being few."""
+    gen = _gen(25)
+    pages = sum(-(-l // 16) for l in lengths)
+    cache, table = _filled(gen, pages, 16, kv_heads, dim, fmt), _table(gen, lengths, 16, pages)
+    q = torch.randn(len(lengths), n, heads, dim, generator=gen, device="cuda").bfloat16()
+    out, lse = nn.cache_attend(q, cache, table, _i32(lengths), return_lse=True)
+    want, want_lse, bound, lse_bound = oc.attend(q, cache, table, _i32(lengths), rounded=2.0 ** -16)
+    _check(out, want, bound, "out")
+    _check(lse, want_lse, lse_bound, "lse")
+
+
 @pytest.mark.parametrize("B, n, heads", [(1024, 1, 16), (1, 128, 128)])
 def test_attend_float16_weights_are_rounded_to_the_nearest(cuda, B, n, heads):
     """Values of 1 and -1 under weights of 1 and exp(-t), t to 2^-6, are tanh(t / 2), small enough for float16 to show the
