@@ -182,6 +182,24 @@ def test_workspace():
     assert 0 < size() == size(T=8) == size(T=40, B=40) <= 64 << 20
 
 
+def test_most_workspace():
+    """Of every type, width, head layout and batch: two parts of a tile for each workgroup, of 128 rows of 128 columns and of 32
+    where there are prompts and tokens in one batch, two workgroups a CU."""
+    lib, most = _lib.load(), {0: 0, 1: 0}
+    for dtype in (0, 1, 2):
+        for dim in (32, 64, 96, 128, 256):
+            for kv_heads, group in ((1, 1), (2, 8), (1, 17), (4, 32), (1, 64), (2, 65), (1, 1024)):
+                for T, B in ((4, 4), (64, 1), (8192, 1), (8192, 23), (512, 64), (600, 300), (100000, 100)):
+                    for pages in (10, 200, 8192):
+                        cache = _lib.CacheSpec(5, dim, 1 << 20, 16, kv_heads)
+                        spec = _lib.AttendSpec(dtype=dtype, causal=1, scale=1.0, T=T, B=B, heads=kv_heads * group, table_pages=pages, table_row=pages)
+                        for ragged in (0, 1):
+                            if ragged or T % B == 0:
+                                most[ragged] = max(most[ragged], lib.mxq_cache_attend_workspace(cache, spec, ragged))
+    part = lambda rows, columns: 2 * 512 * rows * (columns + 2) * 4                                # noqa: E731
+    assert most == {0: part(256, 64), 1: part(128, 128) + part(32, 128)} and most[1] < 86e6
+
+
 @pytest.mark.parametrize("here", [False, True])
 def test_strides_are_of_what_the_call_reads(monkeypatch, here):
     """A view is laid out anew by its copy to the call's device: the spec has the strides of the tensors whose memory the
