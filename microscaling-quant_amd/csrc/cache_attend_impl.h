@@ -26,8 +26,6 @@
 // waves, in LDS, a barrier a step, were fewer instructions (223) and slower, 860 us, the waves waiting for each other.
 #pragma once
 
-#include <type_traits>
-
 #include "cache_common.h"
 
 namespace mxq {
@@ -281,6 +279,38 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
     }
   };
 
+  // The scores of a step's keys once more, where one is NaN: a query's lower planes are zero where it has no more bits, and zero
+  // times an infinite key is NaN, so infinite keys meet the first plane alone, the lower ones the largest finite value.  Seldom
+  // needed, it takes the keys from memory again, eight columns at a time, so that no step holds registers for it.  Scores looked
+  // at in every step, their keys kept, took 142 us where this takes 122 (64 single float32 tokens over 4096 keys, 256 columns of
+  // E4M3) and 505 where it takes 470 (a float16 prompt of 4096, 128 columns).
+  auto scores_with_care = [&](int k0, f32x4 (&z)[RT][2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int asked = k0 + 16 * t + 4 * (c & 3) + (c >> 2), key = asked < s.length ? asked : s.length - 1, of = page_of(key);
+      const bool yes = (uint32_t)of < (uint32_t)a.c.pages;
+      const int page = yes ? of : 0, at = yes ? key - (int)divu31(key, a.by_page) * (int)a.c.page_size : 0;
+      const uint8_t *codes = kc + page * a.c.page_stride[0] + at * a.c.row_stride[0], *scales = ks + page * a.c.page_stride[1] + at * a.c.row_stride[1];
+#pragma unroll
+      for (int m = 0; m < RT; ++m) z[m][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        uint32_t w[EW] = {}, scale = 0;
+        if (q_column(i) / 32 < a.blocks) {
+          __builtin_memcpy(w, codes + q_column(i) * BB / 32, BB / 4);
+          scale = scales[q_column(i) / 32];
+        }
+        const bf16x8 k = eight_codes<FAM>(w, scale_field(scale));
+        bf16x8 lower = k;
+        finite_only(lower);
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) z[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p ? lower : k, q[m][p][i], z[m][t], 0, 0, 0);
+      }
+    }
+  };
+
   Ahead ahead;
   if (begin < end) {                                      // there is a key, and so a page of it
     if constexpr (PAGES16) find_tiles(mine);
@@ -311,34 +341,18 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) vsc[i] = scale_from(ahead, 16 * (i >> 2) + 4 * (i & 3) + g, vblock);
-      auto scores = [&](auto lower_finite) {
 #pragma unroll
-        for (int m = 0; m < RT; ++m) z[m][0] = z[m][1] = f32x4{0, 0, 0, 0};
+      for (int m = 0; m < RT; ++m) z[m][0] = z[m][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < NB; ++i) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const bf16x8 k = eight_codes<FAM>(&kw[t][i * EW], scale_field(ksc[t][NB == 8 ? i >> 2 : 0]));
-            bf16x8 lower = k;
-            if constexpr (decltype(lower_finite)::value) finite_only(lower);
+        for (int t = 0; t < 2; ++t) {
+          const bf16x8 k = eight_codes<FAM>(&kw[t][i * EW], scale_field(ksc[t][NB == 8 ? i >> 2 : 0]));
 #pragma unroll
-            for (int m = 0; m < RT; ++m)
+          for (int m = 0; m < RT; ++m)
 #pragma unroll
-              for (int p = P - 1; p >= 0; --p) z[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p ? lower : k, q[m][p][i], z[m][t], 0, 0, 0);
-          }
+            for (int p = P - 1; p >= 0; --p) z[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[m][p][i], z[m][t], 0, 0, 0);
         }
-      };
-      scores(std::false_type{});
-      // A query's lower planes are zero where it has no more bits, and zero times an infinite key is NaN: where some score is
-      // one, the scores are taken again with the first plane alone meeting infinities.  (Looking at the scores costs four
-      // comparisons for 16 rows, looking at the keys some four instructions for each word of codes.)
-      if constexpr (P > 1) {
-        bool none = false;
-#pragma unroll
-        for (int m = 0; m < RT; ++m)
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) none |= __builtin_isunordered(z[m][i >> 2][i & 3], z[m][i >> 2][(i & 3) + 1]);
-        if (__builtin_expect(__any(none), 0)) scores(std::true_type{});
       }
     }
     Places next{};
@@ -364,18 +378,36 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
         }
       }
     }
-    // The maximum follows only when a weight would pass 2^8: until then weights and sums are relative to an old one.
+    // The maximum follows only when a weight would pass 2^8: until then weights and sums are relative to an old one.  Of several
+    // planes it is NaN where a score is.
     float most[RT];
-    bool past = false;
+    auto find_most = [&] {
+      bool past = false;
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
-      most[m] = z[m][0][0];
+      for (int m = 0; m < RT; ++m) {
+        most[m] = z[m][0][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) most[m] = __builtin_fmaxf(most[m], z[m][i >> 2][i & 3]);
-      most[m] *= a.scale2;
-      past |= most[m] > top[m] + 8.0f;
-    }
-    if (__any(past)) {
+        for (int i = 1; i < 8; ++i)
+          most[m] = P > 1 ? __builtin_elementwise_maximum(most[m], z[m][i >> 2][i & 3]) : __builtin_fmaxf(most[m], z[m][i >> 2][i & 3]);
+        most[m] *= a.scale2;
+        past |= P > 1 ? !(most[m] <= top[m] + 8.0f) : most[m] > top[m] + 8.0f;
+      }
+      return __any(past);
+    };
+    if (find_most()) {
+      if constexpr (P > 1) {
+        bool none = false;
+#pragma unroll
+        for (int m = 0; m < RT; ++m) none |= most[m] != most[m];
+        if (__builtin_expect(__any(none), 0)) {
+          scores_with_care(k0, z);
+#pragma unroll
+          for (int m = 0; m < RT; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[m][i >> 2][i & 3] = seen[m] >> i & 1 ? z[m][i >> 2][i & 3] : -__builtin_inff();
+          find_most();
+        }
+      }
 #pragma unroll
       for (int m = 0; m < RT; ++m) {
         most[m] = __builtin_fmaxf(most[m], __shfl_xor(most[m], 16));
