@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * kWaves, attend_groups(DT, NB, RT)) void k_atte
       if constexpr (P > 1) {
         bool none = false;
 #pragma unroll
-        for (int m = 0; m < RT; ++m) none |= most[m] != most[m];
+        for (int m = 0; m < RT; ++m) none |= most[m] != most[m] && total[m] == total[m];   // a row that is NaN already stays it
         if (__builtin_expect(__any(none), 0)) {
           scores_with_care(k0, z);
 #pragma unroll

@@ -683,6 +683,26 @@ def test_attend_infinite_keys(cuda, n, heads, fmt, code, scale):
             assert (out == 0).all() and (lse == -math.inf).all(), (dtype, dim)
 
 
+@pytest.mark.parametrize("n, heads", [(3, 4), (7, 12), (100, 4)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_attend_queries_that_are_no_numbers(cuda, dtype, n, heads):
+    """A NaN or an infinity in one query makes its own row NaN, and no other."""
+    gen = _gen(26)
+    for fmt, dim, page, keys in (("MXFP8_E4M3", 64, 16, 200), ("MXFP4", 128, 24, 200), ("MXFP8_E5M2", 200, 16, 6000)):
+        cache = _filled(gen, -(-keys // page), page, 1, dim, fmt)
+        cache.k_codes[..., 0] = {"MXFP8_E4M3": 0x38, "MXFP8_E5M2": 0x3C, "MXFP4": 0x22}[fmt]      # no key is zero where they are
+        table, lengths = torch.arange(cache.k_codes.shape[0], device="cuda").int()[None], _i32([keys])
+        q = torch.randn(1, n, heads, dim, generator=gen, device="cuda").to(DTYPES[dtype])
+        want, want_lse, bound, lse_bound = oc.attend(q, cache, table, lengths)
+        bad = torch.zeros(n, heads, dtype=torch.bool, device="cuda")
+        bad[0, 1] = bad[n // 2, 0] = bad[n - 1, heads - 1] = True
+        q[0, 0, 1, 0], q[0, n // 2, 0, 0], q[0, n - 1, heads - 1, 0] = math.nan, math.inf, math.nan
+        out, lse = nn.cache_attend(q, cache, table, lengths, return_lse=True)
+        assert torch.isnan(out[0, bad]).all() and torch.isnan(lse[0, bad]).all()
+        _check(out[0, ~bad], want[0, ~bad], bound[0, ~bad], (fmt, dim))
+        _check(lse[0, ~bad], want_lse[0, ~bad], lse_bound[0, ~bad], (fmt, dim))
+
+
 def test_attend_strides(cuda):
     gen = _gen(12)
     cache = _filled(gen, 9, 16, 2, 72, "MXFP8_E4M3")
