@@ -247,7 +247,8 @@ def _attend_spec(key, q_shape, q_dtype, q_strides, table, table_row, lengths, st
         raise ValueError(f"mxq.nn.cache_attend: q must have {B} sequences, as table has, got shape {tuple(q_shape)}")
     if window is not None:
         _whole(window, who, "window", 1, _MOST)
-    if not 0.0 < scale <= 2.0 ** 127:
+    scale = D ** -0.5 if scale is None else scale
+    if not 0.0 < _lib.c_f32(scale).value <= 2.0 ** 127:                        # as the kernels take it
         raise ValueError(f"mxq.nn.cache_attend: scale must be positive, and 2^127 at most, got {scale}")
     if pages * spec.page_size > _MOST_KEYS:
         raise ValueError(f"mxq.nn.cache_attend: {pages} pages of {spec.page_size} keys a sequence are more than {_MOST_KEYS}")
@@ -269,7 +270,7 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
     one.  table (B x pages, at most 2^31 - 2^16 keys; int32) names each sequence's pages and lengths (B, int32) says how many keys it has, its newest
     tokens', written before, among them.  The last query is at the last key; query j of n is at position
     p = lengths[b] - n + j.  causal: it sees keys up to p; window: from p - window + 1 on.  scale (head_dim ** -0.5 by default)
-    must be positive, and 2^127 at most.
+    must be positive as a float32, and 2^127 at most.
 
     Lengths are held to the table's pages and starts to T.  A key on a page that the cache does not have (-1, say) is not
     there.  A query that sees no key, or that belongs to no sequence, gets zeros and an lse of -inf; so does one whose every
@@ -289,9 +290,9 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
         strides = (qd.stride(0), strides[1])
     td = table if table.ndim != 2 or table.shape[1] < 2 or table.stride(1) == 1 else table.contiguous()
     spec, att, size = _attend_spec(
-        _key(cache, who), q.shape, q.dtype, strides, (table.shape, table.dtype), td.stride(0) if td.ndim == 2 else 0,
-        (lengths.shape, lengths.dtype), None if starts is None else (starts.shape, starts.dtype),
-        cache.head_dim ** -0.5 if scale is None else float(scale), bool(causal), window)
+        _key(cache, who), q.shape, q.dtype, strides, (table.shape, table.dtype),
+        td.stride(0) if td.ndim == 2 else 0, (lengths.shape, lengths.dtype),
+        None if starts is None else (starts.shape, starts.dtype), None if scale is None else float(scale), bool(causal), window)
     _no_grad(who, q)
     dev = _device(cache, who, q)
     if cache.k_codes.device != dev:                             # a cache in host memory

@@ -107,6 +107,17 @@ def test_cache_attend_refuses(change, error, text):
         nn.cache_attend(**args)
 
 
+@pytest.mark.parametrize("change, text", [
+    (dict(cache=_cache()._replace(head_dim=0)), "head_dim must be"),            # before its default scale, 0 to a negative power
+    (dict(cache=_cache()._replace(head_dim="40")), "head_dim must be"),
+    (dict(scale=1e-50), "scale must be positive"),                              # zero as a float32
+    (dict(scale=1e300), "scale must be positive"),
+    (dict(scale=-1.0), "scale must be positive")])
+def test_cache_attend_refuses_by_its_own_errors(change, text):
+    with pytest.raises(ValueError, match=text):
+        nn.cache_attend(**{**dict(q=torch.zeros(3, 1, 6, 40), cache=_cache(), table=_i32(3, 2), lengths=_i32(3)), **change})
+
+
 def test_forward_mode_tangents_are_refused():
     dual = lambda *shape: forward_ad.make_dual(torch.zeros(shape), torch.ones(shape))         # noqa: E731
     plain = torch.zeros
