@@ -288,10 +288,10 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
     strides = qd.stride()[-3:-1]
     if qd.ndim == 4 and qd.shape[1] == 1:
         strides = (qd.stride(0), strides[1])
-    td = table if table.ndim != 2 or table.shape[1] < 2 or table.stride(1) == 1 else table.contiguous()
+    rows = table.ndim != 2 or table.shape[1] < 2 or table.stride(1) == 1       # a row's pages lie next to each other
     spec, att, size = _attend_spec(
         _key(cache, who), q.shape, q.dtype, strides, (table.shape, table.dtype),
-        td.stride(0) if td.ndim == 2 else 0, (lengths.shape, lengths.dtype),
+        0 if table.ndim != 2 else table.stride(0) if rows else table.shape[1], (lengths.shape, lengths.dtype),
         None if starts is None else (starts.shape, starts.dtype), None if scale is None else float(scale), bool(causal), window)
     _no_grad(who, q)
     dev = _device(cache, who, q)
@@ -302,7 +302,7 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
         got = cache_attend(_lib.to_device(q, dev), cache, _lib.to_device(table, dev), lengths, starts, scale=scale,
                            causal=causal, window=window, return_lse=return_lse)
         return tuple(_lib.back(t, q) for t in got) if return_lse else _lib.back(got, q)
-    ld = _lib.to_device(lengths, dev).contiguous()
+    td, ld = table if rows else table.contiguous(), _lib.to_device(lengths, dev).contiguous()
     sd = None if starts is None else _lib.to_device(starts, dev).contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
