@@ -278,16 +278,14 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
     the weights exp(scale q k^T - max) are held to 2^-16 (float32 queries' whole), but those of bfloat16 queries are rounded to
     bfloat16 in a sequence of more than 64 rows (its queries times the heads that share one of keys)."""
     who = "cache_attend"
-    qd = q
-    if qd.ndim and qd.stride(-1) != 1 and qd.shape[-1] > 1:
-        qd = qd.contiguous()
-    if qd.ndim == 4:
-        S, n, h, _ = qd.stride()
-        if S != n * qd.shape[1] and qd.shape[0] > 1 and qd.shape[1] > 1:       # a token's stride is one number
-            qd = qd.contiguous()
-    strides = qd.stride()[-3:-1]
-    if qd.ndim == 4 and qd.shape[1] == 1:
-        strides = (qd.stride(0), strides[1])
+    strides = q.stride()
+    dense = q.ndim < 3 or strides[-1] == 1 or q.shape[-1] < 2
+    if q.ndim == 4 and q.shape[0] > 1 and q.shape[1] > 1:                      # a token's stride is one number
+        dense = dense and strides[0] == strides[1] * q.shape[1]
+    if dense:
+        strides = (strides[0], strides[2]) if q.ndim == 4 and q.shape[1] == 1 else strides[-3:-1]
+    else:
+        strides = (q.shape[-2] * q.shape[-1], q.shape[-1])
     rows = table.ndim != 2 or table.shape[1] < 2 or table.stride(1) == 1       # a row's pages lie next to each other
     spec, att, size = _attend_spec(
         _key(cache, who), q.shape, q.dtype, strides, (table.shape, table.dtype),
@@ -302,7 +300,8 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
         got = cache_attend(_lib.to_device(q, dev), cache, _lib.to_device(table, dev), lengths, starts, scale=scale,
                            causal=causal, window=window, return_lse=return_lse)
         return tuple(_lib.back(t, q) for t in got) if return_lse else _lib.back(got, q)
-    td, ld = table if rows else table.contiguous(), _lib.to_device(lengths, dev).contiguous()
+    qd, td = q if dense else q.contiguous(), table if rows else table.contiguous()
+    ld = _lib.to_device(lengths, dev).contiguous()
     sd = None if starts is None else _lib.to_device(starts, dev).contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None

@@ -118,10 +118,12 @@ def test_cache_attend_refuses_by_its_own_errors(change, text):
         nn.cache_attend(**{**dict(q=torch.zeros(3, 1, 6, 40), cache=_cache(), table=_i32(3, 2), lengths=_i32(3)), **change})
 
 
-def test_a_refused_table_is_not_copied(monkeypatch):
+def test_refused_views_are_not_copied(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "contiguous", lambda t, *args, **more: pytest.fail("copied"))
     with pytest.raises(ValueError, match="keys a sequence"):
         nn.cache_attend(torch.zeros(3, 1, 6, 40), _cache(), _i32(1, 1).expand(3, 2 ** 27), _i32(3))
+    with pytest.raises(ValueError, match="too many"):
+        nn.cache_attend(torch.zeros(3, 1, 1, 1).expand(3, 2 ** 27, 6, 40), _cache(), _i32(3, 2), _i32(3))
 
 
 def test_forward_mode_tangents_are_refused():
