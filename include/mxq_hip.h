@@ -591,7 +591,10 @@ typedef struct mxq_attend_spec {
  * table (int32) names, and the queries [starts[b], starts[b + 1]) (starts NULL: T / B each), whose last one is at the last
  * key: query j of n is at p = lengths[b] - n + j and sees keys up to p where causal, from p - window + 1 on where there is
  * a window.  Lengths are held to the table's pages, starts to T; a key on a page that does not exist is not there.  A
- * query that sees no key, or belongs to no sequence, gets zeros and an lse of -inf.
+ * query that sees no key, or belongs to no sequence, gets zeros and an lse of -inf.  Keys and values below 2^-126 are
+ * rounded to bfloat16's subnormals, those of 2^128 and more are infinite.  Weights exp(scale q k^T - max) are held to 2^-16,
+ * of float32 queries whole, of bfloat16 ones in a sequence of more than 64 rows (queries times heads / kv_heads) rounded to
+ * bfloat16.
  * `workspace`: device memory of mxq_cache_attend_workspace bytes, 256-byte aligned (NULL where that is 0). */
 int64_t mxq_cache_attend_workspace(const mxq_cache_spec* cache, const mxq_attend_spec* spec, int32_t ragged);
 int mxq_cache_attend(const void* q, const uint8_t* k_codes, const uint8_t* k_scales, const uint8_t* v_codes,

@@ -267,16 +267,17 @@ def cache_attend(q: torch.Tensor, cache: PackedCache, table: torch.Tensor, lengt
 
     q: B x n x heads x head_dim, or with starts (B + 1 ascending int32) T x heads x head_dim, sequence b's queries being
     [starts[b], starts[b + 1]); float32, bfloat16 or float16.  heads is a multiple of the cache's; neighbouring heads share
-    one.  table (B x pages, at most 2^31 - 2^16 keys; int32) names each sequence's pages and lengths (B, int32) says how many keys it has, its newest
-    tokens', written before, among them.  The last query is at the last key; query j of n is at position
+    one.  table (B x pages, at most 2^31 - 2^16 keys; int32) names each sequence's pages and lengths (B, int32) says how many
+    keys it has, its newest tokens', written before, among them.  The last query is at the last key; query j of n is at position
     p = lengths[b] - n + j.  causal: it sees keys up to p; window: from p - window + 1 on.  scale (head_dim ** -0.5 by default)
     must be positive as a float32, and 2^127 at most.
 
     Lengths are held to the table's pages and starts to T.  A key on a page that the cache does not have (-1, say) is not
     there.  A query that sees no key, or that belongs to no sequence, gets zeros and an lse of -inf; so does one whose every
-    score is -inf.  A query that sees a value that is no finite number gets no finite number in its column.  Sums are float32;
-    the weights exp(scale q k^T - max) are held to 2^-16 (float32 queries' whole), but those of bfloat16 queries are rounded to
-    bfloat16 in a sequence of more than 64 rows (its queries times the heads that share one of keys)."""
+    score is -inf.  A query that sees a value that is no finite number gets no finite number in its column.  Keys and values
+    below 2^-126 are rounded to bfloat16's subnormals, those of 2^128 and more are infinite.  Sums are float32; the weights
+    exp(scale q k^T - max) are held to 2^-16, float32 queries' whole, but those of bfloat16 queries are rounded to bfloat16 in a
+    sequence of more than 64 rows (its queries times the heads that share one of keys)."""
     who = "cache_attend"
     strides = q.stride()
     dense = q.ndim < 3 or strides[-1] == 1 or q.shape[-1] < 2

@@ -421,6 +421,23 @@ def test_attend_tiny_and_large_scale_bytes(cuda):
             _attend(q, cache, torch.arange(9, dtype=torch.int32, device="cuda")[None], _i32([140]))
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_attend_values_below_the_smallest_normal(cuda, fmt, dtype):
+    """Each value is off by half a step of bfloat16's subnormals at most, 2^-134, and so is their mean by weights; no value is
+    taken for zero that is more than that."""
+    for n in (1, 100):
+        for low in (0, 1, 2, 4, 8):
+            gen = _gen(low)
+            cache = _filled(gen, 5, 16, 1, 64, fmt)
+            cache.v_scales.fill_(low)
+            q = torch.randn(1, n, 4, 64, generator=gen, device="cuda").to(DTYPES[dtype])
+            args = q, cache, torch.arange(5, device="cuda").int()[None], _i32([77])
+            want, _, bound, _ = oc.attend(*args)
+            assert dtype == "f16" or (want != 0).any()
+            _check(nn.cache_attend(*args), want, bound + 2.0 ** -134, (fmt, low, n))
+
+
 @pytest.mark.parametrize("B, n", [(64, 3), (65, 3), (70, 20), (256, 1), (257, 1), (600, 2)])
 def test_attend_sequences_of_short_contexts(cuda, B, n):
     """Contexts too short to be cut, of as many sequences as are looked through for a tile and of more; ragged ones of one
