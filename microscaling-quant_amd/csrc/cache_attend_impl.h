@@ -16,14 +16,15 @@
 // two, all but 2^-16 of them, of others; of bfloat16 queries in tiles of many rows as one, as precise as their output
 // (weight_planes_of).  The sum of weights is of the unrounded ones.
 //
-// Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 110 us, 3.9 TB/s of the 5.2 that
-// a copy reaches, and 8 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step ahead
-// (two and three steps ahead gained nothing), which two workgroups a CU do not keep up with the memory's latency.
-// Many rows: a prompt of 8192 tokens (32 heads on 8, 128 columns, MXFP8): 782 us, 700 TFLOP/s, of the 1350 of a large library
-// product.  Of its cycles 78% issue vector instructions (285 a step of a wave's 32 rows: 96 make bfloat16 of the codes, 16 are
-// exponentials at a quarter of the rate) and 28% the matrix cores'.  Rows that share a step's conversions are as many as
-// registers let two waves a SIMD have: twice the rows with one wave took 2450 us.  Keys and values converted once for the four
-// waves, in LDS, a barrier a step, were fewer instructions (223) and slower, 860 us, the waves waiting for each other.
+// Few rows: 64 sequences of 4 to 8 thousand keys (32 heads on 8, 128 columns, MXFP4, 429 MB): 116 us traced, 3.7 TB/s of the 5.2
+// that a copy reaches, and 9 us of joining; one sequence of 131072: 40 us, 3.6 TB/s, and 8.  A step asks for its 32 keys a step
+// ahead (two and three steps ahead gained nothing), which two workgroups a CU do not keep up with the memory's latency.
+// Many rows: a prompt of 8192 tokens (32 heads on 8, 128 columns, MXFP8): 798 us, 690 TFLOP/s, of the 1350 of a large library
+// product.  Of its cycles 73% issue vector instructions (286 a step of a wave's 32 rows: 96 make bfloat16 of the codes, 16 are
+// exponentials at a quarter of the rate, 32 are the products, which keep the matrix cores busy for 27%).  Rows that share a
+// step's conversions are as many as two waves a SIMD have registers for, or nearly (attend_rows): twice the rows with one wave
+// took 2450 us.  Keys and values converted once for the four waves, in LDS, a barrier a step, were fewer instructions (223) and
+// slower, 860 us, the waves waiting for each other.
 #pragma once
 
 #include "cache_common.h"

@@ -326,11 +326,17 @@ __device__ __forceinline__ int steps_before(int steps, int64_t share, int64_t we
 __device__ __forceinline__ int64_t part_slot(int group, bool first) { return 2 * (int64_t)group + !first; }
 
 constexpr int kWaves = 4;
-// Sixteens of rows that a wave of many queries has: as many as let two waves share a SIMD's registers (of float32's three
-// planes half as many).
+// Sixteens of rows that a wave of many queries has: about as many as let two waves share a SIMD's registers (of float32's three
+// planes half as many).  Not all forms fit.  Bytes a lane in scratch memory, of bfloat16 queries: up to 64 columns 40 to 64 where
+// tiles are whole and 92 to 136 where they are cut, up to 128 none and 8 to 24, past that, of MXFP8 keys, 80 to 96 and 204 to 212
+// (a prompt of 4096 tokens, 32 heads of 64, takes 211 us, 16 heads of 256 take 376).  What finds a piece's tiles, live through
+// its steps, is most of it.
 constexpr int attend_rows(int dtype, int blocks) { return blocks == 8 ? 1 : dtype == MXQ_DT_F32 ? 4 / blocks : 8 / blocks; }
 // Workgroups a CU (of a wave for each of its SIMDs) that the registers are held to; with sixteen rows of 64 columns, where three
-// would nearly fit, 64 sequences' 512 and 1024 tiles took 55 and 92 us of three, 51 and 97 of two.
+// would nearly fit, 64 sequences' 512 and 1024 tiles took 55 and 92 us of three, 51 and 97 of two.  Bytes a lane in scratch
+// memory, of tiles of few rows: bfloat16 queries of more than 128 columns 80 to 84 over MXFP8 keys and 264 to 272 where tiles
+// are cut, over MXFP4 keys 16 there (64 single tokens over 4096 MXFP8 keys of 4 heads of 256: 167 us; float32 ones, of one
+// workgroup a CU, 126); 32 rows of 128 columns 16 to 72 where they are cut; float32 queries of 64 columns 16.
 constexpr int attend_groups(int dtype, int blocks, int tiles) { return dtype == MXQ_DT_BF16 || tiles * blocks < 8 ? 2 : 1; }
 constexpr int blocks_class(int blocks) { return blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8; }
 
